@@ -34,6 +34,7 @@
 // pool[page_table[b, t // P], kvh, t % P], GQA kvh = h // (Hq/Hkv), positions
 // t < seq_len) and cacheir/runtime/cpu.py:342-377 (softmax(q.k * scale) v,
 // prefill causal mask).
+#include "attn_tile.hpp"
 #include "common.hpp"
 
 #include <float.h>
@@ -99,7 +100,6 @@ constexpr int kChunk = 128;  // tokens per partial in the generic path
 // longest-first dispatch also ranks one row per thread in this array.
 constexpr int kPtCache = 64 * kWaves;
 constexpr int kMinSplitTokens = 256;
-constexpr float kLog2e = 1.4426950408889634f;
 
 // Tokens visible to query row `row`, clamped to what the page table can address.
 __device__ __forceinline__ int visible_len(const int32_t* lens, int row, int q_len, int max_ctx) {
@@ -588,23 +588,6 @@ __global__ __launch_bounds__(64 * kWaves) void attn_f16_d128(
 // (28/4) 209 -> 19.  NB = 2 (one max, one rescale and one barrier per 64 tokens of a
 // wavefront) against 1: 2048 after 6000 280 -> 251.
 constexpr int kPfVec = 32;  // query vectors per wavefront (one 32-wide MFMA tile)
-
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-
-// Transposing LDS read: see the kernel's header.
-__device__ __forceinline__ f16x4 lds_read_tr(const uint8_t* p) {
-  typedef __fp16 h4 __attribute__((ext_vector_type(4)));
-  const h4 v = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) h4*)(p));
-  return __builtin_bit_cast(f16x4, v);
-}
-// This wavefront's DMA has landed, then every wavefront's.  The wait is the builtin, not asm: the compiler counts it,
-// and then puts no wait of its own (which would cover the next stage's DMA too) before the reads of the landed stage.
-__device__ __forceinline__ void dma_wait_barrier() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x70);  // vmcnt(0), lgkmcnt(0)
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
 
 template <int VW, int CW, int NB>
 __global__ __launch_bounds__(64 * VW * CW, 2) void attn_prefill_f16_d128(

@@ -27,7 +27,10 @@ CIR_I8_ROW = 65  # ... and int8
 ATTENTION_NOALLOC_MAX_BYTES = 16 << 20  # CIR_ATTENTION_NOALLOC_MAX_BYTES
 GEMM_PARTIALS, GEMM_SWIGLU, GEMM_ARGMAX, GEMM_ATTN_MERGE = 0, 1, 2, 3  # cir_qgemm_plan ops
 
+ROPE_LAYOUTS = {"interleaved": 0, "half": 1}  # CIR_ROPE_*
+
 _c_int, _c_size, _c_float, _vp = ctypes.c_int, ctypes.c_size_t, ctypes.c_float, ctypes.c_void_p
+_c_i64 = ctypes.c_int64
 
 # name -> (restype, argtypes)
 _SIGNATURES = {
@@ -48,6 +51,17 @@ _SIGNATURES = {
     "cir_paged_prefill_split_bytes": (_c_size, [_c_int] * 8),
     "cir_paged_prefill_attention_split": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_size, _c_int, _c_int, _c_int,
                                                    _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _vp]),
+    "cir_shared_attention_workspace_bytes": (_c_size, [_c_int] * 8),
+    "cir_paged_decode_attention_shared": (_c_int, [_vp] * 7 + [_c_int, _vp, _vp, _c_size] + [_c_int] * 6 +
+                                          [_c_float, _c_int, _vp]),
+    "cir_token_logprobs_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int]),
+    "cir_token_logprobs": (_c_int, [_vp, _c_int, _c_i64, _vp, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _c_size,
+                                    _vp]),
+    "cir_extend_page_tables": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int,
+                                        _c_int, _c_int, _vp]),
+    "cir_rope_append": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_int, _vp, _vp, _vp,
+                                 _c_float, _c_int, _c_int, _vp, _c_i64, _c_i64, _vp, _vp, _c_int, _c_i64, _c_int, _c_int,
+                                 _c_int, _c_int, _c_int, _vp]),
     "cir_qweight_tiled_bytes": (_c_size, [_c_int, _c_int, _c_int]),
     "cir_qweight_repack": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _vp]),
     "cir_qweight_repack_rows": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp]),

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -34,6 +35,24 @@ def _cuda(t: torch.Tensor, name: str, rows_only: bool = False) -> None:
         _req(t.dim() == 2 and t.stride(1) == 1, f"{name} rows must be contiguous")
     else:
         _req(t.is_contiguous(), f"{name} must be contiguous")
+
+
+def _call_on(t: torch.Tensor, name: str, *args) -> None:
+    """Launch on the GPU that holds ``t``, on that GPU's current stream (which need not be the current GPU)."""
+    if t.device.index == torch.cuda.current_device():
+        hip.call(name, *args, hip.stream_handle())
+    else:
+        with torch.cuda.device(t.device):
+            hip.call(name, *args, hip.stream_handle())
+
+
+def _tensors(device: torch.device, **named: tuple) -> None:
+    """Each of ``name=(tensor, dtype, shape)``: contiguous, on ``device``, of that dtype and shape."""
+    for name, (t, dtype, shape) in named.items():
+        _cuda(t, name)
+        _req(t.device == device, f"{name} must be on {device}")
+        _req(t.dtype == dtype, f"{name} must be {str(dtype).removeprefix('torch.')}", TypeError)
+        _req(tuple(t.shape) == tuple(shape), f"{name} must be {list(shape)}, got {list(t.shape)}")
 
 
 # ------------------------------------------------------------------ attention --
@@ -159,6 +178,167 @@ def paged_prefill_attention(q, k_pool, v_pool, page_table, seq_lens, q_len: int,
     hip.call(name, q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(),
              out.data_ptr(), workspace.data_ptr(), workspace.numel(), batch, q_len, num_heads, kvh, head_dim, psize,
              max_pages, float(scale), code, hip.stream_handle())
+    return out
+
+
+def shared_attention_workspace(batch: int, groups: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                               page_size: int, max_pages: int, kv_dtype: torch.dtype, device) -> torch.Tensor:
+    """Workspace of ``paged_decode_attention_shared`` at these sizes (one per call that may overlap another)."""
+    n = hip.size_call("cir_shared_attention_workspace_bytes", batch, groups, num_heads, num_kv_heads, head_dim, page_size,
+                      max_pages, hip.dtype_code(kv_dtype))
+    return torch.empty(max(n, 4), dtype=torch.uint8, device=device)
+
+
+def paged_decode_attention_shared(q, k_pool, v_pool, page_table, seq_lens, group_rows, prefix_lens, *,
+                                  scale: float | None = None, out: torch.Tensor | None = None,
+                                  workspace: torch.Tensor | None = None, check_tables: bool = False) -> torch.Tensor:
+    """``paged_decode_attention`` of a batch whose rows share prefixes: rows ``group_rows[g] .. group_rows[g + 1] - 1``
+    (int32 ``[groups + 1]``, ascending) have the same pages for their first ``prefix_lens[g]`` tokens (int32
+    ``[groups]``), and each prefix is read once for all of them.  Both may change between replays of a captured call.
+    ``check_tables`` checks them, the pages and the lengths on the host (a device sync)."""
+    for t, n in ((q, "q"), (k_pool, "k_pool"), (group_rows, "group_rows"), (prefix_lens, "prefix_lens")):
+        _cuda(t, n)
+    _req(q.dim() == 3, "q must be [batch, num_heads, head_dim]")
+    batch, num_heads, head_dim = q.shape
+    slots, kvh, psize, hd = _check_pool(q, k_pool, v_pool, page_table, seq_lens, num_heads, check_tables)
+    _req(hd == head_dim and page_table.dim() == 2 and page_table.shape[0] == batch and seq_lens.shape == (batch,),
+         "shape mismatch")
+    groups, max_pages = prefix_lens.numel(), page_table.shape[1]
+    _tensors(q.device, k_pool=(k_pool, q.dtype, k_pool.shape), v_pool=(v_pool, q.dtype, k_pool.shape),
+             page_table=(page_table, torch.int32, page_table.shape), seq_lens=(seq_lens, torch.int32, (batch,)),
+             group_rows=(group_rows, torch.int32, (groups + 1,)), prefix_lens=(prefix_lens, torch.int32, (groups,)))
+    if check_tables:
+        rows, lens, table = group_rows.tolist(), prefix_lens.tolist(), page_table.cpu()
+        _req(all(a <= b for a, b in zip(rows, rows[1:])) and 0 <= rows[0] and rows[-1] <= batch,
+             "group_rows must ascend within the batch")
+        for g, n in enumerate(lens):
+            part = table[rows[g]: rows[g + 1], : max(0, n) // psize]
+            _req(0 <= n <= max_pages * psize, "prefix_lens exceed the page table capacity")
+            _req(part.numel() == 0 or bool((part == part[:1]).all()), f"group {g}: rows with other pages in the prefix")
+    out = torch.empty_like(q) if out is None else out
+    _tensors(q.device, out=(out, q.dtype, q.shape))
+    if batch == 0:
+        return out
+    if workspace is None:
+        workspace = shared_attention_workspace(batch, groups, num_heads, kvh, head_dim, psize, max_pages, q.dtype,
+                                               q.device)
+    _cuda(workspace, "workspace")
+    _req(workspace.device == q.device, f"workspace must be on {q.device}")
+    scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
+    _call_on(q, "cir_paged_decode_attention_shared", q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
+             page_table.data_ptr(), seq_lens.data_ptr(), group_rows.data_ptr(), prefix_lens.data_ptr(), groups,
+             out.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(), batch, num_heads, kvh,
+             head_dim, psize, max_pages, float(scale), hip.dtype_code(q.dtype))
+    return out
+
+
+# ---------------------------------------------------------------- step inputs --
+class StepTables(NamedTuple):
+    """What ``extend_page_tables`` writes beside the page table (see ``cir_extend_page_tables``)."""
+
+    seq_lens: torch.Tensor   # int32 [batch]: lengths with the granted tokens
+    free_head: torch.Tensor  # int32 [1]: first free slot not taken
+    offsets: torch.Tensor    # int32 [batch + 1]: where each row's new tokens begin
+    positions: torch.Tensor  # int32 [max_tokens]
+    slot_map: torch.Tensor   # int64 [max_tokens]: place in the pools, -1 where there is none
+    granted: torch.Tensor    # int32 [batch]: new tokens that got their pages (all of a row's or none)
+
+    @classmethod
+    def empty(cls, batch: int, max_tokens: int, device) -> "StepTables":
+        i32 = lambda n: torch.empty(n, dtype=torch.int32, device=device)
+        return cls(i32(batch), i32(1), i32(batch + 1), i32(max_tokens),
+                   torch.empty(max_tokens, dtype=torch.int64, device=device), i32(batch))
+
+
+def extend_page_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, new_tokens: torch.Tensor,
+                       free_slots: torch.Tensor, free_head: torch.Tensor, *, page_size: int, max_tokens: int,
+                       out: StepTables | None = None) -> StepTables:
+    """Page tables, positions and slot maps of a step on the GPU: row b's ``new_tokens[b]`` tokens after its
+    ``seq_lens[b]``, new pages taken from ``free_slots[free_head:]`` in row order and written into ``page_table``.
+    ``max_tokens`` bounds the new tokens of all rows (the map's length; its tail is -1).  ``out`` may hold ``seq_lens``
+    and ``free_head`` themselves, which then advance in place (a captured decode step replays without the host)."""
+    _cuda(page_table, "page_table")
+    _req(page_table.dim() == 2 and page_table.shape[1] > 0, "page_table must be [batch, pages]")
+    batch, max_pages = page_table.shape
+    _req(page_size > 0 and max_tokens >= 0, "page_size must be positive and max_tokens not negative")
+    _cuda(free_slots, "free_slots")
+    dev, i32 = page_table.device, torch.int32
+    _tensors(dev, page_table=(page_table, i32, page_table.shape), seq_lens=(seq_lens, i32, (batch,)),
+             new_tokens=(new_tokens, i32, (batch,)), free_slots=(free_slots, i32, (free_slots.numel(),)),
+             free_head=(free_head, i32, (1,)))
+    if out is None:
+        out = StepTables.empty(batch, max_tokens, dev)
+    _tensors(dev, **{"out.seq_lens": (out.seq_lens, i32, (batch,)), "out.free_head": (out.free_head, i32, (1,)),
+                     "out.offsets": (out.offsets, i32, (batch + 1,)),
+                     "out.positions": (out.positions, i32, (max_tokens,)),
+                     "out.slot_map": (out.slot_map, torch.int64, (max_tokens,)),
+                     "out.granted": (out.granted, i32, (batch,))})
+    _call_on(page_table, "cir_extend_page_tables", page_table.data_ptr(), seq_lens.data_ptr(), new_tokens.data_ptr(),
+             free_slots.data_ptr(), free_slots.numel(), free_head.data_ptr(), out.seq_lens.data_ptr(),
+             out.free_head.data_ptr(), out.offsets.data_ptr(), out.granted.data_ptr(), out.positions.data_ptr(),
+             out.slot_map.data_ptr(), batch, max_pages, page_size, max_tokens)
+    return out
+
+
+def rope_frequencies(rotary_dim: int, theta: float, scaling: dict | None = None, device="cuda") -> torch.Tensor:
+    """Angles per position of the ``rotary_dim / 2`` pairs, ``theta ** (-2 i / rotary_dim)`` in float64, for
+    ``rope_append``.  ``scaling`` as model configurations write it: ``{"rope_type": "linear", "factor": s}`` divides
+    every frequency by s; ``"llama3"`` (with ``low_freq_factor`` a, ``high_freq_factor`` b and
+    ``original_max_position_embeddings`` n) keeps frequencies of more than b turns in n positions, divides those of
+    fewer than a by the factor and passes from one to the other linearly in the number of turns.  Other schemes: pass
+    their own table (and their factor on cos and sin) to ``rope_append``."""
+    _req(rotary_dim >= 0 and rotary_dim % 2 == 0, "rotary_dim must be even")
+    _req(theta > 0, "theta must be positive")
+    f = theta ** (-2.0 * torch.arange(rotary_dim // 2, dtype=torch.float64) / max(rotary_dim, 1))
+    kind = (scaling or {}).get("rope_type", (scaling or {}).get("type", "default"))
+    if kind == "linear":
+        f = f / float(scaling["factor"])
+    elif kind == "llama3":
+        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        _req(high > low, "high_freq_factor must exceed low_freq_factor")
+        turns = f * float(scaling["original_max_position_embeddings"]) / (2.0 * math.pi)
+        keep = ((turns - low) / (high - low)).clamp(0.0, 1.0)
+        f = keep * f + (1.0 - keep) * f / float(scaling["factor"])
+    else:
+        _req(kind == "default", f"unsupported rope scaling {kind!r}")
+    return f.to(device)
+
+
+def rope_append(q, k, v, positions, slot_map, inv_freq, k_pool, v_pool, *, layout: str = "interleaved",
+                factor: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions of q ``[T, Hq, D]`` and k ``[T, Hkv, D]`` at ``positions`` and the append of k and v to the pools
+    at ``slot_map`` (int64, a token's page * page_size + offset; outside the pools: padding, nothing is written).  The
+    first ``2 * inv_freq.numel()`` dims of a head turn, in pairs (2i, 2i + 1) (``"interleaved"``) or halves apart
+    (``"half"``); cos and sin are multiplied by ``factor``.  q, k and v may be views (any token and head stride, as the
+    columns of one QKV projection); ``out`` may be q.  Returns the turned q."""
+    for t, n in ((q, "q"), (k, "k"), (v, "v")):
+        _req(isinstance(t, torch.Tensor), f"{n} must be a torch.Tensor", TypeError)
+        _req(t.is_cuda and t.device == q.device, f"{n} must be on the GPU, with q")
+        _req(t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] == 1),
+             f"{n} must be [tokens, heads, head_dim] with contiguous heads")
+        _req(t.dtype == q.dtype, "q, k and v must share a dtype", TypeError)
+    tokens, heads, dim = q.shape
+    kvh = k.shape[1]
+    _req(k.shape == v.shape == (tokens, kvh, dim), "k and v must be [tokens, kv_heads, head_dim] of q's tokens and dims")
+    _req(layout in hip.ROPE_LAYOUTS, f"layout must be one of {sorted(hip.ROPE_LAYOUTS)}")
+    _cuda(k_pool, "k_pool")
+    _req(k_pool.dim() == 4 and k_pool.shape[1] == kvh and k_pool.shape[3] == dim,
+         "pools must be [slots, kv_heads, page_size, head_dim] of k's heads")
+    _cuda(inv_freq, "inv_freq")
+    rot = 2 * inv_freq.numel()
+    _tensors(q.device, k_pool=(k_pool, k_pool.dtype, k_pool.shape), v_pool=(v_pool, k_pool.dtype, k_pool.shape),
+             positions=(positions, torch.int32, (tokens,)), slot_map=(slot_map, torch.int64, (tokens,)),
+             inv_freq=(inv_freq, torch.float64, (inv_freq.numel(),)))
+    _req(rot <= dim, f"inv_freq turns {rot} dims of heads of {dim}")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _req(isinstance(out, torch.Tensor) and out.device == q.device and out.shape == q.shape and
+         (out.stride(2) == 1 or dim == 1) and out.dtype == q.dtype, "out must be like q")
+    _call_on(q, "cir_rope_append", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+             v.data_ptr(), v.stride(0), v.stride(1), hip.dtype_code(q.dtype), positions.data_ptr(), slot_map.data_ptr(),
+             inv_freq.data_ptr(), float(factor), rot, hip.ROPE_LAYOUTS[layout], out.data_ptr(), out.stride(0),
+             out.stride(1), k_pool.data_ptr(), v_pool.data_ptr(), hip.dtype_code(k_pool.dtype),
+             k_pool.shape[0] * k_pool.shape[2], tokens, heads, kvh, dim, k_pool.shape[2])
     return out
 
 
@@ -477,6 +657,47 @@ def argmax(logits: torch.Tensor, out=None) -> torch.Tensor:
         out = torch.empty(rows, dtype=torch.int64, device=logits.device)
     hip.call("cir_argmax", logits.data_ptr(), vocab, out.data_ptr(), rows, vocab, hip.stream_handle())
     return out
+
+
+class TokenLogprobs(NamedTuple):
+    logprobs: torch.Tensor | None  # float32 [rows] of the given tokens
+    entropy: torch.Tensor          # float32 [rows], in nats
+    top_ids: torch.Tensor          # int64 [rows, top_k], most likely first
+    top_logprobs: torch.Tensor     # float32 [rows, top_k]
+
+
+def token_logprobs_workspace(rows: int, vocab: int, top_k: int, device) -> torch.Tensor:
+    return torch.empty(max(hip.size_call("cir_token_logprobs_workspace_bytes", rows, vocab, top_k), 8),
+                       dtype=torch.uint8, device=device)
+
+
+def token_logprobs(logits: torch.Tensor, ids: torch.Tensor | None, top_k: int = 0, *,
+                   workspace: torch.Tensor | None = None) -> TokenLogprobs:
+    """Log probabilities of ``ids`` (int64 ``[rows]``; an id outside the vocabulary gives NaN), entropy and the ``top_k``
+    (0..64) most likely tokens of each row of ``logits`` (float32 or float16 ``[rows, vocab]``, any row stride) in one
+    pass.  Ties go to the lowest id, NaN counts as the largest logit; see ``cir_token_logprobs``."""
+    _req(isinstance(logits, torch.Tensor), "logits must be a torch.Tensor", TypeError)
+    _req(logits.is_cuda, "logits must be on the GPU")
+    _req(logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1),
+         "logits must be [rows, vocab] with contiguous rows")
+    rows, vocab = logits.shape
+    ld = logits.stride(0) if rows > 1 else vocab
+    _req(ld >= vocab, "logits rows overlap")
+    _req(0 <= top_k <= 64 and top_k <= vocab, f"top_k must be 0..64 and at most the vocabulary (got {top_k})")
+    code, dev = hip.dtype_code(logits.dtype), logits.device
+    if ids is not None:
+        _tensors(dev, ids=(ids, torch.int64, (rows,)))
+    f32 = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dev)
+    res = TokenLogprobs(None if ids is None else f32(rows), f32(rows),
+                        torch.empty((rows, top_k), dtype=torch.int64, device=dev), f32(rows, top_k))
+    if workspace is None:
+        workspace = token_logprobs_workspace(rows, vocab, top_k, dev)
+    _cuda(workspace, "workspace")
+    _req(workspace.device == dev, f"workspace must be on {dev}")
+    _call_on(logits, "cir_token_logprobs", logits.data_ptr(), code, ld, hip.ptr(ids), rows, vocab, top_k,
+             hip.ptr(res.logprobs), res.entropy.data_ptr(), res.top_ids.data_ptr(), res.top_logprobs.data_ptr(),
+             workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    return res
 
 
 def stream_read(buf: torch.Tensor, workgroups: int, threads: int, layout: int, out: torch.Tensor,

@@ -156,6 +156,32 @@ int cir_paged_prefill_attention_split(const void* q, const void* k_pool, const v
                                       int batch, int q_len, int num_heads, int num_kv_heads, int head_dim,
                                       int page_size, int max_pages, float scale, int kv_dtype, void* stream);
 
+/* Decode attention of a batch whose rows share prefixes: cir_paged_decode_attention with
+ * the same q, pools, page_table, seq_lens and out, where rows group_rows[g] ..
+ * group_rows[g + 1] - 1 (int32 [groups + 1], on the device, ascending, in 0 .. batch) have
+ * the same page table entries, and so the same K and V, for their first prefix_lens[g]
+ * tokens (int32 [groups], on the device).  Each prefix is then read once for the query
+ * vectors of all its rows instead of once per row; the result is the attention over each
+ * row's whole context, whatever part of it is shared.  The pages of a prefix are taken from
+ * the group's first row; sharing stops at that row's length, and a row shorter than the
+ * prefix, a group of one row and rows in no group read all of their context alone.
+ * group_rows out of order switch sharing off.  A sequence with seq_len 0 yields zeros, one
+ * whose scores are all -inf NaN.
+ * fp16 pools on 16-byte addresses, head_dim 128, page_size a multiple of 16, up to 32 query
+ * heads per KV head, 4096 rows and 512 groups; other calls run cir_paged_decode_attention
+ * (every row reads its prefix).  A row's last bits depend on the batch it is in.
+ * workspace: cir_shared_attention_workspace_bytes bytes on a 16-byte address, written by
+ * the call (calls that overlap need one each); nothing in it needs clearing.
+ * Replaces, for such batches, cacheir/backends/triton_kernels.py:174-217. */
+size_t cir_shared_attention_workspace_bytes(int batch, int groups, int num_heads, int num_kv_heads, int head_dim,
+                                            int page_size, int max_pages, int kv_dtype);
+int cir_paged_decode_attention_shared(const void* q, const void* k_pool, const void* v_pool,
+                                      const int32_t* page_table, const int32_t* seq_lens,
+                                      const int32_t* group_rows, const int32_t* prefix_lens, int groups, void* out,
+                                      void* workspace, size_t workspace_bytes, int batch, int num_heads,
+                                      int num_kv_heads, int head_dim, int page_size, int max_pages, float scale,
+                                      int kv_dtype, void* stream);
+
 /* ------------------------------------------------------------ block weights ---
  * GGUF Q4_0 / Q8_0 blocks (cacheir/importers/gguf.py:36,40,273-310) for a weight
  * W[n, k] stored row-major, blocks along k.  The GEMM reads a tiled copy made once
@@ -314,6 +340,66 @@ int cir_argmax(const float* logits, int ld, int64_t* ids, int rows, int vocab, v
 size_t cir_qgemm_argmax_workspace_bytes(int m, int n);
 int cir_qgemm_argmax(const void* x, int ldx, const void* w_tiled, int fmt, int64_t* ids, void* workspace,
                      size_t ws_bytes, int m, int n, int k, void* stream);
+
+/* Log probabilities of given tokens, entropy and the top_k most likely tokens of rows of
+ * logits (dt CIR_F32 or CIR_F16, row stride ld elements, any alignment of a row):
+ *   logprobs[r] = log softmax(logits[r])[ids[r]]   (NaN for an id outside 0 .. vocab - 1)
+ *   entropy[r]  = -sum p log p                      (natural logarithm; p log p = 0 at p = 0)
+ *   top_ids[r][0 .. top_k), top_logprobs likewise: by decreasing logit, equal ones by index
+ *     (a logit of -inf counts as any other value; NaN is above every number, as in cir_argmax).
+ * A row that holds NaN or +inf, or -inf alone, has NaN probabilities.  ids may be NULL
+ * (logprobs is then not written).  0 <= top_k <= 64, top_k <= vocab; statistics in fp32.
+ * workspace: cir_token_logprobs_workspace_bytes bytes on an 8-byte address (0: NULL will
+ * do), written by the call.  No counterpart in the reference, whose sampling is greedy. */
+size_t cir_token_logprobs_workspace_bytes(int rows, int vocab, int top_k);
+int cir_token_logprobs(const void* logits, int dt, int64_t ld, const int64_t* ids, int rows, int vocab, int top_k,
+                       float* logprobs, float* entropy, int64_t* top_ids, float* top_logprobs, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------- step inputs ---
+ * Page tables and slot maps of a step from its request lengths, on the device: row b holds
+ * seq_lens[b] tokens and gets new_tokens[b] more (a negative count is 0).  Row by row, the
+ * pages ceil(seq_len / page_size) .. ceil((seq_len + new) / page_size) - 1 take
+ * free_slots[free_head[0]], the entry after it, and so on, up to free_slots[free_total - 1]:
+ *   page_table[b][...]  the new entries (others are left as they were)
+ *   granted[b]          new_tokens[b], or 0 for a row that does not get its pages: it needs more
+ *                       than max_pages, its tokens end past max_tokens, or the free slots ran
+ *                       out at it or at a row before it (a row that needs no page is served)
+ *   seq_lens_out[b]     seq_lens[b] + granted[b];  free_head_out[0] = free_head[0] + pages taken
+ *   offsets[0 .. batch] where each row's new tokens begin (a sum over new_tokens, granted or not)
+ *   positions[j], slot_map[j], j < max_tokens: position of token j in its sequence and its place
+ *                       in the pools, page_table[b][position / page_size] * page_size +
+ *                       position % page_size (-1 for tokens of a row that was not granted and,
+ *                       with position 0, past the last row's)
+ * seq_lens_out may be seq_lens and free_head_out free_head (updated in place, so a captured
+ * step advances with every replay); the other outputs may not overlap an input.  The page that a row's
+ * next token falls in must be the row's own (the pool's copy on write does that on the host).
+ * Replaces the host loops of cacheir/runtime/kv_cache.py:110-122 and cuda.py:1218-1237. */
+int cir_extend_page_tables(int32_t* page_table, const int32_t* seq_lens, const int32_t* new_tokens,
+                           const int32_t* free_slots, int free_total, const int32_t* free_head, int32_t* seq_lens_out,
+                           int32_t* free_head_out, int32_t* offsets, int32_t* granted, int32_t* positions,
+                           int64_t* slot_map, int batch, int max_pages, int page_size, int max_tokens, void* stream);
+
+/* Rotary positions of q and k, and the append of k and v to the pages, token by token
+ * (cacheir/runtime/cpu.py:324-340 has interleaved pairs over the whole head): q
+ * [tokens, num_heads, head_dim], k and v [tokens, num_kv_heads, head_dim] of dtype dt with
+ * any token and head stride (elements; the dims of a head are contiguous).  Pair i <
+ * rotary_dim / 2 of a head -- dims (2i, 2i + 1) for CIR_ROPE_INTERLEAVED, (i, i + rotary_dim
+ * / 2) for CIR_ROPE_HALF -- turns by positions[t] * inv_freq[i] (fp64; the angle is formed and
+ * reduced in 64 bits) and is multiplied by factor; dims from rotary_dim on pass unchanged.
+ * q_out has q's dtype and may be q; token t's k and v go to slot_map[t]: page
+ * slot_map[t] / page_size, offset slot_map[t] % page_size of pools of `slots` tokens in all
+ * (pages * page_size).  A token whose slot lies outside 0 .. slots - 1 is padding: nothing
+ * of it is written, q_out included.  Two tokens must not share a slot.  head_dim even and
+ * <= 256, rotary_dim even and <= head_dim. */
+#define CIR_ROPE_INTERLEAVED 0
+#define CIR_ROPE_HALF 1
+int cir_rope_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                    int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride, int dt,
+                    const int32_t* positions, const int64_t* slot_map, const double* inv_freq, float factor,
+                    int rotary_dim, int layout, void* q_out, int64_t o_token_stride, int64_t o_head_stride,
+                    void* k_pool, void* v_pool, int kv_dtype, int64_t slots, int tokens, int num_heads,
+                    int num_kv_heads, int head_dim, int page_size, void* stream);
 
 /* ------------------------------------------------------------- calibration ---
  * Reads `bytes` (a multiple of 16) from buf with `workgroups` x `threads` threads,

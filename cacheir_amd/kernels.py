@@ -37,13 +37,20 @@ def _cuda(t: torch.Tensor, name: str, rows_only: bool = False) -> None:
         _req(t.is_contiguous(), f"{name} must be contiguous")
 
 
-def _call_on(t: torch.Tensor, name: str, *args) -> None:
-    """Launch on the GPU that holds ``t``, on that GPU's current stream (which need not be the current GPU)."""
-    if t.device.index == torch.cuda.current_device():
-        hip.call(name, *args, hip.stream_handle())
+def _call_on(dev: int, name: str, *args) -> None:
+    """Launch on GPU ``dev``, on its current stream (it need not be the current GPU)."""
+    if dev == torch._C._cuda_getDevice():
+        hip.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
     else:
-        with torch.cuda.device(t.device):
-            hip.call(name, *args, hip.stream_handle())
+        with torch.cuda.device(dev):
+            hip.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+
+
+def _fits(t, dev: int, dtype: torch.dtype, shape: tuple) -> bool:
+    """A contiguous tensor of this type and shape on GPU ``dev``: the test of ``_tensors`` without its messages.  The
+    wrappers of small launches ask this first (0.4 us a tensor against 1.5: page tables of 128 rows took 32 us of the host
+    for 8 of the GPU, now 12.5) and look for what is wrong only if something is."""
+    return t.get_device() == dev and t.dtype is dtype and t.shape == shape and t.is_contiguous()
 
 
 def _tensors(device: torch.device, **named: tuple) -> None:
@@ -189,18 +196,18 @@ def shared_attention_workspace(batch: int, groups: int, num_heads: int, num_kv_h
     return torch.empty(max(n, 4), dtype=torch.uint8, device=device)
 
 
-def paged_decode_attention_shared(q, k_pool, v_pool, page_table, seq_lens, group_rows, prefix_lens, *,
-                                  scale: float | None = None, out: torch.Tensor | None = None,
-                                  workspace: torch.Tensor | None = None, check_tables: bool = False) -> torch.Tensor:
-    """``paged_decode_attention`` of a batch whose rows share prefixes: rows ``group_rows[g] .. group_rows[g + 1] - 1``
-    (int32 ``[groups + 1]``, ascending) have the same pages for their first ``prefix_lens[g]`` tokens (int32
-    ``[groups]``), and each prefix is read once for all of them.  Both may change between replays of a captured call.
-    ``check_tables`` checks them, the pages and the lengths on the host (a device sync)."""
+def _check_workspace(workspace, dev: int) -> None:
+    if not (workspace.get_device() == dev and workspace.is_contiguous()):
+        _cuda(workspace, "workspace")
+        _req(False, f"workspace must be on cuda:{dev}")
+
+
+def _check_shared(q, k_pool, v_pool, page_table, seq_lens, group_rows, prefix_lens, check_tables: bool) -> None:
     for t, n in ((q, "q"), (k_pool, "k_pool"), (group_rows, "group_rows"), (prefix_lens, "prefix_lens")):
         _cuda(t, n)
     _req(q.dim() == 3, "q must be [batch, num_heads, head_dim]")
     batch, num_heads, head_dim = q.shape
-    slots, kvh, psize, hd = _check_pool(q, k_pool, v_pool, page_table, seq_lens, num_heads, check_tables)
+    _, _, psize, hd = _check_pool(q, k_pool, v_pool, page_table, seq_lens, num_heads, check_tables)
     _req(hd == head_dim and page_table.dim() == 2 and page_table.shape[0] == batch and seq_lens.shape == (batch,),
          "shape mismatch")
     groups, max_pages = prefix_lens.numel(), page_table.shape[1]
@@ -215,20 +222,42 @@ def paged_decode_attention_shared(q, k_pool, v_pool, page_table, seq_lens, group
             part = table[rows[g]: rows[g + 1], : max(0, n) // psize]
             _req(0 <= n <= max_pages * psize, "prefix_lens exceed the page table capacity")
             _req(part.numel() == 0 or bool((part == part[:1]).all()), f"group {g}: rows with other pages in the prefix")
-    out = torch.empty_like(q) if out is None else out
-    _tensors(q.device, out=(out, q.dtype, q.shape))
+
+
+def paged_decode_attention_shared(q, k_pool, v_pool, page_table, seq_lens, group_rows, prefix_lens, *,
+                                  scale: float | None = None, out: torch.Tensor | None = None,
+                                  workspace: torch.Tensor | None = None, check_tables: bool = False) -> torch.Tensor:
+    """``paged_decode_attention`` of a batch whose rows share prefixes: rows ``group_rows[g] .. group_rows[g + 1] - 1``
+    (int32 ``[groups + 1]``, ascending) have the same pages for their first ``prefix_lens[g]`` tokens (int32
+    ``[groups]``), and each prefix is read once for all of them.  Both may change between replays of a captured call.
+    ``check_tables`` checks them, the pages and the lengths on the host (a device sync)."""
+    dev, dt = q.get_device(), q.dtype
+    if not (dev >= 0 and q.dim() == 3 and k_pool.dim() == 4 and page_table.dim() == 2 and not check_tables
+            and _fits(q, dev, dt, q.shape) and _fits(k_pool, dev, dt, k_pool.shape)
+            and _fits(v_pool, dev, dt, k_pool.shape) and q.shape[2] == k_pool.shape[3]
+            and _fits(page_table, dev, torch.int32, (q.shape[0], page_table.shape[1]))
+            and _fits(seq_lens, dev, torch.int32, (q.shape[0],))
+            and _fits(prefix_lens, dev, torch.int32, (prefix_lens.numel(),))
+            and _fits(group_rows, dev, torch.int32, (prefix_lens.numel() + 1,))):
+        _check_shared(q, k_pool, v_pool, page_table, seq_lens, group_rows, prefix_lens, check_tables)
+    batch, num_heads, head_dim = q.shape
+    kvh, psize = k_pool.shape[1], k_pool.shape[2]
+    groups, max_pages = prefix_lens.numel(), page_table.shape[1]
+    if out is None:
+        out = torch.empty_like(q)
+    elif not _fits(out, dev, dt, q.shape):
+        _tensors(q.device, out=(out, dt, q.shape))
     if batch == 0:
         return out
     if workspace is None:
         workspace = shared_attention_workspace(batch, groups, num_heads, kvh, head_dim, psize, max_pages, q.dtype,
                                                q.device)
-    _cuda(workspace, "workspace")
-    _req(workspace.device == q.device, f"workspace must be on {q.device}")
+    _check_workspace(workspace, dev)
     scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
-    _call_on(q, "cir_paged_decode_attention_shared", q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
+    _call_on(dev, "cir_paged_decode_attention_shared", q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
              page_table.data_ptr(), seq_lens.data_ptr(), group_rows.data_ptr(), prefix_lens.data_ptr(), groups,
-             out.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(), batch, num_heads, kvh,
-             head_dim, psize, max_pages, float(scale), hip.dtype_code(q.dtype))
+             out.data_ptr(), workspace.data_ptr(), workspace.nbytes, batch, num_heads, kvh, head_dim, psize, max_pages,
+             scale, hip.dtype_code(dt))
     return out
 
 
@@ -245,9 +274,11 @@ class StepTables(NamedTuple):
 
     @classmethod
     def empty(cls, batch: int, max_tokens: int, device) -> "StepTables":
-        i32 = lambda n: torch.empty(n, dtype=torch.int32, device=device)
-        return cls(i32(batch), i32(1), i32(batch + 1), i32(max_tokens),
-                   torch.empty(max_tokens, dtype=torch.int64, device=device), i32(batch))
+        # one allocation for what is int32 (six of them took 8 us of a call)
+        lens, head, offsets, positions, granted = torch.empty(
+            3 * batch + 2 + max_tokens, dtype=torch.int32, device=device).split_with_sizes(
+                (batch, 1, batch + 1, max_tokens, batch))
+        return cls(lens, head, offsets, positions, torch.empty(max_tokens, dtype=torch.int64, device=device), granted)
 
 
 def extend_page_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, new_tokens: torch.Tensor,
@@ -257,26 +288,30 @@ def extend_page_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, new_tok
     ``seq_lens[b]``, new pages taken from ``free_slots[free_head:]`` in row order and written into ``page_table``.
     ``max_tokens`` bounds the new tokens of all rows (the map's length; its tail is -1).  ``out`` may hold ``seq_lens``
     and ``free_head`` themselves, which then advance in place (a captured decode step replays without the host)."""
-    _cuda(page_table, "page_table")
-    _req(page_table.dim() == 2 and page_table.shape[1] > 0, "page_table must be [batch, pages]")
+    dev, i32 = page_table.get_device(), torch.int32
+    if not (dev >= 0 and page_table.dim() == 2 and _fits(page_table, dev, i32, page_table.shape)
+            and _fits(seq_lens, dev, i32, page_table.shape[:1]) and _fits(new_tokens, dev, i32, page_table.shape[:1])
+            and _fits(free_slots, dev, i32, (free_slots.numel(),)) and _fits(free_head, dev, i32, (1,))):
+        _cuda(page_table, "page_table")
+        _req(page_table.dim() == 2, "page_table must be [batch, pages]")
+        _cuda(free_slots, "free_slots")
+        _tensors(page_table.device, page_table=(page_table, i32, page_table.shape),
+                 seq_lens=(seq_lens, i32, page_table.shape[:1]), new_tokens=(new_tokens, i32, page_table.shape[:1]),
+                 free_slots=(free_slots, i32, (free_slots.numel(),)), free_head=(free_head, i32, (1,)))
     batch, max_pages = page_table.shape
     _req(page_size > 0 and max_tokens >= 0, "page_size must be positive and max_tokens not negative")
-    _cuda(free_slots, "free_slots")
-    dev, i32 = page_table.device, torch.int32
-    _tensors(dev, page_table=(page_table, i32, page_table.shape), seq_lens=(seq_lens, i32, (batch,)),
-             new_tokens=(new_tokens, i32, (batch,)), free_slots=(free_slots, i32, (free_slots.numel(),)),
-             free_head=(free_head, i32, (1,)))
     if out is None:
-        out = StepTables.empty(batch, max_tokens, dev)
-    _tensors(dev, **{"out.seq_lens": (out.seq_lens, i32, (batch,)), "out.free_head": (out.free_head, i32, (1,)),
-                     "out.offsets": (out.offsets, i32, (batch + 1,)),
-                     "out.positions": (out.positions, i32, (max_tokens,)),
-                     "out.slot_map": (out.slot_map, torch.int64, (max_tokens,)),
-                     "out.granted": (out.granted, i32, (batch,))})
-    _call_on(page_table, "cir_extend_page_tables", page_table.data_ptr(), seq_lens.data_ptr(), new_tokens.data_ptr(),
-             free_slots.data_ptr(), free_slots.numel(), free_head.data_ptr(), out.seq_lens.data_ptr(),
-             out.free_head.data_ptr(), out.offsets.data_ptr(), out.granted.data_ptr(), out.positions.data_ptr(),
-             out.slot_map.data_ptr(), batch, max_pages, page_size, max_tokens)
+        out = StepTables.empty(batch, max_tokens, page_table.device)
+    else:
+        _tensors(page_table.device, **{
+            "out.seq_lens": (out.seq_lens, i32, (batch,)), "out.free_head": (out.free_head, i32, (1,)),
+            "out.offsets": (out.offsets, i32, (batch + 1,)), "out.positions": (out.positions, i32, (max_tokens,)),
+            "out.slot_map": (out.slot_map, torch.int64, (max_tokens,)), "out.granted": (out.granted, i32, (batch,))})
+    lens, head, offsets, positions, slot_map, granted = out
+    _call_on(dev, "cir_extend_page_tables", page_table.data_ptr(), seq_lens.data_ptr(), new_tokens.data_ptr(),
+             free_slots.data_ptr(), free_slots.numel(), free_head.data_ptr(), lens.data_ptr(), head.data_ptr(),
+             offsets.data_ptr(), granted.data_ptr(), positions.data_ptr(), slot_map.data_ptr(), batch, max_pages,
+             page_size, max_tokens)
     return out
 
 
@@ -304,6 +339,26 @@ def rope_frequencies(rotary_dim: int, theta: float, scaling: dict | None = None,
     return f.to(device)
 
 
+def _check_rope(q, k, v, positions, slot_map, inv_freq, k_pool, v_pool) -> None:
+    for t, n in ((q, "q"), (k, "k"), (v, "v")):
+        _req(isinstance(t, torch.Tensor), f"{n} must be a torch.Tensor", TypeError)
+        _req(t.is_cuda and t.device == q.device, f"{n} must be on the GPU, with q")
+        _req(t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] == 1),
+             f"{n} must be [tokens, heads, head_dim] with contiguous heads")
+        _req(t.dtype == q.dtype, "q, k and v must share a dtype", TypeError)
+    tokens, _, dim = q.shape
+    kvh = k.shape[1]
+    _req(k.shape == v.shape == (tokens, kvh, dim), "k and v must be [tokens, kv_heads, head_dim] of q's tokens and dims")
+    _cuda(k_pool, "k_pool")
+    _req(k_pool.dim() == 4 and k_pool.shape[1] == kvh and k_pool.shape[3] == dim,
+         "pools must be [slots, kv_heads, page_size, head_dim] of k's heads")
+    _cuda(inv_freq, "inv_freq")
+    _tensors(q.device, k_pool=(k_pool, k_pool.dtype, k_pool.shape), v_pool=(v_pool, k_pool.dtype, k_pool.shape),
+             positions=(positions, torch.int32, (tokens,)), slot_map=(slot_map, torch.int64, (tokens,)),
+             inv_freq=(inv_freq, torch.float64, (inv_freq.numel(),)))
+    _req(2 * inv_freq.numel() <= dim, f"inv_freq turns {2 * inv_freq.numel()} dims of heads of {dim}")
+
+
 def rope_append(q, k, v, positions, slot_map, inv_freq, k_pool, v_pool, *, layout: str = "interleaved",
                 factor: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
     """Rotary positions of q ``[T, Hq, D]`` and k ``[T, Hkv, D]`` at ``positions`` and the append of k and v to the pools
@@ -311,34 +366,32 @@ def rope_append(q, k, v, positions, slot_map, inv_freq, k_pool, v_pool, *, layou
     first ``2 * inv_freq.numel()`` dims of a head turn, in pairs (2i, 2i + 1) (``"interleaved"``) or halves apart
     (``"half"``); cos and sin are multiplied by ``factor``.  q, k and v may be views (any token and head stride, as the
     columns of one QKV projection); ``out`` may be q.  Returns the turned q."""
-    for t, n in ((q, "q"), (k, "k"), (v, "v")):
-        _req(isinstance(t, torch.Tensor), f"{n} must be a torch.Tensor", TypeError)
-        _req(t.is_cuda and t.device == q.device, f"{n} must be on the GPU, with q")
-        _req(t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] == 1),
-             f"{n} must be [tokens, heads, head_dim] with contiguous heads")
-        _req(t.dtype == q.dtype, "q, k and v must share a dtype", TypeError)
-    tokens, heads, dim = q.shape
-    kvh = k.shape[1]
-    _req(k.shape == v.shape == (tokens, kvh, dim), "k and v must be [tokens, kv_heads, head_dim] of q's tokens and dims")
+    dev, dt = q.get_device(), q.dtype
+    kdt, rot = k_pool.dtype, 2 * inv_freq.numel()
+    if not (dev >= 0 and q.dim() == k.dim() == 3 and k_pool.dim() == 4 and k.get_device() == v.get_device() == dev
+            and k.dtype is dt and v.dtype is dt and v.shape == k.shape and k.shape[0] == q.shape[0]
+            and k.shape[2] == q.shape[2] and q.stride(2) == k.stride(2) == v.stride(2) == 1
+            and k_pool.shape[1] == k.shape[1] and k_pool.shape[3] == q.shape[2] >= rot
+            and _fits(k_pool, dev, kdt, k_pool.shape) and _fits(v_pool, dev, kdt, k_pool.shape)
+            and _fits(positions, dev, torch.int32, q.shape[:1]) and _fits(slot_map, dev, torch.int64, q.shape[:1])
+            and _fits(inv_freq, dev, torch.float64, (rot // 2,))):
+        _check_rope(q, k, v, positions, slot_map, inv_freq, k_pool, v_pool)
     _req(layout in hip.ROPE_LAYOUTS, f"layout must be one of {sorted(hip.ROPE_LAYOUTS)}")
-    _cuda(k_pool, "k_pool")
-    _req(k_pool.dim() == 4 and k_pool.shape[1] == kvh and k_pool.shape[3] == dim,
-         "pools must be [slots, kv_heads, page_size, head_dim] of k's heads")
-    _cuda(inv_freq, "inv_freq")
-    rot = 2 * inv_freq.numel()
-    _tensors(q.device, k_pool=(k_pool, k_pool.dtype, k_pool.shape), v_pool=(v_pool, k_pool.dtype, k_pool.shape),
-             positions=(positions, torch.int32, (tokens,)), slot_map=(slot_map, torch.int64, (tokens,)),
-             inv_freq=(inv_freq, torch.float64, (inv_freq.numel(),)))
-    _req(rot <= dim, f"inv_freq turns {rot} dims of heads of {dim}")
+    tokens, heads, dim = q.shape
+    slots, kvh, psize, _ = k_pool.shape
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _req(isinstance(out, torch.Tensor) and out.device == q.device and out.shape == q.shape and
-         (out.stride(2) == 1 or dim == 1) and out.dtype == q.dtype, "out must be like q")
-    _call_on(q, "cir_rope_append", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-             v.data_ptr(), v.stride(0), v.stride(1), hip.dtype_code(q.dtype), positions.data_ptr(), slot_map.data_ptr(),
-             inv_freq.data_ptr(), float(factor), rot, hip.ROPE_LAYOUTS[layout], out.data_ptr(), out.stride(0),
-             out.stride(1), k_pool.data_ptr(), v_pool.data_ptr(), hip.dtype_code(k_pool.dtype),
-             k_pool.shape[0] * k_pool.shape[2], tokens, heads, kvh, dim, k_pool.shape[2])
+        out = torch.empty(q.shape, dtype=dt, device=q.device)
+    else:
+        _req(isinstance(out, torch.Tensor) and out.device == q.device and out.shape == q.shape and
+             (out.stride(2) == 1 or dim == 1) and out.dtype == dt, "out must be like q")
+    q0, q1, _ = q.stride()
+    k0, k1, _ = k.stride()
+    v0, v1, _ = v.stride()
+    o0, o1, _ = out.stride()
+    _call_on(dev, "cir_rope_append", q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1,
+             hip.dtype_code(dt), positions.data_ptr(), slot_map.data_ptr(), inv_freq.data_ptr(), factor, rot,
+             hip.ROPE_LAYOUTS[layout], out.data_ptr(), o0, o1, k_pool.data_ptr(), v_pool.data_ptr(),
+             hip.dtype_code(kdt), slots * psize, tokens, heads, kvh, dim, psize)
     return out
 
 
@@ -677,26 +730,30 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor | None, top_k: int = 
     (0..64) most likely tokens of each row of ``logits`` (float32 or float16 ``[rows, vocab]``, any row stride) in one
     pass.  Ties go to the lowest id, NaN counts as the largest logit; see ``cir_token_logprobs``."""
     _req(isinstance(logits, torch.Tensor), "logits must be a torch.Tensor", TypeError)
-    _req(logits.is_cuda, "logits must be on the GPU")
+    dev = logits.get_device()
+    _req(dev >= 0, "logits must be on the GPU")
     _req(logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1),
          "logits must be [rows, vocab] with contiguous rows")
     rows, vocab = logits.shape
     ld = logits.stride(0) if rows > 1 else vocab
     _req(ld >= vocab, "logits rows overlap")
-    _req(0 <= top_k <= 64 and top_k <= vocab, f"top_k must be 0..64 and at most the vocabulary (got {top_k})")
-    code, dev = hip.dtype_code(logits.dtype), logits.device
-    if ids is not None:
-        _tensors(dev, ids=(ids, torch.int64, (rows,)))
-    f32 = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dev)
-    res = TokenLogprobs(None if ids is None else f32(rows), f32(rows),
-                        torch.empty((rows, top_k), dtype=torch.int64, device=dev), f32(rows, top_k))
+    if not (0 <= top_k <= 64 and top_k <= vocab):
+        _req(False, f"top_k must be 0..64 and at most the vocabulary (got {top_k})")
+    code = hip.dtype_code(logits.dtype)
+    if ids is not None and not _fits(ids, dev, torch.int64, (rows,)):
+        _tensors(logits.device, ids=(ids, torch.int64, (rows,)))
+    # one allocation for what is float32
+    n = 0 if ids is None else rows
+    lp, entropy, top_lp = torch.empty(n + rows + rows * top_k, dtype=torch.float32,
+                                      device=logits.device).split_with_sizes((n, rows, rows * top_k))
+    res = TokenLogprobs(None if ids is None else lp, entropy,
+                        torch.empty((rows, top_k), dtype=torch.int64, device=logits.device), top_lp.view(rows, top_k))
     if workspace is None:
-        workspace = token_logprobs_workspace(rows, vocab, top_k, dev)
-    _cuda(workspace, "workspace")
-    _req(workspace.device == dev, f"workspace must be on {dev}")
-    _call_on(logits, "cir_token_logprobs", logits.data_ptr(), code, ld, hip.ptr(ids), rows, vocab, top_k,
-             hip.ptr(res.logprobs), res.entropy.data_ptr(), res.top_ids.data_ptr(), res.top_logprobs.data_ptr(),
-             workspace.data_ptr(), workspace.numel() * workspace.element_size())
+        workspace = token_logprobs_workspace(rows, vocab, top_k, logits.device)
+    else:
+        _check_workspace(workspace, dev)
+    _call_on(dev, "cir_token_logprobs", logits.data_ptr(), code, ld, hip.ptr(ids), rows, vocab, top_k, lp.data_ptr(),
+             entropy.data_ptr(), res.top_ids.data_ptr(), top_lp.data_ptr(), workspace.data_ptr(), workspace.nbytes)
     return res
 
 

@@ -6,15 +6,16 @@
 // (max, sum of e^(s - m), sum of e^(s - m) v), and the pieces of a row, its group's prefix
 // among them, are joined by sum 2^(m_i - M) (l_i, O_i) in a second launch.
 //
-// Work.  Two kinds of item: (group, tile of 128 query vectors, KV head) over the prefix, and
-// (row, KV head) over what follows it; a group of up to 32 vectors makes one tile of 32.
-// An item costs kItemCost + its 32-token blocks; the items lie on one axis, prefixes first,
-// and each of kGroups persistent workgroups takes an equal stretch of that axis, whatever
-// rows it crosses: lengths live on the device, and a grid cut by rows or by a fixed number
-// of splits leaves CUs idle behind the longest row.  Every workgroup finds its stretch by a
-// scan over the groups and rows (from L2, ~1 us).  A piece of item i computed by workgroup w
-// has the slot w + i: along the axis one of the two grows from piece to piece, so slots are
-// unique, and the join finds an item's pieces from its start and the stretch alone.
+// Work.  Two kinds of item: (group, tile of 128 query vectors) over the prefix, and a row
+// over what follows it; a group of up to 32 vectors makes one tile of 32.  An item costs
+// kItemCost + its 32-token blocks; the items lie on one axis, prefixes first, and each team
+// of workgroups (one per KV head) takes an equal stretch of that axis, whatever rows it
+// crosses: lengths live on the device, and a grid cut by rows or by a fixed number of splits
+// leaves CUs idle behind the longest row.  Every workgroup finds its stretch by a scan over
+// the groups and rows (from L2, ~1 us).  A piece of item i computed by team w has the slot
+// w + i: along the axis one of the two grows from piece to piece, so slots are unique, and
+// the join finds an item's pieces from its start and the stretch alone.  The workgroups of a
+// team walk the same pages in step, one head of each.
 //
 // Bodies (8 wavefronts, one workgroup per CU, MFMA 32x32x16 f16, S^T = K Q^T and
 // O^T = V^T P^T as in the prefill attention, whose LDS swizzles these are):
@@ -40,7 +41,7 @@ constexpr int kBlock = 32;        // tokens of an MFMA tile
 constexpr int kVec = 32;          // query vectors of an MFMA tile
 constexpr int kWaves = 8;
 constexpr int kThreads = 64 * kWaves;
-constexpr int kGroups = 256;      // workgroups: one per CU
+constexpr int kGroups = 256;      // workgroups, about: one per CU
 constexpr int kTileVec = 128;     // query vectors of a prefix tile
 constexpr int kItemCost = 3;      // start and join of a piece, in blocks
 constexpr int kMinStretch = 8;    // blocks per workgroup at least (one per wavefront)
@@ -48,24 +49,20 @@ constexpr int kMaxPrefixes = 512;   // groups: one per thread
 constexpr int kMaxRows = 4096;
 constexpr int kRowB = 2 * D;      // bytes of a K or V row
 
-// Workspace: header, then one record per group and row, then the pieces.
-struct Plan {
-  int stretch, pad[3];
-};
-struct GroupRec {
-  int start, first_item, blocks, row0;  // blocks 0: nothing shared
+// Workspace: one record per row, then the pieces.
+struct Pieces {
+  int slot, count;  // of an item: piece k lies in slot + k
 };
 struct RowRec {
-  int start, blocks, group, length;  // group -1: the row takes no prefix piece
+  Pieces prefix[2];  // of the tile that holds the row's first query vector of a KV head, and of the next one
+  Pieces own;
+  int first, pad;  // that vector in its group
 };
 struct Layout {
-  size_t groups, rows, pre_o, pre_ml, suf_o, suf_ml, total;  // bytes
-  int pre_slots, suf_slots;
+  size_t rows, pre_o, pre_ml, suf_o, suf_ml, total;  // bytes
 };
 
 struct Args {
-  Plan* plan;
-  GroupRec* groups;
   RowRec* rows;
   float *pre_o, *pre_ml, *suf_o, *suf_ml;
   int B, NG, Hq, Hkv, P16, max_pages;  // P16: page size / 16
@@ -84,25 +81,30 @@ struct Piece {
 
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// Inclusive sum over the workgroup, and its total.
-__device__ __forceinline__ int block_scan(int v, int* scratch, int& total) {
+// Inclusive sums of N values over the workgroup, and their totals.
+template <int N>
+__device__ __forceinline__ void block_scan(int (&v)[N], int (&total)[N], int (*scratch)[kWaves]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int o = __shfl_up(v, off, 64);
-    v += lane >= off ? o : 0;
-  }
-  if (lane == 63) scratch[wave] = v;
-  __syncthreads();
-  total = 0;
-  int before = 0;
+  for (int i = 0; i < N; ++i) {
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    before += w < wave ? scratch[w] : 0;
-    total += scratch[w];
+    for (int off = 1; off < 64; off <<= 1) {
+      const int o = __shfl_up(v[i], off, 64);
+      v[i] += lane >= off ? o : 0;
+    }
+    if (lane == 63) scratch[i][wave] = v[i];
   }
   __syncthreads();
-  return v + before;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    total[i] = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      v[i] += w < wave ? scratch[i][w] : 0;
+      total[i] += scratch[i][w];
+    }
+  }
+  __syncthreads();
 }
 
 // Running softmax of one query vector per lane (lane l and l + 32: the same vector).
@@ -496,10 +498,8 @@ __device__ __forceinline__ void piece_tile(const Args& A, const Piece& p, uint8_
   __syncthreads();
 }
 
-// Blocks of a row's own part, where it starts, the group whose prefix it takes (-1: none) and its length.
-struct Own {
-  int first, blocks, group, length;
-};
+// A row's place on the axis, whether it takes its group's prefix, and the tokens its last block lacks.
+constexpr int kPadBits = 5, kTakes = 1 << kPadBits, kPlace = kPadBits + 1;
 
 __global__ __launch_bounds__(kThreads, 2) void attn_shared_f16_d128(
     const f16* __restrict__ q, const f16* __restrict__ kp, const f16* __restrict__ vp, const int32_t* __restrict__ pt,
@@ -508,137 +508,159 @@ __global__ __launch_bounds__(kThreads, 2) void attn_shared_f16_d128(
   __shared__ __align__(16) uint8_t st0[kStage];
   __shared__ __align__(16) uint8_t st1[kStage];
   __shared__ float sm_ml[kWaves][2][kVec];
-  __shared__ int sm_scan[kWaves];
+  __shared__ int sm_scan[3][kWaves];
   // Group g: rows sm_row0[g] .. sm_row0[g + 1] - 1, shared blocks, place on the axis, first item.
   __shared__ int sm_row0[kMaxPrefixes + 1], sm_eff[kMaxPrefixes], sm_gstart[kMaxPrefixes], sm_item[kMaxPrefixes];
-  __shared__ int sm_rstart[kMaxRows + 1];  // place of row r's items on the axis
+  __shared__ int sm_row[kMaxRows + 1];
   __shared__ int sm_find;
-  const int t = threadIdx.x, w = blockIdx.x;
   const int G = A.Hq / A.Hkv, NG = A.NG, B = A.B, Hkv = A.Hkv;
+  const int t = threadIdx.x, w = blockIdx.x / Hkv, h = blockIdx.x - w * Hkv;  // team, KV head
   const int max_ctx = A.max_pages * A.P16 * 16;
 
-  // Groups.  What is shared ends at the first row's own length (its pages are the ones read) and at whole blocks;
-  // a row alone shares nothing, and rows out of order switch sharing off.
-  bool bad = false;
-  for (int g = t; g <= NG; g += kThreads) {
-    const int r = group_rows[g];
-    bad |= r < 0 || r > B || (g < NG && group_rows[g + 1] < r);
-    sm_row0[g] = r;
-  }
-  const bool off = __syncthreads_or(bad);
-  int eff = 0, cost = 0, n = 0;
+  // Everything the plan needs is loaded at once (it is bound by latency); lengths wait in the staging rows.
+  int* sm_len = reinterpret_cast<int*>(st0);
+  static_assert(kMaxRows * 4 <= kStage, "");
+  int g0 = 0, g1 = 0, prefix = 0;
   if (t < NG) {
-    const int r0 = sm_row0[t], rows = off ? 0 : sm_row0[t + 1] - r0;
-    if (rows > 1) eff = max(0, min(min(prefix_lens[t], lens[r0]), max_ctx)) / kBlock;
-    n = eff > 0 ? (rows * G + kTileVec - 1) / kTileVec * Hkv : 0;
-    cost = n * (eff + kItemCost);
+    g0 = group_rows[t];
+    g1 = group_rows[t + 1];
+    prefix = prefix_lens[t];
+  }
+  for (int r = t; r < B; r += kThreads) sm_len[r] = max(0, min(lens[r], max_ctx));
+  if (t < NG) {
+    sm_row0[t] = g0;
+    if (t == NG - 1) sm_row0[NG] = g1;
+  }
+  // Rows out of order switch sharing off.
+  const bool off = __syncthreads_or(t < NG && (g0 < 0 || g1 > B || g1 < g0)) || NG == 0;
+  // Groups.  What is shared ends at the first row's own length (its pages are the ones read) and at whole blocks; a row
+  // alone shares nothing.
+  int v[3] = {0, 0, 0}, total[3], eff = 0;  // cost of the group's items, their number, cost of a row
+  if (t < NG) {
+    const int rows = off ? 0 : g1 - g0;
+    if (rows > 1) eff = max(0, min(prefix, sm_len[g0])) / kBlock;
+    v[1] = eff > 0 ? (rows * G + kTileVec - 1) / kTileVec : 0;
+    v[0] = v[1] * (eff + kItemCost);
     sm_eff[t] = eff;
   }
-  int total, items;
-  const int gstart = block_scan(cost, sm_scan, total) - cost, item = block_scan(n, sm_scan, items) - n;
-  if (t < NG) {
-    sm_gstart[t] = gstart;
-    sm_item[t] = item;
-    if (w == 0) A.groups[t] = GroupRec{gstart, item, eff, sm_row0[t]};
-  }
   __syncthreads();
-  const int prefix_total = total;
-
-  const auto own_of = [&](int r) __attribute__((always_inline)) {
-    const int L = max(0, min(lens[r], max_ctx));
-    int g = -1;
-    if (!off && NG > 0 && r >= sm_row0[0] && r < sm_row0[NG]) {
-      int lo = 0, hi = NG - 1;  // the last group that starts at or before r (empty ones start where the next does)
-      while (lo < hi) {
-        const int m = (lo + hi + 1) >> 1;
-        if (sm_row0[m] <= r) lo = m;
-        else hi = m - 1;
-      }
-      // a row shorter than the prefix reads it alone
-      if (sm_eff[lo] > 0 && L >= sm_eff[lo] * kBlock) g = lo;
+  const auto group_of = [&](int r) __attribute__((always_inline)) {  // -1: none
+    if (off || r < sm_row0[0] || r >= sm_row0[NG]) return -1;
+    int lo = 0, hi = NG - 1;  // the last group that starts at or before r (empty ones start where the next does)
+    while (lo < hi) {
+      const int m = (lo + hi + 1) >> 1;
+      if (sm_row0[m] <= r) lo = m;
+      else hi = m - 1;
     }
-    const int first = g >= 0 ? sm_eff[g] : 0;
-    return Own{first, (L + kBlock - 1) / kBlock - first, g, L};
+    return lo;
   };
+  int rows_total = 0;
+  const int gcost = v[0], gitems = v[1];
+  int gstart = 0;
   for (int r0 = 0; r0 < B; r0 += kThreads) {  // uniform
     const int r = r0 + t;
-    Own o{0, 0, -1, 0};
-    if (r < B) o = own_of(r);
-    const int c = o.blocks > 0 ? Hkv * (o.blocks + kItemCost) : 0;
-    int sum;
-    const int start = total + block_scan(c, sm_scan, sum) - c;
+    int cost = 0, word = 0;
     if (r < B) {
-      sm_rstart[r] = start;
-      if (w == 0) A.rows[r] = RowRec{start, o.blocks, o.group, o.length};
+      const int L = sm_len[r], g = group_of(r), e = g >= 0 ? sm_eff[g] : 0;
+      const bool takes = e > 0 && L >= e * kBlock;  // a row shorter than the prefix reads it alone
+      const int blocks = (L + kBlock - 1) / kBlock - (takes ? e : 0);
+      cost = blocks > 0 ? blocks + kItemCost : 0;
+      word = (takes ? kTakes : 0) | (-L & (kBlock - 1));
     }
-    total += sum;
+    if (r0 == 0) {
+      v[2] = cost;
+      block_scan<3>(v, total, sm_scan);
+      gstart = v[0] - gcost;
+      if (t < NG) {
+        sm_gstart[t] = gstart;
+        sm_item[t] = v[1] - gitems;
+      }
+    } else {
+      int c[1] = {cost}, sum[1];
+      block_scan<1>(c, sum, sm_scan);
+      v[2] = c[0];
+      total[2] = sum[0];
+    }
+    if (r < B) sm_row[r] = ((total[0] + rows_total + v[2] - cost) << kPlace) | word;
+    rows_total += total[2];
   }
-  if (t == 0) sm_rstart[B] = total;
-  const int stretch = max((total + kGroups - 1) / kGroups, kMinStretch);
-  if (w == 0 && t == 0) A.plan->stretch = stretch;
-  const int a = w * stretch, b = min(total, a + stretch);
+  const int prefix_total = total[0], all = prefix_total + rows_total;
+  if (t == 0) sm_row[B] = all << kPlace;
+  const int teams = gridDim.x / Hkv;
+  const int stretch = max((all + teams - 1) / teams, kMinStretch);
+  const int a = w * stretch, b = min(all, a + stretch);
+  __syncthreads();
+
+  // The join's records, shared out over the workgroups from the last one on (the ones without work of their own).
+  for (int r = (int)(gridDim.x - 1 - blockIdx.x) + t * (int)gridDim.x; r < B; r += kThreads * (int)gridDim.x) {
+    const int word = sm_row[r], place = word >> kPlace, span = (sm_row[r + 1] >> kPlace) - place;
+    const auto pieces = [&](int start, int blocks, int item) {  // item's blocks from `start` on
+      const int w0 = start / stretch;
+      return Pieces{w0 + item, (start + blocks - 1) / stretch - w0 + 1};
+    };
+    RowRec rec{{{0, 0}, {0, 0}}, {0, 0}, 0, 0};
+    if (word & kTakes) {
+      const int g = group_of(r), tiles = ((sm_row0[g + 1] - sm_row0[g]) * G + kTileVec - 1) / kTileVec;
+      const int shared = sm_eff[g];
+      rec.first = (r - sm_row0[g]) * G;
+      const int tile = rec.first / kTileVec;
+      for (int k = 0; k < 2 && tile + k < tiles; ++k)
+        rec.prefix[k] = pieces(sm_gstart[g] + (tile + k) * (shared + kItemCost) + kItemCost, shared,
+                               sm_item[g] + tile + k);
+    }
+    if (span > 0) rec.own = pieces(place + kItemCost, span - kItemCost, r);
+    A.rows[r] = rec;
+  }
   if (a >= b) return;  // uniform
   // The unit (group, then NG + row) in which the stretch begins.
-  __syncthreads();
   if (a < prefix_total) {
-    if (t < NG && gstart <= a && a < gstart + cost) sm_find = t;
+    if (t < NG && gstart <= a && a < gstart + gcost) sm_find = t;
   } else {
     for (int r = t; r < B; r += kThreads)
-      if (sm_rstart[r] <= a && a < sm_rstart[r + 1]) sm_find = NG + r;
+      if ((sm_row[r] >> kPlace) <= a && a < (sm_row[r + 1] >> kPlace)) sm_find = NG + r;
   }
   __syncthreads();
 
   for (int u = uni(sm_find); u < NG + B; ++u) {  // uniform
     const bool pre = u < NG;
     const int r = u - NG;
-    Own o{0, 0, -1, 0};
-    int rows = 0, count = Hkv, start;
+    int rows = 0, count = 1, start, first = 0, blocks, limit;  // items, their place, blocks, tokens
     if (pre) {
       rows = uni(sm_row0[u + 1]) - uni(sm_row0[u]);
-      o.blocks = uni(sm_eff[u]);
-      o.length = o.blocks * kBlock;
-      count = (rows * G + kTileVec - 1) / kTileVec * Hkv;
+      blocks = uni(sm_eff[u]);
+      count = (rows * G + kTileVec - 1) / kTileVec;
       start = uni(sm_gstart[u]);
+      limit = blocks * kBlock;
     } else {
-      o = own_of(r);
-      o.first = uni(o.first);
-      o.blocks = uni(o.blocks);
-      o.length = uni(o.length);
-      start = uni(sm_rstart[r]);
+      const int word = uni(sm_row[r]);
+      start = word >> kPlace;
+      blocks = (uni(sm_row[r + 1]) >> kPlace) - start - kItemCost;
+      if (word & kTakes) first = uni(sm_eff[uni(group_of(r))]);
+      limit = (first + blocks) * kBlock - (word & (kBlock - 1));
     }
     if (start >= b) break;
-    if (o.blocks <= 0) continue;
-    const int c = o.blocks + kItemCost;
+    if (blocks <= 0) continue;
+    const int c = blocks + kItemCost;
     for (int i = max(0, (a - start) / c); i < count && start + i * c < b; ++i) {
       const int st = start + i * c + kItemCost;
-      const int k0 = max(0, min(a - st, o.blocks)), k1 = max(0, min(b - st, o.blocks));
+      const int k0 = max(0, min(a - st, blocks)), k1 = max(0, min(b - st, blocks));
       if (k0 >= k1) continue;
       Piece p;
       p.q = q;
       p.kp = kp;
       p.vp = vp;
-      p.blk0 = o.first + k0;
-      p.blk1 = o.first + k1;
-      p.limit = o.length;
-      if (pre) {
-        const int tile = i / Hkv;
-        p.h = i - tile * Hkv;
-        p.vrow = uni(sm_row0[u]);
-        p.v0 = tile * kTileVec;
-        p.nv = min(kTileVec, rows * G - p.v0);
-        const size_t slot = (size_t)(w + uni(sm_item[u]) + i) * kTileVec;
-        p.o = A.pre_o + slot * D;
-        p.ml = A.pre_ml + slot * 2;
-      } else {
-        p.h = i;
-        p.vrow = r;
-        p.v0 = 0;
-        p.nv = G;
-        const size_t slot = (size_t)(w + r * Hkv + i) * G;
-        p.o = A.suf_o + slot * D;
-        p.ml = A.suf_ml + slot * 2;
-      }
+      p.h = h;
+      p.blk0 = first + k0;
+      p.blk1 = first + k1;
+      p.limit = limit;
+      p.vrow = pre ? uni(sm_row0[u]) : r;
+      p.v0 = pre ? i * kTileVec : 0;
+      p.nv = pre ? min(kTileVec, rows * G - p.v0) : G;
       p.ptrow = pt + (size_t)p.vrow * A.max_pages;
+      const int slot = w + (pre ? uni(sm_item[u]) + i : r);
+      const size_t at = ((size_t)slot * Hkv + h) * (pre ? kTileVec : G);
+      p.o = (pre ? A.pre_o : A.suf_o) + at * D;
+      p.ml = (pre ? A.pre_ml : A.suf_ml) + at * 2;
       if (p.nv > kVec) piece_tile(A, p, st0, st1, sm_ml);
       else piece_stream(A, p, st0, st1, sm_ml);
     }
@@ -646,7 +668,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_shared_f16_d128(
 }
 
 // out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i over the pieces of a query vector: those of its group's prefix, then
-// those of its own part, in order.  32 lanes per vector, four dims each; lane k takes (m, l) of every 32nd piece.
+// those of its own part, in order.  32 lanes per vector, four dims each; lane k takes (m, l) of every 32nd piece.  Bound
+// by latency (record, then pieces), so the first pieces' O are loaded along with their (m, l).
 // A row without tokens gives zeros; one whose scores are all -inf NaN, as a softmax over them does.
 __global__ __launch_bounds__(256) void attn_shared_join(Args A, f16* __restrict__ out) {
   const int id = (int)((blockIdx.x * 256u + threadIdx.x) >> 5), lane = threadIdx.x & 31;
@@ -654,99 +677,98 @@ __global__ __launch_bounds__(256) void attn_shared_join(Args A, f16* __restrict_
   if (row >= A.B) return;
   const int head = id - row * A.Hq, G = A.Hq / A.Hkv;
   const int h = head / G, g = head - h * G;
-  const int stretch = A.plan->stretch;
-  const RowRec rr = A.rows[row];
-  const float *po[2], *pm[2];  // O and (m, l) of the first piece of each kind
-  size_t step[2];              // vectors from one piece to the next
-  int count[2] = {0, 0};
-  if (rr.group >= 0) {
-    const GroupRec gr = A.groups[rr.group];
-    const int v = (row - gr.row0) * G + g, tile = v / kTileVec, i = tile * A.Hkv + h;
-    const int st = gr.start + i * (gr.blocks + kItemCost) + kItemCost;
-    const int w0 = st / stretch, w1 = (st + gr.blocks - 1) / stretch;
-    const size_t at = (size_t)(w0 + gr.first_item + i) * kTileVec + (v - tile * kTileVec);
-    po[0] = A.pre_o + at * D;
-    pm[0] = A.pre_ml + at * 2;
-    step[0] = kTileVec;
-    count[0] = w1 - w0 + 1;
+  const RowRec rec = A.rows[row];
+  const int v = rec.first + g, later = v / kTileVec != rec.first / kTileVec;
+  const Pieces pre = later ? rec.prefix[1] : rec.prefix[0];
+  const int n = pre.count + rec.own.count;
+  if (n == 0) {
+    *reinterpret_cast<f16x4*>(out + (size_t)id * D + 4 * lane) = f16x4{0, 0, 0, 0};
+    return;
   }
-  if (rr.blocks > 0) {
-    const int st = rr.start + h * (rr.blocks + kItemCost) + kItemCost;
-    const int w0 = st / stretch, w1 = (st + rr.blocks - 1) / stretch;
-    const size_t at = (size_t)(w0 + row * A.Hkv + h) * G + g;
-    po[1] = A.suf_o + at * D;
-    pm[1] = A.suf_ml + at * 2;
-    step[1] = G;
-    count[1] = w1 - w0 + 1;
-  }
-  float M = -INFINITY;
+  // Query vector `at` of piece k's slot: (m, l) and O.
+  const size_t pre_at = ((size_t)pre.slot * A.Hkv + h) * kTileVec + v % kTileVec;
+  const size_t own_at = ((size_t)rec.own.slot * A.Hkv + h) * G + g;
+  const auto at = [&](int k) {
+    return k < pre.count ? pre_at + (size_t)k * A.Hkv * kTileVec : own_at + (size_t)(k - pre.count) * A.Hkv * G;
+  };
+  const auto ml_of = [&](int k) {
+    return *reinterpret_cast<const float2*>((k < pre.count ? A.pre_ml : A.suf_ml) + 2 * at(k));
+  };
+  const auto o_of = [&](int k) {
+    return *reinterpret_cast<const f32x4*>((k < pre.count ? A.pre_o : A.suf_o) + D * at(k) + 4 * lane);
+  };
+  constexpr int U = 4;
+  float2 ml = lane < n ? ml_of(lane) : make_float2(-INFINITY, 0.f);
+  f32x4 x[U];
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
-    for (int k = lane; k < count[s]; k += 32) M = fmaxf(M, pm[s][k * step[s] * 2]);
+  for (int j = 0; j < U; ++j) x[j] = o_of(min(j, n - 1));
+  float M = ml.x;
+  for (int k = lane + 32; k < n; k += 32) M = fmaxf(M, ml_of(k).x);
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor(M, x, 32));
+  for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor(M, s, 32));
   const float ms = M == -INFINITY ? 0.f : M;
   float den = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int k0 = 0; k0 < n; k0 += 32) {
+    if (k0) ml = k0 + lane < n ? ml_of(k0 + lane) : make_float2(-INFINITY, 0.f);
+    const float f = __builtin_amdgcn_exp2f(ml.x - ms);
+    den = fmaf(ml.y, f, den);
+    for (int j0 = k0; j0 < min(n, k0 + 32); j0 += U) {
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
-    for (int k0 = 0; k0 < count[s]; k0 += 32) {
-      float f = 0.f;
-      if (k0 + lane < count[s]) {
-        const float* ml = pm[s] + (k0 + lane) * step[s] * 2;
-        f = __builtin_amdgcn_exp2f(ml[0] - ms);
-        den = fmaf(ml[1], f, den);
-      }
-      const int n = min(32, count[s] - k0);
-      for (int j = 0; j < n; ++j) {
-        const float fj = __shfl(f, j, 32);
-        const f32x4 x = *reinterpret_cast<const f32x4*>(po[s] + (k0 + j) * step[s] * D + 4 * lane);
+      for (int j = 0; j < U; ++j) {
+        const float fj = __shfl(f, j0 + j - k0, 32);
+        if (j0 + j < n) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], fj, o[e]);
+          for (int e = 0; e < 4; ++e) o[e] = fmaf(x[j][e], fj, o[e]);
+        }
       }
+#pragma unroll
+      for (int j = 0; j < U; ++j) x[j] = o_of(min(j0 + U + j, n - 1));
     }
+  }
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) den += __shfl_xor(den, x, 32);
-  const float inv = den == 0.f ? (rr.length > 0 ? NAN : 0.f) : 1.f / den;
+  for (int s = 16; s > 0; s >>= 1) den += __shfl_xor(den, s, 32);
+  const float inv = den == 0.f ? NAN : 1.f / den;
   f16x4 y;
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] = static_cast<f16>(as_f32_value(o[e] * inv));
   *reinterpret_cast<f16x4*>(out + (size_t)id * D + 4 * lane) = y;
 }
 
+int teams_of(int Hkv) { return max(1, kGroups / Hkv); }
+
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
 Layout layout(int B, int NG, int Hq, int Hkv) {
   const int G = Hq / Hkv;
   Layout l{};
-  // tiles of n_g rows: ceil(n_g G / 128), so at most B G / 128 + NG in all
-  l.pre_slots = kGroups + (int)(((long)B * G / kTileVec + NG) * Hkv);
-  l.suf_slots = kGroups + B * Hkv;
-  size_t at = round16(sizeof(Plan));
+  size_t at = 0;
   const auto take = [&](size_t bytes) {
     const size_t p = at;
     at += round16(bytes);
     return p;
   };
-  l.groups = take(sizeof(GroupRec) * NG);
+  // tiles of n_g rows: ceil(n_g G / 128), so at most B G / 128 + NG in all
+  const size_t pre = NG ? (size_t)(teams_of(Hkv) + (long)B * G / kTileVec + NG) * Hkv * kTileVec : 0;
+  const size_t suf = (size_t)(teams_of(Hkv) + B) * Hkv * G;
   l.rows = take(sizeof(RowRec) * B);
-  l.pre_o = take((size_t)(NG ? l.pre_slots : 0) * kTileVec * D * sizeof(float));
-  l.pre_ml = take((size_t)(NG ? l.pre_slots : 0) * kTileVec * 2 * sizeof(float));
-  l.suf_o = take((size_t)l.suf_slots * G * D * sizeof(float));
-  l.suf_ml = take((size_t)l.suf_slots * G * 2 * sizeof(float));
+  l.pre_o = take(pre * D * sizeof(float));
+  l.pre_ml = take(pre * 2 * sizeof(float));
+  l.suf_o = take(suf * D * sizeof(float));
+  l.suf_ml = take(suf * 2 * sizeof(float));
   l.total = at;
   return l;
 }
 
-// Sizes that the shared kernel takes: fp16, head_dim 128, pages of a multiple of 16 tokens, up to 32 query heads per KV
-// head, and an axis that 32 bits number.  Others run the decode attention over each row's whole context.
+// Sizes that the shared kernel takes: fp16, head_dim 128, pages of a multiple of 16 tokens, up to 32 query heads per
+// KV head, and an axis that sm_row holds.  Others run the decode attention over each row's whole context.
 bool shares(int B, int NG, int Hq, int Hkv, int head_dim, int P, int max_pages, int kv_dtype) {
   const int G = Hq / Hkv;
   const long per_item = (long)max_pages * P / kBlock + 1 + kItemCost;
-  const long items = ((long)B * G / kTileVec + NG + B) * Hkv;
+  const long items = (long)B * G / kTileVec + NG + B;
   // (page_index is exact while (tokens / 16) (P / 16) < 2^32)
   return kv_dtype == CIR_F16 && head_dim == D && P % 16 == 0 && (long)max_pages * P / 16 * (P / 16) < (1L << 32) &&
-         G <= kVec && NG <= kMaxPrefixes && B <= kMaxRows && per_item < (1L << 30) && items < (1L << 30) && per_item * items < (1L << 30);
+         G <= kVec && NG <= kMaxPrefixes && B <= kMaxRows && per_item < (1L << 31) && per_item * items < (1L << (31 - kPlace));
 }
 
 }  // namespace
@@ -793,14 +815,13 @@ extern "C" int cir_paged_decode_attention_shared(const void* q, const void* k_po
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const float scale_log2 = scale * kLog2e;
   const uint32_t P16 = page_size / 16;
-  const Args A{reinterpret_cast<Plan*>(ws),
-               reinterpret_cast<GroupRec*>(ws + l.groups), reinterpret_cast<RowRec*>(ws + l.rows),
+  const Args A{reinterpret_cast<RowRec*>(ws + l.rows),
                reinterpret_cast<float*>(ws + l.pre_o), reinterpret_cast<float*>(ws + l.pre_ml),
                reinterpret_cast<float*>(ws + l.suf_o), reinterpret_cast<float*>(ws + l.suf_ml), batch, groups, num_heads,
                num_kv_heads, (int)P16, max_pages, (uint32_t)(((1ull << 32) + P16 - 1) / P16),
                scale_log2 == 0.f ? FLT_MIN : scale_log2};  // (a masked score is -inf: -inf * 0 would be NaN)
   hipStream_t s = as_stream(stream);
-  attn_shared_f16_d128<<<kGroups, kThreads, 0, s>>>(
+  attn_shared_f16_d128<<<teams_of(num_kv_heads) * num_kv_heads, kThreads, 0, s>>>(
       static_cast<const f16*>(q), static_cast<const f16*>(k_pool), static_cast<const f16*>(v_pool), page_table, seq_lens,
       group_rows, prefix_lens, A);
   const int st = launch_status();

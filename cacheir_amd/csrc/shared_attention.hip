@@ -17,15 +17,15 @@
 // the join finds an item's pieces from its start and the stretch alone.  The workgroups of a
 // team walk the same pages in step, one head of each.
 //
-// Bodies (8 wavefronts, one workgroup per CU, MFMA 32x32x16 f16, S^T = K Q^T and
-// O^T = V^T P^T as in the prefill attention, whose LDS swizzles these are):
+// Bodies (4 wavefronts, two workgroups per CU, so that one streams while the other starts or
+// ends a piece; MFMA 32x32x16 f16, S^T = K Q^T and O^T = V^T P^T as in the prefill
+// attention, whose LDS swizzles these are):
 //   * piece_stream, up to 32 query vectors: bound by the read of K and V.  Each wavefront
-//     walks blocks of its own (every 8th) and stages them by DMA in LDS of its own: no
+//     walks blocks of its own (every 4th) and stages them by DMA in LDS of its own: no
 //     barriers, K of the next block is on its way once this block's K is in registers, and
 //     V likewise, so a CU has 64 to 128 KiB in flight.
-//   * piece_tile, up to 128 vectors: bound by the matrix cores and the softmax.  Four
-//     wavefronts of 32 vectors, twice: two sets take turns of 64-token pairs of blocks; K
-//     and V go through LDS once for all.
+//   * piece_tile, up to 128 vectors: bound by the matrix cores and the softmax.  Each
+//     wavefront takes 32 vectors; stages of 64 tokens of K and V go through LDS for all.
 // P is rounded to fp16 for the second product (relative 2^-11 of a weight) and l sums the
 // rounded values, so a row's weights still add up to one; everything else is fp32.
 #include "attn_tile.hpp"
@@ -39,14 +39,14 @@ namespace {
 constexpr int D = 128;
 constexpr int kBlock = 32;        // tokens of an MFMA tile
 constexpr int kVec = 32;          // query vectors of an MFMA tile
-constexpr int kWaves = 8;
+constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
-constexpr int kGroups = 256;      // workgroups, about: one per CU
+constexpr int kGroups = 512;      // workgroups, about: two per CU
 constexpr int kTileVec = 128;     // query vectors of a prefix tile
 constexpr int kItemCost = 3;      // start and join of a piece, in blocks
-constexpr int kMinStretch = 8;    // blocks per workgroup at least (one per wavefront)
-constexpr int kMaxPrefixes = 512;   // groups: one per thread
-constexpr int kMaxRows = 4096;
+constexpr int kMinStretch = 4;    // blocks per workgroup at least (one per wavefront)
+constexpr int kMaxPrefixes = 256;   // groups: one per thread
+constexpr int kMaxRows = 2048;
 constexpr int kRowB = 2 * D;      // bytes of a K or V row
 
 // Workspace: one record per row, then the pieces.
@@ -191,7 +191,7 @@ __device__ __forceinline__ void load_vt(const uint8_t* v, const int (&vo)[2], in
     }
 }
 
-constexpr int kStage = 64 * 1024;  // bytes of each of the two LDS arrays
+constexpr int kStage = 32 * 1024;  // bytes of each of the two LDS arrays
 
 // Pool rows of 16 tokens (one page holds them whole), token 16 n first: page table entry, then elements from the pool.
 __device__ __forceinline__ int page_index(const Args& A, int n) {
@@ -350,21 +350,18 @@ __device__ __forceinline__ void piece_stream(const Args& A, const Piece& p, uint
 }
 
 // ------------------------------------------------------ up to 128 vectors -----
-// VW x CW wavefronts: VW tiles of 32 vectors, CW sets that take turns of NB blocks.
-__device__ __forceinline__ void piece_tile(const Args& A, const Piece& p, uint8_t* st0, uint8_t* st1,
-                                           float (*sm_ml)[2][kVec]) {
-  constexpr int VW = 4, CW = 2, NB = 2;
-  constexpr int kTok = kBlock * NB * CW;          // tokens per stage
+__device__ __forceinline__ void piece_tile(const Args& A, const Piece& p, uint8_t* st0, uint8_t* st1) {
+  constexpr int NB = 2;
+  constexpr int kTok = kBlock * NB;               // tokens per stage
   constexpr int kHalf = kTok * kRowB;             // bytes of K, then V
   constexpr int kRows = kTok / kWaves;            // rows of each a wavefront brings in
   static_assert(kRows == 16 && 2 * kHalf == kStage, "a wavefront's rows lie in one page");
   const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int vw = wave % VW, cw = wave / VW;
   const int l32 = lane & 31, h = lane >> 5;
   const float sc = fabsf(A.scale_log2);
-  const int nst = (p.blk1 - p.blk0 + NB * CW - 1) / (NB * CW);  // (every token of the blocks counts)
+  const int nst = (p.blk1 - p.blk0 + NB - 1) / NB;  // (every token of the blocks counts)
   const int first16 = 2 * p.blk0 + wave, last16 = 2 * p.blk1 - 1;
-  const bool busy = vw * kVec < p.nv;  // uniform
+  const bool busy = wave * kVec < p.nv;  // uniform
 
   // DMA of a stage: each wavefront brings in 16 rows of K and of V; past the last block it re-reads the last rows.
   const int lr = lane >> 4, ls = lane & 15;
@@ -391,15 +388,15 @@ __device__ __forceinline__ void piece_tile(const Args& A, const Piece& p, uint8_
   };
 
   f16x8 qb[8];
-  load_q(A, p, vw * kVec + l32, qb);
+  load_q(A, p, wave * kVec + l32, qb);
   Soft a;
   soft_init(a);
-  const int krow = (kBlock * NB * cw + l32) * kRowB, kx = 16 * (h ^ (l32 & 15));
+  const int krow = l32 * kRowB, kx = 16 * (h ^ (l32 & 15));
   const int ti = lane & 15, sub = (lane >> 4) & 1;
   int vo[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    vo[i] = kHalf + (kBlock * NB * cw + 8 * i + 4 * h + (ti >> 2)) * kRowB +
+    vo[i] = kHalf + (8 * i + 4 * h + (ti >> 2)) * kRowB +
             16 * ((2 * sub + ((ti & 3) >> 1)) ^ (2 * i + h)) + 8 * (ti & 1);
 
   auto blocks = [&](const uint8_t* buf, int blk) __attribute__((always_inline)) {
@@ -444,8 +441,7 @@ __device__ __forceinline__ void piece_tile(const Args& A, const Piece& p, uint8_
       issue(other, st + 1);
       fetch(min(st + 2, nst - 1));
     }
-    const int blk = p.blk0 + (st * CW + cw) * NB;
-    if (busy && blk < p.blk1) blocks(cur, blk);
+    if (busy) blocks(cur, p.blk0 + st * NB);
   };
   fetch(0);
   issue(st0, 0);
@@ -458,44 +454,21 @@ __device__ __forceinline__ void piece_tile(const Args& A, const Piece& p, uint8_
   }
   a.l += __shfl_xor(a.l, 32, 64);
 
-  // Join the two sets: the second parks (m, l, O) in the first array.
-  dma_wait_barrier();  // every wavefront has read its last stage
-  float* park = reinterpret_cast<float*>(st0 + vw * (64 * 64 * 4)) + lane;
-  if (cw > 0 && busy) {
+  const int v = wave * kVec + l32;
+  if (v < p.nv) {
+    float* po = p.o + (size_t)v * D + 4 * h;
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) park[(16 * dt + r) * 64] = a.acc[dt][r];
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<f32x4*>(po + 32 * dt + 8 * j) =
+            f32x4{a.acc[dt][4 * j], a.acc[dt][4 * j + 1], a.acc[dt][4 * j + 2], a.acc[dt][4 * j + 3]};
     if (h == 0) {
-      sm_ml[vw][0][l32] = a.m;
-      sm_ml[vw][1][l32] = a.l;
+      p.ml[2 * v] = a.m;
+      p.ml[2 * v + 1] = a.l;
     }
   }
-  __syncthreads();
-  if (cw == 0 && busy) {
-    const float mg = sm_ml[vw][0][l32], lg = sm_ml[vw][1][l32];
-    const float mn = fmaxf(a.m, mg), ms = mn == -INFINITY ? 0.f : mn;
-    const float fa = __builtin_amdgcn_exp2f(a.m - ms), fb = __builtin_amdgcn_exp2f(mg - ms);
-    const int v = vw * kVec + l32;
-    const float l = fmaf(a.l, fa, lg * fb);
-    f32x4 o[D / 32][4];
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[dt][r >> 2][r & 3] = fmaf(a.acc[dt][r], fa, park[(16 * dt + r) * 64] * fb);
-    if (v < p.nv) {
-      float* po = p.o + (size_t)v * D + 4 * h;
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(po + 32 * dt + 8 * j) = o[dt][j];
-      if (h == 0) {
-        p.ml[2 * v] = mn;
-        p.ml[2 * v + 1] = l;
-      }
-    }
-  }
-  __syncthreads();
+  __syncthreads();  // every wavefront has read its last stage
 }
 
 // A row's place on the axis, whether it takes its group's prefix, and the tokens its last block lacks.
@@ -661,7 +634,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_shared_f16_d128(
       const size_t at = ((size_t)slot * Hkv + h) * (pre ? kTileVec : G);
       p.o = (pre ? A.pre_o : A.suf_o) + at * D;
       p.ml = (pre ? A.pre_ml : A.suf_ml) + at * 2;
-      if (p.nv > kVec) piece_tile(A, p, st0, st1, sm_ml);
+      if (p.nv > kVec) piece_tile(A, p, st0, st1);
       else piece_stream(A, p, st0, st1, sm_ml);
     }
   }

@@ -168,7 +168,7 @@ int cir_paged_prefill_attention_split(const void* q, const void* k_pool, const v
  * group_rows out of order switch sharing off.  A sequence with seq_len 0 yields zeros, one
  * whose scores are all -inf NaN.
  * fp16 pools on 16-byte addresses, head_dim 128, page_size a multiple of 16, up to 32 query
- * heads per KV head, 4096 rows and 512 groups; other calls run cir_paged_decode_attention
+ * heads per KV head, 2048 rows and 256 groups; other calls run cir_paged_decode_attention
  * (every row reads its prefix).  A row's last bits depend on the batch it is in.
  * workspace: cir_shared_attention_workspace_bytes bytes on a 16-byte address, written by
  * the call (calls that overlap need one each); nothing in it needs clearing.

@@ -1,15 +1,19 @@
 // Log probabilities of given tokens, entropy and the most likely alternatives of rows of
 // logits, in one pass over the logits.
 //
-// With m = max x, S = sum e^(x - m) and T = sum e^(x - m) (x - m):
-//   log p(i) = x_i - m - log S,   H = -sum p log p = log S - T / S
-// (both terms of H are positive: no cancellation).  Each thread keeps (m, S, T) in fp32 over
-// its share and rescales when its maximum moves: with a = e^(m - m'), S' = a S and
-// T' = a (T + (m - m') S).  The alternatives are the K largest by (value, then lowest
-// index): a wavefront keeps the best 64 of its share sorted across its lanes, as 64-bit keys
-// (order-preserving bits of the value | complement of the index), and inserts what beats
-// the K-th.  Wavefronts, then workgroups of a row, are merged in order, so results do not
-// depend on timing.
+// In base 2, with a reference r near max x, y = (x - r) log2 e, S = sum 2^y, T = sum 2^y y:
+//   log p(i) = ln 2 (y_i - log2 S),   H = -sum p log p = ln 2 (log2 S - T / S)
+// (both terms of H are positive: no cancellation).  Each thread keeps (r, S, T) in fp32 over
+// its share and rescales when its maximum moves: with d = (r - r') log2 e, S' = 2^d S and
+// T' = 2^d (T + d S).
+//
+// The alternatives are the K largest by (value, then lowest index), as 64-bit keys
+// (order-preserving bits of the value | complement of the index).  A wavefront keeps its best
+// 64 sorted across its lanes.  The first values of its share go in as the largest of each
+// lane, sorted by a bitonic network: the K-th of those bounds what can still enter, so of
+// random logits a handful more is inserted one by one (inserting every one of the first 1024
+// took ~100 insertions, 5 us).  Sorted lists are joined in 7 exchange steps: wavefronts, then
+// workgroups of a row, in order, so results do not depend on timing.
 //
 // Bound by the read of the logits.
 #include "common.hpp"
@@ -24,9 +28,10 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxTop = 64;       // a wavefront's lanes
 constexpr int kMinChunk = 4096;   // logits of a workgroup that shares its row with others
-constexpr float kLog2e = 1.4426950408889634f;
-// e^-200 is zero in fp32: differences below it add nothing, and 0 * (x - m) stays 0 for x = -inf.
-constexpr float kFloor = -200.f;
+constexpr int kManyRows = 1024, kShortRow = 4096;  // rows of one wavefront each
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// 2^-300 is zero in fp32: y below it adds nothing, and 0 * y stays 0 for x = -inf.
+constexpr float kFloor = -300.f;
 
 typedef unsigned long long u64;
 
@@ -48,57 +53,137 @@ __device__ __forceinline__ u64 read_lane(u64 v, int l) {
   return ((u64)hi << 32) | lo;
 }
 
-struct Stats {
-  float m, s, t;
+// fp32 logits: the reference is the maximum itself.  fp16 logits: it is fl(max log2 e), so that y is one mixed-precision
+// FMA on the logit as it was loaded (values up to 65504: no overflow); the rounding of the reference is shared by all.
+template <typename T>
+struct Words;
+template <>
+struct Words<float> {
+  static constexpr int kN = 4, kUnroll = 4;
+  typedef float vec __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ float ref_of(float m) { return m; }
+  static __device__ __forceinline__ float y_of(float x, float ref) { return (x - ref) * kLog2e; }
+  static __device__ __forceinline__ float gap(float ref, float to) { return (ref - to) * kLog2e; }
+  static __device__ __forceinline__ float log_p(float x, float ref, float log2_s) { return (x - ref) - log2_s * kLn2; }
 };
+template <>
+struct Words<f16> {
+  static constexpr int kN = 8, kUnroll = 4;
+  typedef f16 vec __attribute__((ext_vector_type(8)));
+  // (as_f32_value: contracted into the subtraction in gap, the unrounded product would not cancel)
+  static __device__ __forceinline__ float ref_of(float m) { return as_f32_value(m * kLog2e); }
+  static __device__ __forceinline__ float y_of(f16 x, float ref) { return fmaf((float)x, kLog2e, -ref); }
+  static __device__ __forceinline__ float gap(float ref, float to) { return ref - to; }
+  static __device__ __forceinline__ float log_p(f16 x, float ref, float log2_s) { return (y_of(x, ref) - log2_s) * kLn2; }
+};
+
+struct Stats {
+  float m, ref, s, t;
+};
+template <typename T>
+__device__ __forceinline__ Stats none() {
+  const float low = sizeof(T) == 2 ? -65504.f : -FLT_MAX;
+  return {low, Words<T>::ref_of(low), 0.f, 0.f};
+}
+template <typename T>
 __device__ __forceinline__ void raise(Stats& a, float m) {  // to a maximum m >= a.m
-  const float d = fmaxf(a.m - m, kFloor), f = __builtin_amdgcn_exp2f(d * kLog2e);
+  const float ref = Words<T>::ref_of(m);
+  const float d = fmaxf(Words<T>::gap(a.ref, ref), kFloor), f = __builtin_amdgcn_exp2f(d);
   a.t = f * fmaf(d, a.s, a.t);
   a.s *= f;
+  a.ref = ref;
   a.m = m;
 }
-__device__ __forceinline__ void add(Stats& a, float x) {  // x <= a.m, or NaN or +inf (S becomes NaN)
-  const float d = x - a.m, e = __builtin_amdgcn_exp2f(d * kLog2e);
+template <typename T>
+__device__ __forceinline__ void add(Stats& a, T x) {  // x <= a.m, or NaN or +inf (S becomes NaN)
+  const float y = Words<T>::y_of(x, a.ref), e = __builtin_amdgcn_exp2f(y);
   a.s += e;
-  a.t = fmaf(e, fmaxf(d, kFloor), a.t);
+  a.t = fmaf(e, fmaxf(y, kFloor), a.t);
 }
+template <typename T>
 __device__ __forceinline__ Stats join(Stats a, Stats b) {
   const float m = fmaxf(a.m, b.m);
-  raise(a, m);
-  raise(b, m);
-  return {m, a.s + b.s, a.t + b.t};
+  raise<T>(a, m);
+  raise<T>(b, m);
+  return {m, a.ref, a.s + b.s, a.t + b.t};
+}
+template <typename T>
+__device__ __forceinline__ Stats join_wave(Stats a) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const Stats b = {__shfl_xor(a.m, off), __shfl_xor(a.ref, off), __shfl_xor(a.s, off), __shfl_xor(a.t, off)};
+    a = join<T>(a, b);
+  }
+  return a;
 }
 
-// The wavefront's sorted list: lane i holds the i-th best key (0: none).
+// The key of lane ^ MASK, by DPP inside a row of 16 lanes and gfx950's lane swaps past it.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false);
+}
+template <int MASK>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+  if constexpr (MASK == 1) return dpp<0xB1>(v);              // quad_perm [1,0,3,2]
+  else if constexpr (MASK == 2) return dpp<0x4E>(v);         // quad_perm [2,3,0,1]
+  else if constexpr (MASK == 4) return dpp<0x1B>(dpp<0x141>(v));  // half-row mirror (^7), quad_perm [3,2,1,0] (^3)
+  else if constexpr (MASK == 8) return dpp<0x128>(v);        // row_ror:8
+  else if constexpr (MASK == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);  // (r0, r0, r2, r2), (r1, r1, r3, r3) by rows
+    const uint32_t a = r[0], b = r[1];
+    return (threadIdx.x & 16) ? a : b;
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);  // (low, low), (high, high) halves
+    const uint32_t a = r[0], b = r[1];
+    return (threadIdx.x & 32) ? a : b;
+  }
+}
+// Compare-exchange with lane ^ MASK; `up`: this lane keeps the larger key.
+template <int MASK>
+__device__ __forceinline__ void exchange(u64& k, bool up) {
+  const u64 o = ((u64)lane_xor<MASK>((uint32_t)(k >> 32)) << 32) | lane_xor<MASK>((uint32_t)k);
+  k = (k > o) == up ? k : o;
+}
+template <int MASK>
+__device__ __forceinline__ void merge_steps(u64& k, int lane, bool desc) {  // a bitonic run of 2 MASK lanes, sorted
+  exchange<MASK>(k, ((lane & MASK) == 0) == desc);
+  if constexpr (MASK > 1) merge_steps<MASK / 2>(k, lane, desc);
+}
+
+// The wavefront's list: lane i holds the i-th best key (0: none).
 struct Top {
   u64 key, least;  // least: the K-th best (uniform)
-  __device__ __forceinline__ void init() { key = least = 0; }
-  // Every lane offers one key (0: none).
+  // One key per lane, sorted: becomes the list.
+  __device__ __forceinline__ void sort(u64 k, int K, int lane) {
+    merge_steps<1>(k, lane, (lane & 2) == 0);
+    merge_steps<2>(k, lane, (lane & 4) == 0);
+    merge_steps<4>(k, lane, (lane & 8) == 0);
+    merge_steps<8>(k, lane, (lane & 16) == 0);
+    merge_steps<16>(k, lane, (lane & 32) == 0);
+    merge_steps<32>(k, lane, true);
+    key = k;
+    least = read_lane(key, K - 1);
+  }
+  // Joins another sorted list: the larger of lane i and lane 63 - i of the other are the best 64, as a bitonic run.
+  __device__ __forceinline__ void join(u64 k, int K, int lane) {
+    const u64 o = __shfl(k, 63 - lane);
+    key = key > o ? key : o;
+    merge_steps<32>(key, lane, true);
+    least = read_lane(key, K - 1);
+  }
+  // Every lane offers one key (0: none); what beats the K-th best is inserted.
   __device__ __forceinline__ void offer(u64 k, int K, int lane) {
     u64 want = __builtin_amdgcn_ballot_w64(k > least);
     while (want) {  // uniform
       const int l = __builtin_ctzll(want);
       const u64 b = read_lane(k, l);
       const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(key > b));
-      const u64 up = __shfl_up(key, 1);
+      const u64 up = ((u64)dpp<0x138>((uint32_t)(key >> 32)) << 32) | dpp<0x138>((uint32_t)key);  // lane - 1 (wave_shr)
       key = lane < at ? key : lane == at ? b : up;
       least = read_lane(key, K - 1);
       want = __builtin_amdgcn_ballot_w64(k > least) & ~((2ull << l) - 1);
     }
   }
-};
-
-template <typename T>
-struct Words;
-template <>
-struct Words<float> {
-  static constexpr int kN = 4;
-  typedef float vec __attribute__((ext_vector_type(4)));
-};
-template <>
-struct Words<f16> {
-  static constexpr int kN = 8;
-  typedef f16 vec __attribute__((ext_vector_type(8)));
 };
 
 struct Out {
@@ -108,35 +193,39 @@ struct Out {
   float* top_lp;
 };
 
-// A row's results from its whole statistics (valid in every lane of the wavefront) and list.
-__device__ __forceinline__ void finish(const Out& o, int64_t row, const Stats& a, const Top& top, int K, float x,
-                                       bool known, int lane) {
+// A row's results from its whole statistics (valid in every lane of the wavefront) and list; x: the given token's logit.
+template <typename T>
+__device__ __forceinline__ void finish(const Out& o, int64_t row, const Stats& a, const Top& top, int K, T x, bool known,
+                                       int lane) {
   // no probability anywhere (logits of -inf alone): NaN, as the log of 0 / 0
-  const float log_s = a.s > 0.f || a.s != a.s ? logf(a.s) : NAN;
+  const float log_s = a.s > 0.f || a.s != a.s ? log2f(a.s) : NAN;
   if (lane == 0) {
-    if (o.lp) o.lp[row] = known ? (x - a.m) - log_s : NAN;
-    o.entropy[row] = log_s - a.t / a.s;
+    if (o.lp) o.lp[row] = known ? Words<T>::log_p(x, a.ref, log_s) : NAN;
+    o.entropy[row] = (log_s - a.t / a.s) * kLn2;
   }
   if (lane < K) {
     const int64_t at = row * K + lane;
     o.top_ids[at] = key_index(top.key);
-    o.top_lp[at] = (key_value(top.key) - a.m) - log_s;
+    o.top_lp[at] = Words<T>::log_p(from_f32<T>(key_value(top.key)), a.ref, log_s);
   }
 }
 
-// One workgroup per (row, split): grid x = row * S + split.
-template <typename T, bool TOP>
+// WPR wavefronts per row: four, one workgroup per (row, split), grid x = row * S + split; or one, four rows per
+// workgroup (S = 1).
+template <typename T, bool TOP, int WPR>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict__ logits, int64_t ld,
-                                                            const int64_t* __restrict__ ids, int vocab, int K, int S,
-                                                            Out out, float* __restrict__ part,
+                                                            const int64_t* __restrict__ ids, int rows, int vocab, int K,
+                                                            int S, Out out, float* __restrict__ part,
                                                             u64* __restrict__ part_top) {
-  constexpr int N = Words<T>::kN, U = 4;
-  typedef typename Words<T>::vec vec;
+  typedef Words<T> W;
+  constexpr int N = W::kN, U = W::kUnroll;
+  typedef typename W::vec vec;
   __shared__ float sm[kWaves][3];
   __shared__ u64 sm_top[kWaves][kMaxTop];
-  const int64_t row = blockIdx.x / (unsigned)S;
-  const int split = blockIdx.x % (unsigned)S;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int64_t row = WPR == 1 ? (int64_t)blockIdx.x * kWaves + wave : blockIdx.x / (unsigned)S;
+  const int split = WPR == 1 ? 0 : blockIdx.x % (unsigned)S, turn = WPR == 1 ? 0 : wave;
+  if (WPR == 1 && row >= rows) return;
   const T* x = logits + row * ld;
   // Vectors of 16 aligned bytes: `skip` values before the first, then nv vectors, then a tail.
   const int skip = min(vocab, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
@@ -144,78 +233,88 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
   const int per = (nv + S - 1) / S, v0 = min(nv, split * per), v1 = min(nv, v0 + per);
   const vec* xv = reinterpret_cast<const vec*>(x + skip);
 
-  Stats a = {-FLT_MAX, 0.f, 0.f};
-  Top top;
-  top.init();
+  Stats a = none<T>();
+  Top top{0, 0};
   const auto one = [&](bool have, int i) __attribute__((always_inline)) {  // a value of the head or tail
-    const float v = have ? to_f32(x[i]) : -INFINITY;
-    raise(a, fmaxf(a.m, v));
-    if (have) add(a, v);
-    if (TOP) top.offer(have ? make_key(v, i) : 0, K, lane);
+    const T v = have ? x[i] : (T)-INFINITY;
+    raise<T>(a, fmaxf(a.m, to_f32(v)));
+    add<T>(a, v);
+    if (TOP) top.offer(have ? make_key(to_f32(v), i) : 0, K, lane);
   };
-  if (split == 0 && wave == 0 && skip) one(lane < skip, lane);
-  for (int base = v0 + wave * 64; base < v1; base += kThreads * U) {  // uniform
+  for (int base = v0 + turn * 64; base < v1; base += 64 * WPR * U) {  // uniform
     vec w[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = base + u * kThreads + lane;
+      const int i = base + u * 64 * WPR + lane;
       if (i < v1) w[u] = xv[i];
       else
 #pragma unroll
         for (int e = 0; e < N; ++e) w[u][e] = (T)-INFINITY;
     }
-    float v[U][N], mx = -FLT_MAX;
+    vec top_of = w[0];
+#pragma unroll
+    for (int u = 1; u < U; ++u) top_of = __builtin_elementwise_max(top_of, w[u]);
+    float mx = -INFINITY;  // of the group, in this lane (NaN aside)
+#pragma unroll
+    for (int e = 0; e < N; ++e) mx = fmaxf(mx, to_f32(top_of[e]));
+    if (mx > a.m) raise<T>(a, mx);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        v[u][e] = to_f32(w[u][e]);
-        mx = fmaxf(mx, v[u][e]);
-      }
-    if (mx > a.m) raise(a, mx);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < N; ++e) add(a, v[u][e]);
+      for (int e = 0; e < N; ++e) add<T>(a, w[u][e]);
     if (TOP) {
-      // A value equal to the K-th best cannot enter: what the list holds came earlier, at lower indices.  A NaN (or an
-      // infinity) has made the sum NaN, and is looked for value by value from then on.
+      const auto key_of = [&](int u, int e) __attribute__((always_inline)) {
+        const int i = base + u * 64 * WPR + lane;
+        return i < v1 ? make_key(to_f32(w[u][e]), skip + i * N + e) : 0;
+      };
+      u64 best = 0;
+      if (read_lane(top.key, 0) == 0) {  // uniform: the first group
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const u64 k = key_of(u, e);
+            best = k > best ? k : best;
+          }
+        top.sort(best, K, lane);
+      }
+      // A value equal to the K-th best of earlier groups cannot enter (they hold lower indices).  A NaN or an infinity
+      // has made the sum NaN, and is looked for from then on.  (No K-th best yet: NaN, which lets every value pass.)
       const float least = key_value(top.least);
-      const bool look = top.least == 0 || mx > least || a.s != a.s;
-      if (__builtin_amdgcn_ballot_w64(look)) {
+      if (__builtin_amdgcn_ballot_w64(best != 0 || !(mx <= least) || a.s != a.s)) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int i = base + u * kThreads + lane;
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int e = 0; e < N; ++e) top.offer(i < v1 ? make_key(v[u][e], skip + i * N + e) : 0, K, lane);
-        }
+          for (int e = 0; e < N; ++e)
+            if (__builtin_amdgcn_ballot_w64(!(to_f32(w[u][e]) < least))) {
+              const u64 k = key_of(u, e);
+              top.offer(k != best ? k : 0, K, lane);
+            }
       }
     }
   }
-  if (split == S - 1 && wave == kWaves - 1 && tail < vocab) one(tail + lane < vocab, tail + lane);
-
+  if (split == 0 && turn == 0 && skip) one(lane < skip, lane);
+  if (split == S - 1 && turn == WPR - 1 && tail < vocab) one(tail + lane < vocab, tail + lane);
+  a = join_wave<T>(a);
+  if constexpr (WPR > 1) {
+    if (lane == 0) {
+      sm[wave][0] = a.m;
+      sm[wave][1] = a.s;
+      sm[wave][2] = a.t;
+    }
+    if (TOP) sm_top[wave][lane] = top.key;
+    __syncthreads();
+    if (wave) return;
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const Stats b = {__shfl_xor(a.m, off), __shfl_xor(a.s, off), __shfl_xor(a.t, off)};
-    a = (lane & off) ? join(b, a) : join(a, b);
-  }
-  if (lane == 0) {
-    sm[wave][0] = a.m;
-    sm[wave][1] = a.s;
-    sm[wave][2] = a.t;
-  }
-  if (TOP) sm_top[wave][lane] = top.key;
-  __syncthreads();
-  if (wave) return;
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) {
-    a = join(a, Stats{sm[w][0], sm[w][1], sm[w][2]});
-    if (TOP) top.offer(lane < K ? sm_top[w][lane] : 0, K, lane);
+    for (int w = 1; w < kWaves; ++w) {
+      a = join<T>(a, Stats{sm[w][0], W::ref_of(sm[w][0]), sm[w][1], sm[w][2]});
+      if (TOP) top.join(sm_top[w][lane], K, lane);
+    }
   }
   if (S == 1) {
     const int64_t id = ids ? ids[row] : -1;
     const bool known = id >= 0 && id < vocab;
-    finish(out, row, a, top, TOP ? K : 0, known ? to_f32(x[id]) : 0.f, known, lane);
+    finish<T>(out, row, a, top, TOP ? K : 0, known ? x[id] : (T)0, known, lane);
     return;
   }
   if (lane == 0) {
@@ -227,33 +326,35 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
   if (TOP && lane < K) part_top[(size_t)blockIdx.x * K + lane] = top.key;
 }
 
-// Joins the S splits of a row, one wavefront per row.
+// Joins the S <= 64 splits of a row: one workgroup per row, every wavefront a quarter of the lists.
 template <typename T, bool TOP>
-__global__ __launch_bounds__(64) void logprobs_merge(const T* __restrict__ logits, int64_t ld,
-                                                     const int64_t* __restrict__ ids, int vocab, int K, int S, Out out,
-                                                     const float* __restrict__ part, const u64* __restrict__ part_top) {
+__global__ __launch_bounds__(kThreads) void logprobs_merge(const T* __restrict__ logits, int64_t ld,
+                                                           const int64_t* __restrict__ ids, int vocab, int K, int S,
+                                                           Out out, const float* __restrict__ part,
+                                                           const u64* __restrict__ part_top) {
+  __shared__ u64 sm_top[kWaves][kMaxTop];
   const int64_t row = blockIdx.x;
-  const int lane = threadIdx.x;
-  const int64_t id = ids ? ids[row] : -1;
-  const bool known = id >= 0 && id < vocab;
-  const float x = known ? to_f32(logits[row * ld + id]) : 0.f;
-  Stats a = {-FLT_MAX, 0.f, 0.f};
-  if (lane < S) {  // (S <= 64)
-    const float* p = part + (row * S + lane) * 3;
-    a = {p[0], p[1], p[2]};
-  }
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const Stats b = {__shfl_xor(a.m, off), __shfl_xor(a.s, off), __shfl_xor(a.t, off)};
-    a = (lane & off) ? join(b, a) : join(a, b);
-  }
-  Top top;
-  top.init();
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  Top top{0, 0};
   if (TOP) {
     const u64* p = part_top + row * S * K;
-    for (int i = 0; i < S * K; i += 64) top.offer(i + lane < S * K ? p[i + lane] : 0, K, lane);
+    for (int i = wave; i < S; i += kWaves) top.join(lane < K ? p[i * K + lane] : 0, K, lane);
+    sm_top[wave][lane] = top.key;
+    __syncthreads();
   }
-  finish(out, row, a, top, TOP ? K : 0, x, known, lane);
+  if (wave) return;
+  const int64_t id = ids ? ids[row] : -1;
+  const bool known = id >= 0 && id < vocab;
+  const T x = known ? logits[row * ld + id] : (T)0;
+  Stats a = none<T>();
+  if (lane < S) {
+    const float* p = part + (row * S + lane) * 3;
+    a = {p[0], Words<T>::ref_of(p[0]), p[1], p[2]};
+  }
+  a = join_wave<T>(a);
+  if (TOP)
+    for (int w = 1; w < kWaves; ++w) top.join(sm_top[w][lane], K, lane);
+  finish<T>(out, row, a, top, TOP ? K : 0, x, known, lane);
 }
 
 // Workgroups that share a row: enough for two per CU, each with kMinChunk logits at least.
@@ -295,10 +396,16 @@ extern "C" int cir_token_logprobs(const void* logits, int dt, int64_t ld, const 
   float* part = reinterpret_cast<float*>(part_top + (size_t)rows * S * top_k);
   const auto go = [&]<typename T, bool TOP>() {
     const T* x = static_cast<const T*>(logits);
-    logprobs_kernel<T, TOP><<<(unsigned)(rows * S), kThreads, 0, s>>>(x, ld, ids, vocab, top_k, S, out, part, part_top);
+    if (rows >= kManyRows && vocab <= kShortRow) {
+      logprobs_kernel<T, TOP, 1><<<(unsigned)((rows + kWaves - 1) / kWaves), kThreads, 0, s>>>(
+          x, ld, ids, rows, vocab, top_k, 1, out, part, part_top);
+      return launch_status();
+    }
+    logprobs_kernel<T, TOP, kWaves><<<(unsigned)(rows * S), kThreads, 0, s>>>(x, ld, ids, rows, vocab, top_k, S, out,
+                                                                              part, part_top);
     const int st = launch_status();
     if (st || S == 1) return st;
-    logprobs_merge<T, TOP><<<rows, 64, 0, s>>>(x, ld, ids, vocab, top_k, S, out, part, part_top);
+    logprobs_merge<T, TOP><<<rows, kThreads, 0, s>>>(x, ld, ids, vocab, top_k, S, out, part, part_top);
     return launch_status();
   };
   if (dt == CIR_F16) return top_k ? go.template operator()<f16, true>() : go.template operator()<f16, false>();

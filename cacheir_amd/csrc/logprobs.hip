@@ -8,12 +8,18 @@
 // T' = 2^d (T + d S).
 //
 // The alternatives are the K largest by (value, then lowest index), as 64-bit keys
-// (order-preserving bits of the value | complement of the index).  A wavefront keeps its best
-// 64 sorted across its lanes.  The first values of its share go in as the largest of each
-// lane, sorted by a bitonic network: the K-th of those bounds what can still enter, so of
-// random logits a handful more is inserted one by one (inserting every one of the first 1024
-// took ~100 insertions, 5 us).  Sorted lists are joined in 7 exchange steps: wavefronts, then
-// workgroups of a row, in order, so results do not depend on timing.
+// (order-preserving bits of the value | complement of the index).  While it streams, a lane
+// only keeps the largest value of each of up to kCells stretches of its share ("cells"), which
+// the statistics need anyway.  The K-th largest of a wavefront's 64 lane maxima bounds the
+// row's K-th largest value from below; so does the largest such bound of the row's
+// wavefronts.  The values that reach the bound lie in the few cells whose maximum does:
+// those are read again, what reaches the bound is gathered in LDS, sorted by a bitonic
+// network and kept as the wavefront's list, 64 keys across its lanes.  Where too many cells
+// qualify (equal logits, a mask that leaves less than K tokens) or a NaN is about, the share
+// is walked in order instead, past every group that cannot change the list.  Sorted lists
+// are joined in 7 exchange steps: wavefronts, then workgroups of a row, in order, so results
+// do not depend on timing.  (Inserting what beat a running K-th best as it streamed by took
+// 101 us where this takes 67, 1021 x 152064 fp16 and K = 2; without alternatives it is 61.)
 //
 // Bound by the read of the logits.
 #include "common.hpp"
@@ -27,24 +33,33 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxTop = 64;       // a wavefront's lanes
+constexpr int kCells = 16;        // maxima a lane keeps
+constexpr int kPicks = 128;       // cells of a wavefront that are read again
+constexpr int kKeys = 256;        // keys a wavefront gathers
+constexpr int kAhead = 8;         // values per lane that are read again at once
 constexpr int kMinChunk = 4096;   // logits of a workgroup that shares its row with others
-constexpr int kManyRows = 1024, kShortRow = 4096;  // rows of one wavefront each
+constexpr int kManyRows = 1024;   // rows of one wavefront each, where they are short
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // 2^-300 is zero in fp32: y below it adds nothing, and 0 * y stays 0 for x = -inf.
 constexpr float kFloor = -300.f;
 
 typedef unsigned long long u64;
 
+// Order-preserving bits (NaN aside).
+__device__ __forceinline__ uint32_t rank_bits(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.f);
+  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float rank_value(uint32_t b) {
+  return __builtin_bit_cast(float, (b & 0x80000000u) ? b & 0x7fffffffu : ~b);
+}
 // Larger key = larger value (NaN above all, -0 as 0), then lower index.
 __device__ __forceinline__ u64 make_key(float v, int i) {
-  uint32_t b = __builtin_bit_cast(uint32_t, v + 0.f);
-  b = (v != v) ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
-  return ((u64)b << 32) | (uint32_t)~i;
+  return ((u64)((v != v) ? 0xffffffffu : rank_bits(v)) << 32) | (uint32_t)~i;
 }
 __device__ __forceinline__ float key_value(u64 k) {
   const uint32_t b = (uint32_t)(k >> 32);
-  if (b == 0xffffffffu) return NAN;
-  return __builtin_bit_cast(float, (b & 0x80000000u) ? b & 0x7fffffffu : ~b);
+  return b == 0xffffffffu ? NAN : rank_value(b);
 }
 __device__ __forceinline__ int key_index(u64 k) { return (int)~(uint32_t)k; }
 
@@ -76,6 +91,13 @@ struct Words<f16> {
   static __device__ __forceinline__ float gap(float ref, float to) { return ref - to; }
   static __device__ __forceinline__ float log_p(f16 x, float ref, float log2_s) { return (y_of(x, ref) - log2_s) * kLn2; }
 };
+
+__device__ __forceinline__ uint32_t read_lane32(uint32_t v, int l) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, l);
+}
+__device__ __forceinline__ int lanes_below(u64 m) {  // set bits of lanes before this one
+  return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+}
 
 struct Stats {
   float m, ref, s, t;
@@ -145,25 +167,30 @@ __device__ __forceinline__ void exchange(u64& k, bool up) {
   k = (k > o) == up ? k : o;
 }
 template <int MASK>
-__device__ __forceinline__ void merge_steps(u64& k, int lane, bool desc) {  // a bitonic run of 2 MASK lanes, sorted
+__device__ __forceinline__ void exchange(uint32_t& k, bool up) {
+  const uint32_t o = lane_xor<MASK>(k), hi = max(k, o), lo = min(k, o);
+  k = up ? hi : lo;
+}
+template <int MASK, typename Key>
+__device__ __forceinline__ void merge_steps(Key& k, int lane, bool desc) {  // a bitonic run of 2 MASK lanes, sorted
   exchange<MASK>(k, ((lane & MASK) == 0) == desc);
   if constexpr (MASK > 1) merge_steps<MASK / 2>(k, lane, desc);
+}
+
+template <typename Key>
+__device__ __forceinline__ Key sorted(Key k, int lane) {  // one key per lane, the largest in lane 0
+  merge_steps<1>(k, lane, (lane & 2) == 0);
+  merge_steps<2>(k, lane, (lane & 4) == 0);
+  merge_steps<4>(k, lane, (lane & 8) == 0);
+  merge_steps<8>(k, lane, (lane & 16) == 0);
+  merge_steps<16>(k, lane, (lane & 32) == 0);
+  merge_steps<32>(k, lane, true);
+  return k;
 }
 
 // The wavefront's list: lane i holds the i-th best key (0: none).
 struct Top {
   u64 key, least;  // least: the K-th best (uniform)
-  // One key per lane, sorted: becomes the list.
-  __device__ __forceinline__ void sort(u64 k, int K, int lane) {
-    merge_steps<1>(k, lane, (lane & 2) == 0);
-    merge_steps<2>(k, lane, (lane & 4) == 0);
-    merge_steps<4>(k, lane, (lane & 8) == 0);
-    merge_steps<8>(k, lane, (lane & 16) == 0);
-    merge_steps<16>(k, lane, (lane & 32) == 0);
-    merge_steps<32>(k, lane, true);
-    key = k;
-    least = read_lane(key, K - 1);
-  }
   // Joins another sorted list: the larger of lane i and lane 63 - i of the other are the best 64, as a bitonic run.
   __device__ __forceinline__ void join(u64 k, int K, int lane) {
     const u64 o = __shfl(k, 63 - lane);
@@ -171,17 +198,15 @@ struct Top {
     merge_steps<32>(key, lane, true);
     least = read_lane(key, K - 1);
   }
-  // Every lane offers one key (0: none); what beats the K-th best is inserted.
-  __device__ __forceinline__ void offer(u64 k, int K, int lane) {
-    u64 want = __builtin_amdgcn_ballot_w64(k > least);
-    while (want) {  // uniform
-      const int l = __builtin_ctzll(want);
-      const u64 b = read_lane(k, l);
-      const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(key > b));
-      const u64 up = ((u64)dpp<0x138>((uint32_t)(key >> 32)) << 32) | dpp<0x138>((uint32_t)key);  // lane - 1 (wave_shr)
-      key = lane < at ? key : lane == at ? b : up;
+  // Every lane offers one key (0: none).
+  __device__ __forceinline__ void absorb(u64 k, int K, int lane) {
+    if (!__builtin_amdgcn_ballot_w64(k > least)) return;
+    k = sorted(k, lane);
+    if (read_lane(key, 0) != 0) {  // uniform
+      join(k, K, lane);
+    } else {
+      key = k;
       least = read_lane(key, K - 1);
-      want = __builtin_amdgcn_ballot_w64(k > least) & ~((2ull << l) - 1);
     }
   }
 };
@@ -211,17 +236,20 @@ __device__ __forceinline__ void finish(const Out& o, int64_t row, const Stats& a
 }
 
 // WPR wavefronts per row: four, one workgroup per (row, split), grid x = row * S + split; or one, four rows per
-// workgroup (S = 1).
-template <typename T, bool TOP, int WPR>
+// workgroup (S = 1).  U vectors per lane and group; ONE: every wavefront's share is one group (what may enter the list
+// is then taken from registers).
+template <typename T, bool TOP, int WPR, int U, bool ONE>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict__ logits, int64_t ld,
                                                             const int64_t* __restrict__ ids, int rows, int vocab, int K,
                                                             int S, Out out, float* __restrict__ part,
                                                             u64* __restrict__ part_top) {
   typedef Words<T> W;
-  constexpr int N = W::kN, U = W::kUnroll;
+  constexpr int N = W::kN;
   typedef typename W::vec vec;
-  __shared__ float sm[kWaves][3];
-  __shared__ u64 sm_top[kWaves][kMaxTop];
+  __shared__ float sm[kWaves][4];
+  __shared__ float sm_cell[TOP && !ONE ? kWaves : 1][TOP && !ONE ? kCells : 1][64];
+  __shared__ u64 sm_keys[TOP ? kWaves : 1][TOP ? kKeys : 1];
+  __shared__ int sm_pick[TOP && !ONE ? kWaves : 1][TOP && !ONE ? kPicks : 1], sm_n[kWaves];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int64_t row = WPR == 1 ? (int64_t)blockIdx.x * kWaves + wave : blockIdx.x / (unsigned)S;
   const int split = WPR == 1 ? 0 : blockIdx.x % (unsigned)S, turn = WPR == 1 ? 0 : wave;
@@ -232,17 +260,19 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
   const int nv = (vocab - skip) / N, tail = skip + nv * N;
   const int per = (nv + S - 1) / S, v0 = min(nv, split * per), v1 = min(nv, v0 + per);
   const vec* xv = reinterpret_cast<const vec*>(x + skip);
+  // The given token's logit, on its way meanwhile.
+  const int64_t id = S == 1 && ids ? ids[row] : -1;
+  const bool known = id >= 0 && id < vocab;
+  const T given = x[known ? id : 0];
 
+  // This wavefront's groups: vectors base0 + g * kGroup + u * 64 WPR + lane, u < U; cells of `wide` groups.
+  constexpr int kGroup = 64 * WPR * U;
+  const int base0 = v0 + turn * 64;
+  const int groups = base0 < v1 ? (ONE ? 1 : (v1 - base0 + kGroup - 1) / kGroup) : 0;
+  const int wide = (groups + kCells - 1) / kCells;
   Stats a = none<T>();
-  Top top{0, 0};
-  const auto one = [&](bool have, int i) __attribute__((always_inline)) {  // a value of the head or tail
-    const T v = have ? x[i] : (T)-INFINITY;
-    raise<T>(a, fmaxf(a.m, to_f32(v)));
-    add<T>(a, v);
-    if (TOP) top.offer(have ? make_key(to_f32(v), i) : 0, K, lane);
-  };
-  for (int base = v0 + turn * 64; base < v1; base += 64 * WPR * U) {  // uniform
-    vec w[U];
+  float most = -INFINITY;  // the lane's largest value (NaN aside)
+  const auto load = [&](vec (&w)[U], int base) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = base + u * 64 * WPR + lane;
@@ -251,50 +281,137 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
 #pragma unroll
         for (int e = 0; e < N; ++e) w[u][e] = (T)-INFINITY;
     }
+  };
+  const auto take = [&](const vec (&w)[U]) __attribute__((always_inline)) {  // into the statistics; the largest value
     vec top_of = w[0];
 #pragma unroll
     for (int u = 1; u < U; ++u) top_of = __builtin_elementwise_max(top_of, w[u]);
-    float mx = -INFINITY;  // of the group, in this lane (NaN aside)
+    float mx = to_f32(top_of[0]);
 #pragma unroll
-    for (int e = 0; e < N; ++e) mx = fmaxf(mx, to_f32(top_of[e]));
+    for (int e = 1; e < N; ++e) mx = fmaxf(mx, to_f32(top_of[e]));
     if (mx > a.m) raise<T>(a, mx);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int e = 0; e < N; ++e) add<T>(a, w[u][e]);
-    if (TOP) {
-      const auto key_of = [&](int u, int e) __attribute__((always_inline)) {
-        const int i = base + u * 64 * WPR + lane;
-        return i < v1 ? make_key(to_f32(w[u][e]), skip + i * N + e) : 0;
-      };
-      u64 best = 0;
-      if (read_lane(top.key, 0) == 0) {  // uniform: the first group
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const u64 k = key_of(u, e);
-            best = k > best ? k : best;
-          }
-        top.sort(best, K, lane);
-      }
-      // A value equal to the K-th best of earlier groups cannot enter (they hold lower indices).  A NaN or an infinity
-      // has made the sum NaN, and is looked for from then on.  (No K-th best yet: NaN, which lets every value pass.)
-      const float least = key_value(top.least);
-      if (__builtin_amdgcn_ballot_w64(best != 0 || !(mx <= least) || a.s != a.s)) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int e = 0; e < N; ++e)
-            if (__builtin_amdgcn_ballot_w64(!(to_f32(w[u][e]) < least))) {
-              const u64 k = key_of(u, e);
-              top.offer(k != best ? k : 0, K, lane);
-            }
+    return mx;
+  };
+  vec one[ONE ? U : 1];
+  if constexpr (ONE) {
+    load(one, base0);
+    most = take(one);
+  } else {
+    float cell = -INFINITY;
+    for (int g = 0; g < groups; ++g) {  // uniform
+      vec w[U];
+      load(w, base0 + g * kGroup);
+      const float mx = take(w);
+      if constexpr (TOP) {
+        cell = fmaxf(cell, mx);
+        if ((g + 1) % wide == 0 || g + 1 == groups) {  // uniform
+          sm_cell[wave][g / wide][lane] = cell;
+          most = fmaxf(most, cell);
+          cell = -INFINITY;
+        }
       }
     }
   }
-  if (split == 0 && turn == 0 && skip) one(lane < skip, lane);
-  if (split == S - 1 && turn == WPR - 1 && tail < vocab) one(tail + lane < vocab, tail + lane);
+  // The values before the first vector and behind the last one (at most N - 1 each), one per lane.
+  const bool has_head = split == 0 && turn == 0 && skip > 0, has_tail = split == S - 1 && turn == WPR - 1 && tail < vocab;
+  const int end_at = has_head && lane < skip                            ? lane
+                     : has_tail && lane >= 32 && tail + lane - 32 < vocab ? tail + lane - 32
+                                                                        : -1;
+  if (has_head || has_tail) {
+    const T v = end_at >= 0 ? x[end_at] : (T)-INFINITY;
+    raise<T>(a, fmaxf(a.m, to_f32(v)));
+    if (end_at >= 0) add<T>(a, v);
+  }
+
+  Top top{0, 0};
+  if constexpr (TOP) {
+    // The bound: at least K values of the row reach it.
+    float bound = rank_value(read_lane32(sorted(rank_bits(most), lane), K - 1));
+    const bool odd = __builtin_amdgcn_ballot_w64(a.s != a.s) != 0;  // uniform: a NaN or an infinity
+    if (WPR > 1) {
+      if (lane == 0) sm[wave][3] = bound;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) bound = fmaxf(bound, sm[w][3]);
+    }
+    int n = 0;  // keys gathered, uniform
+    const auto gather = [&](bool may, float v, int at) __attribute__((always_inline)) {
+      const u64 m = __builtin_amdgcn_ballot_w64(may);
+      if (m) {
+        const int to = n + lanes_below(m);
+        if (may && to < kKeys) sm_keys[wave][to] = make_key(v, at);
+        n += __builtin_popcountll(m);
+      }
+    };
+    if (has_head || has_tail) gather(end_at >= 0, end_at >= 0 ? to_f32(x[end_at]) : 0.f, end_at);
+    const int ends = n;
+    int picks = 0;  // uniform
+    if constexpr (ONE) {
+      if (!odd) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int i = base0 + u * 64 * WPR + lane;
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const float v = to_f32(one[u][e]);
+            gather(i < v1 && v >= bound, v, skip + i * N + e);
+          }
+        }
+      }
+    } else if (!odd) {
+      // The cells that reach the bound.
+      const int cells = wide ? (groups + wide - 1) / wide : 0;
+      for (int c = 0; c < cells; ++c) {
+        const u64 hit = __builtin_amdgcn_ballot_w64(sm_cell[wave][c][lane] >= bound);
+        const int at = picks + lanes_below(hit);
+        if (((hit >> lane) & 1) && at < kPicks) sm_pick[wave][at] = c * 64 + lane;
+        picks += __builtin_popcountll(hit);
+      }
+      if (picks <= kPicks) {
+        for (int g = 0; g < wide; ++g)                                 // (group of the cell)
+          for (int j0 = 0; j0 < picks * U * N; j0 += 64 * kAhead) {    // uniform
+            float v[kAhead];
+            int at[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+              const int j = j0 + 64 * k + lane, p = j / (U * N), r = j % (U * N);
+              const int pick = sm_pick[wave][min(p, kPicks - 1)];
+              const int i = base0 + ((pick >> 6) * wide + g) * kGroup + r / N * 64 * WPR + (pick & 63);
+              const bool in = p < picks && i < v1;
+              at[k] = in ? skip + i * N + r % N : -1;
+              v[k] = to_f32(x[in ? at[k] : 0]);
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) gather(at[k] >= 0 && v[k] >= bound, v[k], at[k]);
+          }
+      }
+    }
+    if (picks > kPicks || n > kKeys || odd) {  // uniform
+      for (int j = 0; j < ends; j += 64) top.absorb(j + lane < ends ? sm_keys[wave][j + lane] : 0, K, lane);
+      for (int g = 0; g < groups; ++g) {           // uniform
+        const float least = key_value(top.least);  // (none yet: NaN)
+        if (!ONE && !odd) {
+          const float m = sm_cell[wave][ONE ? 0 : g / wide][lane];
+          if (!__builtin_amdgcn_ballot_w64(m >= bound && !(m <= least))) continue;
+        }
+        for (int j = 0; j < U * N; ++j) {
+          const int i = base0 + g * kGroup + j / N * 64 * WPR + lane, at = skip + i * N + j % N;
+          const bool in = i < v1;
+          const float v = to_f32(x[in ? at : 0]);
+          top.absorb(in && !(v < bound) ? make_key(v, at) : 0, K, lane);
+        }
+      }
+      n = 64;
+      sm_keys[wave][lane] = top.key;
+      top = Top{0, 0};
+    }
+    if (lane == 0) sm_n[wave] = n;
+  }
+
   a = join_wave<T>(a);
   if constexpr (WPR > 1) {
     if (lane == 0) {
@@ -302,19 +419,29 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
       sm[wave][1] = a.s;
       sm[wave][2] = a.t;
     }
-    if (TOP) sm_top[wave][lane] = top.key;
     __syncthreads();
     if (wave) return;
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) {
-      a = join<T>(a, Stats{sm[w][0], W::ref_of(sm[w][0]), sm[w][1], sm[w][2]});
-      if (TOP) top.join(sm_top[w][lane], K, lane);
+    for (int w = 1; w < kWaves; ++w) a = join<T>(a, Stats{sm[w][0], W::ref_of(sm[w][0]), sm[w][1], sm[w][2]});
+  }
+  if constexpr (TOP) {  // every wavefront's keys, 64 at a time
+    constexpr int kOf = WPR > 1 ? kWaves : 1;
+    int from[kOf + 1];
+    from[0] = 0;
+#pragma unroll
+    for (int w = 0; w < kOf; ++w) from[w + 1] = from[w] + __builtin_amdgcn_readfirstlane(sm_n[WPR > 1 ? w : wave]);
+    for (int j = 0; j < from[kOf]; j += 64) {
+      int w = 0;
+#pragma unroll
+      for (int k = 1; k < kOf; ++k) w += j + lane >= from[k] ? 1 : 0;
+      int start = 0;
+#pragma unroll
+      for (int k = 1; k < kOf; ++k) start = w == k ? from[k] : start;
+      top.absorb(j + lane < from[kOf] ? sm_keys[WPR > 1 ? w : wave][j + lane - start] : 0, K, lane);
     }
   }
   if (S == 1) {
-    const int64_t id = ids ? ids[row] : -1;
-    const bool known = id >= 0 && id < vocab;
-    finish<T>(out, row, a, top, TOP ? K : 0, known ? x[id] : (T)0, known, lane);
+    finish<T>(out, row, a, top, TOP ? K : 0, given, known, lane);
     return;
   }
   if (lane == 0) {
@@ -326,34 +453,55 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
   if (TOP && lane < K) part_top[(size_t)blockIdx.x * K + lane] = top.key;
 }
 
-// Joins the S <= 64 splits of a row: one workgroup per row, every wavefront a quarter of the lists.
+// Joins the S <= 64 splits of a row, one wavefront per row: the K-th largest of the lanes' best keys bounds what can
+// enter, what reaches it is gathered and sorted (all of it, 64 at a time, where equal values make it too much).
 template <typename T, bool TOP>
-__global__ __launch_bounds__(kThreads) void logprobs_merge(const T* __restrict__ logits, int64_t ld,
-                                                           const int64_t* __restrict__ ids, int vocab, int K, int S,
-                                                           Out out, const float* __restrict__ part,
-                                                           const u64* __restrict__ part_top) {
-  __shared__ u64 sm_top[kWaves][kMaxTop];
+__global__ __launch_bounds__(64) void logprobs_merge(const T* __restrict__ logits, int64_t ld,
+                                                     const int64_t* __restrict__ ids, int vocab, int K, int S, Out out,
+                                                     const float* __restrict__ part, const u64* __restrict__ part_top) {
+  __shared__ u64 sm_keys[kKeys];
   const int64_t row = blockIdx.x;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  Top top{0, 0};
-  if (TOP) {
-    const u64* p = part_top + row * S * K;
-    for (int i = wave; i < S; i += kWaves) top.join(lane < K ? p[i * K + lane] : 0, K, lane);
-    sm_top[wave][lane] = top.key;
-    __syncthreads();
-  }
-  if (wave) return;
+  const int lane = threadIdx.x;
   const int64_t id = ids ? ids[row] : -1;
   const bool known = id >= 0 && id < vocab;
-  const T x = known ? logits[row * ld + id] : (T)0;
   Stats a = none<T>();
   if (lane < S) {
     const float* p = part + (row * S + lane) * 3;
     a = {p[0], Words<T>::ref_of(p[0]), p[1], p[2]};
   }
+  const T x = logits[row * ld + (known ? id : 0)];
+  Top top{0, 0};
+  if (TOP) {
+    const u64* p = part_top + row * S * K;
+    const int all = S * K;
+    uint32_t best = 0;
+    for (int i0 = 0; i0 < all; i0 += 64 * kAhead) {
+      u64 k[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) k[j] = p[min(i0 + 64 * j + lane, all - 1)];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) best = max(best, i0 + 64 * j + lane < all ? (uint32_t)(k[j] >> 32) : 0);
+    }
+    const uint32_t bound = read_lane32(sorted(best, lane), K - 1);
+    int n = 0;
+    for (int i0 = 0; i0 < all; i0 += 64 * kAhead) {
+      u64 k[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) k[j] = p[min(i0 + 64 * j + lane, all - 1)];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const bool may = i0 + 64 * j + lane < all && k[j] != 0 && (uint32_t)(k[j] >> 32) >= bound;
+        const u64 m = __builtin_amdgcn_ballot_w64(may);
+        const int to = n + lanes_below(m);
+        if (may && to < kKeys) sm_keys[to] = k[j];
+        n += __builtin_popcountll(m);
+      }
+    }
+    const bool fits = n <= kKeys;
+    if (!fits) n = all;
+    for (int i = 0; i < n; i += 64) top.absorb(i + lane < n ? (fits ? sm_keys[i + lane] : p[i + lane]) : 0, K, lane);
+  }
   a = join_wave<T>(a);
-  if (TOP)
-    for (int w = 1; w < kWaves; ++w) top.join(sm_top[w][lane], K, lane);
   finish<T>(out, row, a, top, TOP ? K : 0, x, known, lane);
 }
 
@@ -396,16 +544,22 @@ extern "C" int cir_token_logprobs(const void* logits, int dt, int64_t ld, const 
   float* part = reinterpret_cast<float*>(part_top + (size_t)rows * S * top_k);
   const auto go = [&]<typename T, bool TOP>() {
     const T* x = static_cast<const T*>(logits);
-    if (rows >= kManyRows && vocab <= kShortRow) {
-      logprobs_kernel<T, TOP, 1><<<(unsigned)((rows + kWaves - 1) / kWaves), kThreads, 0, s>>>(
-          x, ld, ids, rows, vocab, top_k, 1, out, part, part_top);
+    constexpr int kGroup = 64 * 4 * Words<T>::kN;  // logits of a wavefront's group
+    const auto run = [&]<int WPR, int U, bool ONE>() {
+      logprobs_kernel<T, TOP, WPR, U, ONE><<<WPR == 1 ? (unsigned)((rows + kWaves - 1) / kWaves) : (unsigned)(rows * S),
+                                             kThreads, 0, s>>>(x, ld, ids, rows, vocab, top_k, S, out, part, part_top);
+    };
+    if (rows >= kManyRows && vocab <= 4 * kGroup) {
+      if (vocab <= kGroup / 4) run.template operator()<1, 1, true>();
+      else if (vocab <= kGroup) run.template operator()<1, 4, true>();
+      else run.template operator()<1, 4, false>();
       return launch_status();
     }
-    logprobs_kernel<T, TOP, kWaves><<<(unsigned)(rows * S), kThreads, 0, s>>>(x, ld, ids, rows, vocab, top_k, S, out,
-                                                                              part, part_top);
+    if (((vocab / Words<T>::kN + S - 1) / S) <= 64 * 4 * kWaves) run.template operator()<kWaves, 4, true>();
+    else run.template operator()<kWaves, 4, false>();
     const int st = launch_status();
     if (st || S == 1) return st;
-    logprobs_merge<T, TOP><<<rows, kThreads, 0, s>>>(x, ld, ids, vocab, top_k, S, out, part, part_top);
+    logprobs_merge<T, TOP><<<rows, 64, 0, s>>>(x, ld, ids, vocab, top_k, S, out, part, part_top);
     return launch_status();
   };
   if (dt == CIR_F16) return top_k ? go.template operator()<f16, true>() : go.template operator()<f16, false>();

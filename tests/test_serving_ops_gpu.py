@@ -548,9 +548,10 @@ def test_rope_append_refusals(device):
 
 
 # --------------------------------------------------------- log probabilities --
-def check_logprobs(logits, ids, k, r):
-    """``logits`` on the CPU (any dtype), rows without NaN or +inf."""
+def check_logprobs(logits, ids, k, r, which=None):
+    """``logits`` on the CPU (any dtype), rows without NaN or +inf; row i of the results is of logits row ``which[i]``."""
     rows, vocab = logits.shape
+    which = torch.arange(rows) if which is None else which
     x = logits.double()
     lp = torch.log_softmax(x, dim=1)
     p = lp.exp()
@@ -560,14 +561,14 @@ def check_logprobs(logits, ids, k, r):
     near = lambda got, want, tol: bool((((got.cpu().double() - want).abs() <= tol) | (got.cpu().double() == want)).all())
     order = np.argsort(-x.numpy(), axis=1, kind="stable")[:, :k]
     order = torch.from_numpy(np.ascontiguousarray(order))
-    assert torch.equal(r.top_ids.cpu(), order)
+    assert torch.equal(r.top_ids.cpu(), order[which])
     best, away = lp.gather(1, order), (x.gather(1, order) - m).abs()
-    assert near(r.top_logprobs, best, sums + U32 * (away + best.abs()))
-    assert near(r.entropy, h, 2 * sums * (1 + h) + 2 * U32 * h)
+    assert near(r.top_logprobs, best[which], (sums + U32 * (away + best.abs()))[which])
+    assert near(r.entropy, h[which], (2 * sums * (1 + h) + 2 * U32 * h)[which])
     if ids is not None:
         inside = (ids >= 0) & (ids < vocab)
-        at = ids.clamp(0, vocab - 1)[:, None]
-        want, d = lp.gather(1, at).squeeze(1), (x.gather(1, at) - m).abs().squeeze(1)
+        at = ids.clamp(0, vocab - 1)
+        want, d = lp[which, at], (x[which, at] - m[which, 0]).abs()
         got = r.logprobs.cpu()
         assert torch.isnan(got[~inside]).all()
         assert near(got[inside], want[inside], (sums + U32 * (d + want.abs()))[inside])
@@ -611,6 +612,34 @@ def test_logprobs_ties_order_and_masks(device, dtype, vocab):
     x = torch.stack(rows).to(dtype)
     ids = torch.randint(0, vocab, (len(rows),), generator=g)
     check_logprobs(x, ids, 20, kernels.token_logprobs(x.to(device), ids.to(device), 20))
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [
+    (1100, 100, torch.float32), (1100, 100, torch.float16), (1027, 700, torch.float32), (1027, 1900, torch.float16),
+    (1100, 3000, torch.float32), (1030, 8000, torch.float16),           # a wavefront per row, one group and several
+    (520, 90001, torch.float32), (516, 180000, torch.float16), (513, 5000, torch.float32)])  # a workgroup per row
+def test_logprobs_many_rows(device, rows, vocab, dtype):
+    """Copies of a dozen rows (random, rising, equal, masked but for a few, one value repeated, NaN) under other ids."""
+    from cacheir_amd import kernels
+
+    g = torch.Generator().manual_seed(rows + vocab)
+    few = torch.full((vocab,), -math.inf)
+    few[torch.randint(0, vocab, (3,), generator=g)] = 1.5
+    half = torch.randn(vocab, generator=g)
+    half[vocab // 3:] = 2.0
+    kinds = [torch.linspace(-8, 8, vocab), torch.zeros(vocab), few, half,
+             torch.randn(vocab, generator=g).masked_fill(torch.rand(vocab, generator=g) < 0.99, torch.finfo(dtype).min)]
+    kinds += [torch.randn(vocab, generator=g) * 4 for _ in range(6)]
+    x = torch.stack(kinds).to(dtype)
+    which = torch.arange(rows) % len(kinds)
+    ids = torch.randint(0, vocab, (rows,), generator=g)
+    r = kernels.token_logprobs(x.to(device)[which.to(device)].contiguous(), ids.to(device), 7)
+    check_logprobs(x, ids, 7, r, which)
+    bad = x.clone()
+    bad[:, vocab // 2] = math.nan
+    r = kernels.token_logprobs(bad.to(device)[which.to(device)].contiguous(), ids.to(device), 7)
+    order = [vocab // 2] + [i for i in np.argsort(-x[5].float().numpy(), kind="stable")[:8].tolist() if i != vocab // 2]
+    assert r.top_ids[5].tolist() == order[:7] and torch.isnan(r.entropy).all() and torch.isnan(r.logprobs).all()
 
 
 def test_logprobs_rows_without_probabilities(device):

@@ -232,17 +232,16 @@ def paged_decode_attention_shared(q, k_pool, v_pool, page_table, seq_lens, group
     ``[groups]``), and each prefix is read once for all of them.  Both may change between replays of a captured call.
     ``check_tables`` checks them, the pages and the lengths on the host (a device sync)."""
     dev, dt = q.get_device(), q.dtype
-    if not (dev >= 0 and q.dim() == 3 and k_pool.dim() == 4 and page_table.dim() == 2 and not check_tables
-            and _fits(q, dev, dt, q.shape) and _fits(k_pool, dev, dt, k_pool.shape)
-            and _fits(v_pool, dev, dt, k_pool.shape) and q.shape[2] == k_pool.shape[3]
-            and _fits(page_table, dev, torch.int32, (q.shape[0], page_table.shape[1]))
-            and _fits(seq_lens, dev, torch.int32, (q.shape[0],))
-            and _fits(prefix_lens, dev, torch.int32, (prefix_lens.numel(),))
-            and _fits(group_rows, dev, torch.int32, (prefix_lens.numel() + 1,))):
+    qs, ps, ts, i32 = q.shape, k_pool.shape, page_table.shape, torch.int32
+    groups = prefix_lens.numel()
+    if not (dev >= 0 and len(qs) == 3 and len(ps) == 4 and len(ts) == 2 and not check_tables
+            and qs[0] == ts[0] and qs[2] == ps[3] and _fits(q, dev, dt, qs) and _fits(k_pool, dev, dt, ps)
+            and _fits(v_pool, dev, dt, ps) and _fits(page_table, dev, i32, ts) and _fits(seq_lens, dev, i32, qs[:1])
+            and _fits(prefix_lens, dev, i32, (groups,)) and _fits(group_rows, dev, i32, (groups + 1,))):
         _check_shared(q, k_pool, v_pool, page_table, seq_lens, group_rows, prefix_lens, check_tables)
-    batch, num_heads, head_dim = q.shape
-    kvh, psize = k_pool.shape[1], k_pool.shape[2]
-    groups, max_pages = prefix_lens.numel(), page_table.shape[1]
+    batch, num_heads, head_dim = qs
+    _, kvh, psize, _ = ps
+    max_pages = ts[1]
     if out is None:
         out = torch.empty_like(q)
     elif not _fits(out, dev, dt, q.shape):
@@ -289,16 +288,17 @@ def extend_page_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, new_tok
     ``max_tokens`` bounds the new tokens of all rows (the map's length; its tail is -1).  ``out`` may hold ``seq_lens``
     and ``free_head`` themselves, which then advance in place (a captured decode step replays without the host)."""
     dev, i32 = page_table.get_device(), torch.int32
-    if not (dev >= 0 and page_table.dim() == 2 and _fits(page_table, dev, i32, page_table.shape)
-            and _fits(seq_lens, dev, i32, page_table.shape[:1]) and _fits(new_tokens, dev, i32, page_table.shape[:1])
-            and _fits(free_slots, dev, i32, (free_slots.numel(),)) and _fits(free_head, dev, i32, (1,))):
+    shape, rows = page_table.shape, page_table.shape[:1]
+    if not (dev >= 0 and len(shape) == 2 and _fits(page_table, dev, i32, shape) and _fits(seq_lens, dev, i32, rows)
+            and _fits(new_tokens, dev, i32, rows) and _fits(free_slots, dev, i32, (free_slots.numel(),))
+            and _fits(free_head, dev, i32, (1,))):
         _cuda(page_table, "page_table")
         _req(page_table.dim() == 2, "page_table must be [batch, pages]")
         _cuda(free_slots, "free_slots")
         _tensors(page_table.device, page_table=(page_table, i32, page_table.shape),
                  seq_lens=(seq_lens, i32, page_table.shape[:1]), new_tokens=(new_tokens, i32, page_table.shape[:1]),
                  free_slots=(free_slots, i32, (free_slots.numel(),)), free_head=(free_head, i32, (1,)))
-    batch, max_pages = page_table.shape
+    batch, max_pages = shape
     _req(page_size > 0 and max_tokens >= 0, "page_size must be positive and max_tokens not negative")
     if out is None:
         out = StepTables.empty(batch, max_tokens, page_table.device)
@@ -366,21 +366,21 @@ def rope_append(q, k, v, positions, slot_map, inv_freq, k_pool, v_pool, *, layou
     first ``2 * inv_freq.numel()`` dims of a head turn, in pairs (2i, 2i + 1) (``"interleaved"``) or halves apart
     (``"half"``); cos and sin are multiplied by ``factor``.  q, k and v may be views (any token and head stride, as the
     columns of one QKV projection); ``out`` may be q.  Returns the turned q."""
-    dev, dt = q.get_device(), q.dtype
-    kdt, rot = k_pool.dtype, 2 * inv_freq.numel()
-    if not (dev >= 0 and q.dim() == k.dim() == 3 and k_pool.dim() == 4 and k.get_device() == v.get_device() == dev
-            and k.dtype is dt and v.dtype is dt and v.shape == k.shape and k.shape[0] == q.shape[0]
-            and k.shape[2] == q.shape[2] and q.stride(2) == k.stride(2) == v.stride(2) == 1
-            and k_pool.shape[1] == k.shape[1] and k_pool.shape[3] == q.shape[2] >= rot
-            and _fits(k_pool, dev, kdt, k_pool.shape) and _fits(v_pool, dev, kdt, k_pool.shape)
-            and _fits(positions, dev, torch.int32, q.shape[:1]) and _fits(slot_map, dev, torch.int64, q.shape[:1])
-            and _fits(inv_freq, dev, torch.float64, (rot // 2,))):
+    dev, dt, kdt = q.get_device(), q.dtype, k_pool.dtype
+    qs, ks, ps, fs = q.shape, k.shape, k_pool.shape, inv_freq.shape
+    if not (dev >= 0 and len(qs) == len(ks) == 3 and len(ps) == 4 and len(fs) == 1
+            and k.get_device() == dev == v.get_device() and k.dtype is dt is v.dtype and v.shape == ks
+            and qs[0] == ks[0] and ps[3] == qs[2] == ks[2] >= 2 * fs[0] and ps[1] == ks[1]
+            and q.stride(2) == k.stride(2) == v.stride(2) == 1
+            and _fits(k_pool, dev, kdt, ps) and _fits(v_pool, dev, kdt, ps) and _fits(positions, dev, torch.int32, qs[:1])
+            and _fits(slot_map, dev, torch.int64, qs[:1]) and _fits(inv_freq, dev, torch.float64, fs)):
         _check_rope(q, k, v, positions, slot_map, inv_freq, k_pool, v_pool)
     _req(layout in hip.ROPE_LAYOUTS, f"layout must be one of {sorted(hip.ROPE_LAYOUTS)}")
-    tokens, heads, dim = q.shape
-    slots, kvh, psize, _ = k_pool.shape
+    tokens, heads, dim = qs
+    slots, kvh, psize, _ = ps
+    rot = 2 * inv_freq.numel()
     if out is None:
-        out = torch.empty(q.shape, dtype=dt, device=q.device)
+        out = q.new_empty(qs)
     else:
         _req(isinstance(out, torch.Tensor) and out.device == q.device and out.shape == q.shape and
              (out.stride(2) == 1 or dim == 1) and out.dtype == dt, "out must be like q")

@@ -20,58 +20,64 @@ bool valid_dt(int dt) { return dt == CIR_F32 || dt == CIR_F16; }
 // free_slots[head + upto_b - need_b + p - ceil(lens[b] / P)], so no workgroup reads an entry
 // that another writes, and every workgroup runs the scan over the rows by itself and then
 // takes its span of the tokens (the first token of a new page also writes the table entry).
-// Bound by latency: three dependent loads (lengths; table entry or free slot) and two
-// block scans of kRows rows each.
+// Bound by latency: three dependent loads (lengths; table entry or free slot) and a block
+// scan of kRows rows.  Sums saturate at kCap, above any max_tokens or free_total, so 32 bits
+// hold them (64-bit sums and divisions made 128 rows of a token each 8.3 us instead of 4.3).
 constexpr int kRows = 256;     // rows per scan = threads
 constexpr int kSpan = 1024;    // tokens per workgroup
 constexpr int kFill = 1;       // write tables, positions, slots, offsets and granted
 constexpr int kAdvance = 2;    // write seq_lens_out and free_head_out
+constexpr uint32_t kCap = 1u << 30;
 
-// Inclusive sum over the workgroup; the last thread's value is the total.
-__device__ __forceinline__ long block_scan(long v, long* scratch) {
+__device__ __forceinline__ uint32_t sat_add(uint32_t a, uint32_t b) { return min(a + b, kCap); }  // (each <= kCap)
+
+// Inclusive saturating sum over the workgroup, from `before` on; the last thread's value is the total.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t before, uint32_t* scratch) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-    const long o = __shfl_up(v, off, 64);
-    v += lane >= off ? o : 0;
+    const uint32_t o = __shfl_up(v, off, 64);
+    v = sat_add(v, lane >= off ? o : 0);
   }
   if (lane == 63) scratch[wave] = v;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) v += scratch[w];
-  __syncthreads();
-  return v;
+#pragma unroll
+  for (int w = 0; w < kRows / 64; ++w) before = sat_add(before, w < wave ? scratch[w] : 0);
+  return sat_add(v, before);
 }
+__device__ __forceinline__ uint32_t pages_of(uint32_t tokens, uint32_t P) { return tokens / P + (tokens % P ? 1 : 0); }
 
 __global__ __launch_bounds__(kRows) void extend_tables_kernel(
     int32_t* table, const int32_t* lens, const int32_t* news, const int32_t* __restrict__ free_slots, int free_total,
     const int32_t* head_in, int32_t* lens_out, int32_t* head_out, int32_t* __restrict__ offsets,
     int32_t* __restrict__ granted, int32_t* __restrict__ positions, int64_t* __restrict__ slot_map, int batch,
     int max_pages, int P, int max_tokens, int what) {
-  __shared__ long sm_scan[kRows / 64];
-  __shared__ long sm_end[kRows];   // tokens up to and with the row
-  __shared__ int sm_len[kRows], sm_new[kRows], sm_ok[kRows];
-  __shared__ long sm_from[kRows];  // free_slots index of the row's page 0, were it new
-  __shared__ long sm_total[2];
+  __shared__ uint32_t sm_tok[kRows / 64], sm_pag[kRows / 64];
+  __shared__ uint32_t sm_end[kRows];  // tokens up to and with the row
+  __shared__ uint32_t sm_len[kRows], sm_old[kRows];  // sm_old: pages held
+  __shared__ int sm_from[kRows];      // free_slots index of the row's page 0, were it new; kNone: not granted
+  __shared__ uint32_t sm_total[2];
+  constexpr int kNone = INT_MIN;
   const int t = threadIdx.x;
   const bool first = blockIdx.x == 0;
-  const long head = head_in[0];
-  const long span0 = (long)blockIdx.x * kSpan, span1 = min(span0 + kSpan, (long)max_tokens);
-  long tokens = 0, pages = 0, used = 0;  // of the rows before this chunk; `used`: pages handed out
+  const int head = head_in[0];
+  const uint32_t room = head >= 0 && head < free_total ? free_total - head : 0;  // free slots left
+  const uint32_t span0 = blockIdx.x * (uint32_t)kSpan, span1 = min(span0 + kSpan, (uint32_t)max_tokens);
+  uint32_t tokens = 0, pages = 0, used = 0;  // of the rows before this chunk; `used`: pages handed out
   for (int r0 = 0; r0 < batch; r0 += kRows) {  // uniform
     const int r = r0 + t;
     const bool in = r < batch;
-    const int len = in ? max(lens[r], 0) : 0, add = in ? max(news[r], 0) : 0;
-    const long have = (len + (long)P - 1) / P, want = ((long)len + add + P - 1) / P;
-    const long end = tokens + block_scan(add, sm_scan);
-    const bool fits = want <= max_pages && end <= max_tokens && (long)len + add <= INT_MAX;
-    const long need = fits ? want - have : 0;
-    const long upto = pages + block_scan(need, sm_scan);
-    const bool ok = fits && (need == 0 || (head >= 0 && head + upto <= free_total));
+    const uint32_t len = in ? max(lens[r], 0) : 0, add = in ? max(news[r], 0) : 0;
+    const uint32_t have = pages_of(len, P), want = pages_of(len + add, P);  // (len + add < 2^32)
+    const uint32_t end = block_scan(min(add, kCap), tokens, sm_tok);
+    const bool fits = want <= (uint32_t)max_pages && end <= (uint32_t)max_tokens && len + add <= (uint32_t)INT_MAX;
+    const uint32_t need = fits ? want - have : 0;
+    const uint32_t upto = block_scan(need, pages, sm_pag);
+    const bool ok = fits && (need == 0 || upto <= room);
     sm_end[t] = end;
     sm_len[t] = len;
-    sm_new[t] = add;
-    sm_ok[t] = ok;
-    sm_from[t] = head + upto - need - have;
+    sm_old[t] = have;
+    sm_from[t] = ok ? head + (int)(upto - need) - (int)have : kNone;
     if (t == kRows - 1) {
       sm_total[0] = end;
       sm_total[1] = upto;
@@ -80,32 +86,29 @@ __global__ __launch_bounds__(kRows) void extend_tables_kernel(
     used = (ok && need > 0) ? upto : used;
     if (first && in) {
       if (what & kFill) {
-        offsets[r + 1] = (int)min(end, (long)INT_MAX);
+        offsets[r + 1] = (int)end;
         granted[r] = ok ? add : 0;
       }
-      if (what & kAdvance) lens_out[r] = len + (ok ? add : 0);
+      if (what & kAdvance) lens_out[r] = (int)(len + (ok ? add : 0));
     }
     __syncthreads();
     if (what & kFill) {
-      const long lo = max(span0, tokens), hi = min(span1, sm_total[0]);
-      for (long j = lo + t; j < hi; j += kRows) {
-        int a = 0, b = kRows - 1;  // first row whose end lies past j
-        while (a < b) {
-          const int m = (a + b) >> 1;
-          if (sm_end[m] > j) b = m;
-          else a = m + 1;
-        }
-        const long pos = sm_len[a] + (j - (sm_end[a] - sm_new[a]));
-        const int page = (int)(pos / P), off = (int)(pos - (long)page * P);
-        const int old = (int)((sm_len[a] + (long)P - 1) / P);
+      const uint32_t lo = max(span0, tokens), hi = min(span1, sm_total[0]);
+      for (uint32_t j = lo + t; j < hi; j += kRows) {
+        int a = 0;  // first row whose end lies past j
+#pragma unroll
+        for (int step = kRows / 2; step > 0; step >>= 1) a += sm_end[a + step - 1] <= j ? step : 0;
+        const uint32_t pos = sm_len[a] + (j - (a ? sm_end[a - 1] : tokens));
+        const uint32_t page = pos / (uint32_t)P, off = pos - page * P;
+        const int from = sm_from[a];
         int64_t slot = -1;
-        if (sm_ok[a]) {
+        if (from != kNone) {
           int32_t* entry = table + (size_t)(r0 + a) * max_pages + page;
-          const int s = page < old ? *entry : free_slots[sm_from[a] + page];
-          if (page >= old && off == 0) *entry = s;
+          const int s = page < sm_old[a] ? *entry : free_slots[from + (int)page];
+          if (page >= sm_old[a] && off == 0) *entry = s;
           slot = (int64_t)s * P + off;
         }
-        positions[j] = (int)min(pos, (long)INT_MAX);
+        positions[j] = (int)min(pos, (uint32_t)INT_MAX);
         slot_map[j] = slot;
       }
     }
@@ -114,18 +117,21 @@ __global__ __launch_bounds__(kRows) void extend_tables_kernel(
     __syncthreads();  // the next chunk writes the same arrays
   }
   if (what & kFill) {  // tokens past the last row's
-    for (long j = max(span0, tokens) + t; j < span1; j += kRows) {
+    for (uint32_t j = max(span0, tokens) + t; j < span1; j += kRows) {
       positions[j] = 0;
       slot_map[j] = -1;
     }
     if (first && t == 0) offsets[0] = 0;
   }
   if ((what & kAdvance) && first) {
-    sm_end[t] = used;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) used = max(used, (uint32_t)__shfl_xor(used, off, 64));
+    if ((t & 63) == 0) sm_tok[t >> 6] = used;
     __syncthreads();
     if (t == 0) {
-      for (int i = 1; i < kRows; ++i) used = max(used, sm_end[i]);
-      head_out[0] = (int)(head + used);
+#pragma unroll
+      for (int w = 1; w < kRows / 64; ++w) used = max(used, sm_tok[w]);
+      head_out[0] = head + (int)used;
     }
   }
 }
@@ -268,6 +274,7 @@ extern "C" int cir_extend_page_tables(int32_t* page_table, const int32_t* seq_le
                                       int max_pages, int page_size, int max_tokens, void* stream) {
   CIR_CHECK_ARG(batch >= 0 && max_tokens >= 0 && free_total >= 0, "extend_page_tables: bad sizes");
   CIR_CHECK_ARG(page_size > 0 && max_pages > 0, "extend_page_tables: page_size and max_pages must be positive");
+  CIR_CHECK_ARG(max_tokens < (int)kCap && free_total < (int)kCap, "extend_page_tables: 2^30 tokens or free slots");
   // (no rows: the slot map is still filled with -1)
   CIR_CHECK_ARG((page_table && seq_lens && new_tokens && seq_lens_out && granted) || batch == 0,
                 "extend_page_tables: null pointer");

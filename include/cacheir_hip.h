@@ -366,7 +366,8 @@ int cir_token_logprobs(const void* logits, int dt, int64_t ld, const int64_t* id
  *                       than max_pages, its tokens end past max_tokens, or the free slots ran
  *                       out at it or at a row before it (a row that needs no page is served)
  *   seq_lens_out[b]     seq_lens[b] + granted[b];  free_head_out[0] = free_head[0] + pages taken
- *   offsets[0 .. batch] where each row's new tokens begin (a sum over new_tokens, granted or not)
+ *   offsets[0 .. batch] where each row's new tokens begin (a sum over new_tokens, granted or not;
+ *                       sums stay at 2^30 from there on; max_tokens and free_total are below)
  *   positions[j], slot_map[j], j < max_tokens: position of token j in its sequence and its place
  *                       in the pools, page_table[b][position / page_size] * page_size +
  *                       position % page_size (-1 for tokens of a row that was not granted and,

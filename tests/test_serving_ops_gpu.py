@@ -270,7 +270,7 @@ def tables_ref(table, lens, new, free, head, psize, max_tokens):
     for b, n in enumerate(new.tolist()):
         n = max(n, 0)
         at = offsets[-1]
-        offsets.append(at + n)
+        offsets.append(min(at + n, 2 ** 30))
         have, want = -(-lens[b] // psize), -(-(lens[b] + n) // psize)
         ok = want <= table.shape[1] and at + n <= max_tokens
         if ok and want > have:
@@ -280,12 +280,11 @@ def tables_ref(table, lens, new, free, head, psize, max_tokens):
             for i in range(have, want):
                 table[b, i] = free[head]
                 head += 1
-        for j in range(n):
-            if at + j < max_tokens:
-                p = lens[b] + j
-                positions[at + j] = p
-                if ok:
-                    slots[at + j] = int(table[b, p // psize]) * psize + p % psize
+        for j in range(min(n, max_tokens - at)):
+            p = lens[b] + j
+            positions[at + j] = p
+            if ok:
+                slots[at + j] = int(table[b, p // psize]) * psize + p % psize
         granted.append(n if ok else 0)
         lens[b] += granted[-1]
     i32 = lambda v: torch.tensor(v, dtype=torch.int32)
@@ -296,7 +295,7 @@ def tables_ref(table, lens, new, free, head, psize, max_tokens):
 def tables_case(seed, lens, new, psize=16, width=None, spare=4, taken=2):
     rng = np.random.default_rng(seed)
     have = [-(-n // psize) for n in lens]
-    need = sum(max(0, -(-(n + max(a, 0)) // psize) - h) for n, a, h in zip(lens, new, have))
+    need = sum(max(0, -(-(n + max(a, 0)) // psize) - h) for n, a, h in zip(lens, new, have) if a < 10 ** 6)
     width = width or max([1] + [-(-(n + max(a, 0)) // psize) for n, a in zip(lens, new)])
     perm = rng.permutation(sum(have) + taken + need + max(spare, 0)).astype(np.int32)
     table = np.full((len(lens), width), 77777, dtype=np.int32)
@@ -332,6 +331,7 @@ def check_tables(case, device, psize, max_tokens):
     ([30, 0, 16], [40, 500, 1], 16, 5, 4, 0),                 # a row too long for its table
     ([3, 4, 5], [10, 10, 10], 16, None, 4, -11),              # the map ends inside a row
     ([3, 9], [7, 7], 1, None, 2, 0),
+    ([3, 9], [7, 2 ** 31 - 5], 16, 9, 2, 30 - 2 ** 31),       # a count no 32-bit sum or table holds
 ])
 def test_page_tables(device, lens, new, psize, width, spare, slack):
     case = tables_case(len(lens), lens, new, psize, width, spare)

@@ -61,6 +61,10 @@ __device__ __forceinline__ rsrc_t make_rsrc(const void* p, uint32_t bytes) {
 __device__ __forceinline__ void buf16_to_lds(rsrc_t r, uint8_t* lds, uint32_t voff, uint32_t soff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, voff, soff, 0, 0);
 }
+// The same for data that is read once: a non-temporal load, which leaves the caches to what is read again.
+__device__ __forceinline__ void buf16_to_lds_once(rsrc_t r, uint8_t* lds, uint32_t voff, uint32_t soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, voff, soff, 0, 2);
+}
 
 // Wavefront (64-lane) reductions through DPP/swizzle-backed shuffles.
 __device__ __forceinline__ float wave_sum(float v) {

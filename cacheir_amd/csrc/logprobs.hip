@@ -38,6 +38,9 @@ constexpr int kPicks = 128;       // cells of a wavefront that are read again
 constexpr int kKeys = 256;        // keys a wavefront gathers
 constexpr int kAhead = 8;         // values per lane that are read again at once
 constexpr int kMinChunk = 4096;   // logits of a workgroup that shares its row with others
+// Logits that the last cache cannot hold are read past it (1021 x 152064 fp16 66.9 -> 62.5 us; 32 x 128256, which a
+// product has just written, 14.6 -> 15.4).
+constexpr size_t kCacheBytes = (size_t)256 << 20;
 constexpr int kManyRows = 1024;   // rows of one wavefront each, where they are short
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // 2^-300 is zero in fp32: y below it adds nothing, and 0 * y stays 0 for x = -inf.
@@ -237,8 +240,8 @@ __device__ __forceinline__ void finish(const Out& o, int64_t row, const Stats& a
 
 // WPR wavefronts per row: four, one workgroup per (row, split), grid x = row * S + split; or one, four rows per
 // workgroup (S = 1).  U vectors per lane and group; ONE: every wavefront's share is one group (what may enter the list
-// is then taken from registers).
-template <typename T, bool TOP, int WPR, int U, bool ONE>
+// is then taken from registers); ONCE: non-temporal loads.
+template <typename T, bool TOP, int WPR, int U, bool ONE, bool ONCE>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict__ logits, int64_t ld,
                                                             const int64_t* __restrict__ ids, int rows, int vocab, int K,
                                                             int S, Out out, float* __restrict__ part,
@@ -276,7 +279,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = base + u * 64 * WPR + lane;
-      if (i < v1) w[u] = xv[i];
+      if (i < v1) w[u] = ONCE ? __builtin_nontemporal_load(xv + i) : xv[i];
       else
 #pragma unroll
         for (int e = 0; e < N; ++e) w[u][e] = (T)-INFINITY;
@@ -545,18 +548,20 @@ extern "C" int cir_token_logprobs(const void* logits, int dt, int64_t ld, const 
   const auto go = [&]<typename T, bool TOP>() {
     const T* x = static_cast<const T*>(logits);
     constexpr int kGroup = 64 * 4 * Words<T>::kN;  // logits of a wavefront's group
-    const auto run = [&]<int WPR, int U, bool ONE>() {
-      logprobs_kernel<T, TOP, WPR, U, ONE><<<WPR == 1 ? (unsigned)((rows + kWaves - 1) / kWaves) : (unsigned)(rows * S),
-                                             kThreads, 0, s>>>(x, ld, ids, rows, vocab, top_k, S, out, part, part_top);
+    const auto run = [&]<int WPR, int U, bool ONE, bool ONCE>() {
+      const unsigned wgs = WPR == 1 ? (unsigned)((rows + kWaves - 1) / kWaves) : (unsigned)(rows * S);
+      logprobs_kernel<T, TOP, WPR, U, ONE, ONCE><<<wgs, kThreads, 0, s>>>(x, ld, ids, rows, vocab, top_k, S, out, part,
+                                                                          part_top);
     };
     if (rows >= kManyRows && vocab <= 4 * kGroup) {
-      if (vocab <= kGroup / 4) run.template operator()<1, 1, true>();
-      else if (vocab <= kGroup) run.template operator()<1, 4, true>();
-      else run.template operator()<1, 4, false>();
+      if (vocab <= kGroup / 4) run.template operator()<1, 1, true, false>();
+      else if (vocab <= kGroup) run.template operator()<1, 4, true, false>();
+      else run.template operator()<1, 4, false, false>();
       return launch_status();
     }
-    if (((vocab / Words<T>::kN + S - 1) / S) <= 64 * 4 * kWaves) run.template operator()<kWaves, 4, true>();
-    else run.template operator()<kWaves, 4, false>();
+    if (((vocab / Words<T>::kN + S - 1) / S) <= 64 * 4 * kWaves) run.template operator()<kWaves, 4, true, false>();
+    else if ((size_t)rows * vocab * sizeof(T) < kCacheBytes) run.template operator()<kWaves, 4, false, false>();
+    else run.template operator()<kWaves, 4, false, true>();
     const int st = launch_status();
     if (st || S == 1) return st;
     logprobs_merge<T, TOP><<<rows, 64, 0, s>>>(x, ld, ids, vocab, top_k, S, out, part, part_top);

@@ -23,7 +23,8 @@
 //   * piece_stream, up to 32 query vectors: bound by the read of K and V.  Each wavefront
 //     walks blocks of its own (every 4th) and stages them by DMA in LDS of its own: no
 //     barriers, K of the next block is on its way once this block's K is in registers, and
-//     V likewise, so a CU has 64 to 128 KiB in flight.
+//     V likewise, so a CU has 64 to 128 KiB in flight.  The loads are non-temporal (128 rows
+//     of 64 to 7168 tokens, 28/4 heads: 180 -> 158 us, 6.0 TB/s).
 //   * piece_tile, up to 128 vectors: bound by the matrix cores and the softmax.  Each
 //     wavefront takes 32 vectors; stages of 64 tokens of K and V go through LDS for all.
 // P is rounded to fp16 for the second product (relative 2^-11 of a weight) and l sums the
@@ -154,9 +155,12 @@ __device__ __forceinline__ void soft_step(Soft& a, f32x16 (&c)[NB], float sc, f1
   for (int j = 0; j < NB; ++j) {
     ps[j] = 0.f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      pa[j][r >> 3][r & 7] = static_cast<f16>(__builtin_amdgcn_exp2f(fmaf(c[j][r], pc, -ms)));
-      ps[j] += static_cast<float>(pa[j][r >> 3][r & 7]);
+    for (int r = 0; r < 16; r += 2) {
+      const f16x2 two = {static_cast<f16>(__builtin_amdgcn_exp2f(fmaf(c[j][r], pc, -ms))),
+                         static_cast<f16>(__builtin_amdgcn_exp2f(fmaf(c[j][r + 1], pc, -ms)))};
+      pa[j][r >> 3][r & 7] = two.x;
+      pa[j][r >> 3][(r & 7) + 1] = two.y;
+      ps[j] = __builtin_amdgcn_fdot2(two, f16x2{(f16)1.f, (f16)1.f}, ps[j], false);  // exact products, fp32 sum
     }
   }
 }
@@ -235,7 +239,7 @@ __device__ __forceinline__ void piece_stream(const Args& A, const Piece& p, uint
       for (int u = 0; u < 4; ++u) {
         uint32_t off = at[u];
         if (end < 15) off = off - max(0, 4 * u + lr - end) * kRowB;  // uniform
-        buf16_to_lds(r, buf + (16 * j + 4 * u) * kRowB, off, 0);
+        buf16_to_lds_once(r, buf + (16 * j + 4 * u) * kRowB, off, 0);
       }
     }
   };

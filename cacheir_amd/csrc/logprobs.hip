@@ -508,6 +508,9 @@ __global__ __launch_bounds__(64) void logprobs_merge(const T* __restrict__ logit
   finish<T>(out, row, a, top, TOP ? K : 0, x, known, lane);
 }
 
+template <typename T>
+constexpr int kGroupOf = 64 * 4 * Words<T>::kN;  // logits of a wavefront's group
+
 // Workgroups that share a row: enough for two per CU, each with kMinChunk logits at least.
 int row_splits(int rows, int vocab) {
   const int fill = 512 / max(1, min(rows, 512)), most = max(1, vocab / kMinChunk);
@@ -540,20 +543,22 @@ extern "C" int cir_token_logprobs(const void* logits, int dt, int64_t ld, const 
   const size_t need = cir_token_logprobs_workspace_bytes(rows, vocab, top_k);
   CIR_CHECK_ARG((workspace || need == 0) && workspace_bytes >= need && (uintptr_t)workspace % 8 == 0,
                 "token_logprobs: workspace too small or not on 8 bytes (%zu < %zu)", workspace_bytes, need);
-  CIR_CHECK_ARG((long)rows * S < (1L << 31), "token_logprobs: grid too large");
+  const bool many = rows >= kManyRows && vocab <= 4 * (dt == CIR_F16 ? kGroupOf<f16> : kGroupOf<float>);
+  CIR_CHECK_ARG((many ? ((long)rows + kWaves - 1) / kWaves : (long)rows * S) * kThreads < (1L << 32),
+                "token_logprobs: %d rows are too many for a launch", rows);
   hipStream_t s = as_stream(stream);
   const Out out{ids ? logprobs : nullptr, entropy, top_ids, top_logprobs};
   u64* part_top = static_cast<u64*>(workspace);
   float* part = reinterpret_cast<float*>(part_top + (size_t)rows * S * top_k);
   const auto go = [&]<typename T, bool TOP>() {
     const T* x = static_cast<const T*>(logits);
-    constexpr int kGroup = 64 * 4 * Words<T>::kN;  // logits of a wavefront's group
+    constexpr int kGroup = kGroupOf<T>;
     const auto run = [&]<int WPR, int U, bool ONE, bool ONCE>() {
-      const unsigned wgs = WPR == 1 ? (unsigned)((rows + kWaves - 1) / kWaves) : (unsigned)(rows * S);
+      const unsigned wgs = WPR == 1 ? (unsigned)(((long)rows + kWaves - 1) / kWaves) : (unsigned)(rows * S);
       logprobs_kernel<T, TOP, WPR, U, ONE, ONCE><<<wgs, kThreads, 0, s>>>(x, ld, ids, rows, vocab, top_k, S, out, part,
                                                                           part_top);
     };
-    if (rows >= kManyRows && vocab <= 4 * kGroup) {
+    if (many) {
       if (vocab <= kGroup / 4) run.template operator()<1, 1, true, false>();
       else if (vocab <= kGroup) run.template operator()<1, 4, true, false>();
       else run.template operator()<1, 4, false, false>();

@@ -50,6 +50,7 @@ constexpr int kItemCost = 6;
 constexpr int kMinStretch = 8;
 constexpr int kMaxPrefixes = 256;  // groups: one per thread
 constexpr int kMaxRows = 2048;
+constexpr long kMaxVectors = 1L << 27;  // of the batch: the join's threads stay below 2^32
 constexpr int kRowB = 2 * D;      // bytes of a K or V row
 
 // Workspace: one record per row, then the pieces.
@@ -747,7 +748,8 @@ bool shares(int B, int NG, int Hq, int Hkv, int head_dim, int P, int max_pages, 
   const long items = (long)B * G / kTileVec + NG + B;
   // (page_index is exact while (tokens / 16) (P / 16) < 2^32)
   return kv_dtype == CIR_F16 && head_dim == D && P % 16 == 0 && (long)max_pages * P / 16 * (P / 16) < (1L << 32) &&
-         G <= kVec && NG <= kMaxPrefixes && B <= kMaxRows && per_item < (1L << 31) && per_item * items < (1L << (31 - kPlace));
+         G <= kVec && NG <= kMaxPrefixes && B <= kMaxRows && (long)B * Hq < kMaxVectors && per_item < (1L << 31) &&
+         per_item * items < (1L << (31 - kPlace));
 }
 
 }  // namespace
@@ -783,9 +785,9 @@ extern "C" int cir_paged_decode_attention_shared(const void* q, const void* k_po
   CIR_CHECK_ARG(page_size > 0 && max_pages > 0 && (long)page_size * max_pages <= 0x7fffffffL,
                 "attention_shared: page_size and max_pages must be positive, and their product a 32-bit number");
   CIR_CHECK_ARG(kv_dtype == CIR_F16 || kv_dtype == CIR_F32, "attention_shared: kv_dtype must be CIR_F16 or CIR_F32");
-  // DMA takes 16-byte groups of the pools.
+  // DMA takes 16-byte groups of the pools; q is read by 16 bytes, out written by 8.
   if (!shares(batch, groups, num_heads, num_kv_heads, head_dim, page_size, max_pages, kv_dtype) ||
-      ((uintptr_t)k_pool | (uintptr_t)v_pool) % 16)
+      ((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool) % 16 || (uintptr_t)out % 8)
     return cir_paged_decode_attention(q, k_pool, v_pool, page_table, seq_lens, out, workspace, workspace_bytes, batch,
                                       num_heads, num_kv_heads, head_dim, page_size, max_pages, scale, kv_dtype, stream);
   const Layout l = layout(batch, groups, num_heads, num_kv_heads);

@@ -145,6 +145,8 @@ __global__ __launch_bounds__(kRows) void extend_tables_kernel(
 constexpr int kRopeThreads = 256;
 constexpr int kMaxDim = 256;
 constexpr int kTokens = 4;
+constexpr int kMaxTokens = 1 << 26;  // (a grid has fewer than 2^32 threads)
+constexpr int kMaxHeads = 1 << 20;
 
 template <typename T, int N>
 struct Vec {
@@ -312,10 +314,20 @@ extern "C" int cir_rope_append(const void* q, int64_t q_token_stride, int64_t q_
                 "rope_append: rotary_dim %d must be even and at most head_dim", rotary_dim);
   CIR_CHECK_ARG(tokens >= 0 && num_heads >= 0 && num_kv_heads > 0 && page_size > 0 && slots >= 0,
                 "rope_append: bad sizes");
+  CIR_CHECK_ARG(tokens <= kMaxTokens && num_heads <= kMaxHeads && num_kv_heads <= kMaxHeads,
+                "rope_append: more than 2^26 tokens or 2^20 heads");
   if (tokens == 0) return 0;
   CIR_CHECK_ARG((num_heads == 0 || (q && q_out)) && k && v && positions && slot_map && k_pool && v_pool &&
                     (inv_freq || rotary_dim == 0),
                 "rope_append: null pointer");
+  // Written heads that overlap, or q in place at other strides, would be read and written by different threads.
+  const auto apart = [&](int64_t stride, int n) { return n <= 1 || stride >= head_dim || stride <= -head_dim; };
+  CIR_CHECK_ARG(num_heads == 0 || (apart(o_token_stride, tokens) && apart(o_head_stride, num_heads)),
+                "rope_append: heads of q_out overlap");
+  CIR_CHECK_ARG(num_heads == 0 || q_out != q ||
+                    ((tokens == 1 || o_token_stride == q_token_stride) &&
+                     (num_heads == 1 || o_head_stride == q_head_stride)),
+                "rope_append: q_out is q with other strides");
   hipStream_t s = as_stream(stream);
   const RopeIn in{q, k, v, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride,
                   o_token_stride, o_head_stride};

@@ -172,6 +172,18 @@ def test_shared_attention_pools_off_16_bytes(device):
     check_shared(case, kernels.paged_decode_attention_shared(**dev))
 
 
+def test_shared_attention_q_and_out_off_their_alignment(device):
+    """q off 16 bytes or out off 8 (the rows of a larger buffer): each row alone."""
+    case = shared_case(7, [(3, 96)], [1, 20, 17], 8, 2)
+    dev = {k: v.to(device) for k, v in case.items()}
+    from cacheir_amd import kernels
+
+    raw = torch.empty(dev["q"].numel() + 4, dtype=torch.float16, device=device)
+    check_shared(case, kernels.paged_decode_attention_shared(**(dev | {"q": raw[4:].view(dev["q"].shape).copy_(dev["q"])})))
+    raw = torch.empty(dev["q"].numel() + 2, dtype=torch.float16, device=device)
+    check_shared(case, kernels.paged_decode_attention_shared(**dev, out=raw[2:].view(dev["q"].shape)))
+
+
 def test_shared_attention_scores_at_the_limits(device):
     """Scores past 2^24, keys that make every score -inf (NaN), and infinities behind the last token (which stay out)."""
     case = shared_case(8, [(5, 128), (2, 0)], [5, 1, 40, 33, 70, 20, 64], 8, 2)

@@ -1,0 +1,160 @@
+"""Sizes and refusals of the serving operators' entry points that the host decides (no GPU calls)."""
+import math
+
+import pytest
+import torch
+
+from cacheir_amd import hip, kernels
+
+pytestmark = pytest.mark.skipif(not hip.library_path().exists(), reason="libcacheir_hip.so not built")
+
+F16, F32 = hip.CIR_F16, hip.CIR_F32
+
+
+def refuses(name, match, *args):
+    with pytest.raises(RuntimeError, match=match):
+        hip.call(name, *args)
+
+
+@pytest.mark.parametrize("batch,groups,hq,hkv", [(1, 0, 8, 8), (3, 1, 28, 4), (128, 16, 32, 8), (2048, 256, 32, 1)])
+def test_shared_attention_workspace(batch, groups, hq, hkv):
+    """Room for both paths (the pools' addresses, which a size query does not see, decide between them): at least the
+    plain decode's, and fp32 (m, l, O) of every row's own piece and of a 128-vector prefix tile per group."""
+    size = hip.size_call("cir_shared_attention_workspace_bytes", batch, groups, hq, hkv, 128, 16, 64, F16)
+    assert size >= hip.size_call("cir_paged_attention_workspace_bytes", batch, hq, 128, 1024)
+    assert size >= 4 * 130 * (batch * hq + groups * hkv * 128)
+    for plain in ((64, 16, F16), (128, 16, F32), (128, 8, F16)):  # sizes that read each row alone
+        d, page, dt = plain
+        assert (hip.size_call("cir_shared_attention_workspace_bytes", batch, groups, hq, hkv, d, page, 64, dt)
+                == hip.size_call("cir_paged_attention_workspace_bytes", batch, hq, d, 64 * page))
+
+
+@pytest.mark.parametrize("bad", [(0, 1, 8, 2, 128, 16, 4), (2, -1, 8, 2, 128, 16, 4), (2, 1, 7, 2, 128, 16, 4),
+                                 (2, 1, 8, 0, 128, 16, 4), (2, 1, 8, 2, 0, 16, 4), (2, 1, 8, 2, 128, 0, 4),
+                                 (2, 1, 8, 2, 128, 16, 0), (2, 1, 8, 2, 128, 1 << 16, 1 << 16)])
+def test_shared_attention_workspace_of_bad_sizes(bad):
+    assert hip.size_call("cir_shared_attention_workspace_bytes", *bad, F16) == 0
+
+
+def test_shared_attention_refusals():
+    def call(match, groups=1, batch=2, hq=8, hkv=2, d=128, page=16, pages=4, dt=F16, p=None):
+        refuses("cir_paged_decode_attention_shared", match, p, p, p, p, p, None, None, groups, p, None, 0, batch, hq, hkv,
+                d, page, pages, 1.0, dt, None)
+
+    p = torch.zeros(64).data_ptr()
+    call("batch and groups", groups=-1)
+    call("batch and groups", batch=-1)
+    call("null pointer")
+    call("null group_rows", p=p)
+    call("multiple of num_kv_heads", groups=0, hq=7, p=p)
+    call("head_dim 257", groups=0, d=257, p=p)
+    call("32-bit", groups=0, page=1 << 16, pages=1 << 16, p=p)
+    call("kv_dtype", groups=0, dt=7, p=p)
+    call("workspace too small", groups=0, p=p)
+    hip.call("cir_paged_decode_attention_shared", *[None] * 7, 0, None, None, 0, 0, 8, 2, 128, 16, 4, 1.0, F16, None)
+
+
+def test_page_tables_refusals():
+    def call(match, free_total=4, batch=2, pages=4, page=16, tokens=8, p=None):
+        refuses("cir_extend_page_tables", match, p, p, p, p, free_total, p, p, p, p, p, p, p, batch, pages, page, tokens,
+                None)
+
+    call("bad sizes", batch=-1)
+    call("bad sizes", tokens=-1)
+    call("bad sizes", free_total=-1)
+    call("must be positive", page=0)
+    call("must be positive", pages=0)
+    call(r"2\^30", tokens=1 << 30)
+    call(r"2\^30", free_total=1 << 30)
+    call("null pointer")
+    call("null pointer", batch=0)
+
+
+def rope(tokens=2, heads=2, kv_heads=1, d=8, rot=8, layout=0, dt=F32, kvdt=F32, page=4, slots=16, q=(16, 8), o=(16, 8), p=None,
+         out=None):
+    hip.call("cir_rope_append", p, *q, p, 8, 8, p, 8, 8, dt, p, p, p, 1.0, rot, layout, out or p, *o, p, p, kvdt, slots,
+             tokens, heads, kv_heads, d, page, None)
+
+
+@pytest.mark.parametrize("match,kw", [
+    ("bad dtype", dict(dt=9)), ("bad dtype", dict(kvdt=9)), ("bad layout", dict(layout=2)), ("head_dim 7", dict(d=7)),
+    ("head_dim 258", dict(d=258)), ("rotary_dim 10", dict(rot=10)), ("rotary_dim 3", dict(rot=3)),
+    ("bad sizes", dict(tokens=-1)), ("bad sizes", dict(kv_heads=0)), ("bad sizes", dict(page=0)),
+    ("bad sizes", dict(slots=-1)), (r"2\^26", dict(tokens=(1 << 26) + 1)), (r"2\^20", dict(heads=(1 << 20) + 1)),
+    ("null pointer", {})])
+def test_rope_refusals(match, kw):
+    with pytest.raises(RuntimeError, match=match):
+        rope(**kw)
+
+
+def test_rope_refuses_outputs_that_overlap():
+    """Tokens or heads of q_out on one another (an expanded tensor), and q in place as a view with other strides."""
+    x, y = torch.zeros(64), torch.zeros(64)
+    for o in ((0, 8), (16, 0), (16, 4), (7, 8)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            rope(p=x.data_ptr(), out=y.data_ptr(), o=o)
+    with pytest.raises(RuntimeError, match="other strides"):
+        rope(p=x.data_ptr(), o=(8, 16))
+    rope(tokens=0)
+
+
+def test_logprobs_workspace():
+    """Nothing where a row has a workgroup of its own; 12 bytes of sums and top_k keys of 8 per split elsewhere."""
+    size = lambda *a: hip.size_call("cir_token_logprobs_workspace_bytes", *a)
+    assert size(512, 128256, 20) == size(1, 1000, 5) == size(0, 1000, 5) == size(4, 0, 5) == size(4, 100, -1) == 0
+    one = size(3, 128256, 0)
+    assert one > 0 and one % (3 * 12) == 0
+    assert size(3, 128256, 20) == one // 12 * (12 + 160)
+
+
+def test_logprobs_refusals():
+    def call(match, dt=F16, ld=100, rows=2, vocab=100, k=5, p=None, ids=None):
+        refuses("cir_token_logprobs", match, p, dt, ld, ids, rows, vocab, k, None, p, p, p, None, 0, None)
+
+    p = torch.zeros(64).data_ptr()
+    call("bad dtype", dt=9)
+    call("bad sizes", rows=-1)
+    call("bad sizes", vocab=0, k=0)
+    call("bad sizes", ld=99)
+    call("top_k 65", k=65)
+    call("top_k 6", vocab=5, k=6)
+    call("top_k -1", k=-1)
+    call("null pointer")
+    call("null pointer", p=p, ids=p)
+    call("alignment", p=p + 1)
+    call("workspace too small", p=p, rows=3, vocab=128256, ld=128256)
+    call("too many", p=p, rows=1 << 26, vocab=5, ld=5)  # 2^24 workgroups of 256 threads
+    call("too many", p=p, rows=1 << 24, vocab=5000, ld=5000)
+    hip.call("cir_token_logprobs", None, F16, 100, None, 0, 100, 5, *[None] * 5, 0, None)
+
+
+def test_rope_frequencies_on_the_host():
+    f = kernels.rope_frequencies(8, 10000.0, device="cpu")
+    assert f.dtype == torch.float64 and torch.equal(f, 10000.0 ** (-torch.arange(4, dtype=torch.float64) / 4))
+    assert torch.equal(kernels.rope_frequencies(8, 10000.0, {"rope_type": "linear", "factor": 4}, "cpu"), f / 4)
+    assert kernels.rope_frequencies(0, 10000.0, device="cpu").numel() == 0
+    scaled = kernels.rope_frequencies(128, 500000.0, {
+        "rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+        "original_max_position_embeddings": 8192}, "cpu")
+    plain = kernels.rope_frequencies(128, 500000.0, device="cpu")
+    turns = plain * 8192 / (2 * math.pi)
+    assert torch.equal(scaled[turns > 4], plain[turns > 4]) and torch.equal(scaled[turns < 1], plain[turns < 1] / 8)
+    mid = (turns > 1) & (turns < 4)
+    assert bool(((scaled[mid] < plain[mid]) & (scaled[mid] > plain[mid] / 8)).all()) and bool(mid.any())
+    for bad in (dict(rotary_dim=3, theta=10000.0), dict(rotary_dim=8, theta=0.0),
+                dict(rotary_dim=8, theta=10000.0, scaling={"rope_type": "other"})):
+        with pytest.raises(ValueError):
+            kernels.rope_frequencies(**bad, device="cpu")
+
+
+def test_the_wrappers_refuse_host_tensors():
+    i32 = lambda *n: torch.zeros(n, dtype=torch.int32)
+    q, pool = torch.zeros(2, 8, 128, dtype=torch.float16), torch.zeros(4, 2, 16, 128, dtype=torch.float16)
+    with pytest.raises(ValueError, match="on the GPU"):
+        kernels.paged_decode_attention_shared(q, pool, pool, i32(2, 4), i32(2), i32(2), i32(1))
+    with pytest.raises(ValueError, match="on the GPU"):
+        kernels.extend_page_tables(i32(2, 4), i32(2), i32(2), i32(8), i32(1), page_size=16, max_tokens=2)
+    with pytest.raises(ValueError, match="on the GPU"):
+        kernels.rope_append(q, q[:, :2], q[:, :2], i32(2), i32(2).long(), torch.zeros(64, dtype=torch.float64), pool, pool)
+    with pytest.raises(ValueError, match="on the GPU"):
+        kernels.token_logprobs(torch.zeros(2, 100), torch.zeros(2, dtype=torch.int64))

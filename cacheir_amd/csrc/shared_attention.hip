@@ -25,8 +25,10 @@
 //     barriers, K of the next block is on its way once this block's K is in registers, and
 //     V likewise, so a CU has 64 to 128 KiB in flight.  The loads are non-temporal (128 rows
 //     of 64 to 7168 tokens, 28/4 heads: 180 -> 158 us, 6.0 TB/s).
-//   * piece_tile, up to 128 vectors: bound by the matrix cores and the softmax.  Each
-//     wavefront takes 32 vectors; stages of 64 tokens of K and V go through LDS for all.
+//   * piece_tile, up to 128 vectors: bound by the chain of a stage (LDS reads, products,
+//     softmax), which the second workgroup hides in part.  Each wavefront takes 32 vectors;
+//     stages of 64 tokens of K and V go through LDS for all.  64 rows after 32672 tokens,
+//     32/8 heads: 59 us, 576 TFLOP/s.
 // P is rounded to fp16 for the second product (relative 2^-11 of a weight) and l sums the
 // rounded values, so a row's weights still add up to one; everything else is fp32.
 #include "attn_tile.hpp"
@@ -44,13 +46,14 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kGroups = 512;      // workgroups, about: two per CU
 constexpr int kTileVec = 128;     // query vectors of a prefix tile
-// A piece's start and join in blocks, and the blocks per workgroup at least.  6 and 8 against 3 and 4, 28/4 heads: 64 rows
-// after 16000 tokens 55.6 -> 50.7 us, 32 after 8000 27.3 -> 25.7, 8 after 3000 19.3 -> 16.7; 4 rows 12.6 -> 12.8.
+// A piece's start and join in blocks (6 against 3, us: 64 rows after 16000 tokens 49.3 -> 47.9, 64 after 2048 22.3 -> 20.8,
+// 32 after 8000 24.5 -> 22.6), and the blocks per workgroup at least (one per wavefront; 4 against 8: 4 rows after 500
+// tokens 12.8 -> 11.8, 16 after 1000 16.8 -> 15.6, 8 after 3000 14.3 -> 15.6).
 constexpr int kItemCost = 6;
-constexpr int kMinStretch = 8;
+constexpr int kMinStretch = 4;
 constexpr int kMaxPrefixes = 256;  // groups: one per thread
 constexpr int kMaxRows = 2048;
-constexpr long kMaxVectors = 1L << 27;  // of the batch: the join's threads stay below 2^32
+constexpr long kMaxVectors = 1L << 26;  // of the batch: the join's threads stay below 2^32
 constexpr int kRowB = 2 * D;      // bytes of a K or V row
 
 // Workspace: one record per row, then the pieces.
@@ -128,14 +131,17 @@ __device__ __forceinline__ void soft_init(Soft& a) {
 }
 // Scores c (unscaled) of NB blocks -> p in fp16, the B operand of the second product, with the running max and the
 // accumulators moved; `ps` are the sums of p.  A vector that has seen no finite score keeps m = -inf and subtracts 0.
+// m follows the maximum only once some score lies more than 8 above it: p stays at 2^8 or less, which fp16 holds as
+// exactly as p <= 1, and after a piece's first blocks the 64 accumulators are hardly ever scaled (128 rows after 16384
+// shared tokens, 28/4 heads: 61 -> 57 us).  The two lanes of a vector compare their own halves of the scores.
 template <int NB>
 __device__ __forceinline__ void soft_step(Soft& a, f32x16 (&c)[NB], float sc, f16x8 (&pa)[NB][2], float (&ps)[NB]) {
   float mx = c[0][0];
 #pragma unroll
   for (int r = 1; r < 16 * NB; ++r) mx = fmaxf(mx, c[r >> 4][r & 15]);
-  mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * sc;
-  if (__builtin_amdgcn_ballot_w64(mx > a.m) != 0) {  // uniform
-    const float mn = fmaxf(a.m, mx);
+  mx *= sc;
+  if (__builtin_amdgcn_ballot_w64(mx > a.m + 8.f) != 0) {  // uniform
+    const float mn = fmaxf(a.m, fmaxf(mx, __shfl_xor(mx, 32, 64)));
     const float alpha = __builtin_amdgcn_exp2f(a.m - (mn == -INFINITY ? 0.f : mn));
     a.l *= alpha;
     a.m = mn;
@@ -406,7 +412,10 @@ __device__ __forceinline__ void piece_tile(const Args& A, const Piece& p, uint8_
     vo[i] = kHalf + (8 * i + 4 * h + (ti >> 2)) * kRowB +
             16 * ((2 * sub + ((ti & 3) >> 1)) ^ (2 * i + h)) + 8 * (ti & 1);
 
+  // The products run at a higher wave priority than the softmax: of the two wavefronts of a SIMD the one that feeds the
+  // matrix cores goes first (64 rows after 32672 tokens 64.5 -> 62.6 us).
   auto blocks = [&](const uint8_t* buf, int blk) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_setprio(1);
     f32x16 c[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
@@ -421,15 +430,18 @@ __device__ __forceinline__ void piece_tile(const Args& A, const Piece& p, uint8_
     }
     f16x8 va[NB][D / 32][2];
     load_vt(buf, vo, ti, va[0]);  // before the softmax, which hides the LDS latency
+    __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
     const bool both = blk + 1 < p.blk1;  // uniform
     if (!both) {
+      asm volatile("" : "+v"(c[1]));  // (stays a branch: 16 selects a stage otherwise)
 #pragma unroll
       for (int r = 0; r < 16; ++r) c[1][r] = -INFINITY;
     }
     f16x8 pa[NB][2];
     float ps[NB];
     soft_step<NB>(a, c, sc, pa, ps);
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       if (j > 0 && !both) break;  // uniform
@@ -449,6 +461,7 @@ __device__ __forceinline__ void piece_tile(const Args& A, const Piece& p, uint8_
       fetch(min(st + 2, nst - 1));
     }
     if (busy) blocks(cur, p.blk0 + st * NB);
+    __builtin_amdgcn_s_setprio(0);
   };
   fetch(0);
   issue(st0, 0);
@@ -648,23 +661,24 @@ __global__ __launch_bounds__(kThreads, 2) void attn_shared_f16_d128(
 }
 
 // out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i over the pieces of a query vector: those of its group's prefix, then
-// those of its own part, in order.  32 lanes per vector, four dims each; lane k takes (m, l) of every 32nd piece.  Bound
-// by latency (record, then pieces), so the first pieces' O are loaded along with their (m, l).
+// those of its own part.  Two half-wavefronts per vector, each with every second piece, four dims a lane; lane k takes
+// (m, l) of every 32nd piece.  Bound by latency (record, then pieces), so a half-wavefront has four O on their way, the
+// first ones along with the (m, l).  Half-wavefronts per vector, us of the whole call: 64 rows after 2048 tokens, 9
+// pieces a vector, 24.8 with one, 21.0 with two, 24.6 with four; 20 groups of 4 rows 31.4, 30.9, 32.7.
 // A row without tokens gives zeros; one whose scores are all -inf NaN, as a softmax over them does.
 __global__ __launch_bounds__(256) void attn_shared_join(Args A, f16* __restrict__ out) {
-  const int id = (int)((blockIdx.x * 256u + threadIdx.x) >> 5), lane = threadIdx.x & 31;
-  const int row = id / A.Hq;
-  if (row >= A.B) return;
-  const int head = id - row * A.Hq, G = A.Hq / A.Hkv;
+  constexpr int W = 2, U = 4, kVecs = 8 / W;
+  __shared__ f32x4 sm_o[kVecs][32];
+  const int part = threadIdx.x >> 5, lane = threadIdx.x & 31, s = part % W, vec = part / W;
+  const int id = blockIdx.x * kVecs + vec;
+  const bool live = id < A.B * A.Hq;
+  const int row = live ? id / A.Hq : 0;
+  const int head = live ? id - row * A.Hq : 0, G = A.Hq / A.Hkv;
   const int h = head / G, g = head - h * G;
   const RowRec rec = A.rows[row];
   const int v = rec.first + g, later = v / kTileVec != rec.first / kTileVec;
   const Pieces pre = later ? rec.prefix[1] : rec.prefix[0];
-  const int n = pre.count + rec.own.count;
-  if (n == 0) {
-    *reinterpret_cast<f16x4*>(out + (size_t)id * D + 4 * lane) = f16x4{0, 0, 0, 0};
-    return;
-  }
+  const int n = live ? pre.count + rec.own.count : 0;
   // Query vector `at` of piece k's slot: (m, l) and O.
   const size_t pre_at = ((size_t)pre.slot * A.Hkv + h) * kTileVec + v % kTileVec;
   const size_t own_at = ((size_t)rec.own.slot * A.Hkv + h) * G + g;
@@ -677,38 +691,49 @@ __global__ __launch_bounds__(256) void attn_shared_join(Args A, f16* __restrict_
   const auto o_of = [&](int k) {
     return *reinterpret_cast<const f32x4*>((k < pre.count ? A.pre_o : A.suf_o) + D * at(k) + 4 * lane);
   };
-  constexpr int U = 4;
-  float2 ml = lane < n ? ml_of(lane) : make_float2(-INFINITY, 0.f);
-  f32x4 x[U];
-#pragma unroll
-  for (int j = 0; j < U; ++j) x[j] = o_of(min(j, n - 1));
-  float M = ml.x;
-  for (int k = lane + 32; k < n; k += 32) M = fmaxf(M, ml_of(k).x);
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor(M, s, 32));
-  const float ms = M == -INFINITY ? 0.f : M;
   float den = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int k0 = 0; k0 < n; k0 += 32) {
-    if (k0) ml = k0 + lane < n ? ml_of(k0 + lane) : make_float2(-INFINITY, 0.f);
-    const float f = __builtin_amdgcn_exp2f(ml.x - ms);
-    den = fmaf(ml.y, f, den);
-    for (int j0 = k0; j0 < min(n, k0 + 32); j0 += U) {
+  if (n > 0) {
+    float2 ml = lane < n ? ml_of(lane) : make_float2(-INFINITY, 0.f);
+    f32x4 x[U];
+    const auto load = [&](int k0) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const float fj = __shfl(f, j0 + j - k0, 32);
-        if (j0 + j < n) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = fmaf(x[j][e], fj, o[e]);
-        }
+        const int k = k0 + s + W * j;
+        x[j] = o_of(min(k, n - 1));
       }
+    };
+    load(0);
+    float M = ml.x;
+    for (int k = lane + 32; k < n; k += 32) M = fmaxf(M, ml_of(k).x);
 #pragma unroll
-      for (int j = 0; j < U; ++j) x[j] = o_of(min(j0 + U + j, n - 1));
+    for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 32));
+    const float ms = M == -INFINITY ? 0.f : M;
+    for (int k0 = 0; k0 < n; k0 += 32) {
+      if (k0) ml = k0 + lane < n ? ml_of(k0 + lane) : make_float2(-INFINITY, 0.f);
+      const float f = __builtin_amdgcn_exp2f(ml.x - ms);
+      den = fmaf(ml.y, f, den);
+      for (int j0 = k0; j0 < min(n, k0 + 32); j0 += W * U) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+          const int k = j0 + s + W * j;
+          const float fk = __shfl(f, k - k0, 32);
+          if (k < n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(x[j][e], fk, o[e]);
+          }
+        }
+        if (j0 + W * U < n) load(j0 + W * U);
+      }
     }
-  }
 #pragma unroll
-  for (int s = 16; s > 0; s >>= 1) den += __shfl_xor(den, s, 32);
-  const float inv = den == 0.f ? NAN : 1.f / den;
+    for (int d = 16; d > 0; d >>= 1) den += __shfl_xor(den, d, 32);
+  }
+  if (s > 0) sm_o[vec][lane] = o;
+  __syncthreads();
+  if (s > 0 || !live) return;
+  o += sm_o[vec][lane];
+  const float inv = n == 0 ? 0.f : den == 0.f ? NAN : 1.f / den;
   f16x4 y;
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] = static_cast<f16>(as_f32_value(o[e] * inv));
@@ -808,6 +833,6 @@ extern "C" int cir_paged_decode_attention_shared(const void* q, const void* k_po
   const int st = launch_status();
   if (st) return st;
   const unsigned vectors = (unsigned)batch * num_heads;
-  attn_shared_join<<<(vectors + 7) / 8, 256, 0, s>>>(A, static_cast<f16*>(out));
+  attn_shared_join<<<(vectors + 3) / 4, 256, 0, s>>>(A, static_cast<f16*>(out));
   return launch_status();
 }

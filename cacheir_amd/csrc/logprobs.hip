@@ -293,10 +293,14 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
 #pragma unroll
     for (int e = 1; e < N; ++e) mx = fmaxf(mx, to_f32(top_of[e]));
     if (mx > a.m) raise<T>(a, mx);
+    // (a sum of its own per group: next to a likely token's 1 hundreds of terms below 2^-25 would be lost one by one)
+    Stats b = {a.m, a.ref, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < N; ++e) add<T>(a, w[u][e]);
+      for (int e = 0; e < N; ++e) add<T>(b, w[u][e]);
+    a.s += b.s;
+    a.t += b.t;
     return mx;
   };
   vec one[ONE ? U : 1];

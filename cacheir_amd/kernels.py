@@ -368,29 +368,28 @@ def rope_append(q, k, v, positions, slot_map, inv_freq, k_pool, v_pool, *, layou
     columns of one QKV projection); ``out`` may be q.  Returns the turned q."""
     dev, dt, kdt = q.get_device(), q.dtype, k_pool.dtype
     qs, ks, ps, fs = q.shape, k.shape, k_pool.shape, inv_freq.shape
+    qt, kt, vt = q.stride(), k.stride(), v.stride()
     if not (dev >= 0 and len(qs) == len(ks) == 3 and len(ps) == 4 and len(fs) == 1
             and k.get_device() == dev == v.get_device() and k.dtype is dt is v.dtype and v.shape == ks
             and qs[0] == ks[0] and ps[3] == qs[2] == ks[2] >= 2 * fs[0] and ps[1] == ks[1]
-            and q.stride(2) == k.stride(2) == v.stride(2) == 1
+            and qt[2] == kt[2] == vt[2] == 1
             and _fits(k_pool, dev, kdt, ps) and _fits(v_pool, dev, kdt, ps) and _fits(positions, dev, torch.int32, qs[:1])
             and _fits(slot_map, dev, torch.int64, qs[:1]) and _fits(inv_freq, dev, torch.float64, fs)):
         _check_rope(q, k, v, positions, slot_map, inv_freq, k_pool, v_pool)
-    _req(layout in hip.ROPE_LAYOUTS, f"layout must be one of {sorted(hip.ROPE_LAYOUTS)}")
+    if layout not in hip.ROPE_LAYOUTS:
+        _req(False, f"layout must be one of {sorted(hip.ROPE_LAYOUTS)}")
     tokens, heads, dim = qs
     slots, kvh, psize, _ = ps
-    rot = 2 * inv_freq.numel()
     if out is None:
         out = q.new_empty(qs)
+        ot = (heads * dim, dim)
     else:
         _req(isinstance(out, torch.Tensor) and out.device == q.device and out.shape == q.shape and
              (out.stride(2) == 1 or dim == 1) and out.dtype == dt, "out must be like q")
-    q0, q1, _ = q.stride()
-    k0, k1, _ = k.stride()
-    v0, v1, _ = v.stride()
-    o0, o1, _ = out.stride()
-    _call_on(dev, "cir_rope_append", q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1,
-             hip.dtype_code(dt), positions.data_ptr(), slot_map.data_ptr(), inv_freq.data_ptr(), factor, rot,
-             hip.ROPE_LAYOUTS[layout], out.data_ptr(), o0, o1, k_pool.data_ptr(), v_pool.data_ptr(),
+        ot = out.stride()
+    _call_on(dev, "cir_rope_append", q.data_ptr(), qt[0], qt[1], k.data_ptr(), kt[0], kt[1], v.data_ptr(), vt[0], vt[1],
+             hip.dtype_code(dt), positions.data_ptr(), slot_map.data_ptr(), inv_freq.data_ptr(), factor, 2 * fs[0],
+             hip.ROPE_LAYOUTS[layout], out.data_ptr(), ot[0], ot[1], k_pool.data_ptr(), v_pool.data_ptr(),
              hip.dtype_code(kdt), slots * psize, tokens, heads, kvh, dim, psize)
     return out
 
@@ -748,12 +747,13 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor | None, top_k: int = 
                                       device=logits.device).split_with_sizes((n, rows, rows * top_k))
     res = TokenLogprobs(None if ids is None else lp, entropy,
                         torch.empty((rows, top_k), dtype=torch.int64, device=logits.device), top_lp.view(rows, top_k))
-    if workspace is None:
-        workspace = token_logprobs_workspace(rows, vocab, top_k, logits.device)
-    else:
+    if workspace is not None:
         _check_workspace(workspace, dev)
+    elif hip.size_call("cir_token_logprobs_workspace_bytes", rows, vocab, top_k):
+        workspace = token_logprobs_workspace(rows, vocab, top_k, logits.device)
+    ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
     _call_on(dev, "cir_token_logprobs", logits.data_ptr(), code, ld, hip.ptr(ids), rows, vocab, top_k, lp.data_ptr(),
-             entropy.data_ptr(), res.top_ids.data_ptr(), top_lp.data_ptr(), workspace.data_ptr(), workspace.nbytes)
+             entropy.data_ptr(), res.top_ids.data_ptr(), top_lp.data_ptr(), ws, ws_bytes)
     return res
 
 

@@ -218,6 +218,21 @@ def test_shared_attention_scores_at_the_limits(device):
     assert bool((got[1] == 0).all()) and torch.isnan(got[[0, 2]]).all()
 
 
+@pytest.mark.parametrize("slope", [0.002, 0.05, 0.17, 1.0, -0.05, -1.0])
+@pytest.mark.parametrize("rows,hq,hkv", [(40, 8, 2), (3, 4, 1)])
+def test_shared_attention_scores_that_rise_and_fall(device, slope, rows, hq, hkv):
+    """Scores of slope * t: the running maximum is passed by little or much, once or in every block, and later pieces
+    outweigh earlier ones (or weigh nothing)."""
+    case = shared_case(14, [(rows, 640)], [(7 * b) % 300 for b in range(rows)], hq, hkv)
+    sign = torch.randint(0, 2, (128,), generator=torch.Generator().manual_seed(0)) * 2.0 - 1.0
+    case["q"] = (sign * (1 + torch.arange(rows * hq).view(rows, hq, 1) % 3 / 4)).half()
+    for b in range(rows):
+        t = torch.arange(int(case["seq_lens"][b]))
+        pages = case["page_table"][b].long()[t // 16]
+        case["k_pool"][pages, :, t % 16] = (sign * (slope * t / 128).view(-1, 1, 1)).half().expand(-1, hkv, -1)
+    check_shared(case, run_shared(case, device, scale=1.0), 1.0)
+
+
 def test_shared_attention_captured_and_on_a_stream(device):
     """Two graphs with workspaces of their own, replayed in turn with other lengths and prefixes between the replays,
     and a call on a stream of its own, all bit for bit the eager call's."""
@@ -652,6 +667,23 @@ def test_logprobs_many_rows(device, rows, vocab, dtype):
     r = kernels.token_logprobs(bad.to(device)[which.to(device)].contiguous(), ids.to(device), 7)
     order = [vocab // 2] + [i for i in np.argsort(-x[5].float().numpy(), kind="stable")[:8].tolist() if i != vocab // 2]
     assert r.top_ids[5].tolist() == order[:7] and torch.isnan(r.entropy).all() and torch.isnan(r.logprobs).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_logprobs_of_a_likely_token_among_many_unlikely_ones(device, dtype):
+    """1 + 150000 times 1e-8: added one by one to the 1, some 600 of a thread's terms (6e-6) would be lost.  A thread adds
+    19 groups of 32 (38 of 16) sums to it and 12 joins follow, each off by 2^-24 at most; the rest is exact to 2e-10."""
+    from cacheir_amd import kernels
+
+    rows, vocab, low = 512, 150001, -18.40625
+    x = torch.full((rows, vocab), low, dtype=dtype, device=device)
+    ids = (torch.arange(rows, device=device) * 293) % vocab
+    x[torch.arange(rows, device=device), ids] = 0.0
+    got = kernels.token_logprobs(x, ids, 2)
+    want = -np.log1p((vocab - 1) * np.exp(low))
+    bound = (19 + 12 if dtype == torch.float16 else 38 + 12) * U32 + 2e-10
+    assert float((got.logprobs.double() - want).abs().max()) <= bound
+    assert torch.equal(got.top_ids[:, 0], ids) and torch.equal(got.top_logprobs[:, 0], got.logprobs)
 
 
 def test_logprobs_rows_without_probabilities(device):

@@ -741,6 +741,41 @@ def test_logprobs_graph_stream_and_refusals(device):
         kernels.token_logprobs(x, ids, 8, workspace=torch.empty(8, dtype=torch.uint8, device=device))
 
 
+# ------------------------------------------------------------------------ far --
+def test_pages_past_32_bit_offsets(device):
+    """Pages whose elements lie past 2^32 in their pools: what is appended there and read from there has the bits of the
+    same pages at the start of small pools.  Logits of rows that lie 2^32 elements
+    apart likewise."""
+    from cacheir_amd import kernels
+
+    case = shared_case(15, [(3, 96), (1, 0)], [5, 40, 17, 33], 8, 2)
+    near = {k: v.to(device) for k, v in case.items()}
+    pages = case["k_pool"].shape[0]
+    first = (1 << 32) // case["k_pool"][0].numel() - pages // 2  # the pages lie on both sides of 2^32
+    far = dict(near, page_table=near["page_table"] + first)
+    for name in ("k_pool", "v_pool"):
+        far[name] = torch.empty((first + pages, *near[name].shape[1:]), dtype=torch.float16, device=device)
+        far[name][first:] = near[name]
+    assert far["k_pool"].numel() > 1 << 32
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn((pages, 12, 128), generator=g).half().to(device)
+    pos = torch.arange(pages, dtype=torch.int32, device=device) * 1000
+    freq = kernels.rope_frequencies(128, 1e4, None, device)
+    slot = torch.arange(pages, device=device) * 16 + 3  # one token in every page
+    outs = [kernels.rope_append(x[:, :8], x[:, 8:10], x[:, 10:], pos, slot + at * 16, freq, c["k_pool"], c["v_pool"])
+            for c, at in ((near, 0), (far, first))]
+    assert torch.equal(*outs)
+    for name in ("k_pool", "v_pool"):
+        assert torch.equal(far[name][first:], near[name])
+    assert torch.equal(kernels.paged_decode_attention_shared(**far), kernels.paged_decode_attention_shared(**near))
+
+    rows = torch.as_strided(far["k_pool"].view(-1), (2, 1000), ((1 << 32) - 1000, 1))  # the second ends at 2^32
+    rows.copy_(torch.randn((2, 1000), generator=g))
+    ids = torch.tensor([5, 999], device=device)
+    for a, b in zip(kernels.token_logprobs(rows, ids, 4), kernels.token_logprobs(rows.contiguous(), ids, 4)):
+        assert torch.equal(a, b)
+
+
 # ------------------------------------------------------------------- together --
 def test_decode_steps_of_the_operators_together(device):
     """Samples of two prompts: pages and slots built on the GPU, rotary append, attention over the shared prefixes and

@@ -44,6 +44,7 @@ constexpr int kMinChunk = 4096;   // logits of a workgroup that shares its row w
 // product has just written, 14.6 -> 15.4).
 constexpr size_t kCacheBytes = (size_t)256 << 20;
 constexpr int kManyRows = 1024;   // rows of one wavefront each, where they are short
+constexpr int kMaxRows = 1 << 24; // (rows * kThreads < 2^32)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // 2^-300 is zero in fp32: y below it adds nothing, and 0 * y stays 0 for x = -inf.
 constexpr float kFloor = -300.f;
@@ -517,7 +518,7 @@ __global__ __launch_bounds__(64) void logprobs_merge(const T* __restrict__ logit
 template <typename T>
 constexpr int kGroupOf = 64 * 4 * Words<T>::kN;  // logits of a wavefront's group
 
-// Workgroups that share a row: enough for two per CU, each with kMinChunk logits at least.
+// Workgroups that share a row: enough for two per CU, each with kMinChunk logits at least (one from 257 rows on).
 int row_splits(int rows, int vocab) {
   const int fill = 512 / max(1, min(rows, 512)), most = max(1, vocab / kMinChunk);
   return max(1, min(min(fill, most), 64));
@@ -541,6 +542,8 @@ extern "C" int cir_token_logprobs(const void* logits, int dt, int64_t ld, const 
   CIR_CHECK_ARG(rows >= 0 && vocab > 0 && ld >= vocab, "token_logprobs: bad sizes");
   CIR_CHECK_ARG(top_k >= 0 && top_k <= kMaxTop && top_k <= vocab, "token_logprobs: top_k %d out of range (0..%d, at most "
                 "the vocabulary)", top_k, kMaxTop);
+  // A grid has fewer than 2^32 threads: one bound for all forms, which asks for a workgroup per row at most.
+  CIR_CHECK_ARG(rows < kMaxRows, "token_logprobs: %d rows are too many for a launch (fewer than 2^24)", rows);
   if (rows == 0) return 0;
   CIR_CHECK_ARG(logits && entropy && (!ids || logprobs) && (top_k == 0 || (top_ids && top_logprobs)),
                 "token_logprobs: null pointer");
@@ -550,8 +553,6 @@ extern "C" int cir_token_logprobs(const void* logits, int dt, int64_t ld, const 
   CIR_CHECK_ARG((workspace || need == 0) && workspace_bytes >= need && (uintptr_t)workspace % 8 == 0,
                 "token_logprobs: workspace too small or not on 8 bytes (%zu < %zu)", workspace_bytes, need);
   const bool many = rows >= kManyRows && vocab <= 4 * (dt == CIR_F16 ? kGroupOf<f16> : kGroupOf<float>);
-  CIR_CHECK_ARG((many ? ((long)rows + kWaves - 1) / kWaves : (long)rows * S) * kThreads < (1L << 32),
-                "token_logprobs: %d rows are too many for a launch", rows);
   hipStream_t s = as_stream(stream);
   const Out out{ids ? logprobs : nullptr, entropy, top_ids, top_logprobs};
   u64* part_top = static_cast<u64*>(workspace);

@@ -349,7 +349,8 @@ int cir_qgemm_argmax(const void* x, int ldx, const void* w_tiled, int fmt, int64
  *   top_ids[r][0 .. top_k), top_logprobs likewise: by decreasing logit, equal ones by index
  *     (a logit of -inf counts as any other value; NaN is above every number, as in cir_argmax).
  * A row that holds NaN or +inf, or -inf alone, has NaN probabilities.  ids may be NULL
- * (logprobs is then not written).  0 <= top_k <= 64, top_k <= vocab; statistics in fp32.
+ * (logprobs is then not written).  rows < 2^24, 0 <= top_k <= 64, top_k <= vocab; statistics
+ * in fp32.
  * workspace: cir_token_logprobs_workspace_bytes bytes on an 8-byte address (0: NULL will
  * do), written by the call.  No counterpart in the reference, whose sampling is greedy. */
 size_t cir_token_logprobs_workspace_bytes(int rows, int vocab, int top_k);

@@ -128,6 +128,16 @@ def test_logprobs_refusals():
     hip.call("cir_token_logprobs", None, F16, 100, None, 0, 100, 5, *[None] * 5, 0, None)
 
 
+@pytest.mark.parametrize("dt", [F16, F32])
+@pytest.mark.parametrize("vocab", [5, 1000, 5000, 100000])
+def test_logprobs_of_too_many_rows_never_reach_a_launch(dt, vocab):
+    """Status 1 is the argument check's own; a launch without a GPU fails with another one."""
+    p = torch.zeros(64).data_ptr()
+    for rows in (1 << 24, (1 << 26) + 1, 2 ** 31 - 1):
+        refuses("cir_token_logprobs", "status 1: .*too many", p, dt, vocab, None, rows, vocab, 5, None, p, p, p, None, 0,
+                None)
+
+
 def test_rope_frequencies_on_the_host():
     f = kernels.rope_frequencies(8, 10000.0, device="cpu")
     assert f.dtype == torch.float64 and torch.equal(f, 10000.0 ** (-torch.arange(4, dtype=torch.float64) / 4))

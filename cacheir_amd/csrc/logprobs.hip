@@ -358,7 +358,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
       }
     };
     if (has_head || has_tail) gather(end_at >= 0, end_at >= 0 ? to_f32(x[end_at]) : 0.f, end_at);
-    const int ends = n;
+    const int ends = n;  // (at most 2 N - 2, those before the first vector first)
     int picks = 0;  // uniform
     if constexpr (ONE) {
       if (!odd) {
@@ -401,7 +401,10 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
       }
     }
     if (picks > kPicks || n > kKeys || odd) {  // uniform
-      for (int j = 0; j < ends; j += 64) top.absorb(j + lane < ends ? sm_keys[wave][j + lane] : 0, K, lane);
+      // What lies before the groups, then the groups, then what lies behind them: a group whose values are no larger than
+      // the list's least can be passed over because the list holds lower indices only.
+      const int head = has_head ? skip : 0;
+      top.absorb(lane < head ? sm_keys[wave][lane] : 0, K, lane);
       for (int g = 0; g < groups; ++g) {           // uniform
         const float least = key_value(top.least);  // (none yet: NaN)
         if (!ONE && !odd) {
@@ -415,6 +418,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
           top.absorb(in && !(v < bound) ? make_key(v, at) : 0, K, lane);
         }
       }
+      top.absorb(lane >= head && lane < ends ? sm_keys[wave][lane] : 0, K, lane);
       n = 64;
       sm_keys[wave][lane] = top.key;
       top = Top{0, 0};

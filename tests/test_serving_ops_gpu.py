@@ -704,6 +704,37 @@ def test_logprobs_rows_without_probabilities(device):
         assert r.top_ids[2].tolist() == [0, 1, 2, 3]
 
 
+@pytest.mark.parametrize("rows,vocab,dtype", [
+    (1031, 1029, torch.float32), (1031, 3001, torch.float32), (1031, 4095, torch.float32),   # a wavefront per row,
+    (1031, 2051, torch.float16), (1031, 8189, torch.float16),                                # several groups each
+    (517, 4999, torch.float32), (517, 20001, torch.float32), (517, 20003, torch.float16),    # a workgroup per row
+    (26, 60001, torch.float32), (32, 140007, torch.float16)])                                # several workgroups per row
+def test_logprobs_equal_values_by_index(device, rows, vocab, dtype):
+    """Rows of equal values and plateaus of the largest value that begin in every wavefront's share (and none, a few or
+    many values before the end), where the values behind the last whole vector are equal too: the lowest ids win.  Rows
+    lie next to one another, so they begin and end at every place within 16 bytes."""
+    from cacheir_amd import kernels
+
+    n = 4 if dtype == torch.float32 else 8  # values of a vector; a wavefront's turn is 64 of them
+    assert vocab % 2 == 1
+    low = -torch.rand(vocab, generator=torch.Generator().manual_seed(vocab)) * 4 - 1
+    starts = [0, 3, 64 * n, 128 * n, 192 * n, 192 * n + 5, 256 * n + 64 * n, vocab // 2, vocab - 70 * n, vocab - n - 2,
+              vocab - 1] + [max(0, vocab - turns * 64 * n) for turns in (8, 9, 10, 11)]
+    kinds = []
+    for at in starts:
+        row = low.clone()
+        row[min(at, vocab - 1):] = 2.0
+        kinds.append(row)
+    few = torch.full((vocab,), -math.inf)  # fewer than top_k tokens left
+    few[[vocab // 3, vocab - 1]] = 1.0
+    kinds += [few, torch.full((vocab,), torch.finfo(dtype).min)]
+    x = torch.stack(kinds).to(dtype)  # 17 kinds: each meets every alignment
+    which = torch.arange(rows) % len(kinds)
+    dev = x.to(device)[which.to(device)].contiguous()
+    for k in (1, 2, 3, 5, 7):
+        check_logprobs(x, None, k, kernels.token_logprobs(dev, None, k), which)
+
+
 def test_logprobs_graph_stream_and_refusals(device):
     from cacheir_amd import kernels
 

@@ -142,8 +142,9 @@ __device__ __forceinline__ void soft_step(Soft& a, f32x16 (&c)[NB], float sc, f1
   float mx = c[0][0];
 #pragma unroll
   for (int r = 1; r < 16 * NB; ++r) mx = fmaxf(mx, c[r >> 4][r & 15]);
-  mx *= sc;
-  if (__builtin_amdgcn_ballot_w64(mx > a.m + 8.f) != 0) {  // uniform
+  mx = as_f32_value(mx * sc);
+  // The difference, not a.m + 8: from |m| = 2^27 on that can round up to the next score, 16 above, whose p is no fp16.
+  if (__builtin_amdgcn_ballot_w64(mx - a.m > 8.f) != 0) {  // uniform
     const float mn = fmaxf(a.m, fmaxf(mx, __shfl_xor(mx, 32, 64)));
     const float alpha = __builtin_amdgcn_exp2f(a.m - (mn == -INFINITY ? 0.f : mn));
     a.l *= alpha;

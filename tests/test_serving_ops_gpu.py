@@ -218,6 +218,49 @@ def test_shared_attention_scores_at_the_limits(device):
     assert bool((got[1] == 0).all()) and torch.isnan(got[[0, 2]]).all()
 
 
+@pytest.mark.parametrize("rows,hq,hkv,prefix", [
+    (3, 64, 64, 2048),     # 3 vectors of a KV head, about 12 blocks a piece: every wavefront meets both scores
+    (40, 64, 16, 4096)])   # 160: a tile of 128 and one of 32
+@pytest.mark.parametrize("low,high,times", [
+    (2 ** 27 + 16, 2 ** 27 + 32, 1.0), (2 ** 26 + 8, 2 ** 26 + 16, 1.0), (2 ** 28 - 16, 2 ** 28, 1.0),
+    (2 ** 24 + 2, 2 ** 24 + 10, 1.0), (-2 ** 27 - 32, -2 ** 27 - 16, 1.0),
+    (89479112, 89479120, 1.5)])  # products 134218668 and ...680 round to ...672 and ...688
+def test_shared_attention_scores_one_step_apart(device, rows, hq, hkv, prefix, low, high, times):
+    """Scores so large that the next fp32 number is 2 to 16 further, every second 128 tokens the higher one.  The sums
+    are exact here and the scale makes the exponents ``times`` the scores, rounded once, so a weight is 1 or 2 to their
+    difference, and what is left are the roundings of the weights and the output and n sums in fp32."""
+    scale = 0.6931471824645996 * times
+    assert np.float32(scale) * np.float32(1.4426950408889634) == np.float32(times)
+    case = shared_case(16, [(rows, prefix)], [(37 * b) % 50 + 1 for b in range(rows)], hq, hkv)
+    parts = torch.tensor([2.0 ** 14, 2.0 ** 10, 2.0], dtype=torch.float64)
+    case["q"].zero_()
+    case["q"][:, :, :3] = parts.half()
+    ref, tol = torch.zeros(case["q"].shape, dtype=torch.float64), torch.zeros(case["q"].shape, dtype=torch.float64)
+    big = float(torch.tensor(high / 2 ** 14).half())
+    for b in range(rows):
+        n = int(case["seq_lens"][b])
+        t = torch.arange(n)
+        pages = case["page_table"][b].long()[t // 16]
+        c = torch.where(t // 128 % 2 == 1, high, low).double()
+        mid = ((c - big * 2 ** 14) / 2 ** 10).trunc()
+        key = torch.zeros((n, hkv, 128), dtype=torch.float16)
+        key[:, :, :3] = torch.stack([torch.full((n,), big, dtype=torch.float64), mid,
+                                     (c - big * 2 ** 14 - mid * 2 ** 10) / 2], dim=1)[:, None].half()
+        assert torch.equal(key[:, 0, :3].double() @ parts, c)
+        case["k_pool"][pages, :, t % 16] = key
+        v = case["v_pool"][pages, :, t % 16].double()
+        s = (c * times).float().double()
+        w = torch.exp2(s - s.max())
+        l = w.sum()
+        out, mass = ((w / l).view(-1, 1, 1).mul(x).sum(dim=0) for x in (v, v.abs()))
+        off = mass * (2 * U16 + (n + 64) * U32) + v.abs().sum(dim=0) * 2.0 ** -25 / l + U16 * out.abs()
+        ref[b], tol[b] = (x.repeat_interleave(hq // hkv, dim=0) for x in (out, off))
+    got = run_shared(case, device, scale=scale)
+    assert torch.isfinite(got).all()
+    err = (got.cpu().double() - ref).abs()
+    assert bool((err <= tol).all()), f"max excess {(err - tol).max():.3e}, max error {err.max():.3e}"
+
+
 @pytest.mark.parametrize("slope", [0.002, 0.05, 0.17, 1.0, -0.05, -1.0])
 @pytest.mark.parametrize("rows,hq,hkv", [(40, 8, 2), (3, 4, 1)])
 def test_shared_attention_scores_that_rise_and_fall(device, slope, rows, hq, hkv):

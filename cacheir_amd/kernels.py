@@ -219,7 +219,7 @@ def _check_shared(q, k_pool, v_pool, page_table, seq_lens, group_rows, prefix_le
         _req(all(a <= b for a, b in zip(rows, rows[1:])) and 0 <= rows[0] and rows[-1] <= batch,
              "group_rows must ascend within the batch")
         for g, n in enumerate(lens):
-            part = table[rows[g]: rows[g + 1], : max(0, n) // psize]
+            part = table[rows[g]: rows[g + 1], : -(-max(0, n) // psize)]  # the page it ends in too
             _req(0 <= n <= max_pages * psize, "prefix_lens exceed the page table capacity")
             _req(part.numel() == 0 or bool((part == part[:1]).all()), f"group {g}: rows with other pages in the prefix")
 
@@ -229,8 +229,9 @@ def paged_decode_attention_shared(q, k_pool, v_pool, page_table, seq_lens, group
                                   workspace: torch.Tensor | None = None, check_tables: bool = False) -> torch.Tensor:
     """``paged_decode_attention`` of a batch whose rows share prefixes: rows ``group_rows[g] .. group_rows[g + 1] - 1``
     (int32 ``[groups + 1]``, ascending) have the same pages for their first ``prefix_lens[g]`` tokens (int32
-    ``[groups]``), and each prefix is read once for all of them.  Both may change between replays of a captured call.
-    ``check_tables`` checks them, the pages and the lengths on the host (a device sync)."""
+    ``[groups]``; the page in which they end is the same too), and each prefix is read once for all of them.  Both may
+    change between replays of a captured call.  ``check_tables`` checks them, the pages and the lengths on the host (a
+    device sync)."""
     dev, dt = q.get_device(), q.dtype
     qs, ps, ts, i32 = q.shape, k_pool.shape, page_table.shape, torch.int32
     groups = prefix_lens.numel()

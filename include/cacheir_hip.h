@@ -160,7 +160,8 @@ int cir_paged_prefill_attention_split(const void* q, const void* k_pool, const v
  * the same q, pools, page_table, seq_lens and out, where rows group_rows[g] ..
  * group_rows[g + 1] - 1 (int32 [groups + 1], on the device, ascending, in 0 .. batch) have
  * the same page table entries, and so the same K and V, for their first prefix_lens[g]
- * tokens (int32 [groups], on the device).  Each prefix is then read once for the query
+ * tokens (int32 [groups], on the device), the entry of the page in which they end among
+ * them: where that page is each row's own copy, give the tokens before it.  Each prefix is then read once for the query
  * vectors of all its rows instead of once per row; the result is the attention over each
  * row's whole context, whatever part of it is shared.  The pages of a prefix are taken from
  * the group's first row; sharing stops at that row's length, and a row shorter than the

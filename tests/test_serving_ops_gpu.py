@@ -111,6 +111,24 @@ def test_shared_attention_shapes(device, hq, hkv, groups, suffix, psize):
     check_shared(case, run_shared(case, device, check_tables=True))
 
 
+@pytest.mark.parametrize("psize,whole,prefixes", [
+    (64, [64, 128, 192, 640], [32, 100, 191, 577]), (48, [48, 96, 144, 480], [47, 95, 97, 479]),
+    (16, [16, 32, 48, 640], [1, 31, 33, 639]), (128, [128, 128, 256, 640], [33, 127, 160, 600])])
+@pytest.mark.parametrize("rows,hq,hkv", [(3, 8, 2), (20, 16, 2)])
+def test_shared_attention_prefixes_that_end_inside_a_page(device, psize, whole, prefixes, rows, hq, hkv):
+    """Prefixes that are no whole number of pages, of 32-token blocks or of either, the last page common to the rows (what
+    follows the prefix in it is theirs too); some rows end inside the prefix or that page."""
+    case = shared_case(17, [(rows, p) for p in whole], [(13 * b) % 70 for b in range(4 * rows)], hq, hkv, psize)
+    case["prefix_lens"] = torch.tensor(prefixes, dtype=torch.int32)
+    for g, p in enumerate(prefixes):
+        case["seq_lens"][g * rows + 1] = p
+        case["seq_lens"][g * rows + 2] = p - 1
+    check_shared(case, run_shared(case, device, check_tables=True))
+    case["page_table"][1, 0] = case["page_table"][1, 0] + (1 if case["page_table"][1, 0] == 0 else -1)
+    with pytest.raises(ValueError, match="group 0: rows with other pages"):
+        run_shared(case, device, check_tables=True)
+
+
 @pytest.mark.parametrize("seed", range(8))
 def test_shared_attention_random_groups(device, seed):
     rng = np.random.default_rng(seed)

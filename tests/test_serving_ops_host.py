@@ -29,6 +29,29 @@ def test_shared_attention_workspace(batch, groups, hq, hkv):
                 == hip.size_call("cir_paged_attention_workspace_bytes", batch, hq, d, 64 * page))
 
 
+@pytest.mark.parametrize("page,prefix", [(64, 32), (64, 33), (64, 63), (64, 100), (48, 47), (48, 95), (16, 1), (16, 96)])
+def test_checked_tables_cover_the_page_in_which_a_prefix_ends(monkeypatch, page, prefix):
+    """Every page that holds a token of the prefix is the same in all rows of a group: the kernel reads whole 32-token
+    blocks of the prefix from the first row's pages, the part of a page among them."""
+    monkeypatch.setattr(kernels, "_cuda", lambda *a, **k: None)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32)
+    q, pool = torch.zeros(5, 8, 128, dtype=torch.float16), torch.zeros(40, 2, page, 128, dtype=torch.float16)
+    table = torch.arange(35, dtype=torch.int32).view(5, 7)
+    last = (prefix - 1) // page
+    table[1:4, : last + 1] = table[1, : last + 1]
+    check = lambda t: kernels._check_shared(q, pool, pool, t, i32([prefix + 1] * 5), i32([1, 4, 5]), i32([prefix, 40]),
+                                            True)
+    check(table)
+    for col in range(last + 1):
+        other = table.clone()
+        other[3, col] = 39
+        with pytest.raises(ValueError, match="group 0: rows with other pages"):
+            check(other)
+    other = table.clone()
+    other[3, last + 1] = 39  # behind the prefix
+    check(other)
+
+
 @pytest.mark.parametrize("bad", [(0, 1, 8, 2, 128, 16, 4), (2, -1, 8, 2, 128, 16, 4), (2, 1, 7, 2, 128, 16, 4),
                                  (2, 1, 8, 0, 128, 16, 4), (2, 1, 8, 2, 0, 16, 4), (2, 1, 8, 2, 128, 0, 4),
                                  (2, 1, 8, 2, 128, 16, 0), (2, 1, 8, 2, 128, 1 << 16, 1 << 16)])

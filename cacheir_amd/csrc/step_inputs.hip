@@ -5,6 +5,8 @@
 
 #include <limits.h>
 
+#include <utility>
+
 namespace cir {
 namespace {
 
@@ -265,6 +267,28 @@ __global__ __launch_bounds__(kRopeThreads) void rope_append_kernel(
   }
 }
 
+// Whether any two of the heads at t * ts + h * hs (t < nt, h < nh; `len` elements each) overlap: some (i, j) != (0, 0),
+// |i| < nt, |j| < nh, has |i ts + j hs| < len.
+bool heads_overlap(int64_t ts, int nt, int64_t hs, int nh, int len) {
+  typedef __int128 wide;  // (any strides)
+  const auto mag = [](wide v) { return v < 0 ? -v : v; };
+  wide a = ts, b = hs;
+  int na = nt, nb = nh;
+  if (na < nb) {
+    std::swap(a, b);
+    std::swap(na, nb);
+  }
+  if (na <= 1) return false;
+  if (mag(a) < len || (nb > 1 && mag(b) < len)) return true;
+  // One axis lies within a step of the other, as in every ordinary tensor.
+  if (nb <= 1 || mag(a) >= (nb - 1) * mag(b) + len || mag(b) >= (na - 1) * mag(a) + len) return false;
+  for (int j = 1; j < nb; ++j) {  // i = -j b / a, rounded to both sides, comes nearest
+    const wide i = mag(j * b) / mag(a), rest = mag(j * b) - i * mag(a);
+    if ((i < na && rest < len) || (i + 1 < na && mag(a) - rest < len)) return true;
+  }
+  return false;
+}
+
 }  // namespace
 }  // namespace cir
 
@@ -322,8 +346,7 @@ extern "C" int cir_rope_append(const void* q, int64_t q_token_stride, int64_t q_
                     (inv_freq || rotary_dim == 0),
                 "rope_append: null pointer");
   // Written heads that overlap, or q in place at other strides, would be read and written by different threads.
-  const auto apart = [&](int64_t stride, int n) { return n <= 1 || stride >= head_dim || stride <= -head_dim; };
-  CIR_CHECK_ARG(num_heads == 0 || (apart(o_token_stride, tokens) && apart(o_head_stride, num_heads)),
+  CIR_CHECK_ARG(num_heads == 0 || !heads_overlap(o_token_stride, tokens, o_head_stride, num_heads, head_dim),
                 "rope_append: heads of q_out overlap");
   CIR_CHECK_ARG(num_heads == 0 || q_out != q ||
                     ((tokens == 1 || o_token_stride == q_token_stride) &&

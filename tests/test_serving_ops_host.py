@@ -121,6 +121,31 @@ def test_rope_refuses_outputs_that_overlap():
     rope(tokens=0)
 
 
+def test_rope_refuses_exactly_the_outputs_that_overlap():
+    """Token and head stride together, against the heads' elements counted out.  (q_out is q here, at strides that q does
+    not have, so no call reaches a launch.)"""
+    x = torch.zeros(64)
+    for tokens, heads, d in ((2, 4, 8), (4, 2, 8), (3, 3, 4), (5, 2, 2), (1, 4, 8), (4, 1, 8)):
+        strides = [s for s in range(-5 * d - 3, 5 * d + 4)]
+        for ts in strides[:: 1 if d < 8 else 3] + [8, 16, 24, 32, -8, -32]:
+            for hs in strides[:: 1 if d < 8 else 5] + [8, 16, 24, 32, -8, -32]:
+                first = {t * ts + h * hs for t in range(tokens) for h in range(heads)}
+                at = {e + i for e in first for i in range(d)}
+                apart = len(at) == tokens * heads * d
+                with pytest.raises(RuntimeError, match="other strides" if apart else "overlap"):
+                    rope(tokens=tokens, heads=heads, d=d, rot=d, p=x.data_ptr(), o=(ts, hs), q=(999, 999))
+
+
+@pytest.mark.parametrize("o", [(2 ** 63 - 1, -2 ** 63), (-2 ** 63, 8), (2 ** 40 + 1, 2 ** 40), (2 ** 62, 2 ** 62)])
+def test_rope_overlap_of_far_strides(o):
+    x = torch.zeros(64)
+    for tokens, heads in ((1 << 20, 3), (3, 1 << 20), (2, 2)):
+        # 1: t = h = 1 of (2^63 - 1, -2^63); 1 - 2^20 + ... of neighbours; equal strides
+        match = "other strides" if o == (-2 ** 63, 8) else "overlap"
+        with pytest.raises(RuntimeError, match=match):
+            rope(tokens=tokens, heads=heads, p=x.data_ptr(), o=o, q=(16, 9))
+
+
 def test_logprobs_workspace():
     """Nothing where a row has a workgroup of its own; 12 bytes of sums and top_k keys of 8 per split elsewhere."""
     size = lambda *a: hip.size_call("cir_token_logprobs_workspace_bytes", *a)

@@ -352,6 +352,9 @@ extern "C" int cir_rope_append(const void* q, int64_t q_token_stride, int64_t q_
                     ((tokens == 1 || o_token_stride == q_token_stride) &&
                      (num_heads == 1 || o_head_stride == q_head_stride)),
                 "rope_append: q_out is q with other strides");
+  const uintptr_t pool_bytes = (uintptr_t)slots * num_kv_heads * head_dim * (kv_dtype == CIR_F16 ? 2 : 4);
+  const uintptr_t k_at = (uintptr_t)k_pool, v_at = (uintptr_t)v_pool;
+  CIR_CHECK_ARG((k_at < v_at ? v_at - k_at : k_at - v_at) >= pool_bytes, "rope_append: k_pool and v_pool overlap");
   hipStream_t s = as_stream(stream);
   const RopeIn in{q, k, v, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride,
                   o_token_stride, o_head_stride};

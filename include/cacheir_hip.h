@@ -395,7 +395,8 @@ int cir_extend_page_tables(int32_t* page_table, const int32_t* seq_lens, const i
  * slot_map[t] / page_size, offset slot_map[t] % page_size of pools of `slots` tokens in all
  * (pages * page_size).  A token whose slot lies outside 0 .. slots - 1 is padding: nothing
  * of it is written, q_out included.  Two tokens must not share a slot, and q_out, unless it is
- * q at q's strides, overlaps no input; strides that lay its heads on one another are refused.  head_dim even and <= 256, rotary_dim even and <=
+ * q at q's strides, overlaps no input; strides that lay its heads on one another are refused,
+ * and so are pools that overlap.  head_dim even and <= 256, rotary_dim even and <=
  * head_dim, tokens <= 2^26, heads <= 2^20. */
 #define CIR_ROPE_INTERLEAVED 0
 #define CIR_ROPE_HALF 1

@@ -595,6 +595,21 @@ def test_rope_append_matches_the_step_epilogue(device):
     assert (pools[0].float() - pools[2].float()).abs().max() <= 10 * 2 * 72 * U32 + 2 * U16 * 7
 
 
+def test_rope_append_to_the_halves_of_one_allocation(device):
+    """K and V pools one behind the other in memory, as a stacked cache holds them; one tensor as both is refused."""
+    from cacheir_amd import kernels
+
+    x = torch.randn((9, 8, 64), device=device).half()
+    pos, slots = (torch.arange(9, device=device, dtype=t) for t in (torch.int32, torch.int64))
+    both, kp, vp = (torch.zeros((*n, 2, 2, 16, 64), dtype=torch.float16, device=device) for n in ((2,), (), ()))
+    freq = kernels.rope_frequencies(64, 1e4, None, device)
+    args = x[:, :4], x[:, 4:6], x[:, 6:], pos, slots, freq
+    assert torch.equal(kernels.rope_append(*args, both[0], both[1]), kernels.rope_append(*args, kp, vp))
+    assert torch.equal(both[0], kp) and torch.equal(both[1], vp)
+    with pytest.raises(RuntimeError, match="k_pool and v_pool overlap"):
+        kernels.rope_append(*args, kp, kp)
+
+
 def test_rope_frequencies_by_the_formula():
     from cacheir_amd import kernels
 

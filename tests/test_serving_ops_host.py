@@ -146,6 +146,21 @@ def test_rope_overlap_of_far_strides(o):
             rope(tokens=tokens, heads=heads, p=x.data_ptr(), o=o, q=(16, 9))
 
 
+def test_rope_refuses_pools_that_overlap():
+    """K and V of different threads in the same elements: one tensor as both pools, or one that begins inside the other."""
+    pools = torch.zeros(600)
+
+    def call(k, v, slots=16, kvdt=F32):
+        a, p = pools.data_ptr(), torch.zeros(64).data_ptr()
+        refuses("cir_rope_append", "k_pool and v_pool overlap", p, 16, 8, p, 8, 8, p, 8, 8, F32, p, p, p, 1.0, 8, 0, p, 16,
+                8, a + k, a + v, kvdt, slots, 2, 2, 1, 8, 4, None)
+
+    size = 16 * 8 * 4  # slots x head_dim floats
+    for k, v in ((0, 0), (0, 4), (size - 4, 0), (0, size - 4)):
+        call(k, v)
+    call(0, size // 2 - 2, kvdt=F16)
+
+
 def test_logprobs_workspace():
     """Nothing where a row has a workgroup of its own; 12 bytes of sums and top_k keys of 8 per split elsewhere."""
     size = lambda *a: hip.size_call("cir_token_logprobs_workspace_bytes", *a)

@@ -341,6 +341,7 @@ extern "C" int cir_rope_append(const void* q, int64_t q_token_stride, int64_t q_
                 "rope_append: bad sizes");
   CIR_CHECK_ARG(tokens <= kMaxTokens && num_heads <= kMaxHeads && num_kv_heads <= kMaxHeads,
                 "rope_append: more than 2^26 tokens or 2^20 heads");
+  CIR_CHECK_ARG(slots % page_size == 0, "rope_append: slots must be whole pages");
   if (tokens == 0) return 0;
   CIR_CHECK_ARG((num_heads == 0 || (q && q_out)) && k && v && positions && slot_map && k_pool && v_pool &&
                     (inv_freq || rotary_dim == 0),

@@ -161,6 +161,18 @@ def test_rope_refuses_pools_that_overlap():
     call(0, size // 2 - 2, kvdt=F16)
 
 
+def test_rope_refuses_a_part_of_a_page():
+    """Slots are whole pages: head 1 of a slot in a page cut short would lie behind the pool.  (The pools are one here: the
+    last check, so that no call reaches a launch.)"""
+    x = torch.zeros(64)
+    for slots, page in ((17, 16), (15, 16), (1, 2), (2 ** 40 + 1, 4)):
+        with pytest.raises(RuntimeError, match="whole pages"):
+            rope(p=x.data_ptr(), slots=slots, page=page)
+    for slots, page in ((16, 16), (2 ** 40, 4), (7, 1)):
+        with pytest.raises(RuntimeError, match="pools overlap"):
+            rope(p=x.data_ptr(), slots=slots, page=page)
+
+
 def test_logprobs_workspace():
     """Nothing where a row has a workgroup of its own; 12 bytes of sums and top_k keys of 8 per split elsewhere."""
     size = lambda *a: hip.size_call("cir_token_logprobs_workspace_bytes", *a)

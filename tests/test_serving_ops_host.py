@@ -169,7 +169,7 @@ def test_rope_refuses_a_part_of_a_page():
         with pytest.raises(RuntimeError, match="whole pages"):
             rope(p=x.data_ptr(), slots=slots, page=page)
     for slots, page in ((16, 16), (2 ** 40, 4), (7, 1)):
-        with pytest.raises(RuntimeError, match="pools overlap"):
+        with pytest.raises(RuntimeError, match="k_pool and v_pool overlap"):
             rope(p=x.data_ptr(), slots=slots, page=page)
 
 

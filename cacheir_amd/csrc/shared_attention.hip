@@ -56,7 +56,10 @@ constexpr int kItemCost = 6;
 constexpr int kMinStretch = 4;
 constexpr int kMaxPrefixes = 256;  // groups: one per thread
 constexpr int kMaxRows = 2048;
-constexpr long kMaxVectors = 1L << 26;  // of the batch: the join's threads stay below 2^32
+// Fewer query vectors than this in the batch (the join's rounded-up grid stays below 2^32 threads), and fewer KV heads (a
+// workgroup each at least; the records' loop steps by kThreads grids in 32 bits).
+constexpr long kMaxVectors = (1L << 26) - 3;
+constexpr int kMaxKvHeads = 1 << 23;
 constexpr int kRowB = 2 * D;      // bytes of a K or V row
 
 // Workspace: one record per row, then the pieces.
@@ -777,8 +780,8 @@ bool shares(int B, int NG, int Hq, int Hkv, int head_dim, int P, int max_pages, 
   const long items = (long)B * G / kTileVec + NG + B;
   // (page_index is exact while (tokens / 16) (P / 16) < 2^32)
   return kv_dtype == CIR_F16 && head_dim == D && P % 16 == 0 && (long)max_pages * P / 16 * (P / 16) < (1L << 32) &&
-         G <= kVec && NG <= kMaxPrefixes && B <= kMaxRows && (long)B * Hq < kMaxVectors && per_item < (1L << 31) &&
-         per_item * items < (1L << (31 - kPlace));
+         G <= kVec && NG <= kMaxPrefixes && B <= kMaxRows && (long)B * Hq < kMaxVectors && Hkv < kMaxKvHeads &&
+         per_item < (1L << 31) && per_item * items < (1L << (31 - kPlace));
 }
 
 }  // namespace

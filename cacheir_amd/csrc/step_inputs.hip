@@ -148,7 +148,7 @@ __global__ __launch_bounds__(kRows) void extend_tables_kernel(
 constexpr int kRopeThreads = 256;
 constexpr int kMaxDim = 256;
 constexpr int kTokens = 4;
-constexpr int kMaxTokens = 1 << 26;  // (a grid has fewer than 2^32 threads)
+constexpr int kMaxTokens = (1 << 26) - kTokens;  // (a grid, whole workgroups, has fewer than 2^32 threads)
 constexpr int kMaxHeads = 1 << 20;
 
 template <typename T, int N>
@@ -340,7 +340,7 @@ extern "C" int cir_rope_append(const void* q, int64_t q_token_stride, int64_t q_
   CIR_CHECK_ARG(tokens >= 0 && num_heads >= 0 && num_kv_heads > 0 && page_size > 0 && slots >= 0,
                 "rope_append: bad sizes");
   CIR_CHECK_ARG(tokens <= kMaxTokens && num_heads <= kMaxHeads && num_kv_heads <= kMaxHeads,
-                "rope_append: more than 2^26 tokens or 2^20 heads");
+                "rope_append: more than 2^26 - 4 tokens or 2^20 heads");
   CIR_CHECK_ARG(slots % page_size == 0, "rope_append: slots must be whole pages");
   if (tokens == 0) return 0;
   CIR_CHECK_ARG((num_heads == 0 || (q && q_out)) && k && v && positions && slot_map && k_pool && v_pool &&

@@ -168,8 +168,9 @@ int cir_paged_prefill_attention_split(const void* q, const void* k_pool, const v
  * prefix, a group of one row and rows in no group read all of their context alone.
  * group_rows out of order switch sharing off.  A sequence with seq_len 0 yields zeros, one
  * whose scores are all -inf NaN.
- * fp16 pools and q on 16-byte addresses, head_dim 128, page_size a multiple of 16, up to 32
- * query heads per KV head, 2048 rows and 256 groups; other calls run
+ * Shared: fp16 pools and q on 16-byte addresses, out on 8, head_dim 128, page_size a multiple
+ * of 16, up to 32 query heads per KV head, 2048 rows, 256 groups, fewer than 2^23 KV heads and
+ * 2^26 - 3 query vectors (batch * num_heads).  Other calls run
  * cir_paged_decode_attention (every row reads its prefix; scores that are all -inf as there).
  * A row's last bits depend on the batch it is in.
  * workspace: cir_shared_attention_workspace_bytes bytes on a 16-byte address, written by
@@ -397,7 +398,7 @@ int cir_extend_page_tables(int32_t* page_table, const int32_t* seq_lens, const i
  * of it is written, q_out included.  Two tokens must not share a slot, and q_out, unless it is
  * q at q's strides, overlaps no input; strides that lay its heads on one another are refused,
  * and so are pools that overlap.  head_dim even and <= 256, rotary_dim even and <=
- * head_dim, tokens <= 2^26, heads <= 2^20. */
+ * head_dim, tokens <= 2^26 - 4, heads <= 2^20, slots a multiple of page_size. */
 #define CIR_ROPE_INTERLEAVED 0
 #define CIR_ROPE_HALF 1
 int cir_rope_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,

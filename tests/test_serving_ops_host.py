@@ -173,6 +173,27 @@ def test_rope_refuses_a_part_of_a_page():
             rope(p=x.data_ptr(), slots=slots, page=page)
 
 
+@pytest.mark.parametrize("tokens", [(1 << 26) - 3, 1 << 26])
+def test_rope_refuses_launches_of_2_32_threads(tokens):
+    """Four tokens to a workgroup of 256: 2^26 - 4 are the most whose rounded-up grid stays below 2^32 threads."""
+    p = torch.zeros(64).data_ptr()
+    with pytest.raises(RuntimeError, match=r"2\^26 - 4 tokens"):
+        rope(tokens=tokens, p=p)
+    with pytest.raises(RuntimeError, match="k_pool and v_pool overlap"):
+        rope(tokens=(1 << 26) - 4, p=p)
+
+
+@pytest.mark.parametrize("batch,hq,hkv", [
+    (601, 111662, 3602),            # 2^26 - 2 query vectors, 31 a KV head: the join's 2^24 workgroups of 256
+    (1, 1 << 25, 1 << 25),          # as many KV heads: a workgroup each in the first launch
+    (1, 1 << 24, 1 << 24), (2, 1 << 23, 1 << 23)])  # (its record loop steps by 256 grids: 2^31)
+def test_shared_attention_sizes_past_a_launch_read_each_row_alone(batch, hq, hkv):
+    size = hip.size_call("cir_shared_attention_workspace_bytes", batch, 1, hq, hkv, 128, 16, 1, F16)
+    assert size == hip.size_call("cir_paged_attention_workspace_bytes", batch, hq, 128, 16)
+    less = hip.size_call("cir_shared_attention_workspace_bytes", batch, 1, hq // hkv * 1000, 1000, 128, 16, 1, F16)
+    assert less > hip.size_call("cir_paged_attention_workspace_bytes", batch, hq // hkv * 1000, 128, 16)
+
+
 def test_logprobs_workspace():
     """Nothing where a row has a workgroup of its own; 12 bytes of sums and top_k keys of 8 per split elsewhere."""
     size = lambda *a: hip.size_call("cir_token_logprobs_workspace_bytes", *a)

@@ -161,16 +161,22 @@ int cir_paged_prefill_attention_split(const void* q, const void* k_pool, const v
  * group_rows[g + 1] - 1 (int32 [groups + 1], on the device, ascending, in 0 .. batch) have
  * the same page table entries, and so the same K and V, for their first prefix_lens[g]
  * tokens (int32 [groups], on the device), the entry of the page in which they end among
- * them: where that page is each row's own copy, give the tokens before it.  Each prefix is then read once for the query
- * vectors of all its rows instead of once per row; the result is the attention over each
- * row's whole context, whatever part of it is shared.  The pages of a prefix are taken from
- * the group's first row; sharing stops at that row's length, and a row shorter than the
- * prefix, a group of one row and rows in no group read all of their context alone.
+ * them: where that page is each row's own copy, give the tokens before it.  Each prefix is
+ * then read once for the query vectors of all its rows instead of once per row; the result is
+ * the attention over each row's whole context, whatever part of it is shared.  The pages of a
+ * prefix are taken from the group's first row; sharing stops at that row's length, and a row
+ * shorter than the prefix, a group of one row and rows in no group read all of their context
+ * alone.
  * group_rows out of order switch sharing off.  A sequence with seq_len 0 yields zeros, one
  * whose scores are all -inf NaN.
  * Shared: fp16 pools and q on 16-byte addresses, out on 8, head_dim 128, page_size a multiple
  * of 16, up to 32 query heads per KV head, 2048 rows, 256 groups, fewer than 2^23 KV heads and
- * 2^26 - 3 query vectors (batch * num_heads).  Other calls run
+ * 2^26 - 3 query vectors (batch * num_heads), max_pages * page_size / 16 * (page_size / 16)
+ * < 2^32, and work that an axis of 2^25 blocks holds at the table's full width, with
+ * G = num_heads / num_kv_heads:
+ *   (max_pages * page_size / 32 + 7) * (batch + groups + batch * G / 128) < 2^25
+ * (at G = 8 tables of 480 thousand tokens for 2048 rows, of 7 million for 128; a wider table
+ * stops the sharing even where lengths are short).  Other calls run
  * cir_paged_decode_attention (every row reads its prefix; scores that are all -inf as there).
  * A row's last bits depend on the batch it is in.
  * workspace: cir_shared_attention_workspace_bytes bytes on a 16-byte address, written by

@@ -16,13 +16,18 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// Per-thread text of the last argument error (read by cir_last_error_string).
+// Per-thread text of the last error (read by cir_last_error_string).
 void set_error(const char* fmt, ...);
 
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
-// Launch-status helper: returns the launch error of the most recent launch.
-inline int launch_status() { return static_cast<int>(hipGetLastError()); }
+// Launch-status helper: returns the launch error of the most recent launch, and leaves its text (an earlier argument
+// error's would be read beside it).
+inline int launch_status() {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) set_error("launch failed: %s", hipGetErrorString(e));
+  return static_cast<int>(e);
+}
 
 #define CIR_CHECK_ARG(cond, ...)                 \
   do {                                           \

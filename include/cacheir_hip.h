@@ -4,8 +4,8 @@
  * Conventions (modelled on the reference's only C-ABI kernel boundary,
  * cpp/src/cacheir_cuda_kernels.cu:273-411):
  *   - every entry point returns an int status: 0 (hipSuccess) or a hipError_t
- *     value; argument errors return hipErrorInvalidValue (1) and set the text
- *     returned by cir_last_error_string();
+ *     value; argument errors return hipErrorInvalidValue (1); an error sets the
+ *     text returned by cir_last_error_string();
  *   - all pointers are device pointers owned by the caller; nothing is allocated
  *     or freed inside the library; scratch memory is passed in as `workspace`
  *     with its size from the matching *_workspace_bytes() call;

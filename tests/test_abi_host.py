@@ -504,3 +504,15 @@ def test_row_packer_matches_reference_restatement(bits, cols):
     assert np.array_equal(packed, ref["packed_values"])
     assert np.array_equal(scales, ref["scales"]) and np.array_equal(zps, ref["zero_points"])
     assert row_bits("int4_awq") == 4 and row_bits("gptq") == 4 and row_bits("int8") == 8 and row_bits("q4_0") is None
+
+
+@pytest.mark.skipif(not hip.library_path().exists(), reason="libcacheir_hip.so not built")
+@pytest.mark.skipif(torch.cuda.device_count() > 0, reason="the launch has to fail, for want of a GPU")
+def test_a_failed_launch_does_not_report_an_earlier_argument_error():
+    """The text beside a launch's status is that status', not the one that an earlier refusal left."""
+    p = torch.zeros(64).data_ptr()
+    with pytest.raises(RuntimeError, match="bad sizes"):
+        hip.call("cir_argmax", p, 3, p, 1, 4, None)
+    with pytest.raises(RuntimeError) as e:
+        hip.call("cir_argmax", p, 4, p, 1, 4, None)
+    assert "bad sizes" not in str(e.value) and "status 1:" not in str(e.value) and "launch" in str(e.value), e.value

@@ -53,6 +53,12 @@ def _fits(t, dev: int, dtype: torch.dtype, shape: tuple) -> bool:
     return t.get_device() == dev and t.dtype is dtype and t.shape == shape and t.is_contiguous()
 
 
+def _int32(*sizes: int) -> None:
+    """Sizes that go to the library as C ints (ctypes passes the low 32 bits of larger ones)."""
+    if max(sizes) >= 1 << 31:
+        _req(False, f"sizes {sizes} do not fit 32 bits")
+
+
 def _tensors(device: torch.device, **named: tuple) -> None:
     """Each of ``name=(tensor, dtype, shape)``: contiguous, on ``device``, of that dtype and shape."""
     for name, (t, dtype, shape) in named.items():
@@ -243,6 +249,7 @@ def paged_decode_attention_shared(q, k_pool, v_pool, page_table, seq_lens, group
     batch, num_heads, head_dim = qs
     _, kvh, psize, _ = ps
     max_pages = ts[1]
+    _int32(batch, num_heads, kvh, head_dim, psize, max_pages, groups)
     if out is None:
         out = torch.empty_like(q)
     elif not _fits(out, dev, dt, q.shape):
@@ -301,6 +308,7 @@ def extend_page_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, new_tok
                  free_slots=(free_slots, i32, (free_slots.numel(),)), free_head=(free_head, i32, (1,)))
     batch, max_pages = shape
     _req(page_size > 0 and max_tokens >= 0, "page_size must be positive and max_tokens not negative")
+    _int32(batch, max_pages, page_size, max_tokens, free_slots.numel())
     if out is None:
         out = StepTables.empty(batch, max_tokens, page_table.device)
     else:
@@ -381,6 +389,7 @@ def rope_append(q, k, v, positions, slot_map, inv_freq, k_pool, v_pool, *, layou
         _req(False, f"layout must be one of {sorted(hip.ROPE_LAYOUTS)}")
     tokens, heads, dim = qs
     slots, kvh, psize, _ = ps
+    _int32(tokens, heads, kvh, dim, psize)
     if out is None:
         out = q.new_empty(qs)
         ot = (heads * dim, dim)
@@ -735,6 +744,7 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor | None, top_k: int = 
     _req(logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1),
          "logits must be [rows, vocab] with contiguous rows")
     rows, vocab = logits.shape
+    _int32(rows, vocab)
     ld = logits.stride(0) if rows > 1 else vocab
     _req(ld >= vocab, "logits rows overlap")
     if not (0 <= top_k <= 64 and top_k <= vocab):

@@ -883,6 +883,28 @@ def test_pages_past_32_bit_offsets(device):
         assert torch.equal(a, b)
 
 
+def test_sizes_past_32_bits_are_refused(device):
+    """Sizes that a C int does not hold (ctypes would pass their low 32 bits: a vocabulary of 5 for 2^32 + 5, the first
+    page for a table of 2^32 + 1)."""
+    from cacheir_amd import kernels
+
+    far = (1 << 32) + 5
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device=device)
+    for kw in (dict(page_size=far, max_tokens=4), dict(page_size=16, max_tokens=far)):
+        with pytest.raises(ValueError, match="32 bits"):
+            kernels.extend_page_tables(i32(2, 4), i32(2), i32(2), i32(8), i32(1), **kw)
+    with pytest.raises(ValueError, match="32 bits"):
+        kernels.token_logprobs(torch.empty((1, far), dtype=torch.float16, device=device), None, 3)
+    q, pool = (torch.zeros(s, dtype=torch.float16, device=device) for s in ((1, 8, 128), (4, 2, 16, 128)))
+    with pytest.raises(ValueError, match="32 bits"):
+        kernels.paged_decode_attention_shared(q, pool, pool, torch.empty((1, far), dtype=torch.int32, device=device), i32(1),
+                                              i32(2), i32(1))
+    k, none = (torch.empty((n, far, 2), dtype=torch.float16, device=device) for n in (1, 0))
+    with pytest.raises(ValueError, match="32 bits"):
+        kernels.rope_append(torch.zeros((1, 1, 2), dtype=torch.float16, device=device), k, k, i32(1), i32(1).long(),
+                            torch.zeros(1, dtype=torch.float64, device=device), none.unsqueeze(2), none.unsqueeze(2))
+
+
 # ------------------------------------------------------------------- together --
 def test_decode_steps_of_the_operators_together(device):
     """Samples of two prompts: pages and slots built on the GPU, rotary append, attention over the shared prefixes and

@@ -178,6 +178,14 @@ def test_shared_attention_sizes_that_read_each_row_alone(device, dtype, d, psize
     check_shared(case, run_shared(case, device))
 
 
+@pytest.mark.parametrize("rows,groups", [(2048, 256), (2049, 200), (514, 257)])
+def test_shared_attention_at_the_limits_of_rows_and_groups(device, rows, groups):
+    """The most rows and groups that share, and one more of each (every row alone)."""
+    sizes = [rows // groups + (g < rows % groups) for g in range(groups)]
+    case = shared_case(18, [(n, 32 * (g % 4)) for g, n in enumerate(sizes)], [b % 37 for b in range(rows)], 2, 1)
+    check_shared(case, run_shared(case, device, check_tables=True))
+
+
 def test_shared_attention_pools_off_16_bytes(device):
     case = shared_case(7, [(3, 96)], [1, 20, 17], 8, 2)
     dev = {k: v.to(device) for k, v in case.items()}
@@ -569,6 +577,17 @@ def test_rope_append(device, tokens, hq, hkv, d, rot, layout, dtype, kvdt, psize
     again = kernels.rope_append(dq, dk, dv, pos.to(device), slots.to(device), freq, kp, vp, layout=layout, factor=factor,
                                 out=dq)
     assert torch.equal(again[live.to(device)], got[live.to(device)])
+
+
+@pytest.mark.parametrize("tokens,hq,hkv,d,rot,layout,dtype,kvdt", [
+    (5, 8, 8, 80, 20, "half", torch.float16, torch.float16),         # 10 pairs: no whole vectors of 4 or 8
+    (9, 8, 8, 80, 20, "interleaved", torch.float16, torch.float32),
+    (6, 4, 2, 128, 36, "half", torch.float32, torch.float16),
+    (7, 16, 8, 96, 24, "half", torch.float16, torch.float16),        # vectors of 4 where the pools would take 8
+    (130, 3, 1, 80, 78, "half", torch.float16, torch.float16),
+])
+def test_rope_append_of_parts_that_are_no_whole_vectors(device, tokens, hq, hkv, d, rot, layout, dtype, kvdt):
+    test_rope_append(device, tokens, hq, hkv, d, rot, layout, dtype, kvdt, 16)
 
 
 def test_rope_append_matches_the_step_epilogue(device):

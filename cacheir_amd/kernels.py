@@ -48,8 +48,8 @@ def _call_on(dev: int, name: str, *args) -> None:
 
 def _fits(t, dev: int, dtype: torch.dtype, shape: tuple) -> bool:
     """A contiguous tensor of this type and shape on GPU ``dev``: the test of ``_tensors`` without its messages.  The
-    wrappers of small launches ask this first (0.4 us a tensor against 1.5: page tables of 128 rows took 32 us of the host
-    for 8 of the GPU, now 12.5) and look for what is wrong only if something is."""
+    wrappers of small launches ask this first (0.4 us a tensor against 1.5: page tables of 128 rows, 4.3 us of the GPU, took
+    32 us of the host, now 12.5) and look for what is wrong only if something is."""
     return t.get_device() == dev and t.dtype is dtype and t.shape == shape and t.is_contiguous()
 
 
@@ -374,7 +374,7 @@ def rope_append(q, k, v, positions, slot_map, inv_freq, k_pool, v_pool, *, layou
     at ``slot_map`` (int64, a token's page * page_size + offset; outside the pools: padding, nothing is written).  The
     first ``2 * inv_freq.numel()`` dims of a head turn, in pairs (2i, 2i + 1) (``"interleaved"``) or halves apart
     (``"half"``); cos and sin are multiplied by ``factor``.  q, k and v may be views (any token and head stride, as the
-    columns of one QKV projection); ``out`` may be q.  Returns the turned q."""
+    columns of one QKV projection); ``out`` may be q, and otherwise overlaps no input.  Returns the turned q."""
     dev, dt, kdt = q.get_device(), q.dtype, k_pool.dtype
     qs, ks, ps, fs = q.shape, k.shape, k_pool.shape, inv_freq.shape
     qt, kt, vt = q.stride(), k.stride(), v.stride()
@@ -737,7 +737,8 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor | None, top_k: int = 
                    workspace: torch.Tensor | None = None) -> TokenLogprobs:
     """Log probabilities of ``ids`` (int64 ``[rows]``; an id outside the vocabulary gives NaN), entropy and the ``top_k``
     (0..64) most likely tokens of each row of ``logits`` (float32 or float16 ``[rows, vocab]``, any row stride) in one
-    pass.  Ties go to the lowest id, NaN counts as the largest logit; see ``cir_token_logprobs``."""
+    pass, for fewer than 2**24 rows.  Ties go to the lowest id, NaN counts as the largest logit; see
+    ``cir_token_logprobs``."""
     _req(isinstance(logits, torch.Tensor), "logits must be a torch.Tensor", TypeError)
     dev = logits.get_device()
     _req(dev >= 0, "logits must be on the GPU")

@@ -44,7 +44,7 @@ constexpr int kMinChunk = 4096;   // logits of a workgroup that shares its row w
 // product has just written, 14.6 -> 15.4).
 constexpr size_t kCacheBytes = (size_t)256 << 20;
 constexpr int kManyRows = 1024;   // rows of one wavefront each, where they are short
-constexpr int kMaxRows = 1 << 24; // (rows * kThreads < 2^32)
+constexpr int kMaxRows = 1 << 24;  // (rows * kThreads < 2^32)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // 2^-300 is zero in fp32: y below it adds nothing, and 0 * y stays 0 for x = -inf.
 constexpr float kFloor = -300.f;

@@ -19,7 +19,8 @@ OBJ = PKG / "_build"
 LIB_DIR = PKG / "_lib"
 LIB = LIB_DIR / "libcacheir_hip.so"
 SOURCES = ["attention.hip", "qgemm.hip", "qgemm_xl.hip", "rowops.hip", "shared_attention.hip", "step_inputs.hip",
-           "logprobs.hip", "probe.hip"]
+           "logprobs.hip", "drafts.hip", "adjust_logits.hip", "tree_attention.hip",
+           "probe.hip"]
 ARCH = os.environ.get("CACHEIR_HIP_ARCH", "gfx950")
 
 

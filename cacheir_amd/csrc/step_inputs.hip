@@ -173,6 +173,16 @@ __device__ __forceinline__ void store_vec(T* p, const float (&y)[N]) {
   *reinterpret_cast<vt*>(p) = x;
 }
 
+// factor (cos, sin) of pos * f: the product reduced by 2 pi rint(a / 2 pi), 2 pi in two parts
+__device__ __forceinline__ float2 turn_of(int pos, double f, float factor) {
+  const double a = (double)pos * f;
+  const double n = rint(a * 0.15915494309189535);
+  const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586, a));
+  float s, c;
+  sincosf((float)r, &s, &c);
+  return make_float2(c * factor, s * factor);
+}
+
 struct RopeIn {
   const void *q, *k, *v;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head;  // strides, elements
@@ -189,13 +199,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_append_kernel(
   const int half = rot / 2;
   for (int i = threadIdx.x; i < nt * half; i += kRopeThreads) {
     const int u = i / half, p = i - u * half;
-    const double a = (double)positions[t0 + u] * freq[p];
-    // a - 2 pi rint(a / 2 pi), 2 pi in two parts
-    const double n = rint(a * 0.15915494309189535);
-    const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586, a));
-    float s, c;
-    sincosf((float)r, &s, &c);
-    sm_cs[u][p] = make_float2(c * factor, s * factor);
+    sm_cs[u][p] = turn_of(positions[t0 + u], freq[p], factor);
   }
   if ((int)threadIdx.x < nt) {
     const int64_t s = slot_map[t0 + threadIdx.x];
@@ -267,6 +271,130 @@ __global__ __launch_bounds__(kRopeThreads) void rope_append_kernel(
   }
 }
 
+// ---------------------------------------------------- norm and rotary append --
+// y = factor * R(pos * f_i) (x / sqrt(mean x^2 + eps) * w), heads of q and k; v is copied: the rotary append with the
+// norm of each head before the turn, x read once and y rounded once.  A head is taken by LPH lanes (a power of two, items
+// of NP pairs as above, at most two a lane), which join their sums of squares by shuffles, so nothing passes through LDS
+// but the sines.  A lane keeps its own part of both weights.
+struct NormIn {
+  const void *qw, *kw;
+  int wf32;  // weights in fp32 (else fp16)
+  float eps;
+};
+constexpr int kNormItems = 2;
+
+template <typename T, typename TK, int NP>
+__global__ __launch_bounds__(kRopeThreads) void norm_rope_append_kernel(
+    RopeIn in, NormIn nm, const int32_t* __restrict__ positions, const int64_t* __restrict__ slot_map,
+    const double* __restrict__ freq, float factor, T* q_out, TK* __restrict__ kp, TK* __restrict__ vp, int tokens,
+    int Hq, int Hkv, int D, int rot, int halves, int P, int64_t slots, int lph) {
+  __shared__ float2 sm_cs[kTokens][kMaxDim / 2];
+  __shared__ int64_t sm_at[kTokens];  // pool element of the token's row in KV head 0 (negative: padding)
+  const int t0 = blockIdx.x * kTokens, nt = min(kTokens, tokens - t0);
+  const int half = rot / 2;
+  const int per_head = D / 2 / NP;
+  const int lane = threadIdx.x & (lph - 1), group = threadIdx.x / lph, groups = kRopeThreads / lph;
+  // The lane's items: pair p0 = c NP on, whose elements are lo .. lo + NP - 1 and hi .. hi + NP - 1.
+  int lo[kNormItems], hi[kNormItems];
+  bool live[kNormItems];
+  float qw[kNormItems][2 * NP], kw[kNormItems][2 * NP];
+#pragma unroll
+  for (int i = 0; i < kNormItems; ++i) {
+    const int c = lane + i * lph, p0 = c * NP;
+    live[i] = c < per_head;
+    const bool apart = halves && p0 < half;
+    lo[i] = apart ? p0 : 2 * p0;
+    hi[i] = apart ? p0 + half : 2 * p0 + NP;
+    if (live[i]) {
+#pragma unroll
+      for (int e = 0; e < 2 * NP; ++e) {
+        const int at = e < NP ? lo[i] + e : hi[i] + e - NP;
+        qw[i][e] = nm.wf32 ? ((const float*)nm.qw)[at] : to_f32(((const f16*)nm.qw)[at]);
+        kw[i][e] = nm.wf32 ? ((const float*)nm.kw)[at] : to_f32(((const f16*)nm.kw)[at]);
+      }
+    }
+  }
+  for (int i = threadIdx.x; i < nt * half; i += kRopeThreads) {
+    const int u = i / half, p = i - u * half;
+    sm_cs[u][p] = turn_of(positions[t0 + u], freq[p], factor);
+  }
+  if ((int)threadIdx.x < nt) {
+    const int64_t s = slot_map[t0 + threadIdx.x];
+    int64_t at = -1;
+    if (s >= 0 && s < slots) {
+      const int64_t page = s / P;
+      at = (page * Hkv * P + (s - page * P)) * (int64_t)D;
+    }
+    sm_at[threadIdx.x] = at;
+  }
+  __syncthreads();
+  const int heads = Hq + 2 * Hkv, share = (heads + gridDim.y - 1) / gridDim.y;
+  const int h0 = blockIdx.y * share, n = max(0, min(heads, h0 + share) - h0);
+  const float inv_d = 1.f / (float)D;
+  for (int id = group; id < nt * n; id += groups) {  // (the lanes of a head stay together)
+    const int u = id / n, h = h0 + id - u * n;
+    const int64_t at = sm_at[u];
+    if (at < 0) continue;
+    const int64_t tok = t0 + u;
+    const T* src = h < Hq         ? (const T*)in.q + tok * in.q_token + h * in.q_head
+                   : h < Hq + Hkv ? (const T*)in.k + tok * in.k_token + (h - Hq) * in.k_head
+                                  : (const T*)in.v + tok * in.v_token + (h - Hq - Hkv) * in.v_head;
+    float x[kNormItems][2 * NP], sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kNormItems; ++i) {
+      if (!live[i]) continue;
+      const Vec<T, NP> a = load_vec<T, NP>(src + lo[i]), b = load_vec<T, NP>(src + hi[i]);
+#pragma unroll
+      for (int e = 0; e < NP; ++e) {
+        x[i][e] = to_f32(a.v[e]);
+        x[i][NP + e] = to_f32(b.v[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 2 * NP; ++e) sum = fmaf(x[i][e], x[i][e], sum);
+    }
+    if (h < Hq + Hkv) {
+      for (int off = lph >> 1; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+      const float r = 1.f / sqrtf(fmaf(sum, inv_d, nm.eps));
+      const bool is_q = h < Hq;
+#pragma unroll
+      for (int i = 0; i < kNormItems; ++i) {
+        if (!live[i]) continue;
+        const int p0 = (lane + i * lph) * NP;
+#pragma unroll
+        for (int e = 0; e < 2 * NP; ++e) x[i][e] = x[i][e] * r * (is_q ? qw[i][e] : kw[i][e]);
+        if (p0 >= half) continue;
+#pragma unroll
+        for (int e = 0; e < NP; ++e) {
+          const float2 cs = sm_cs[u][p0 + e];
+          const int re = halves ? e : 2 * e, im = halves ? NP + e : 2 * e + 1;
+          const float a = x[i][re], b = x[i][im];
+          x[i][re] = as_f32_value(fmaf(a, cs.x, -(b * cs.y)));
+          x[i][im] = as_f32_value(fmaf(a, cs.y, b * cs.x));
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kNormItems; ++i) {
+      if (!live[i]) continue;
+      float ya[NP], yb[NP];
+#pragma unroll
+      for (int e = 0; e < NP; ++e) {
+        ya[e] = as_f32_value(x[i][e]);
+        yb[e] = as_f32_value(x[i][NP + e]);
+      }
+      if (h < Hq) {
+        T* dst = q_out + tok * in.o_token + h * in.o_head;
+        store_vec<T, NP>(dst + lo[i], ya);
+        store_vec<T, NP>(dst + hi[i], yb);
+      } else {
+        TK* dst = (h < Hq + Hkv ? kp + (int64_t)(h - Hq) * P * D : vp + (int64_t)(h - Hq - Hkv) * P * D) + at;
+        store_vec<TK, NP>(dst + lo[i], ya);
+        store_vec<TK, NP>(dst + hi[i], yb);
+      }
+    }
+  }
+}
+
 // Whether any two of the heads at t * ts + h * hs (t < nt, h < nh; `len` elements each) overlap: some (i, j) != (0, 0),
 // |i| < nt, |j| < nh, has |i ts + j hs| < len.
 bool heads_overlap(int64_t ts, int nt, int64_t hs, int nh, int len) {
@@ -287,6 +415,67 @@ bool heads_overlap(int64_t ts, int nt, int64_t hs, int nh, int len) {
     if ((i < na && rest < len) || (i + 1 < na && mag(a) - rest < len)) return true;
   }
   return false;
+}
+
+// What rope_append and norm_rope_append take (a call without tokens passes with null pointers).
+int check_rope(const char* who, const RopeIn& in, int dt, const int32_t* positions, const int64_t* slot_map,
+               const double* inv_freq, int rotary_dim, int layout, void* q_out, void* k_pool, void* v_pool, int kv_dtype,
+               int64_t slots, int tokens, int num_heads, int num_kv_heads, int head_dim, int page_size) {
+  CIR_CHECK_ARG(valid_dt(dt) && valid_dt(kv_dtype), "%s: bad dtype", who);
+  CIR_CHECK_ARG(layout == CIR_ROPE_INTERLEAVED || layout == CIR_ROPE_HALF, "%s: bad layout %d", who, layout);
+  CIR_CHECK_ARG(head_dim > 0 && head_dim <= kMaxDim && head_dim % 2 == 0, "%s: head_dim %d must be even, 2..%d", who,
+                head_dim, kMaxDim);
+  CIR_CHECK_ARG(rotary_dim >= 0 && rotary_dim <= head_dim && rotary_dim % 2 == 0,
+                "%s: rotary_dim %d must be even and at most head_dim", who, rotary_dim);
+  CIR_CHECK_ARG(tokens >= 0 && num_heads >= 0 && num_kv_heads > 0 && page_size > 0 && slots >= 0,
+                "%s: bad sizes", who);
+  CIR_CHECK_ARG(tokens <= kMaxTokens && num_heads <= kMaxHeads && num_kv_heads <= kMaxHeads,
+                "%s: more than 2^26 - 4 tokens or 2^20 heads", who);
+  CIR_CHECK_ARG(slots % page_size == 0, "%s: slots must be whole pages", who);
+  if (tokens == 0) return 0;
+  CIR_CHECK_ARG((num_heads == 0 || (in.q && q_out)) && in.k && in.v && positions && slot_map && k_pool && v_pool &&
+                    (inv_freq || rotary_dim == 0),
+                "%s: null pointer", who);
+  // Written heads that overlap, or q in place at other strides, would be read and written by different threads.
+  CIR_CHECK_ARG(num_heads == 0 || !heads_overlap(in.o_token, tokens, in.o_head, num_heads, head_dim),
+                "%s: heads of q_out overlap", who);
+  CIR_CHECK_ARG(num_heads == 0 || q_out != in.q ||
+                    ((tokens == 1 || in.o_token == in.q_token) &&
+                     (num_heads == 1 || in.o_head == in.q_head)),
+                "%s: q_out is q with other strides", who);
+  const uintptr_t pool_bytes = (uintptr_t)slots * num_kv_heads * head_dim * (kv_dtype == CIR_F16 ? 2 : 4);
+  const uintptr_t k_at = (uintptr_t)k_pool, v_at = (uintptr_t)v_pool;
+  CIR_CHECK_ARG((k_at < v_at ? v_at - k_at : k_at - v_at) >= pool_bytes, "%s: k_pool and v_pool overlap", who);
+  return 0;
+}
+
+// Values in a vector of an item (NP pairs take two): every row, head and half starts on a whole vector.
+int rope_vector(const RopeIn& in, int dt, int rotary_dim, const void* q_out, const void* k_pool, const void* v_pool,
+                int kv_dtype, int num_heads, int head_dim) {
+  const auto aligned = [&](int np) {
+    const int64_t strides = in.q_token | in.q_head | in.k_token | in.k_head | in.v_token | in.v_head | in.o_token | in.o_head;
+    const uintptr_t io = (num_heads ? (uintptr_t)in.q | (uintptr_t)q_out : 0) | (uintptr_t)in.k | (uintptr_t)in.v;
+    const uintptr_t pool = (uintptr_t)k_pool | (uintptr_t)v_pool;
+    return head_dim % (2 * np) == 0 && rotary_dim % (2 * np) == 0 && strides % np == 0 &&
+           io % (np * (dt == CIR_F16 ? 2 : 4)) == 0 && pool % (np * (kv_dtype == CIR_F16 ? 2 : 4)) == 0;
+  };
+  return dt == CIR_F16 && kv_dtype == CIR_F16 && aligned(8) ? 8 : aligned(4) ? 4 : 1;
+}
+
+// go<T, TK, NP>() for these types and vectors.
+template <typename F>
+void by_rope_types(int dt, int kv_dtype, int np, const F& go) {
+  const auto by_pool = [&]<typename T, int NP>() {
+    kv_dtype == CIR_F16 ? go.template operator()<T, f16, NP>() : go.template operator()<T, float, NP>();
+  };
+  if (dt == CIR_F16) {
+    if (np == 8) go.template operator()<f16, f16, 8>();
+    else if (np == 4) by_pool.template operator()<f16, 4>();
+    else by_pool.template operator()<f16, 1>();
+  } else {
+    if (np == 4) by_pool.template operator()<float, 4>();
+    else by_pool.template operator()<float, 1>();
+  }
 }
 
 }  // namespace
@@ -331,64 +520,56 @@ extern "C" int cir_rope_append(const void* q, int64_t q_token_stride, int64_t q_
                                int64_t o_token_stride, int64_t o_head_stride, void* k_pool, void* v_pool, int kv_dtype,
                                int64_t slots, int tokens, int num_heads, int num_kv_heads, int head_dim, int page_size,
                                void* stream) {
-  CIR_CHECK_ARG(valid_dt(dt) && valid_dt(kv_dtype), "rope_append: bad dtype");
-  CIR_CHECK_ARG(layout == CIR_ROPE_INTERLEAVED || layout == CIR_ROPE_HALF, "rope_append: bad layout %d", layout);
-  CIR_CHECK_ARG(head_dim > 0 && head_dim <= kMaxDim && head_dim % 2 == 0, "rope_append: head_dim %d must be even, 2..%d",
-                head_dim, kMaxDim);
-  CIR_CHECK_ARG(rotary_dim >= 0 && rotary_dim <= head_dim && rotary_dim % 2 == 0,
-                "rope_append: rotary_dim %d must be even and at most head_dim", rotary_dim);
-  CIR_CHECK_ARG(tokens >= 0 && num_heads >= 0 && num_kv_heads > 0 && page_size > 0 && slots >= 0,
-                "rope_append: bad sizes");
-  CIR_CHECK_ARG(tokens <= kMaxTokens && num_heads <= kMaxHeads && num_kv_heads <= kMaxHeads,
-                "rope_append: more than 2^26 - 4 tokens or 2^20 heads");
-  CIR_CHECK_ARG(slots % page_size == 0, "rope_append: slots must be whole pages");
-  if (tokens == 0) return 0;
-  CIR_CHECK_ARG((num_heads == 0 || (q && q_out)) && k && v && positions && slot_map && k_pool && v_pool &&
-                    (inv_freq || rotary_dim == 0),
-                "rope_append: null pointer");
-  // Written heads that overlap, or q in place at other strides, would be read and written by different threads.
-  CIR_CHECK_ARG(num_heads == 0 || !heads_overlap(o_token_stride, tokens, o_head_stride, num_heads, head_dim),
-                "rope_append: heads of q_out overlap");
-  CIR_CHECK_ARG(num_heads == 0 || q_out != q ||
-                    ((tokens == 1 || o_token_stride == q_token_stride) &&
-                     (num_heads == 1 || o_head_stride == q_head_stride)),
-                "rope_append: q_out is q with other strides");
-  const uintptr_t pool_bytes = (uintptr_t)slots * num_kv_heads * head_dim * (kv_dtype == CIR_F16 ? 2 : 4);
-  const uintptr_t k_at = (uintptr_t)k_pool, v_at = (uintptr_t)v_pool;
-  CIR_CHECK_ARG((k_at < v_at ? v_at - k_at : k_at - v_at) >= pool_bytes, "rope_append: k_pool and v_pool overlap");
-  hipStream_t s = as_stream(stream);
   const RopeIn in{q, k, v, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride,
                   o_token_stride, o_head_stride};
-  // Items of NP pairs take two vectors of NP values, so every row, head and half has to start on a whole vector.
-  const auto aligned = [&](int np) {
-    const int64_t strides = q_token_stride | q_head_stride | k_token_stride | k_head_stride | v_token_stride |
-                            v_head_stride | o_token_stride | o_head_stride;
-    const uintptr_t io = (num_heads ? (uintptr_t)q | (uintptr_t)q_out : 0) | (uintptr_t)k | (uintptr_t)v;
-    const uintptr_t pool = (uintptr_t)k_pool | (uintptr_t)v_pool;
-    return head_dim % (2 * np) == 0 && rotary_dim % (2 * np) == 0 && strides % np == 0 &&
-           io % (np * (dt == CIR_F16 ? 2 : 4)) == 0 && pool % (np * (kv_dtype == CIR_F16 ? 2 : 4)) == 0;
-  };
-  const int np = dt == CIR_F16 && kv_dtype == CIR_F16 && aligned(8) ? 8 : aligned(4) ? 4 : 1;
+  if (const int bad = check_rope("rope_append", in, dt, positions, slot_map, inv_freq, rotary_dim, layout, q_out, k_pool,
+                                 v_pool, kv_dtype, slots, tokens, num_heads, num_kv_heads, head_dim, page_size))
+    return bad;
+  if (tokens == 0) return 0;
+  hipStream_t s = as_stream(stream);
+  const int np = rope_vector(in, dt, rotary_dim, q_out, k_pool, v_pool, kv_dtype, num_heads, head_dim);
   const unsigned blocks = (unsigned)((tokens + kTokens - 1) / kTokens);
   const int items = (num_heads + 2 * num_kv_heads) * (head_dim / 2 / np);
   // Few tokens: a workgroup takes a share of the heads (one item per thread and token at least).
   const unsigned shares = (unsigned)max(1, min(min(16, (items * kTokens + kRopeThreads - 1) / kRopeThreads),
                                                (int)(512 / blocks)));
-  const auto go = [&]<typename T, typename TK, int NP>() {
+  by_rope_types(dt, kv_dtype, np, [&]<typename T, typename TK, int NP>() {
     rope_append_kernel<T, TK, NP><<<dim3(blocks, shares), kRopeThreads, 0, s>>>(
         in, positions, slot_map, inv_freq, factor, (T*)q_out, (TK*)k_pool, (TK*)v_pool, tokens, num_heads, num_kv_heads,
         head_dim, rotary_dim, layout == CIR_ROPE_HALF, page_size, slots);
-  };
-  const auto by_pool = [&]<typename T, int NP>() {
-    kv_dtype == CIR_F16 ? go.template operator()<T, f16, NP>() : go.template operator()<T, float, NP>();
-  };
-  if (dt == CIR_F16) {
-    if (np == 8) go.template operator()<f16, f16, 8>();
-    else if (np == 4) by_pool.template operator()<f16, 4>();
-    else by_pool.template operator()<f16, 1>();
-  } else {
-    if (np == 4) by_pool.template operator()<float, 4>();
-    else by_pool.template operator()<float, 1>();
-  }
+  });
+  return launch_status();
+}
+
+extern "C" int cir_norm_rope_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                                    int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                                    int64_t v_head_stride, int dt, const void* q_weight, const void* k_weight, int wdt,
+                                    float eps, const int32_t* positions, const int64_t* slot_map, const double* inv_freq,
+                                    float factor, int rotary_dim, int layout, void* q_out, int64_t o_token_stride,
+                                    int64_t o_head_stride, void* k_pool, void* v_pool, int kv_dtype, int64_t slots,
+                                    int tokens, int num_heads, int num_kv_heads, int head_dim, int page_size,
+                                    void* stream) {
+  const RopeIn in{q, k, v, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride,
+                  o_token_stride, o_head_stride};
+  CIR_CHECK_ARG(valid_dt(wdt), "norm_rope_append: bad dtype");
+  if (const int bad = check_rope("norm_rope_append", in, dt, positions, slot_map, inv_freq, rotary_dim, layout, q_out,
+                                 k_pool, v_pool, kv_dtype, slots, tokens, num_heads, num_kv_heads, head_dim, page_size))
+    return bad;
+  if (tokens == 0) return 0;
+  CIR_CHECK_ARG((q_weight || num_heads == 0) && k_weight, "norm_rope_append: null pointer");
+  const int np = rope_vector(in, dt, rotary_dim, q_out, k_pool, v_pool, kv_dtype, num_heads, head_dim);
+  const int per_head = head_dim / 2 / np;  // (at most 128: two items a lane)
+  int lph = 1;
+  while (lph < per_head && lph < 64) lph *= 2;
+  const unsigned blocks = (unsigned)((tokens + kTokens - 1) / kTokens);
+  // Few tokens: a workgroup takes a share of the heads (a head per group of lanes and token at least).
+  const int heads = num_heads + 2 * num_kv_heads, groups = kRopeThreads / lph;
+  const unsigned shares = (unsigned)max(1, min(min(64, (heads * kTokens + groups - 1) / groups), (int)(512 / blocks)));
+  by_rope_types(dt, kv_dtype, np, [&]<typename T, typename TK, int NP>() {
+    norm_rope_append_kernel<T, TK, NP><<<dim3(blocks, shares), kRopeThreads, 0, as_stream(stream)>>>(
+        in, NormIn{num_heads ? q_weight : k_weight, k_weight, wdt == CIR_F32, eps}, positions, slot_map, inv_freq, factor,
+        (T*)q_out, (TK*)k_pool, (TK*)v_pool, tokens, num_heads, num_kv_heads, head_dim, rotary_dim,
+        layout == CIR_ROPE_HALF, page_size, slots, lph);
+  });
   return launch_status();
 }

@@ -54,6 +54,15 @@ _SIGNATURES = {
     "cir_shared_attention_workspace_bytes": (_c_size, [_c_int] * 8),
     "cir_paged_decode_attention_shared": (_c_int, [_vp] * 7 + [_c_int, _vp, _vp, _c_size] + [_c_int] * 6 +
                                           [_c_float, _c_int, _vp]),
+    "cir_tree_attention_workspace_bytes": (_c_size, [_c_int] * 8),
+    "cir_paged_tree_attention": (_c_int, [_vp] * 8 + [_c_int, _vp, _vp, _c_size] + [_c_int] * 7 + [_c_float, _c_int, _vp]),
+    "cir_adjust_logits": (_c_int, [_vp, _c_i64, _vp, _c_i64, _c_int, _vp, _vp, _vp, _vp, _c_int, _vp, _vp, _c_int, _vp,
+                                   _vp, _vp, _vp, _vp, _c_int, _vp, _c_int, _c_int, _c_int, _vp]),
+    "cir_draft_tree": (_c_int, [_vp] * 6 + [_c_int] * 3 + [_vp]),
+    "cir_accept_drafts": (_c_int, [_vp] * 13 + [_c_int, _c_i64, _vp, _c_int, _vp] + [_c_int] * 8 + [_vp]),
+    "cir_norm_rope_append": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_int, _vp, _vp,
+                                      _c_int, _c_float, _vp, _vp, _vp, _c_float, _c_int, _c_int, _vp, _c_i64, _c_i64, _vp,
+                                      _vp, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _vp]),
     "cir_token_logprobs_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int]),
     "cir_token_logprobs": (_c_int, [_vp, _c_int, _c_i64, _vp, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _c_size,
                                     _vp]),

@@ -268,6 +268,79 @@ def paged_decode_attention_shared(q, k_pool, v_pool, page_table, seq_lens, group
     return out
 
 
+def tree_attention_workspace(tokens: int, batch: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
+                             max_pages: int, kv_dtype: torch.dtype, device) -> torch.Tensor:
+    """Workspace of ``paged_tree_attention`` at these sizes (one per call that may overlap another)."""
+    n = hip.size_call("cir_tree_attention_workspace_bytes", tokens, batch, num_heads, num_kv_heads, head_dim, page_size,
+                      max_pages, hip.dtype_code(kv_dtype))
+    return torch.empty(max(n, 4), dtype=torch.uint8, device=device)
+
+
+def _check_tree(q, k_pool, v_pool, page_table, seq_lens, offsets, counts, masks, check_tables: bool) -> None:
+    for t, n in ((q, "q"), (k_pool, "k_pool"), (masks, "masks")):
+        _cuda(t, n)
+    _req(q.dim() == 3, "q must be [tokens, num_heads, head_dim]")
+    tokens, num_heads, head_dim = q.shape
+    _, _, psize, hd = _check_pool(q, k_pool, v_pool, page_table, seq_lens, num_heads, False)
+    _req(hd == head_dim and page_table.dim() == 2, "shape mismatch")
+    _req(masks.dim() == 2 and masks.shape[0] == tokens, "masks must be [tokens, words]")
+    batch, max_pages = page_table.shape
+    _tensors(q.device, k_pool=(k_pool, q.dtype, k_pool.shape), v_pool=(v_pool, q.dtype, k_pool.shape),
+             page_table=(page_table, torch.int32, page_table.shape), seq_lens=(seq_lens, torch.int32, (batch,)),
+             offsets=(offsets, torch.int32, (batch + 1,)), counts=(counts, torch.int32, (batch,)),
+             masks=(masks, torch.int64, masks.shape))
+    if check_tables:
+        at, n, lens, table = offsets.tolist(), counts.tolist(), seq_lens.tolist(), page_table.cpu()
+        _req(all(a <= b for a, b in zip(at, at[1:])) and 0 <= at[0] and at[-1] <= tokens,
+             "offsets must ascend within the tokens")
+        for b in range(batch):
+            _req(0 <= n[b] <= min(at[b + 1] - at[b], 64 * masks.shape[1], lens[b]),
+                 f"row {b}: counts exceed its tokens, the masks or its length")
+            _req(lens[b] <= max_pages * psize, "seq_lens exceed the page table capacity")
+            used = table[b, : -(-lens[b] // psize)]
+            _req(used.numel() == 0 or (int(used.min()) >= 0 and int(used.max()) < k_pool.shape[0]),
+                 "page_table has slots outside the pool")
+
+
+def paged_tree_attention(q, k_pool, v_pool, page_table, seq_lens, offsets, counts, masks, *, scale: float | None = None,
+                         out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                         check_tables: bool = False) -> torch.Tensor:
+    """Attention of drafted tokens q ``[T, Hq, D]``: row b's are ``q[offsets[b] : offsets[b] + counts[b]]`` (int32
+    ``[B + 1]``, ``[B]``; ``StepTables.offsets`` and ``.granted``), the last of its ``seq_lens[b]`` tokens in the pages.
+    Each sees the tokens before the drafted ones, and drafted token k of its row where bit k % 64 of its
+    ``masks[:, k // 64]`` (int64 ``[T, words]``, ``draft_tree``) is set.  Rows of q that no row counts keep their ``out``.
+    ``check_tables`` checks lengths, offsets and pages on the host (a device sync)."""
+    dev, dt, i32 = q.get_device(), q.dtype, torch.int32
+    qs, ps, ts, ms = q.shape, k_pool.shape, page_table.shape, masks.shape
+    if not (dev >= 0 and len(qs) == 3 and len(ps) == 4 and len(ts) == 2 and len(ms) == 2 and not check_tables
+            and qs[2] == ps[3] and ms[0] == qs[0] and _fits(q, dev, dt, qs) and _fits(k_pool, dev, dt, ps)
+            and _fits(v_pool, dev, dt, ps) and _fits(page_table, dev, i32, ts) and _fits(seq_lens, dev, i32, ts[:1])
+            and _fits(offsets, dev, i32, (ts[0] + 1,)) and _fits(counts, dev, i32, ts[:1])
+            and _fits(masks, dev, torch.int64, ms)):
+        _check_tree(q, k_pool, v_pool, page_table, seq_lens, offsets, counts, masks, check_tables)
+    tokens, num_heads, head_dim = qs
+    _, kvh, psize, _ = ps
+    batch, max_pages = ts
+    words = ms[1]
+    _int32(tokens, num_heads, kvh, head_dim, psize, batch, max_pages, words)
+    code = hip.dtype_code(dt)
+    if out is None:
+        out = torch.empty_like(q)
+    elif not _fits(out, dev, dt, qs):
+        _tensors(q.device, out=(out, dt, qs))
+    if workspace is None:
+        n = hip.size_call("cir_tree_attention_workspace_bytes", tokens, batch, num_heads, kvh, head_dim, psize, max_pages,
+                          code)
+        workspace = torch.empty(max(n, 4), dtype=torch.uint8, device=q.device)
+    else:
+        _check_workspace(workspace, dev)
+    _call_on(dev, "cir_paged_tree_attention", q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr(),
+             seq_lens.data_ptr(), offsets.data_ptr(), counts.data_ptr(), masks.data_ptr(), words, out.data_ptr(),
+             workspace.data_ptr(), workspace.nbytes, tokens, batch, num_heads, kvh, head_dim, psize, max_pages,
+             1.0 / math.sqrt(head_dim) if scale is None else scale, code)
+    return out
+
+
 # ---------------------------------------------------------------- step inputs --
 class StepTables(NamedTuple):
     """What ``extend_page_tables`` writes beside the page table (see ``cir_extend_page_tables``)."""
@@ -368,13 +441,9 @@ def _check_rope(q, k, v, positions, slot_map, inv_freq, k_pool, v_pool) -> None:
     _req(2 * inv_freq.numel() <= dim, f"inv_freq turns {2 * inv_freq.numel()} dims of heads of {dim}")
 
 
-def rope_append(q, k, v, positions, slot_map, inv_freq, k_pool, v_pool, *, layout: str = "interleaved",
-                factor: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
-    """Rotary positions of q ``[T, Hq, D]`` and k ``[T, Hkv, D]`` at ``positions`` and the append of k and v to the pools
-    at ``slot_map`` (int64, a token's page * page_size + offset; outside the pools: padding, nothing is written).  The
-    first ``2 * inv_freq.numel()`` dims of a head turn, in pairs (2i, 2i + 1) (``"interleaved"``) or halves apart
-    (``"half"``); cos and sin are multiplied by ``factor``.  q, k and v may be views (any token and head stride, as the
-    columns of one QKV projection); ``out`` may be q, and otherwise overlaps no input.  Returns the turned q."""
+def _rope_call(name: str, q, k, v, norm: tuple, positions, slot_map, inv_freq, k_pool, v_pool, layout: str,
+               factor: float, out: torch.Tensor | None) -> torch.Tensor:
+    """The checks and the call of ``rope_append`` and ``norm_rope_append`` (``norm``: the latter's arguments)."""
     dev, dt, kdt = q.get_device(), q.dtype, k_pool.dtype
     qs, ks, ps, fs = q.shape, k.shape, k_pool.shape, inv_freq.shape
     qt, kt, vt = q.stride(), k.stride(), v.stride()
@@ -397,10 +466,125 @@ def rope_append(q, k, v, positions, slot_map, inv_freq, k_pool, v_pool, *, layou
         _req(isinstance(out, torch.Tensor) and out.device == q.device and out.shape == q.shape and
              (out.stride(2) == 1 or dim == 1) and out.dtype == dt, "out must be like q")
         ot = out.stride()
-    _call_on(dev, "cir_rope_append", q.data_ptr(), qt[0], qt[1], k.data_ptr(), kt[0], kt[1], v.data_ptr(), vt[0], vt[1],
-             hip.dtype_code(dt), positions.data_ptr(), slot_map.data_ptr(), inv_freq.data_ptr(), factor, 2 * fs[0],
+    _call_on(dev, name, q.data_ptr(), qt[0], qt[1], k.data_ptr(), kt[0], kt[1], v.data_ptr(), vt[0], vt[1],
+             hip.dtype_code(dt), *norm, positions.data_ptr(), slot_map.data_ptr(), inv_freq.data_ptr(), factor, 2 * fs[0],
              hip.ROPE_LAYOUTS[layout], out.data_ptr(), ot[0], ot[1], k_pool.data_ptr(), v_pool.data_ptr(),
              hip.dtype_code(kdt), slots * psize, tokens, heads, kvh, dim, psize)
+    return out
+
+
+def rope_append(q, k, v, positions, slot_map, inv_freq, k_pool, v_pool, *, layout: str = "interleaved",
+                factor: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions of q ``[T, Hq, D]`` and k ``[T, Hkv, D]`` at ``positions`` and the append of k and v to the pools
+    at ``slot_map`` (int64, a token's page * page_size + offset; outside the pools: padding, nothing is written).  The
+    first ``2 * inv_freq.numel()`` dims of a head turn, in pairs (2i, 2i + 1) (``"interleaved"``) or halves apart
+    (``"half"``); cos and sin are multiplied by ``factor``.  q, k and v may be views (any token and head stride, as the
+    columns of one QKV projection); ``out`` may be q, and otherwise overlaps no input.  Returns the turned q."""
+    return _rope_call("cir_rope_append", q, k, v, (), positions, slot_map, inv_freq, k_pool, v_pool, layout, factor, out)
+
+
+def norm_rope_append(q, k, v, q_weight, k_weight, eps: float, positions, slot_map, inv_freq, k_pool, v_pool, *,
+                     layout: str = "interleaved", factor: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``rope_append`` with an RMS norm of each head of q and k before it turns: ``x / sqrt(mean(x ** 2) + eps) *
+    weight``, ``q_weight`` and ``k_weight`` ``[head_dim]`` (float32 or float16).  Rounded once, to the output."""
+    dev, wdt, shape = q.get_device(), q_weight.dtype, q.shape[-1:]
+    if not (dev >= 0 and _fits(q_weight, dev, wdt, shape) and _fits(k_weight, dev, wdt, shape)):
+        _cuda(q, "q") if dev < 0 else None
+        _tensors(q.device, q_weight=(q_weight, wdt, shape), k_weight=(k_weight, wdt, shape))
+    return _rope_call("cir_norm_rope_append", q, k, v, (q_weight.data_ptr(), k_weight.data_ptr(), hip.dtype_code(wdt), eps),
+                      positions, slot_map, inv_freq, k_pool, v_pool, layout, factor, out)
+
+
+# -------------------------------------------------------------- drafted trees --
+class DraftTree(NamedTuple):
+    masks: torch.Tensor      # int64 [tokens, words]: bit k % 64 of word k / 64 where token k of the row is seen
+    positions: torch.Tensor  # int32 [tokens]
+
+
+def draft_tree(parents: torch.Tensor, seq_lens: torch.Tensor, offsets: torch.Tensor, counts: torch.Tensor, *, words: int,
+               out: DraftTree | None = None) -> DraftTree:
+    """What each drafted token sees of its row's tree (itself and its ancestors) and its rotary position, from
+    ``parents`` (int32 ``[T]``, places in the row's tree, negative: it follows the context).  Row b's tokens are
+    ``offsets[b] .. offsets[b] + counts[b] - 1``, up to ``64 * words`` (words 1..4), and the last of its ``seq_lens[b]``;
+    see ``cir_draft_tree``."""
+    dev, i32 = parents.get_device(), torch.int32
+    tokens, batch = parents.numel(), counts.numel()
+    if not (dev >= 0 and _fits(parents, dev, i32, (tokens,)) and _fits(counts, dev, i32, (batch,))
+            and _fits(seq_lens, dev, i32, (batch,)) and _fits(offsets, dev, i32, (batch + 1,))):
+        _cuda(parents, "parents")
+        _tensors(parents.device, parents=(parents, i32, (tokens,)), counts=(counts, i32, (batch,)),
+                 seq_lens=(seq_lens, i32, (batch,)), offsets=(offsets, i32, (batch + 1,)))
+    _req(1 <= words <= 4, f"words must be 1..4 (got {words})")
+    _int32(tokens, batch)
+    if out is None:
+        out = DraftTree(torch.empty((tokens, words), dtype=torch.int64, device=parents.device),
+                        torch.empty(tokens, dtype=i32, device=parents.device))
+    else:
+        _tensors(parents.device, **{"out.masks": (out.masks, torch.int64, (tokens, words)),
+                                    "out.positions": (out.positions, i32, (tokens,))})
+    _call_on(dev, "cir_draft_tree", parents.data_ptr(), seq_lens.data_ptr(), offsets.data_ptr(), counts.data_ptr(),
+             out.masks.data_ptr(), out.positions.data_ptr(), tokens, batch, words)
+    return out
+
+
+class AcceptedDrafts(NamedTuple):
+    accepted: torch.Tensor  # int32 [batch]: drafted tokens that stand, and so tokens said
+    path: torch.Tensor      # int32 [batch, most]: their places in the row's tree, then -1
+    tokens: torch.Tensor    # int64 [batch, most]: what the model chose after each, then -1
+    seq_lens: torch.Tensor  # int32 [batch]: lengths with them
+
+    @classmethod
+    def empty(cls, batch: int, most: int, device) -> "AcceptedDrafts":
+        # one allocation for what is int32
+        accepted, path, lens = torch.empty(batch * (most + 2), dtype=torch.int32,
+                                           device=device).split_with_sizes((batch, batch * most, batch))
+        return cls(accepted, path.view(batch, most), torch.empty((batch, most), dtype=torch.int64, device=device), lens)
+
+
+def accept_drafts(parents: torch.Tensor, drafts: torch.Tensor, targets: torch.Tensor, seq_lens: torch.Tensor,
+                  offsets: torch.Tensor, counts: torch.Tensor, page_table: torch.Tensor, k_pools: torch.Tensor,
+                  v_pools: torch.Tensor, *, most: int, free_slots: torch.Tensor | None = None,
+                  free_head: torch.Tensor | None = None, out: AcceptedDrafts | None = None) -> AcceptedDrafts:
+    """The drafted tokens that the model's choices confirm: from the row's token 0 on, the child whose ``drafts`` (int64
+    ``[T]``) equals ``targets`` (int64 ``[T]``, chosen after each token), ``most`` tokens at most.  K and V of the path
+    move behind the context in the pools of all layers (``[layers, slots, kv_heads, page_size, head_dim]``).  With
+    ``free_slots`` and ``free_head`` (as ``extend_page_tables`` takes them) pages behind the new lengths go back.
+    ``out.seq_lens`` may be ``seq_lens``.  See ``cir_accept_drafts``."""
+    dev, i32, i64 = parents.get_device(), torch.int32, torch.int64
+    tokens, ts, ps, dt = parents.numel(), page_table.shape, k_pools.shape, k_pools.dtype
+    rows = ts[:1]
+    if not (dev >= 0 and len(ts) == 2 and len(ps) == 5 and _fits(parents, dev, i32, (tokens,))
+            and _fits(drafts, dev, i64, (tokens,)) and _fits(targets, dev, i64, (tokens,))
+            and _fits(seq_lens, dev, i32, rows) and _fits(counts, dev, i32, rows)
+            and _fits(offsets, dev, i32, (ts[0] + 1,)) and _fits(page_table, dev, i32, ts)
+            and _fits(k_pools, dev, dt, ps) and _fits(v_pools, dev, dt, ps)):
+        _cuda(parents, "parents")
+        _req(page_table.dim() == 2, "page_table must be [batch, pages]")
+        _req(k_pools.dim() == 5, "pools must be [layers, slots, kv_heads, page_size, head_dim]")
+        _tensors(parents.device, parents=(parents, i32, (tokens,)), drafts=(drafts, i64, (tokens,)),
+                 targets=(targets, i64, (tokens,)), seq_lens=(seq_lens, i32, rows), counts=(counts, i32, rows),
+                 offsets=(offsets, i32, (ts[0] + 1,)), page_table=(page_table, i32, ts), k_pools=(k_pools, dt, ps),
+                 v_pools=(v_pools, dt, ps))
+    batch, max_pages = ts
+    layers, slots, kvh, psize, head_dim = ps
+    _req(1 <= most <= 256, f"most must be 1..256 (got {most})")
+    _int32(tokens, batch, max_pages, layers, kvh, psize, head_dim)
+    _req((free_slots is None) == (free_head is None), "free_slots and free_head go together")
+    total = 0
+    if free_slots is not None:
+        total = free_slots.numel()
+        _tensors(parents.device, free_slots=(free_slots, i32, (total,)), free_head=(free_head, i32, (1,)))
+        _int32(total)
+    if out is None:
+        out = AcceptedDrafts.empty(batch, most, parents.device)
+    else:
+        _tensors(parents.device, **{"out.accepted": (out.accepted, i32, rows), "out.path": (out.path, i32, (batch, most)),
+                                    "out.tokens": (out.tokens, i64, (batch, most)), "out.seq_lens": (out.seq_lens, i32, rows)})
+    _call_on(dev, "cir_accept_drafts", parents.data_ptr(), drafts.data_ptr(), targets.data_ptr(), seq_lens.data_ptr(),
+             offsets.data_ptr(), counts.data_ptr(), page_table.data_ptr(), out.accepted.data_ptr(), out.path.data_ptr(),
+             out.tokens.data_ptr(), out.seq_lens.data_ptr(), k_pools.data_ptr(), v_pools.data_ptr(), hip.dtype_code(dt),
+             slots, hip.ptr(free_slots), total, hip.ptr(free_head), tokens, batch, most, max_pages, layers, kvh, head_dim,
+             psize)
     return out
 
 
@@ -718,6 +902,60 @@ def argmax(logits: torch.Tensor, out=None) -> torch.Tensor:
     if out is None:
         out = torch.empty(rows, dtype=torch.int64, device=logits.device)
     hip.call("cir_argmax", logits.data_ptr(), vocab, out.data_ptr(), rows, vocab, hip.stream_handle())
+    return out
+
+
+def adjust_logits(logits: torch.Tensor, offsets: torch.Tensor | None = None, *, history: torch.Tensor | None = None,
+                  history_lens: torch.Tensor | None = None, prompt_lens: torch.Tensor | None = None,
+                  drafts: torch.Tensor | None = None, masks: torch.Tensor | None = None,
+                  repetition: torch.Tensor | None = None, presence: torch.Tensor | None = None,
+                  frequency: torch.Tensor | None = None, bias_ids: torch.Tensor | None = None,
+                  bias: torch.Tensor | None = None, allowed: torch.Tensor | None = None,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """Penalties for repeated tokens, biases and masks on rows of ``logits`` (float32 or float16 ``[rows, vocab]``, any
+    row stride).  Sequence b has the rows ``offsets[b] .. offsets[b + 1] - 1`` (int32 ``[B + 1]``; None: a row each),
+    tokens ``history[b, : history_lens[b]]`` (int64 ``[B, L]``, int32 ``[B]``; the first ``prompt_lens[b]`` count for
+    ``repetition`` only), and, where ``drafts`` (int64 ``[rows]``) and ``masks`` (``draft_tree``) are given, the drafted
+    tokens on the row's path.  ``repetition``, ``presence``, ``frequency``: float32 ``[B]``; ``bias_ids`` (int64, -1:
+    unused) and ``bias`` (float32) ``[B, K]``; ``allowed``: int32 ``[rows, ceil(vocab / 32)]``, a bit per token.  ``out``
+    may be ``logits``.  See ``cir_adjust_logits``."""
+    _req(isinstance(logits, torch.Tensor), "logits must be a torch.Tensor", TypeError)
+    dev, dt, i32, i64, f32 = logits.get_device(), logits.dtype, torch.int32, torch.int64, torch.float32
+    _req(dev >= 0, "logits must be on the GPU")
+    shape = logits.shape
+    _req(len(shape) == 2 and shape[1] > 0 and (logits.stride(1) == 1 or shape[1] == 1),
+         "logits must be [rows, vocab] with contiguous rows")
+    rows, vocab = shape
+    batch = rows if offsets is None else offsets.numel() - 1
+    width = 0 if history is None else history.shape[-1]
+    listed = 0 if bias_ids is None else bias_ids.shape[-1]
+    words = 0 if masks is None else masks.shape[-1]
+    _int32(rows, vocab, batch, width, listed, words)
+    for name, t, dtype, want in (
+            ("offsets", offsets, i32, (batch + 1,)), ("history", history, i64, (batch, width)),
+            ("history_lens", history_lens, i32, (batch,)), ("prompt_lens", prompt_lens, i32, (batch,)),
+            ("drafts", drafts, i64, (rows,)), ("masks", masks, i64, (rows, words)),
+            ("repetition", repetition, f32, (batch,)), ("presence", presence, f32, (batch,)),
+            ("frequency", frequency, f32, (batch,)), ("bias_ids", bias_ids, i64, (batch, listed)),
+            ("bias", bias, f32, (batch, listed)), ("allowed", allowed, i32, (rows, (vocab + 31) // 32))):
+        if t is not None and not _fits(t, dev, dtype, want):
+            _tensors(logits.device, **{name: (t, dtype, want)})
+    if (history is None) != (history_lens is None) or (drafts is None) != (masks is None) or (bias is None) != (bias_ids is None):
+        _req(False, "history and history_lens, drafts and masks, bias and bias_ids go together")
+    _req(prompt_lens is None or history is not None, "prompt_lens needs history")
+    _req(drafts is None or offsets is not None, "drafts need offsets")
+    ld = logits.stride(0) if rows > 1 else vocab
+    if out is None:
+        out = torch.empty(shape, dtype=dt, device=logits.device)
+        ld_out = vocab
+    else:
+        _req(isinstance(out, torch.Tensor) and out.device == logits.device and out.shape == shape and out.dtype == dt and
+             (out.stride(1) == 1 or vocab == 1), "out must be like logits")
+        ld_out = out.stride(0) if rows > 1 else vocab
+    ptr = hip.ptr
+    _call_on(dev, "cir_adjust_logits", logits.data_ptr(), ld, out.data_ptr(), ld_out, hip.dtype_code(dt), ptr(offsets),
+             ptr(history), ptr(history_lens), ptr(prompt_lens), width, ptr(drafts), ptr(masks), words, ptr(repetition),
+             ptr(presence), ptr(frequency), ptr(bias_ids), ptr(bias), listed, ptr(allowed), rows, batch, vocab)
     return out
 
 

@@ -191,6 +191,32 @@ int cir_paged_decode_attention_shared(const void* q, const void* k_pool, const v
                                       int num_kv_heads, int head_dim, int page_size, int max_pages, float scale,
                                       int kv_dtype, void* stream);
 
+/* Attention of drafted tokens, a tree of them per row, over the paged cache.  Row b holds
+ * seq_lens[b] tokens, its n = counts[b] drafted ones last (their K and V already in the
+ * pages): query row offsets[b] + i of q [tokens, num_heads, head_dim] is its drafted token i
+ * and sees the seq_lens[b] - n tokens before the drafted ones, and drafted token k where bit
+ * k % 64 of masks[offsets[b] + i][k / 64] is set (masks int64 [tokens, words], as
+ * cir_draft_tree writes them, or any others).  Head h reads KV head h / (num_heads /
+ * num_kv_heads).  offsets int32 [batch + 1] and counts int32 [batch] are as
+ * cir_extend_page_tables writes them (offsets, granted); a row has at most
+ * offsets[b + 1] - offsets[b] and 64 * words tokens, words 1..4.  Rows of q that no row
+ * counts are not read and their out is left as it was.  A token that sees nothing yields
+ * zeros, one whose scores are all -inf NaN; K and V that a token does not see do not enter
+ * its result, NaN and infinities among them.  Tokens past the table (max_pages * page_size)
+ * are not seen.  fp16 with head_dim 128 runs on MFMA, other sizes (head_dim <= 256) in fp32
+ * arithmetic.  A row's last bits depend on the batch it is in.  tokens * num_heads < 2^26,
+ * num_kv_heads < 2^16, batch < 2^20.
+ * workspace: cir_tree_attention_workspace_bytes bytes on a 16-byte address (0: NULL will do),
+ * written by the call (calls that overlap need one each); nothing in it needs clearing.
+ * The reference attends one new token a row (cacheir/backends/triton_kernels.py:174-217). */
+size_t cir_tree_attention_workspace_bytes(int tokens, int batch, int num_heads, int num_kv_heads, int head_dim,
+                                          int page_size, int max_pages, int kv_dtype);
+int cir_paged_tree_attention(const void* q, const void* k_pool, const void* v_pool, const int32_t* page_table,
+                             const int32_t* seq_lens, const int32_t* offsets, const int32_t* counts,
+                             const int64_t* masks, int words, void* out, void* workspace, size_t workspace_bytes,
+                             int tokens, int batch, int num_heads, int num_kv_heads, int head_dim, int page_size,
+                             int max_pages, float scale, int kv_dtype, void* stream);
+
 /* ------------------------------------------------------------ block weights ---
  * GGUF Q4_0 / Q8_0 blocks (cacheir/importers/gguf.py:36,40,273-310) for a weight
  * W[n, k] stored row-major, blocks along k.  The GEMM reads a tiled copy made once
@@ -366,6 +392,34 @@ int cir_token_logprobs(const void* logits, int dt, int64_t ld, const int64_t* id
                        float* logprobs, float* entropy, int64_t* top_ids, float* top_logprobs, void* workspace,
                        size_t workspace_bytes, void* stream);
 
+/* Penalties, biases and masks on rows of logits (dt CIR_F32 or CIR_F16, row strides ld_in and
+ * ld_out elements), before sampling.  Sequence b has the rows offsets[b] .. offsets[b + 1] - 1
+ * (int32 [batch + 1], ascending; NULL: row b alone, rows == batch).  With c the times that
+ * token v stands in history[b][prompt_lens[b] .. history_lens[b] - 1] and on the row's drafted
+ * path, and g whether it stands there or in history[b][0 .. prompt_lens[b] - 1]:
+ *   x = logit;  if g: x = x > 0 ? x / repetition[b] : x * repetition[b]
+ *   x -= frequency[b] * c;  if c > 0: x -= presence[b]
+ *   x += bias[b][k] where bias_ids[b][k] == v (the last such k)
+ *   out = allowed bit v % 32 of allowed[row][v / 32] ? x : -inf
+ * computed in fp32 and rounded once; tokens that none of it names keep their bits.
+ * history int64 [batch, history_width] (entries from history_lens[b] on are not read, and
+ * ids outside 0 .. vocab - 1 name no token), prompt_lens NULL: no prompt; drafts int64 and
+ * masks int64 [rows, words] as cir_draft_tree writes them: the row's path are the tokens
+ * drafts[offsets[b] + k] of the bits k of masks[row], its own among them; repetition (> 0),
+ * presence and frequency float [batch] (NULL: 1, 0, 0); bias_ids int64 and bias float
+ * [batch, bias_width] (ids outside the vocabulary: unused); allowed int32 [rows,
+ * ceil(vocab / 32)].  What is NULL is left out.  out may be logits (at the same stride, then
+ * only what changes is written) and otherwise overlaps no input.  Rows that offsets do not
+ * name are left as they were.  rows < 2^24, batch < 2^16, vocab <= 2^30, history_width <=
+ * 2^20 - 257, bias_width <= 2047, words 1..4.  No counterpart in the reference, whose
+ * sampling is greedy over all tokens (scheduler.py:535-543). */
+int cir_adjust_logits(const void* logits, int64_t ld_in, void* out, int64_t ld_out, int dt, const int32_t* offsets,
+                      const int64_t* history, const int32_t* history_lens, const int32_t* prompt_lens,
+                      int history_width, const int64_t* drafts, const int64_t* masks, int words,
+                      const float* repetition, const float* presence, const float* frequency,
+                      const int64_t* bias_ids, const float* bias, int bias_width, const int32_t* allowed, int rows,
+                      int batch, int vocab, void* stream);
+
 /* ------------------------------------------------------------- step inputs ---
  * Page tables and slot maps of a step from its request lengths, on the device: row b holds
  * seq_lens[b] tokens and gets new_tokens[b] more (a negative count is 0).  Row by row, the
@@ -413,6 +467,54 @@ int cir_rope_append(const void* q, int64_t q_token_stride, int64_t q_head_stride
                     int rotary_dim, int layout, void* q_out, int64_t o_token_stride, int64_t o_head_stride,
                     void* k_pool, void* v_pool, int kv_dtype, int64_t slots, int tokens, int num_heads,
                     int num_kv_heads, int head_dim, int page_size, void* stream);
+
+/* cir_rope_append with a norm of each head of q and k before the turn: head x becomes
+ * x / sqrt(mean x^2 + eps) * w, w = q_weight or k_weight [head_dim] of dtype wdt, then turns;
+ * rounded once, to the output.  v is stored as it is.  All else as there. */
+int cir_norm_rope_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                         int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                         int64_t v_head_stride, int dt, const void* q_weight, const void* k_weight, int wdt, float eps,
+                         const int32_t* positions, const int64_t* slot_map, const double* inv_freq, float factor,
+                         int rotary_dim, int layout, void* q_out, int64_t o_token_stride, int64_t o_head_stride,
+                         void* k_pool, void* v_pool, int kv_dtype, int64_t slots, int tokens, int num_heads,
+                         int num_kv_heads, int head_dim, int page_size, void* stream);
+
+/* ------------------------------------------------------------ drafted trees ---
+ * What each drafted token of a step sees of its row's tree, and its position.  Row b's n =
+ * counts[b] tokens are offsets[b] .. offsets[b] + n - 1 of the step's (at most
+ * offsets[b + 1] - offsets[b] and 64 * words, words 1..4), and the last n of its seq_lens[b];
+ * parents[j] is the place of j's parent in the same row's tree and lies before j's own, or is
+ * negative (a token that follows the context; so does one whose parent does not lie before it).
+ *   masks[j][w] (int64 [tokens, words]): bit k of word w set where token 64 w + k of the row is
+ *     j or one of its ancestors
+ *   positions[j] = seq_lens[b] - n + the number of j's ancestors
+ * Tokens that no row counts get empty masks and position 0.  batch < 2^24.  No counterpart in
+ * the reference, which decodes one token at a time. */
+int cir_draft_tree(const int32_t* parents, const int32_t* seq_lens, const int32_t* offsets, const int32_t* counts,
+                   int64_t* masks, int32_t* positions, int tokens, int batch, int words, void* stream);
+
+/* The drafted tokens that the model confirms.  Rows as in cir_draft_tree (up to 256 tokens
+ * each, later ones are never taken); drafts int64 [tokens] are the tokens fed to the model,
+ * targets int64 [tokens] what it chose after each.  The path starts at the row's token 0,
+ * which stands, and goes on from token p to its first child whose draft equals targets[p]:
+ *   accepted[b]   tokens on the path: at least 1 (0 in a row without tokens), at most `most`
+ *   path[b][i]    their places in the row's tree, then -1         int32 [batch, most]
+ *   tokens_out[b][i]  targets[path[i]], what the row says, then -1  int64 [batch, most]
+ *   seq_lens_out[b]   seq_lens[b] - n + accepted[b] (may be seq_lens)
+ * K and V of token path[i] move from position seq_lens[b] - n + path[i] to seq_lens[b] - n + i
+ * in the pools of all layers ([layers, slots, num_kv_heads, page_size, head_dim] each).  With
+ * free_slots (int32 [free_total]) and free_head (int32 [1]) given, the pages behind the new
+ * lengths go back: they are written before free_slots[free_head[0]], in row order, and
+ * free_head[0] falls by their number (if that would be negative nothing is given back).  1 <=
+ * most <= 256, layers, heads and head_dim up to 4096, batch < 2^20, fewer than 2^30 vectors
+ * of 16 bytes (or single values, where heads or pools are no whole ones) in a token of all
+ * layers.  No counterpart in the reference. */
+int cir_accept_drafts(const int32_t* parents, const int64_t* drafts, const int64_t* targets, const int32_t* seq_lens,
+                      const int32_t* offsets, const int32_t* counts, const int32_t* page_table, int32_t* accepted,
+                      int32_t* path, int64_t* tokens_out, int32_t* seq_lens_out, void* k_pools, void* v_pools,
+                      int kv_dtype, int64_t slots, int32_t* free_slots, int free_total, int32_t* free_head, int tokens,
+                      int batch, int most, int max_pages, int layers, int num_kv_heads, int head_dim, int page_size,
+                      void* stream);
 
 /* ------------------------------------------------------------- calibration ---
  * Reads `bytes` (a multiple of 16) from buf with `workgroups` x `threads` threads,

@@ -8,6 +8,8 @@
 #include <float.h>
 #include <math.h>
 
+#include <algorithm>
+
 namespace cir {
 namespace {
 
@@ -276,6 +278,670 @@ size_t generic_floats(const GenericPlan& p, int tokens, int Hq, int D) {
   return p.splits > 1 ? (size_t)tokens * Hq * p.splits * (D + 2) : 0;
 }
 
+// Whether x is an infinity or NaN (not 0: it is), in a form that ors.
+__device__ __forceinline__ uint32_t not_finite(f16 x) {
+  const uint16_t u = __builtin_bit_cast(uint16_t, x);
+  return (u & 0x7c00) == 0x7c00;
+}
+
+// ------------------------------------------------- fp16, head_dim 128: MFMA -----
+// Work.  An item is a row's tile of up to 256 query vectors (drafted token and head of the KV head's group) over all that
+// the row holds; it costs kItemCost + its 32-token blocks.  The items lie on one axis and each team of workgroups (one per
+// KV head) takes an equal stretch of it: lengths and counts live on the device, and a grid cut by rows leaves CUs idle
+// behind the longest.  Every workgroup scans the rows for itself.  A stretch's part of an item is a piece, which leaves
+// (max, sum, O) of its vectors; the piece of team w and of the tile that begins at vector e of all (e = first token * G +
+// 256 tile) lies at vector 256 w + e of the workspace: along the axis one of the two grows by at least the piece's
+// vectors, so pieces do not overlap, and the join finds a tile's pieces from its start and the stretch alone.
+//
+// Body (4 wavefronts, one workgroup per CU, up to 512 registers a lane).  Each wavefront takes NG groups of 32 query
+// vectors (Q in registers) and, of VW = 4 / CW wavefronts side by side, every CW-th block.  Stages of 64 tokens of K and V
+// come by DMA into a ring of four in LDS: two are on their way while one is worked on.  S^T = K Q^T and O^T = V^T P^T on
+// MFMA 32x32x16: a lane holds one vector's scores and sums, 64 vectors a wavefront halve the LDS reads of 32.  The scores
+// of the next block run on the matrix cores while the VALU takes this block's exponentials.
+constexpr int D = 128;
+constexpr int kBlock = 32;       // tokens of an MFMA tile
+constexpr int kGroup = 32;       // query vectors of an MFMA tile
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kTileVec = 256;    // query vectors of a tile
+constexpr int kWorkgroups = 256;
+constexpr int kItemCost = 6;     // a piece's start and join, in blocks
+constexpr int kMinStretch = 4;
+constexpr int kMaxRows = 1024;
+constexpr int kRowB = 2 * D;     // bytes of a K or V row
+constexpr int kStageTok = 64;    // tokens of a stage
+constexpr int kStage = 2 * kStageTok * kRowB;  // bytes: K, then V
+
+struct RowRec {
+  int first, n, start, blocks;  // first token, their number, place of the first tile's blocks, blocks
+};
+struct Fast {
+  Args a;
+  RowRec* rows;
+  int* row_of;      // [tokens]: the row that counts a token, or -1
+  int* stretch;
+  float *o, *ml;    // [vector of the workspace][KV head][D] and [2]
+  int P16;          // page size / 16
+  uint32_t page_magic;  // ceil(2^32 / P16): n / P16 = n * page_magic >> 32 (P16 > 1)
+};
+
+__device__ __forceinline__ int page_index(const Fast& F, int n) {
+  return F.P16 == 1 ? n : (int)__umulhi((uint32_t)n, F.page_magic);
+}
+__device__ __forceinline__ size_t rows16_at(const Fast& F, int h, int page, int n, int index) {
+  return (((size_t)page * F.a.Hkv + h) * F.P16 + (n - index * F.P16)) * (16 * D);
+}
+
+// A piece: vectors v0 .. v0 + nv - 1 of row r (its tile) and KV head h over blocks blk0 .. blk1 - 1.
+struct Piece {
+  const f16 *q, *kp, *vp;
+  const int32_t* ptrow;
+  Row r;
+  int h, v0, nv, blk0, blk1;
+  size_t at;  // first vector in the workspace
+};
+
+struct Smem {
+  float ml[kWaves][2][2 * kGroup];
+  uint32_t mask[kTileVec][2 * kMaxDrafts / 64 + 1];
+  int place[kMaxRows + 1], len[kMaxRows], first[kMaxRows];
+  int16_t n[kMaxRows];
+  int scan[kWaves], find;
+};
+
+// Running softmax of one query vector per lane (lane l and l + 32: the same vector).
+struct Soft {
+  float m, ms, l;  // ms: m, or 0 while there is no finite score
+  f32x16 acc[D / 32];
+};
+
+template <int VW, int NG>
+__device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& sm, uint8_t* st0, uint8_t* st1,
+                                           uint8_t* st2, uint8_t* st3) {
+  constexpr int CW = kWaves / VW;     // wavefronts that take turns at the blocks
+  constexpr int PW = 2 / CW;          // blocks of a stage that a wavefront takes
+  static_assert(CW == 1 || CW == 2, "");
+  const Args& A = F.a;
+  const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int l32 = lane & 31, h = lane >> 5;
+  const int col = wave % VW, par = wave / VW;
+  const float sc = fabsf(A.scale_log2);
+  const int G = A.Hq / A.Hkv;
+  const int limit = min(p.r.limit, p.blk1 * kBlock);  // tokens of the piece end here
+  const int nst = (p.blk1 - p.blk0 + 1) / 2;
+
+  // Q^T as the B operand: lane l32's vector of each group, dims 16 s + 8 h + e (zero past the last vector); a negative
+  // scale goes into its sign, so that the maximum can be taken before scaling.
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const uint32_t flip = A.scale_log2 < 0.f ? 0x80008000u : 0u;
+  f16x8 qb[NG][8];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    const int v = (col * NG + g) * kGroup + l32;
+    const bool live = v < p.nv;
+    const int vv = p.v0 + (live ? v : 0), tok = vv / G;
+    const f16* row = p.q + ((size_t)(p.r.first + tok) * A.Hq + (size_t)p.h * G + (vv - tok * G)) * D + 8 * h;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(row + 16 * s) ^ flip;
+      qb[g][s] = live ? __builtin_bit_cast(f16x8, x) : f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    }
+  }
+  // The masks of the tile's vectors, where a block of the piece holds drafted tokens.
+  const int drafts = min(p.r.n, p.r.limit - p.r.context);  // of the row, as far as the table holds them
+  if (p.blk1 * kBlock > p.r.context) {                     // uniform
+    for (int i = threadIdx.x; i < p.nv * 2 * A.words; i += kThreads) {
+      const int v = i / (2 * A.words), w = i - v * (2 * A.words);
+      sm.mask[v][w] = mask_word(A, p.r.first + (p.v0 + v) / G, w, drafts);
+    }
+  }
+
+  // DMA of a stage: each wavefront brings in 16 rows of K and of V, 4 rows per instruction (lane / 16 = row, lane % 16 =
+  // LDS slot); chunk c of K row r goes to slot c ^ (r % 16), of V row r to slot c ^ (4 (r % 4) + r / 4 % 4).  Rows past the
+  // piece's last token lie past the buffer's end and are zero.
+  const int lr = lane >> 4, ls = lane & 15;
+  uint32_t at_k[4], at_v[4];  // byte offsets of the lane's chunk in 16 whole rows
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    at_k[u] = (4 * u + lr) * kRowB + 16 * (ls ^ (4 * u + lr));
+    at_v[u] = (4 * u + lr) * kRowB + 16 * (ls ^ ((lr << 2) | u));
+  }
+  const int first16 = 2 * p.blk0 + wave, last16 = (limit - 1) >> 4;
+  int page = 0;
+  auto fetch = [&](int st) __attribute__((always_inline)) {
+    page = p.ptrow[page_index(F, min(first16 + 4 * st, last16))];
+  };
+  auto issue = [&](uint8_t* buf, int st) __attribute__((always_inline)) {
+    const int n = first16 + 4 * st, m = min(n, last16);
+    const size_t base = rows16_at(F, p.h, page, m, page_index(F, m));
+    const int bytes = max(0, min(16, limit - 16 * n)) * kRowB;
+    const rsrc_t rk = make_rsrc(p.kp + base, bytes), rv = make_rsrc(p.vp + base, bytes);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      uint8_t* to = buf + (16 * wave + 4 * u) * kRowB;
+      buf16_to_lds(rk, to, at_k[u], 0);
+      buf16_to_lds(rv, to + kStage / 2, at_v[u], 0);
+    }
+  };
+  fetch(0);
+  issue(st0, 0);
+  fetch(1);
+  issue(st1, 1);
+  fetch(2);
+  issue(st2, 2);
+  fetch(3);
+
+  Soft a[NG];
+  bool huge = false;  // uniform: some vector's |m| is 2^24 or more
+  uint32_t dirty = 0;
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    a[g].m = -INFINITY;
+    a[g].ms = a[g].l = 0.f;
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) a[g].acc[t][r] = 0.f;
+  }
+  const int krow = l32 * kRowB, kx = 16 * (h ^ (l32 & 15));
+  const int ti = lane & 15, sub = (lane >> 4) & 1;
+  int vo[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    vo[i] = kStage / 2 + (8 * i + 4 * h + (ti >> 2)) * kRowB + 16 * ((2 * sub + ((ti & 3) >> 1)) ^ (2 * i + h)) +
+            8 * (ti & 1);
+  const auto load_k = [&](const uint8_t* buf, f16x8 (&ka)[8]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < 8; ++s) ka[s] = *reinterpret_cast<const f16x8*>(buf + krow + (kx ^ (32 * s)));
+  };
+  const auto load_v = [&](const uint8_t* buf, f16x8 (&va)[D / 32][2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const uint8_t* x = buf + 64 * (dt ^ (ti >> 2)) + ks * 16 * kRowB;
+        const f16x4 lo = lds_read_tr(x + vo[0]), hi = lds_read_tr(x + vo[1]);
+        va[dt][ks] = f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      }
+  };
+  const auto scores = [&](const f16x8 (&ka)[8], f32x16 (&c)[NG]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) c[g][r] = 0.f;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) c[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[s], qb[g][s], c[g], 0, 0, 0);
+    }
+  };
+  // Tokens of a block that the lane's vector of group g sees; score r is that of token bit_of(r).
+  const auto seen_of = [&](int g, int blk) __attribute__((always_inline)) {
+    const int k = blk * kBlock - p.r.context, rest = limit - blk * kBlock;  // drafted token of the block's first
+    const uint32_t* m = sm.mask[(col * NG + g) * kGroup + l32];
+    const int w = k >> 5, s = k & 31;
+    const uint32_t lo = k < 0 ? 0xffffffffu : w < 2 * A.words ? m[w] : 0;
+    const uint32_t hi = w + 1 >= 0 && w + 1 < 2 * A.words ? m[w + 1] : 0;
+    const uint32_t seen = k <= -32 ? 0xffffffffu : s ? (lo >> s) | (hi << (32 - s)) : lo;
+    return rest >= 32 ? seen : rest <= 0 ? 0u : seen & ((1u << rest) - 1);
+  };
+  const auto bit_of = [&](int r) { return 8 * (r >> 2) + 4 * h + (r & 3); };
+
+  // Blocks from here on hold tokens that not every vector sees, or none.
+  const int special = min(p.r.context, limit) / kBlock;
+  f32x16 c[NG];
+  // One block (K of the next one at `knext`, V of this one at `vcur`).
+  auto block = [&](int blk, const uint8_t* knext, const uint8_t* vcur, auto between) __attribute__((always_inline)) {
+    if (blk >= special) {  // uniform
+      // Scores of tokens that a vector does not see become -inf.
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const uint32_t seen = seen_of(g, blk);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) c[g][r] = seen >> bit_of(r) & 1 ? c[g][r] : -INFINITY;
+      }
+    }
+    // Each group's maximum follows the scores only once some score lies more than 8 above it: p stays at 2^8 or less,
+    // which fp16 holds as exactly as p <= 1, and after a piece's first blocks the accumulators are hardly ever scaled.  The
+    // difference is compared, not m + 8: from |m| = 2^27 on that can round up to the next score.
+    float mx[NG];
+    bool rises = huge;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      mx[g] = c[g][0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mx[g] = fmaxf(mx[g], c[g][r]);
+      mx[g] = as_f32_value(mx[g] * sc);
+      rises |= mx[g] - a[g].m > 8.f;
+    }
+    float pc = sc;
+    if (__builtin_amdgcn_ballot_w64(rises) != 0) {  // uniform
+      bool far = false;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const float mn = fmaxf(a[g].m, fmaxf(mx[g], __shfl_xor(mx[g], 32, 64)));
+        const float alpha = __builtin_amdgcn_exp2f(a[g].m - (mn == -INFINITY ? 0.f : mn));
+        a[g].l *= alpha;
+        a[g].m = mn;
+        a[g].ms = mn == -INFINITY ? 0.f : mn;
+        far |= fabsf(a[g].ms) >= 0x1p24f;
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t) a[g].acc[t] *= alpha;
+      }
+      huge = __builtin_amdgcn_ballot_w64(far) != 0;
+      if (huge) {
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) c[g][r] = as_f32_value(c[g][r] * sc) - a[g].ms;
+        }
+        pc = 1.f;
+      }
+    }
+    between();
+    f16x8 ka[8], va[D / 32][2];
+    load_k(knext, ka);
+    load_v(vcur, va);
+    if (blk >= special) {  // uniform
+      // V that is no finite number must not meet the zero weights of what is not seen: it is left out here and added after
+      // the last block (below).
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const f16 x = va[dt][ks][e];
+            dirty |= not_finite(x);
+            va[dt][ks][e] = not_finite(x) ? (f16)0.f : x;
+          }
+    }
+    // The next block's scores, and p = 2^(c sc - m) by one FMA, in fp16: the B operand of the second product.  m is a
+    // rounded product, off by up to half an ulp: a factor that all p of the vector share.  From |m| = 2^24 on (where it
+    // could leave fp16) the rounded products are subtracted instead (above).
+    f32x16 cn[NG];
+    scores(ka, cn);
+    f16x8 pa[NG][2];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const float ps = huge ? 0.f : a[g].ms;
+      float sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const f16x2 two = {static_cast<f16>(__builtin_amdgcn_exp2f(fmaf(c[g][r], pc, -ps))),
+                           static_cast<f16>(__builtin_amdgcn_exp2f(fmaf(c[g][r + 1], pc, -ps)))};
+        pa[g][r >> 3][r & 7] = two.x;
+        pa[g][r >> 3][(r & 7) + 1] = two.y;
+        sum = __builtin_amdgcn_fdot2(two, f16x2{(f16)1.f, (f16)1.f}, sum, false);  // exact products, fp32 sum
+      }
+      a[g].l += sum;
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+          a[g].acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[dt][ks], pa[g][ks], a[g].acc[dt], 0, 0, 0);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) c[g] = cn[g];
+  };
+  // One stage, `cur`; the next one, whose K the last block takes, has landed after its wait, and stage st + 3 goes to `far`,
+  // which every wavefront has left by then.
+  constexpr int kOther = kBlock * kRowB;  // the stage's second block
+  auto stage = [&](int st, const uint8_t* cur, const uint8_t* next, uint8_t* far) __attribute__((always_inline)) {
+    const int blk = p.blk0 + 2 * st;
+    const auto turn = [&]() __attribute__((always_inline)) {
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0x0F78);  // vmcnt(8): the next stage has landed, the one after it may not
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      issue(far, st + 3);
+      fetch(st + 4);
+    };
+    if constexpr (PW == 2) {
+      block(blk, cur + kOther, cur, [] {});
+      block(blk + 1, next, cur + kOther, turn);
+    } else {
+      block(blk + par, next + par * kOther, cur + par * kOther, turn);
+    }
+  };
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x4070);  // vmcnt(16), lgkmcnt(0): stage 0 has landed, the masks are written
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  {
+    f16x8 ka[8];
+    load_k(st0 + (PW == 1 ? par * kOther : 0), ka);
+    scores(ka, c);
+  }
+  for (int st = 0;;) {  // uniform
+    stage(st, st0, st1, st3);
+    if (++st >= nst) break;
+    stage(st, st1, st2, st0);
+    if (++st >= nst) break;
+    stage(st, st2, st3, st1);
+    if (++st >= nst) break;
+    stage(st, st3, st0, st2);
+    if (++st >= nst) break;
+  }
+  // Infinities and NaN of V among the drafted tokens: each is added to the sums of the vectors that see its token.
+  if (__builtin_amdgcn_ballot_w64(dirty) != 0) {  // uniform
+    for (int blk = p.blk0 + (PW == 1 ? par : 0); blk < p.blk1; blk += CW) {
+      if (blk < special) continue;
+#pragma unroll 1
+      for (int dt = 0; dt < D / 32; ++dt) {
+        f16x8 plus[2], minus[2];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int tok = min(blk * kBlock + bit_of(r), limit - 1), n = tok >> 4, index = page_index(F, n);
+          const f16 x = p.vp[rows16_at(F, p.h, p.ptrow[index], n, index) + (tok & 15) * D + 32 * dt + l32];
+          const uint16_t u = __builtin_bit_cast(uint16_t, x);
+          const bool bad = not_finite(x), nan = bad && (u & 0x3ff);
+          plus[r >> 3][r & 7] = nan || (bad && !(u & 0x8000)) ? (f16)1.f : (f16)0.f;
+          minus[r >> 3][r & 7] = nan || (bad && (u & 0x8000)) ? (f16)1.f : (f16)0.f;
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const uint32_t seen = seen_of(g, blk);
+          f16x8 on[2];  // the vector's tokens as 0 or 1, laid out as its weights
+#pragma unroll
+          for (int r = 0; r < 16; ++r) on[r >> 3][r & 7] = seen >> bit_of(r) & 1 ? (f16)1.f : (f16)0.f;
+          f32x16 up, down;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) up[r] = down[r] = 0.f;
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            up = __builtin_amdgcn_mfma_f32_32x32x16_f16(plus[ks], on[ks], up, 0, 0, 0);
+            down = __builtin_amdgcn_mfma_f32_32x32x16_f16(minus[ks], on[ks], down, 0, 0, 0);
+          }
+#pragma unroll
+          for (int t = 0; t < D / 32; ++t) {
+            if (t != dt) continue;  // (uniform: dt is no constant, the accumulators are registers)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              a[g].acc[t][r] += up[r] > 0.f ? INFINITY : 0.f;
+              a[g].acc[t][r] -= down[r] > 0.f ? INFINITY : 0.f;
+            }
+          }
+        }
+      }
+    }
+  }
+
+  // Wavefronts that took turns at the blocks are joined through LDS: the second leaves its (m, l, O) there, the first adds
+  // its own and writes.  16-byte chunk c of vector v in slot c ^ (v % 32) of its 512 bytes.
+#pragma unroll
+  for (int g = 0; g < NG; ++g) a[g].l += __shfl_xor(a[g].l, 32, 64);
+  float part[NG][2];  // the factors of the two parts' O, and (m, l) of both
+#pragma unroll
+  for (int g = 0; g < NG; ++g) part[g][0] = 1.f, part[g][1] = 0.f;
+  if constexpr (CW == 2) {
+    dma_wait_barrier();  // (every wavefront is done with its blocks, and no DMA is on its way into them)
+    if (par == 1) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        uint8_t* to = (col == 0 ? st0 : st1) + (g * kGroup + l32) * 512;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<f32x4*>(to + 16 * ((8 * dt + 2 * j + h) ^ l32)) =
+                f32x4{a[g].acc[dt][4 * j], a[g].acc[dt][4 * j + 1], a[g].acc[dt][4 * j + 2], a[g].acc[dt][4 * j + 3]};
+        if (h == 0) {
+          sm.ml[wave][0][g * kGroup + l32] = a[g].m;
+          sm.ml[wave][1][g * kGroup + l32] = a[g].l;
+        }
+      }
+    }
+    __syncthreads();
+    if (par == 0) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const float m1 = sm.ml[wave + VW][0][g * kGroup + l32], l1 = sm.ml[wave + VW][1][g * kGroup + l32];
+        const float M = fmaxf(a[g].m, m1), ms = M == -INFINITY ? 0.f : M;
+        part[g][0] = __builtin_amdgcn_exp2f(a[g].m - ms);
+        part[g][1] = __builtin_amdgcn_exp2f(m1 - ms);
+        a[g].l = fmaf(l1, part[g][1], a[g].l * part[g][0]);
+        a[g].m = M;
+      }
+    }
+  }
+  if (CW == 1 || par == 0) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const int v = (col * NG + g) * kGroup + l32;
+      if (v >= p.nv) continue;
+      const size_t at = (p.at + v) * A.Hkv + p.h;
+      const uint8_t* other = (col == 0 ? st0 : st1) + (g * kGroup + l32) * 512;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f32x4 o = {a[g].acc[dt][4 * j], a[g].acc[dt][4 * j + 1], a[g].acc[dt][4 * j + 2], a[g].acc[dt][4 * j + 3]};
+          if constexpr (CW == 2) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(other + 16 * ((8 * dt + 2 * j + h) ^ l32));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], part[g][1], o[e] * part[g][0]);
+          }
+          *reinterpret_cast<f32x4*>(F.o + at * D + 32 * dt + 8 * j + 4 * h) = o;
+        }
+      if (h == 0) {
+        F.ml[2 * at] = a[g].m;
+        F.ml[2 * at + 1] = a[g].l;
+      }
+    }
+  }
+  dma_wait_barrier();  // the next piece writes the same LDS
+}
+
+__global__ __launch_bounds__(kThreads, 1) void tree_f16_d128(const f16* __restrict__ q, const f16* __restrict__ kp,
+                                                             const f16* __restrict__ vp,
+                                                             const int32_t* __restrict__ table, Fast F) {
+  __shared__ __align__(16) uint8_t st0[kStage];
+  __shared__ __align__(16) uint8_t st1[kStage];
+  __shared__ __align__(16) uint8_t st2[kStage];
+  __shared__ __align__(16) uint8_t st3[kStage];
+  __shared__ Smem sm;
+  const Args& A = F.a;
+  const int G = A.Hq / A.Hkv, B = A.batch, Hkv = A.Hkv;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int w = blockIdx.x / Hkv, h = blockIdx.x - w * Hkv;  // team, KV head
+
+  int all = 0;
+  for (int b0 = 0; b0 < B; b0 += kThreads) {  // uniform
+    const int b = b0 + t;
+    int cost = 0;
+    if (b < B) {
+      const Row r = row_of(A, b);
+      const int blocks = (r.limit + kBlock - 1) / kBlock, tiles = (r.n * G + kTileVec - 1) / kTileVec;
+      cost = blocks > 0 ? tiles * (blocks + kItemCost) : 0;
+      sm.first[b] = r.first;
+      sm.n[b] = (int16_t)r.n;
+      sm.len[b] = A.lens[b];
+    }
+    int upto = cost;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int o = __shfl_up(upto, off, 64);
+      upto += lane >= off ? o : 0;
+    }
+    if (lane == 63) sm.scan[wave] = upto;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      upto += i < wave ? sm.scan[i] : 0;
+      total += sm.scan[i];
+    }
+    if (b < B) sm.place[b] = all + upto - cost;
+    all += total;
+    __syncthreads();
+  }
+  if (t == 0) sm.place[B] = all;
+  const int teams = gridDim.x / Hkv;
+  const int stretch = max((all + teams - 1) / teams, kMinStretch);
+  const int lo = w * stretch, hi = min(all, lo + stretch);
+  __syncthreads();
+  const auto row_at = [&](int b) __attribute__((always_inline)) {
+    Row r;
+    r.first = uni(sm.first[b]);
+    r.n = uni(sm.n[b]);
+    const int len = uni(sm.len[b]);
+    r.context = max(0, len - r.n);
+    r.limit = max(0, min(len, A.max_pages * A.P));
+    return r;
+  };
+
+  // What the join needs, shared out over the workgroups from the last one on (the ones without work of their own).
+  const int id = (int)(gridDim.x - 1 - blockIdx.x) + t * (int)gridDim.x, step = kThreads * (int)gridDim.x;
+  if (id == 0) F.stretch[0] = stretch;
+  for (int b = id; b < B; b += step)
+    F.rows[b] = RowRec{sm.first[b], sm.n[b], sm.place[b] + kItemCost,
+                       (max(0, min(sm.len[b], A.max_pages * A.P)) + kBlock - 1) / kBlock};
+  for (int j = id; j < A.tokens; j += step) {
+    int a = 0, z = B - 1;  // the last row that begins at or before j (rows without tokens begin where the next does)
+    while (a < z) {
+      const int m = (a + z + 1) >> 1;
+      if (sm.first[m] <= j) a = m;
+      else z = m - 1;
+    }
+    F.row_of[j] = j >= sm.first[a] && j < sm.first[a] + sm.n[a] ? a : -1;
+  }
+  if (lo >= hi) return;  // uniform
+  for (int b = t; b < B; b += kThreads)
+    if (sm.place[b] <= lo && lo < sm.place[b + 1]) sm.find = b;
+  __syncthreads();
+
+  for (int b = uni(sm.find); b < B; ++b) {  // uniform
+    const int start = uni(sm.place[b]);
+    if (start >= hi) break;
+    if (uni(sm.place[b + 1]) == start) continue;
+    Piece p;
+    p.r = row_at(b);
+    const int blocks = (p.r.limit + kBlock - 1) / kBlock, cost = blocks + kItemCost;
+    const int tiles = (p.r.n * G + kTileVec - 1) / kTileVec;
+    for (int i = max(0, (lo - start) / cost); i < tiles && start + i * cost < hi; ++i) {
+      const int at = start + i * cost + kItemCost;
+      const int k0 = max(0, min(lo - at, blocks)), k1 = max(0, min(hi - at, blocks));
+      if (k0 >= k1) continue;
+      p.q = q;
+      p.kp = kp;
+      p.vp = vp;
+      p.h = h;
+      p.ptrow = table + (size_t)b * A.max_pages;
+      p.v0 = i * kTileVec;
+      p.nv = min(kTileVec, p.r.n * G - p.v0);
+      p.blk0 = k0;
+      p.blk1 = k1;
+      p.at = (size_t)w * kTileVec + (size_t)p.r.first * G + p.v0;
+      if (p.nv <= 2 * kGroup) tree_piece<2, 1>(F, p, sm, st0, st1, st2, st3);
+      else if (p.nv <= 4 * kGroup) tree_piece<2, 2>(F, p, sm, st0, st1, st2, st3);
+      else tree_piece<4, 2>(F, p, sm, st0, st1, st2, st3);
+    }
+  }
+}
+
+// out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i over the pieces of a vector's tile.  Two half-wavefronts per vector, each
+// with every second piece, four dims a lane; lane k takes (m, l) of every 32nd piece.  Bound by latency (row, record, then
+// pieces), so a half-wavefront has four O on their way, the first ones along with the (m, l).
+__global__ __launch_bounds__(256) void tree_join(Fast F, f16* __restrict__ out) {
+  constexpr int W = 2, U = 4, kVecs = 8 / W;
+  __shared__ f32x4 sm_o[kVecs][32];
+  const Args& A = F.a;
+  const int part = threadIdx.x >> 5, lane = threadIdx.x & 31, s = part % W, vec = part / W;
+  const int id = blockIdx.x * kVecs + vec, G = A.Hq / A.Hkv;
+  const int j = id / A.Hq, head = id - j * A.Hq, h = head / G;
+  const int b = id < A.tokens * A.Hq ? F.row_of[j] : -1;
+  const bool live = b >= 0;
+  const RowRec rec = F.rows[live ? b : 0];
+  const int stretch = F.stretch[0];
+  const int v = (j - rec.first) * G + (head - h * G), tile = v / kTileVec;
+  const int start = rec.start + tile * (rec.blocks + kItemCost), w0 = start / stretch;
+  const int n = live && rec.blocks > 0 ? (start + rec.blocks - 1) / stretch - w0 + 1 : 0;
+  const auto at = [&](int k) {
+    return ((size_t)(w0 + k) * kTileVec + (size_t)rec.first * G + v) * A.Hkv + h;
+  };
+  const auto ml_of = [&](int k) { return *reinterpret_cast<const float2*>(F.ml + 2 * at(k)); };
+  const auto o_of = [&](int k) { return *reinterpret_cast<const f32x4*>(F.o + D * at(k) + 4 * lane); };
+  float den = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  if (n > 0) {
+    float2 ml = lane < n ? ml_of(lane) : make_float2(-INFINITY, 0.f);
+    f32x4 x[U];
+    const auto load = [&](int k0) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < U; ++i) x[i] = o_of(min(k0 + s + W * i, n - 1));
+    };
+    load(0);
+    float M = ml.x;
+    for (int k = lane + 32; k < n; k += 32) M = fmaxf(M, ml_of(k).x);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 32));
+    const float ms = M == -INFINITY ? 0.f : M;
+    for (int k0 = 0; k0 < n; k0 += 32) {
+      if (k0) ml = k0 + lane < n ? ml_of(k0 + lane) : make_float2(-INFINITY, 0.f);
+      const float f = __builtin_amdgcn_exp2f(ml.x - ms);
+      den = fmaf(ml.y, f, den);
+      for (int j0 = k0; j0 < min(n, k0 + 32); j0 += W * U) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          const int k = j0 + s + W * i;
+          const float fk = __shfl(f, k - k0, 32);
+          if (k < n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(x[i][e], fk, o[e]);
+          }
+        }
+        if (j0 + W * U < n) load(j0 + W * U);
+      }
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) den += __shfl_xor(den, d, 32);
+  }
+  if (s > 0) sm_o[vec][lane] = o;
+  __syncthreads();
+  if (s > 0 || !live) return;
+  o += sm_o[vec][lane];
+  float inv = 1.f / den;
+  if (den == 0.f) inv = n > 0 && sees(A, row_of(A, b), j) ? NAN : 0.f;
+  f16x4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = static_cast<f16>(as_f32_value(o[e] * inv));
+  *reinterpret_cast<f16x4*>(out + (size_t)id * D + 4 * lane) = y;
+}
+
+int teams_of(int Hkv) { return max(1, kWorkgroups / Hkv); }
+
+size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+
+struct Layout {
+  size_t rows, row_of, stretch, o, ml, total;  // bytes
+};
+Layout layout(int tokens, int batch, int Hq, int Hkv) {
+  Layout l{};
+  size_t at = 0;
+  const auto take = [&](size_t bytes) {
+    const size_t p = at;
+    at += round16(bytes);
+    return p;
+  };
+  const size_t vectors = ((size_t)teams_of(Hkv) * kTileVec + (size_t)tokens * (Hq / Hkv)) * Hkv;
+  l.rows = take(sizeof(RowRec) * batch);
+  l.row_of = take(sizeof(int) * tokens);
+  l.stretch = take(sizeof(int));
+  l.o = take(vectors * D * sizeof(float));
+  l.ml = take(vectors * 2 * sizeof(float));
+  l.total = at;
+  return l;
+}
+
+// Sizes that the MFMA kernel takes; others run the generic one.
+bool fast_sizes(int tokens, int batch, int Hq, int Hkv, int head_dim, int P, int max_pages, int kv_dtype) {
+  const long blocks = (long)max_pages * P / kBlock + 1 + kItemCost;
+  const long tiles = (long)tokens * (Hq / Hkv) / kTileVec + batch;
+  return kv_dtype == CIR_F16 && head_dim == D && P % 16 == 0 && (long)max_pages * P / 16 * (P / 16) < (1L << 32) &&
+         batch <= kMaxRows && blocks * tiles < (1L << 31) - kWorkgroups;
+}
+
 }  // namespace
 }  // namespace cir
 
@@ -287,8 +953,11 @@ extern "C" size_t cir_tree_attention_workspace_bytes(int tokens, int batch, int 
       head_dim > kMaxD || page_size <= 0 || max_pages <= 0 || (long)page_size * max_pages > 0x7fffffffL ||
       (long)tokens * num_heads >= 1L << 26)
     return 0;
+  // (the larger of the two paths: the addresses, which are not known here, decide between them too)
   const GenericPlan g = generic_plan(tokens, batch, num_heads, num_kv_heads, page_size, max_pages);
-  return generic_floats(g, tokens, num_heads, head_dim) * sizeof(float);
+  const size_t plain = generic_floats(g, tokens, num_heads, head_dim) * sizeof(float);
+  if (!fast_sizes(tokens, batch, num_heads, num_kv_heads, head_dim, page_size, max_pages, kv_dtype)) return plain;
+  return std::max(plain, layout(tokens, batch, num_heads, num_kv_heads).total);
 }
 
 extern "C" int cir_paged_tree_attention(const void* q, const void* k_pool, const void* v_pool,
@@ -311,16 +980,37 @@ extern "C" int cir_paged_tree_attention(const void* q, const void* k_pool, const
                 words);
   CIR_CHECK_ARG((long)tokens * num_heads < 1L << 26 && num_kv_heads < 1 << 16 && batch < 1 << 20,
                 "tree_attention: 2^26 query vectors, 2^16 KV heads or 2^20 rows and more");
+  const float scale_log2 = scale * kLog2e;
+  hipStream_t s = as_stream(stream);
+  Args A{page_table, seq_lens, offsets, counts, reinterpret_cast<const uint32_t*>(masks), nullptr, nullptr, tokens, batch,
+         num_heads, num_kv_heads, head_dim, page_size, max_pages, words, 1,
+         scale_log2 == 0.f ? FLT_MIN : scale_log2};  // (a masked score is -inf: -inf * 0 would be NaN)
+  // DMA takes 16-byte groups of the pools; q is read by 16 bytes, out written by 8.
+  if (fast_sizes(tokens, batch, num_heads, num_kv_heads, head_dim, page_size, max_pages, kv_dtype) &&
+      ((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool) % 16 == 0 && (uintptr_t)out % 8 == 0) {
+    const Layout l = layout(tokens, batch, num_heads, num_kv_heads);
+    CIR_CHECK_ARG(workspace && workspace_bytes >= l.total && (uintptr_t)workspace % 16 == 0,
+                  "tree_attention: workspace too small or not on 16 bytes (%zu < %zu)", workspace_bytes, l.total);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    const uint32_t P16 = page_size / 16;
+    const Fast F{A, reinterpret_cast<RowRec*>(ws + l.rows), reinterpret_cast<int*>(ws + l.row_of),
+                 reinterpret_cast<int*>(ws + l.stretch), reinterpret_cast<float*>(ws + l.o),
+                 reinterpret_cast<float*>(ws + l.ml), (int)P16, (uint32_t)(((1ull << 32) + P16 - 1) / P16)};
+    tree_f16_d128<<<teams_of(num_kv_heads) * num_kv_heads, kThreads, 0, s>>>(
+        static_cast<const f16*>(q), static_cast<const f16*>(k_pool), static_cast<const f16*>(v_pool), page_table, F);
+    const int st = launch_status();
+    if (st) return st;
+    tree_join<<<((unsigned)tokens * num_heads + 3) / 4, 256, 0, s>>>(F, static_cast<f16*>(out));
+    return launch_status();
+  }
   const GenericPlan g = generic_plan(tokens, batch, num_heads, num_kv_heads, page_size, max_pages);
   const size_t floats = generic_floats(g, tokens, num_heads, head_dim), need = floats * sizeof(float);
   CIR_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0),
                 "tree_attention: workspace too small or not on 16 bytes (%zu < %zu)", workspace_bytes, need);
-  float* ws = static_cast<float*>(workspace);
-  const float scale_log2 = scale * kLog2e;
-  const Args A{page_table, seq_lens, offsets, counts, reinterpret_cast<const uint32_t*>(masks), ws,
-               ws + (size_t)tokens * num_heads * g.splits * head_dim, tokens, batch, num_heads, num_kv_heads, head_dim,
-               page_size, max_pages, words, g.splits, scale_log2};
-  hipStream_t s = as_stream(stream);
+  A.part_o = static_cast<float*>(workspace);
+  A.part_ml = A.part_o + (size_t)tokens * num_heads * g.splits * head_dim;
+  A.splits = g.splits;
+  A.scale_log2 = scale_log2;
   const auto go = [&]<typename T>() {
     const dim3 grid(g.tiles, num_kv_heads, g.splits);
     const T *qt = static_cast<const T*>(q), *kt = static_cast<const T*>(k_pool), *vt = static_cast<const T*>(v_pool);

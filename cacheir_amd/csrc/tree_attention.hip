@@ -349,15 +349,51 @@ struct Smem {
   int scan[kWaves], find;
 };
 
+// 16 bytes per lane from a buffer (raw, bytes past its end read as 0) into LDS: lane l's land at lds + 16 l.  In asm, and so
+// unknown to the compiler's counts: for a DMA that it knows it puts a wait before every read of the same LDS array, the
+// ring's other stages among them.  The waits are the ones written out below (those that the compiler puts for loads of its
+// own can only come out stricter); no register is written.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ i32x4 buffer_of(const void* p, int bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  return i32x4{uni((int)a), uni((int)(a >> 32) & 0xffff), uni(bytes), 0x00020000};
+}
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // (m0 is reserved; nothing else here uses it)
+template <int ROWS4>  // 4 ROWS4 rows further, in the buffer and in LDS
+__device__ __forceinline__ void dma16(i32x4 buffer, uint32_t lds, uint32_t offset) {
+  constexpr int kMore = 4 * ROWS4 * kRowB;
+  if constexpr (kMore == 0)
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %1, %2, 0 offen lds"
+        :: "s"(lds), "v"(offset), "s"(buffer) : "memory", "m0");
+  else
+    asm volatile(
+        "s_add_u32 m0, %0, %3\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %1, %2, %4 offen lds"
+        :: "s"(lds), "v"(offset), "s"(buffer), "n"(kMore), "s"(kMore) : "memory", "m0", "scc");
+}
+#pragma clang diagnostic pop
+
+template <typename F>
+__device__ __forceinline__ void for_each4(const F& f) {
+  f.template operator()<0>();
+  f.template operator()<1>();
+  f.template operator()<2>();
+  f.template operator()<3>();
+}
+
 // Running softmax of one query vector per lane (lane l and l + 32: the same vector).
 struct Soft {
-  float m, ms, l;  // ms: m, or 0 while there is no finite score
+  float m, l;
   f32x16 acc[D / 32];
 };
 
 template <int VW, int NG>
-__device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& sm, uint8_t* st0, uint8_t* st1,
-                                           uint8_t* st2, uint8_t* st3) {
+__device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& sm, uint8_t* ring) {
   constexpr int CW = kWaves / VW;     // wavefronts that take turns at the blocks
   constexpr int PW = 2 / CW;          // blocks of a stage that a wavefront takes
   static_assert(CW == 1 || CW == 2, "");
@@ -369,6 +405,39 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
   const int G = A.Hq / A.Hkv;
   const int limit = min(p.r.limit, p.blk1 * kBlock);  // tokens of the piece end here
   const int nst = (p.blk1 - p.blk0 + 1) / 2;
+
+  // DMA of a stage: each wavefront brings in 16 rows of K and of V, 4 rows per instruction (lane / 16 = row, lane % 16 =
+  // LDS slot); chunk c of K row r goes to slot c ^ (r % 16), of V row r to slot c ^ (4 (r % 4) + r / 4 % 4).  Rows past the
+  // piece's last token lie past the buffer's end and are zero.
+  const int lr = lane >> 4, ls = lane & 15;
+  // Byte offset of the lane's chunk in the first four rows; rows 4 u on: ^ 64 u or 16 u, and 1024 u further.
+  const uint32_t at_k = lr * kRowB + 16 * (ls ^ lr), at_v = lr * kRowB + 16 * (ls ^ (lr << 2));
+  const int first16 = 2 * p.blk0 + wave, last16 = (limit - 1) >> 4;
+  // Pages of 64 stages' rows, one a lane.  (Scalar loads count with those from LDS and return in any order, so that every
+  // wait for LDS would wait for them: some 700 cycles a stage.)
+  int pages;
+  const auto fetch = [&](int st) __attribute__((always_inline)) {
+    pages = p.ptrow[page_index(F, min(first16 + 4 * (st + lane), last16))];
+    asm volatile("" : "+v"(pages));  // (waits here)
+  };
+  struct Rows {  // the rows of a stage
+    i32x4 k, v;
+    uint32_t to;  // in LDS
+  };
+  const uint32_t ring_at = uni((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)ring) + 16 * wave * kRowB;
+  const auto rows_of = [&](int st) __attribute__((always_inline)) {
+    const int n = first16 + 4 * st, m = min(n, last16);
+    const size_t base = rows16_at(F, p.h, __builtin_amdgcn_readlane(pages, st & 63), m, page_index(F, m));
+    const int bytes = max(0, min(16, limit - 16 * n)) * kRowB;
+    return Rows{buffer_of(p.kp + base, bytes), buffer_of(p.vp + base, bytes), ring_at + (st & 3) * kStage};
+  };
+  const auto issue = [&](int st) __attribute__((always_inline)) {
+    const Rows r = rows_of(st);
+    for_each4([&]<int U>() __attribute__((always_inline)) { dma16<U>(r.k, r.to, at_k ^ (64 * U)); });
+    for_each4([&]<int U>() __attribute__((always_inline)) { dma16<U>(r.v, r.to + kStage / 2, at_v ^ (16 * U)); });
+  };
+  fetch(0);
+  issue(0);
 
   // Q^T as the B operand: lane l32's vector of each group, dims 16 s + 8 h + e (zero past the last vector); a negative
   // scale goes into its sign, so that the maximum can be taken before scaling.
@@ -385,6 +454,9 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
     for (int s = 0; s < 8; ++s) {
       const u32x4 x = *reinterpret_cast<const u32x4*>(row + 16 * s) ^ flip;
       qb[g][s] = live ? __builtin_bit_cast(f16x8, x) : f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      // (Here, before the next stages are on their way: its wait would be for them too.  In accumulator registers, which an
+      // MFMA reads as well as the others.)
+      asm volatile("" : "+a"(qb[g][s]));
     }
   }
   // The masks of the tile's vectors, where a block of the piece holds drafted tokens.
@@ -396,83 +468,27 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
     }
   }
 
-  // DMA of a stage: each wavefront brings in 16 rows of K and of V, 4 rows per instruction (lane / 16 = row, lane % 16 =
-  // LDS slot); chunk c of K row r goes to slot c ^ (r % 16), of V row r to slot c ^ (4 (r % 4) + r / 4 % 4).  Rows past the
-  // piece's last token lie past the buffer's end and are zero.
-  const int lr = lane >> 4, ls = lane & 15;
-  uint32_t at_k[4], at_v[4];  // byte offsets of the lane's chunk in 16 whole rows
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    at_k[u] = (4 * u + lr) * kRowB + 16 * (ls ^ (4 * u + lr));
-    at_v[u] = (4 * u + lr) * kRowB + 16 * (ls ^ ((lr << 2) | u));
-  }
-  const int first16 = 2 * p.blk0 + wave, last16 = (limit - 1) >> 4;
-  int page = 0;
-  auto fetch = [&](int st) __attribute__((always_inline)) {
-    page = p.ptrow[page_index(F, min(first16 + 4 * st, last16))];
-  };
-  auto issue = [&](uint8_t* buf, int st) __attribute__((always_inline)) {
-    const int n = first16 + 4 * st, m = min(n, last16);
-    const size_t base = rows16_at(F, p.h, page, m, page_index(F, m));
-    const int bytes = max(0, min(16, limit - 16 * n)) * kRowB;
-    const rsrc_t rk = make_rsrc(p.kp + base, bytes), rv = make_rsrc(p.vp + base, bytes);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      uint8_t* to = buf + (16 * wave + 4 * u) * kRowB;
-      buf16_to_lds(rk, to, at_k[u], 0);
-      buf16_to_lds(rv, to + kStage / 2, at_v[u], 0);
-    }
-  };
-  fetch(0);
-  issue(st0, 0);
-  fetch(1);
-  issue(st1, 1);
-  fetch(2);
-  issue(st2, 2);
-  fetch(3);
-
   Soft a[NG];
   bool huge = false;  // uniform: some vector's |m| is 2^24 or more
   uint32_t dirty = 0;
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
     a[g].m = -INFINITY;
-    a[g].ms = a[g].l = 0.f;
+    a[g].l = 0.f;
 #pragma unroll
     for (int t = 0; t < D / 32; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) a[g].acc[t][r] = 0.f;
   }
-  const int krow = l32 * kRowB, kx = 16 * (h ^ (l32 & 15));
+  // LDS bytes of the lane's part of K rows (chunk 2 s + h: ^ 32 s) and of V rows (dims from 32 dt on: ^ 64 dt; token rows
+  // 8 i + 4 h ..).
   const int ti = lane & 15, sub = (lane >> 4) & 1;
-  int vo[2];
+  const uint32_t k_at = l32 * kRowB + 16 * (h ^ (l32 & 15));
+  uint32_t v_at[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    vo[i] = kStage / 2 + (8 * i + 4 * h + (ti >> 2)) * kRowB + 16 * ((2 * sub + ((ti & 3) >> 1)) ^ (2 * i + h)) +
-            8 * (ti & 1);
-  const auto load_k = [&](const uint8_t* buf, f16x8 (&ka)[8]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int s = 0; s < 8; ++s) ka[s] = *reinterpret_cast<const f16x8*>(buf + krow + (kx ^ (32 * s)));
-  };
-  const auto load_v = [&](const uint8_t* buf, f16x8 (&va)[D / 32][2]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        const uint8_t* x = buf + 64 * (dt ^ (ti >> 2)) + ks * 16 * kRowB;
-        const f16x4 lo = lds_read_tr(x + vo[0]), hi = lds_read_tr(x + vo[1]);
-        va[dt][ks] = f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      }
-  };
-  const auto scores = [&](const f16x8 (&ka)[8], f32x16 (&c)[NG]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) c[g][r] = 0.f;
-#pragma unroll
-      for (int s = 0; s < 8; ++s) c[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[s], qb[g][s], c[g], 0, 0, 0);
-    }
-  };
+    v_at[i] = kStage / 2 + (8 * i + 4 * h + (ti >> 2)) * kRowB + 64 * (ti >> 2) +
+              16 * ((2 * sub + ((ti & 3) >> 1)) ^ (2 * i + h)) + 8 * (ti & 1);
   // Tokens of a block that the lane's vector of group g sees; score r is that of token bit_of(r).
   const auto seen_of = [&](int g, int blk) __attribute__((always_inline)) {
     const int k = blk * kBlock - p.r.context, rest = limit - blk * kBlock;  // drafted token of the block's first
@@ -487,142 +503,212 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
 
   // Blocks from here on hold tokens that not every vector sees, or none.
   const int special = min(p.r.context, limit) / kBlock;
-  f32x16 c[NG];
-  // One block (K of the next one at `knext`, V of this one at `vcur`).
-  auto block = [&](int blk, const uint8_t* knext, const uint8_t* vcur, auto between) __attribute__((always_inline)) {
-    if (blk >= special) {  // uniform
-      // Scores of tokens that a vector does not see become -inf.
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const uint32_t seen = seen_of(g, blk);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) c[g][r] = seen >> bit_of(r) & 1 ? c[g][r] : -INFINITY;
-      }
+  f32x16 c[NG];  // scores of the block at hand
+  f16x8 ka[8];   // K of the next one
+  const auto read_k = [&](uint32_t at, int s) __attribute__((always_inline)) {
+    ka[s] = *reinterpret_cast<const f16x8*>(ring + ((at + k_at) ^ (32 * s)));
+  };
+  // Rows of a stage on their way, in eight parts (K, then V): from a turn (below) on, a quarter of a stage's beside the
+  // second products of a block and beside the first ones of the next, spread out: an LDS load takes a CU's four wavefronts
+  // some 170 cycles together, and a wavefront that issues several at once stands still.
+  Rows rows{};
+  const auto load_part = [&]<int B, int U>(int i) __attribute__((always_inline)) {  // B: beside second products; U < 4 / PW
+    if constexpr (PW == 1) {
+      if constexpr (B) dma16<U>(rows.k, rows.to, at_k ^ (64 * U));
+      else dma16<U>(rows.v, rows.to + kStage / 2, at_v ^ (16 * U));
+    } else {
+      const bool v = B ? (i & 1) : !(i & 1);
+      constexpr int W = B ? U : U + 2;
+      dma16<W>(v ? rows.v : rows.k, rows.to + (v ? kStage / 2 : 0), (v ? at_v : at_k) ^ ((v ? 16 : 64) * W));
     }
-    // Each group's maximum follows the scores only once some score lies more than 8 above it: p stays at 2^8 or less,
-    // which fp16 holds as exactly as p <= 1, and after a piece's first blocks the accumulators are hardly ever scaled.  The
-    // difference is compared, not m + 8: from |m| = 2^27 on that can round up to the next score.
-    float mx[NG];
-    bool rises = huge;
+  };
+  // One block, `blk` (its V at byte `vcur` of the ring), and the scores of the next one, `bnext`; K of the one after that
+  // (at `kafter`) is read beside the second products.
+  //
+  // p = 2^(c sc - m) by one FMA, in fp16: the B operand of the second product.  The first block's scores set m, which
+  // follows the maximum only once a lane's 16 weights of a block sum to more than 2^8: then no p is larger, and fp16 holds it
+  // as exactly as p <= 1; after a piece's first blocks the accumulators are hardly ever scaled, and no maximum is taken.
+  // m is a rounded product, off by up to half an ulp: a factor that all p of the vector share.  From |m| = 2^24 on (where it
+  // could leave fp16) the rounded products are subtracted instead.
+  //
+  // One wavefront per SIMD issues one instruction in 4 to 5 cycles, whatever it is for: products, exponentials and loads
+  // stand by turns in the order wanted (sched_barrier), and what the 32 cycles of a product leave is filled.
+  auto block = [&]<bool SPECIAL>(int i, int blk, int bnext, uint32_t kafter, uint32_t vcur) __attribute__((always_inline)) {
+    f16x8 va[D / 32][2], pa[NG][2];
+    f32x16 cn[NG];
+    float sum[NG], e0, e1;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      mx[g] = c[g][0];
+      sum[g] = 0.f;
 #pragma unroll
-      for (int r = 1; r < 16; ++r) mx[g] = fmaxf(mx[g], c[g][r]);
-      mx[g] = as_f32_value(mx[g] * sc);
-      rises |= mx[g] - a[g].m > 8.f;
+      for (int r = 0; r < 16; ++r) cn[g][r] = 0.f;
     }
-    float pc = sc;
-    if (__builtin_amdgcn_ballot_w64(rises) != 0) {  // uniform
+    const auto put = [&](int g, int r, float x, float y) __attribute__((always_inline)) {  // weights r and r + 1
+      const f16x2 two = {static_cast<f16>(x), static_cast<f16>(y)};
+      pa[g][r >> 3][r & 7] = two.x;
+      pa[g][r >> 3][(r & 7) + 1] = two.y;
+      sum[g] = __builtin_amdgcn_fdot2(two, f16x2{(f16)1.f, (f16)1.f}, sum[g], false);  // exact products, fp32 sum
+    };
+    const auto exps = [&](int g, int r) __attribute__((always_inline)) {
+      e0 = __builtin_amdgcn_exp2f(fmaf(c[g][r], sc, -a[g].m));
+      e1 = __builtin_amdgcn_exp2f(fmaf(c[g][r + 1], sc, -a[g].m));
+    };
+    exps(0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    const auto first = [&]<int S>() __attribute__((always_inline)) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        cn[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[S], qb[g][S], cn[g], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        const int pair = S * NG + g, gp = pair >> 3, r = 2 * (pair & 7);  // the pair whose exponentials were taken before
+        const float x = e0, y = e1;
+        if (pair + 1 < 8 * NG) exps((pair + 1) >> 3, 2 * ((pair + 1) & 7));
+        put(gp, r, x, y);
+        if (g == 0) {
+          constexpr int dt = S & 3, ks = S >> 2;
+          const f16x4 lo = lds_read_tr(ring + (((vcur + v_at[0]) ^ (64 * dt)) + ks * 16 * kRowB));
+          const f16x4 hi = lds_read_tr(ring + (((vcur + v_at[1]) ^ (64 * dt)) + ks * 16 * kRowB));
+          va[dt][ks] = f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        }
+        if constexpr (S % (2 * PW) == PW) {
+          if (g == NG - 1) load_part.template operator()<0, S / (2 * PW)>(i);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    for_each4([&]<int U>() __attribute__((always_inline)) { first.template operator()<U>(); });
+    for_each4([&]<int U>() __attribute__((always_inline)) { first.template operator()<U + 4>(); });
+    bool over = huge;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) over |= !(sum[g] <= 256.f);
+    if (__builtin_amdgcn_ballot_w64(over) != 0) {  // uniform
       bool far = false;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const float mn = fmaxf(a[g].m, fmaxf(mx[g], __shfl_xor(mx[g], 32, 64)));
-        const float alpha = __builtin_amdgcn_exp2f(a[g].m - (mn == -INFINITY ? 0.f : mn));
+        float mx = c[g][0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, c[g][r]);
+        mx = as_f32_value(mx * sc);
+        const float mn = fmaxf(a[g].m, fmaxf(mx, __shfl_xor(mx, 32, 64)));
+        const float ms = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(a[g].m - ms);
         a[g].l *= alpha;
         a[g].m = mn;
-        a[g].ms = mn == -INFINITY ? 0.f : mn;
-        far |= fabsf(a[g].ms) >= 0x1p24f;
+        far |= fabsf(ms) >= 0x1p24f;
 #pragma unroll
         for (int t = 0; t < D / 32; ++t) a[g].acc[t] *= alpha;
+        sum[g] = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          const float x = fabsf(ms) >= 0x1p24f ? as_f32_value(c[g][r] * sc) - ms : fmaf(c[g][r], sc, -ms);
+          const float y = fabsf(ms) >= 0x1p24f ? as_f32_value(c[g][r + 1] * sc) - ms : fmaf(c[g][r + 1], sc, -ms);
+          put(g, r, __builtin_amdgcn_exp2f(x), __builtin_amdgcn_exp2f(y));
+        }
       }
       huge = __builtin_amdgcn_ballot_w64(far) != 0;
-      if (huge) {
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) c[g][r] = as_f32_value(c[g][r] * sc) - a[g].ms;
-        }
-        pc = 1.f;
-      }
     }
-    between();
-    f16x8 ka[8], va[D / 32][2];
-    load_k(knext, ka);
-    load_v(vcur, va);
-    if (blk >= special) {  // uniform
+    if constexpr (SPECIAL) {
+      // Scores of tokens that a vector does not see become -inf.
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const uint32_t seen = seen_of(g, bnext);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) cn[g][r] = seen >> bit_of(r) & 1 ? cn[g][r] : -INFINITY;
+      }
       // V that is no finite number must not meet the zero weights of what is not seen: it is left out here and added after
       // the last block (below).
+      if (blk >= special) {  // uniform
 #pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
+        for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+          for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const f16 x = va[dt][ks][e];
-            dirty |= not_finite(x);
-            va[dt][ks][e] = not_finite(x) ? (f16)0.f : x;
-          }
+            for (int e = 0; e < 8; ++e) {
+              const f16 x = va[dt][ks][e];
+              dirty |= not_finite(x);
+              va[dt][ks][e] = not_finite(x) ? (f16)0.f : x;
+            }
+      }
     }
-    // The next block's scores, and p = 2^(c sc - m) by one FMA, in fp16: the B operand of the second product.  m is a
-    // rounded product, off by up to half an ulp: a factor that all p of the vector share.  From |m| = 2^24 on (where it
-    // could leave fp16) the rounded products are subtracted instead (above).
-    f32x16 cn[NG];
-    scores(ka, cn);
-    f16x8 pa[NG][2];
+    // A turn, before the block's second products and with V of it in registers: K of the block after the next one is to
+    // have landed (all but the youngest eight loads), and every wavefront has left the stage that stage `far` takes.
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    if (PW == 1 || !(i & 1)) {  // uniform
+      const int far = i / PW + (PW == 1 ? 4 : 3);
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0x0F78);  // vmcnt(8)
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if ((far & 63) == 0) fetch(far);  // uniform
+    }
+    const auto second = [&]<int J>() __attribute__((always_inline)) {
+      constexpr int g = J >> 3, dt = J & 3, ks = (J >> 2) & 1;  // (ks, then dt: four chains)
+      a[g].acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[dt][ks], pa[g][ks], a[g].acc[dt], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (J == 0) rows = rows_of(i / PW + (PW == 1 ? 4 : 3));
+      if constexpr (NG == 1 || J >= 8) read_k(kafter, J & 7);
+      if constexpr (J % (2 * PW * NG) == 2 * PW * NG - 1) load_part.template operator()<1, J / (2 * PW * NG)>(i);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    for_each4([&]<int U>() __attribute__((always_inline)) { second.template operator()<U>(); });
+    for_each4([&]<int U>() __attribute__((always_inline)) { second.template operator()<U + 4>(); });
+    if constexpr (NG == 2) {
+      for_each4([&]<int U>() __attribute__((always_inline)) { second.template operator()<U + 8>(); });
+      for_each4([&]<int U>() __attribute__((always_inline)) { second.template operator()<U + 12>(); });
+    }
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      const float ps = huge ? 0.f : a[g].ms;
-      float sum = 0.f;
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        const f16x2 two = {static_cast<f16>(__builtin_amdgcn_exp2f(fmaf(c[g][r], pc, -ps))),
-                           static_cast<f16>(__builtin_amdgcn_exp2f(fmaf(c[g][r + 1], pc, -ps)))};
-        pa[g][r >> 3][r & 7] = two.x;
-        pa[g][r >> 3][(r & 7) + 1] = two.y;
-        sum = __builtin_amdgcn_fdot2(two, f16x2{(f16)1.f, (f16)1.f}, sum, false);  // exact products, fp32 sum
-      }
-      a[g].l += sum;
+      c[g] = cn[g];
+      a[g].l += sum[g];
     }
+  };
+  // A wavefront's blocks in order: block i lies in stage i / PW.
+  constexpr int kOther = kBlock * kRowB;  // the stage's second block
+  const auto place = [&](int i) { return (uint32_t)((i / PW) & 3) * kStage + (PW == 1 ? par : i & 1) * kOther; };
+  issue(1);
+  if constexpr (PW == 1) issue(2);
+  rows = rows_of(PW == 1 ? 3 : 2);
+  for_each4([&]<int U>() __attribute__((always_inline)) { dma16<U>(rows.k, rows.to, at_k ^ (64 * U)); });
+  if constexpr (PW == 2) {
+    dma16<0>(rows.v, rows.to + kStage / 2, at_v);
+    dma16<1>(rows.v, rows.to + kStage / 2, at_v ^ 16);
+  }
+  asm volatile("" ::: "memory");
+  // Block 0 and K of block 1 have landed, the masks are written: lgkmcnt(0), vmcnt(12) (a stage and K of one) or 14.
+  __builtin_amdgcn_s_waitcnt(PW == 1 ? 0x007C : 0x007E);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  {  // scores of the first block, and K of the second
+    const int first = p.blk0 + (PW == 1 ? par : 0);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) read_k(place(0), s);
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
+      for (int r = 0; r < 16; ++r) c[g][r] = 0.f;
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
-          a[g].acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[dt][ks], pa[g][ks], a[g].acc[dt], 0, 0, 0);
+    for (int s = 0; s < 8; ++s)
 #pragma unroll
-    for (int g = 0; g < NG; ++g) c[g] = cn[g];
-  };
-  // One stage, `cur`; the next one, whose K the last block takes, has landed after its wait, and stage st + 3 goes to `far`,
-  // which every wavefront has left by then.
-  constexpr int kOther = kBlock * kRowB;  // the stage's second block
-  auto stage = [&](int st, const uint8_t* cur, const uint8_t* next, uint8_t* far) __attribute__((always_inline)) {
-    const int blk = p.blk0 + 2 * st;
-    const auto turn = [&]() __attribute__((always_inline)) {
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_waitcnt(0x0F78);  // vmcnt(8): the next stage has landed, the one after it may not
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      issue(far, st + 3);
-      fetch(st + 4);
-    };
-    if constexpr (PW == 2) {
-      block(blk, cur + kOther, cur, [] {});
-      block(blk + 1, next, cur + kOther, turn);
-    } else {
-      block(blk + par, next + par * kOther, cur + par * kOther, turn);
+      for (int g = 0; g < NG; ++g) c[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[s], qb[g][s], c[g], 0, 0, 0);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) read_k(place(1), s);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const uint32_t seen = first >= special ? seen_of(g, first) : 0xffffffffu;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) c[g][r] = seen >> bit_of(r) & 1 ? c[g][r] : -INFINITY;
+    }
+  }
+  const auto turns = [&]<bool SPECIAL>(int from, int to) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int i = from; i < to; ++i) {
+      const int blk = p.blk0 + (PW == 1 ? 2 * i + par : i);
+      block.template operator()<SPECIAL>(i, blk, blk + CW, place(i + 2), place(i));
     }
   };
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x4070);  // vmcnt(16), lgkmcnt(0): stage 0 has landed, the masks are written
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-  {
-    f16x8 ka[8];
-    load_k(st0 + (PW == 1 ? par * kOther : 0), ka);
-    scores(ka, c);
-  }
-  for (int st = 0;;) {  // uniform
-    stage(st, st0, st1, st3);
-    if (++st >= nst) break;
-    stage(st, st1, st2, st0);
-    if (++st >= nst) break;
-    stage(st, st2, st3, st1);
-    if (++st >= nst) break;
-    stage(st, st3, st0, st2);
-    if (++st >= nst) break;
-  }
+  // (a block scores the next one too)
+  const int plain = max(0, min(nst * PW, (special - p.blk0) / CW - 1));
+  turns.template operator()<false>(0, plain);
+  turns.template operator()<true>(plain, nst * PW);
   // Infinities and NaN of V among the drafted tokens: each is added to the sums of the vectors that see its token.
   if (__builtin_amdgcn_ballot_w64(dirty) != 0) {  // uniform
     for (int blk = p.blk0 + (PW == 1 ? par : 0); blk < p.blk1; blk += CW) {
@@ -679,7 +765,7 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
     if (par == 1) {
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        uint8_t* to = (col == 0 ? st0 : st1) + (g * kGroup + l32) * 512;
+        uint8_t* to = ring + col * kStage + (g * kGroup + l32) * 512;
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
@@ -711,7 +797,7 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
       const int v = (col * NG + g) * kGroup + l32;
       if (v >= p.nv) continue;
       const size_t at = (p.at + v) * A.Hkv + p.h;
-      const uint8_t* other = (col == 0 ? st0 : st1) + (g * kGroup + l32) * 512;
+      const uint8_t* other = ring + col * kStage + (g * kGroup + l32) * 512;
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
@@ -736,10 +822,7 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
 __global__ __launch_bounds__(kThreads, 1) void tree_f16_d128(const f16* __restrict__ q, const f16* __restrict__ kp,
                                                              const f16* __restrict__ vp,
                                                              const int32_t* __restrict__ table, Fast F) {
-  __shared__ __align__(16) uint8_t st0[kStage];
-  __shared__ __align__(16) uint8_t st1[kStage];
-  __shared__ __align__(16) uint8_t st2[kStage];
-  __shared__ __align__(16) uint8_t st3[kStage];
+  __shared__ __align__(16) uint8_t ring[4 * kStage];
   __shared__ Smem sm;
   const Args& A = F.a;
   const int G = A.Hq / A.Hkv, B = A.batch, Hkv = A.Hkv;
@@ -833,9 +916,9 @@ __global__ __launch_bounds__(kThreads, 1) void tree_f16_d128(const f16* __restri
       p.blk0 = k0;
       p.blk1 = k1;
       p.at = (size_t)w * kTileVec + (size_t)p.r.first * G + p.v0;
-      if (p.nv <= 2 * kGroup) tree_piece<2, 1>(F, p, sm, st0, st1, st2, st3);
-      else if (p.nv <= 4 * kGroup) tree_piece<2, 2>(F, p, sm, st0, st1, st2, st3);
-      else tree_piece<4, 2>(F, p, sm, st0, st1, st2, st3);
+      if (p.nv <= 2 * kGroup) tree_piece<2, 1>(F, p, sm, ring);
+      else if (p.nv <= 4 * kGroup) tree_piece<2, 2>(F, p, sm, ring);
+      else tree_piece<4, 2>(F, p, sm, ring);
     }
   }
 }

@@ -308,6 +308,7 @@ constexpr int kWorkgroups = 256;
 constexpr int kItemCost = 6;     // a piece's start and join, in blocks
 constexpr int kMinStretch = 4;
 constexpr int kMaxRows = 1024;
+constexpr int kMaxGroup = 2048;   // query heads per KV head (256 G G < 2^32: token_of is exact)
 constexpr int kRowB = 2 * D;     // bytes of a K or V row
 constexpr int kStageTok = 64;    // tokens of a stage
 constexpr int kStage = 2 * kStageTok * kRowB;  // bytes: K, then V
@@ -323,10 +324,14 @@ struct Fast {
   float *o, *ml;    // [vector of the workspace][KV head][D] and [2]
   int P16;          // page size / 16
   uint32_t page_magic;  // ceil(2^32 / P16): n / P16 = n * page_magic >> 32 (P16 > 1)
+  uint32_t head_magic;  // the same of G = Hq / Hkv, for a row's vectors (fewer than 256 G + 256, G <= kMaxGroup)
 };
 
 __device__ __forceinline__ int page_index(const Fast& F, int n) {
   return F.P16 == 1 ? n : (int)__umulhi((uint32_t)n, F.page_magic);
+}
+__device__ __forceinline__ int token_of(const Fast& F, int G, int v) {  // v / G
+  return G == 1 ? v : (int)__umulhi((uint32_t)v, F.head_magic);
 }
 __device__ __forceinline__ size_t rows16_at(const Fast& F, int h, int page, int n, int index) {
   return (((size_t)page * F.a.Hkv + h) * F.P16 + (n - index * F.P16)) * (16 * D);
@@ -448,7 +453,7 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
   for (int g = 0; g < NG; ++g) {
     const int v = (col * NG + g) * kGroup + l32;
     const bool live = v < p.nv;
-    const int vv = p.v0 + (live ? v : 0), tok = vv / G;
+    const int vv = p.v0 + (live ? v : 0), tok = token_of(F, G, vv);
     const f16* row = p.q + ((size_t)(p.r.first + tok) * A.Hq + (size_t)p.h * G + (vv - tok * G)) * D + 8 * h;
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
@@ -462,9 +467,12 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
   // The masks of the tile's vectors, where a block of the piece holds drafted tokens.
   const int drafts = min(p.r.n, p.r.limit - p.r.context);  // of the row, as far as the table holds them
   if (p.blk1 * kBlock > p.r.context) {                     // uniform
-    for (int i = threadIdx.x; i < p.nv * 2 * A.words; i += kThreads) {
-      const int v = i / (2 * A.words), w = i - v * (2 * A.words);
-      sm.mask[v][w] = mask_word(A, p.r.first + (p.v0 + v) / G, w, drafts);
+    const int v = threadIdx.x;
+    static_assert(kTileVec <= kThreads, "");
+    if (v < p.nv) {
+      const int j = p.r.first + token_of(F, G, p.v0 + v);
+#pragma unroll 1
+      for (int w = 0; w < 2 * A.words; ++w) sm.mask[v][w] = mask_word(A, j, w, drafts);
     }
   }
 
@@ -664,8 +672,8 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
   // A wavefront's blocks in order: block i lies in stage i / PW.
   constexpr int kOther = kBlock * kRowB;  // the stage's second block
   const auto place = [&](int i) { return (uint32_t)((i / PW) & 3) * kStage + (PW == 1 ? par : i & 1) * kOther; };
-  issue(1);
-  if constexpr (PW == 1) issue(2);
+#pragma unroll 1
+  for (int st = 1; st < (PW == 1 ? 3 : 2); ++st) issue(st);
   rows = rows_of(PW == 1 ? 3 : 2);
   for_each4([&]<int U>() __attribute__((always_inline)) { dma16<U>(rows.k, rows.to, at_k ^ (64 * U)); });
   if constexpr (PW == 2) {
@@ -693,10 +701,19 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
     for (int s = 0; s < 8; ++s) read_k(place(1), s);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      const uint32_t seen = first >= special ? seen_of(g, first) : 0xffffffffu;
+      if (first >= special) {  // uniform
+        const uint32_t seen = seen_of(g, first);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) c[g][r] = seen >> bit_of(r) & 1 ? c[g][r] : -INFINITY;
+        for (int r = 0; r < 16; ++r) c[g][r] = seen >> bit_of(r) & 1 ? c[g][r] : -INFINITY;
+      }
+      float mx = c[g][0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, c[g][r]);
+      mx = as_f32_value(mx * sc);
+      a[g].m = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      huge |= fabsf(a[g].m) >= 0x1p24f && a[g].m != -INFINITY;
     }
+    huge = __builtin_amdgcn_ballot_w64(huge) != 0;
   }
   const auto turns = [&]<bool SPECIAL>(int from, int to) __attribute__((always_inline)) {
 #pragma unroll 1
@@ -705,8 +722,9 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
       block.template operator()<SPECIAL>(i, blk, blk + CW, place(i + 2), place(i));
     }
   };
-  // (a block scores the next one too)
-  const int plain = max(0, min(nst * PW, (special - p.blk0) / CW - 1));
+  // (A block scores the next one too.  Short pieces stay with the code of the special blocks, which they need besides: each
+  // line of code is loaded once a launch, and a piece of 8 blocks waits for that most of its time.)
+  const int plain = nst <= 6 ? 0 : max(0, min(nst * PW, (special - p.blk0) / CW - 1));
   turns.template operator()<false>(0, plain);
   turns.template operator()<true>(plain, nst * PW);
   // Infinities and NaN of V among the drafted tokens: each is added to the sums of the vectors that see its token.
@@ -1021,7 +1039,7 @@ Layout layout(int tokens, int batch, int Hq, int Hkv) {
 bool fast_sizes(int tokens, int batch, int Hq, int Hkv, int head_dim, int P, int max_pages, int kv_dtype) {
   const long blocks = (long)max_pages * P / kBlock + 1 + kItemCost;
   const long tiles = (long)tokens * (Hq / Hkv) / kTileVec + batch;
-  return kv_dtype == CIR_F16 && head_dim == D && P % 16 == 0 && (long)max_pages * P / 16 * (P / 16) < (1L << 32) &&
+  return kv_dtype == CIR_F16 && head_dim == D && P % 16 == 0 && Hq / Hkv <= kMaxGroup && (long)max_pages * P / 16 * (P / 16) < (1L << 32) &&
          batch <= kMaxRows && blocks * tiles < (1L << 31) - kWorkgroups;
 }
 
@@ -1075,10 +1093,11 @@ extern "C" int cir_paged_tree_attention(const void* q, const void* k_pool, const
     CIR_CHECK_ARG(workspace && workspace_bytes >= l.total && (uintptr_t)workspace % 16 == 0,
                   "tree_attention: workspace too small or not on 16 bytes (%zu < %zu)", workspace_bytes, l.total);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    const uint32_t P16 = page_size / 16;
+    const uint32_t P16 = page_size / 16, G = num_heads / num_kv_heads;
     const Fast F{A, reinterpret_cast<RowRec*>(ws + l.rows), reinterpret_cast<int*>(ws + l.row_of),
                  reinterpret_cast<int*>(ws + l.stretch), reinterpret_cast<float*>(ws + l.o),
-                 reinterpret_cast<float*>(ws + l.ml), (int)P16, (uint32_t)(((1ull << 32) + P16 - 1) / P16)};
+                 reinterpret_cast<float*>(ws + l.ml), (int)P16, (uint32_t)(((1ull << 32) + P16 - 1) / P16),
+                 (uint32_t)(((1ull << 32) + G - 1) / G)};
     tree_f16_d128<<<teams_of(num_kv_heads) * num_kv_heads, kThreads, 0, s>>>(
         static_cast<const f16*>(q), static_cast<const f16*>(k_pool), static_cast<const f16*>(v_pool), page_table, F);
     const int st = launch_status();

@@ -281,42 +281,75 @@ struct NormIn {
   int wf32;  // weights in fp32 (else fp16)
   float eps;
 };
-constexpr int kNormItems = 2;
+template <int NP>
+__device__ __forceinline__ void load_weights(const void* w, int f32, int at, float* y) {  // (any address)
+  typedef float wide __attribute__((ext_vector_type(NP), aligned(4)));
+  typedef f16 half __attribute__((ext_vector_type(NP), aligned(2)));
+  if (f32) {  // uniform
+    const wide x = *reinterpret_cast<const wide*>((const float*)w + at);
+#pragma unroll
+    for (int e = 0; e < NP; ++e) y[e] = x[e];
+  } else {
+    const half x = *reinterpret_cast<const half*>((const f16*)w + at);
+#pragma unroll
+    for (int e = 0; e < NP; ++e) y[e] = to_f32(x[e]);
+  }
+}
 
 template <typename T, typename TK, int NP>
 __global__ __launch_bounds__(kRopeThreads) void norm_rope_append_kernel(
     RopeIn in, NormIn nm, const int32_t* __restrict__ positions, const int64_t* __restrict__ slot_map,
     const double* __restrict__ freq, float factor, T* q_out, TK* __restrict__ kp, TK* __restrict__ vp, int tokens,
     int Hq, int Hkv, int D, int rot, int halves, int P, int64_t slots, int lph) {
+  constexpr int kItems = 64 * 2 * NP >= kMaxDim ? 1 : 2;  // of a lane: 64 lanes at most have a head
   __shared__ float2 sm_cs[kTokens][kMaxDim / 2];
   __shared__ int64_t sm_at[kTokens];  // pool element of the token's row in KV head 0 (negative: padding)
   const int t0 = blockIdx.x * kTokens, nt = min(kTokens, tokens - t0);
   const int half = rot / 2;
   const int per_head = D / 2 / NP;
   const int lane = threadIdx.x & (lph - 1), group = threadIdx.x / lph, groups = kRopeThreads / lph;
+  const int heads = Hq + 2 * Hkv, share = (heads + gridDim.y - 1) / gridDim.y;
+  const int h0 = blockIdx.y * share, n = max(0, min(heads, h0 + share) - h0);
   // The lane's items: pair p0 = c NP on, whose elements are lo .. lo + NP - 1 and hi .. hi + NP - 1.
-  int lo[kNormItems], hi[kNormItems];
-  bool live[kNormItems];
-  float qw[kNormItems][2 * NP], kw[kNormItems][2 * NP];
+  int lo[kItems], hi[kItems];
+  bool live[kItems];
 #pragma unroll
-  for (int i = 0; i < kNormItems; ++i) {
+  for (int i = 0; i < kItems; ++i) {
     const int c = lane + i * lph, p0 = c * NP;
     live[i] = c < per_head;
     const bool apart = halves && p0 < half;
     lo[i] = apart ? p0 : 2 * p0;
     hi[i] = apart ? p0 + half : 2 * p0 + NP;
-    if (live[i]) {
+  }
+  // Head `h` of token t0 + u, and the group's next one; its x is on its way while the one before is worked on.
+  int u = n > 0 ? group / n : nt, h = n > 0 ? group - u * n : 0;
+  Vec<T, NP> na[kItems], nb[kItems];
+  const auto load = [&]() __attribute__((always_inline)) {
+    const int64_t tok = t0 + u;
+    const int hh = h0 + h;
+    const T* src = hh < Hq         ? (const T*)in.q + tok * in.q_token + hh * in.q_head
+                   : hh < Hq + Hkv ? (const T*)in.k + tok * in.k_token + (hh - Hq) * in.k_head
+                                   : (const T*)in.v + tok * in.v_token + (hh - Hq - Hkv) * in.v_head;
 #pragma unroll
-      for (int e = 0; e < 2 * NP; ++e) {
-        const int at = e < NP ? lo[i] + e : hi[i] + e - NP;
-        qw[i][e] = nm.wf32 ? ((const float*)nm.qw)[at] : to_f32(((const f16*)nm.qw)[at]);
-        kw[i][e] = nm.wf32 ? ((const float*)nm.kw)[at] : to_f32(((const f16*)nm.kw)[at]);
-      }
+    for (int i = 0; i < kItems; ++i) {
+      if (!live[i]) continue;
+      na[i] = load_vec<T, NP>(src + lo[i]);
+      nb[i] = load_vec<T, NP>(src + hi[i]);
     }
+  };
+  if (u < nt) load();
+  float qw[kItems][2 * NP], kw[kItems][2 * NP];
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
+    if (!live[i]) continue;
+    load_weights<NP>(nm.qw, nm.wf32, lo[i], qw[i]);
+    load_weights<NP>(nm.qw, nm.wf32, hi[i], qw[i] + NP);
+    load_weights<NP>(nm.kw, nm.wf32, lo[i], kw[i]);
+    load_weights<NP>(nm.kw, nm.wf32, hi[i], kw[i] + NP);
   }
   for (int i = threadIdx.x; i < nt * half; i += kRopeThreads) {
-    const int u = i / half, p = i - u * half;
-    sm_cs[u][p] = turn_of(positions[t0 + u], freq[p], factor);
+    const int w = i / half, p = i - w * half;
+    sm_cs[w][p] = turn_of(positions[t0 + w], freq[p], factor);
   }
   if ((int)threadIdx.x < nt) {
     const int64_t s = slot_map[t0 + threadIdx.x];
@@ -328,36 +361,32 @@ __global__ __launch_bounds__(kRopeThreads) void norm_rope_append_kernel(
     sm_at[threadIdx.x] = at;
   }
   __syncthreads();
-  const int heads = Hq + 2 * Hkv, share = (heads + gridDim.y - 1) / gridDim.y;
-  const int h0 = blockIdx.y * share, n = max(0, min(heads, h0 + share) - h0);
   const float inv_d = 1.f / (float)D;
-  for (int id = group; id < nt * n; id += groups) {  // (the lanes of a head stay together)
-    const int u = id / n, h = h0 + id - u * n;
-    const int64_t at = sm_at[u];
-    if (at < 0) continue;
-    const int64_t tok = t0 + u;
-    const T* src = h < Hq         ? (const T*)in.q + tok * in.q_token + h * in.q_head
-                   : h < Hq + Hkv ? (const T*)in.k + tok * in.k_token + (h - Hq) * in.k_head
-                                  : (const T*)in.v + tok * in.v_token + (h - Hq - Hkv) * in.v_head;
-    float x[kNormItems][2 * NP], sum = 0.f;
+  while (u < nt) {  // (the lanes of a head stay together)
+    const int64_t at = sm_at[u], tok = t0 + u;
+    const int hh = h0 + h, was = u;
+    float x[kItems][2 * NP], sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < kNormItems; ++i) {
+    for (int i = 0; i < kItems; ++i) {
       if (!live[i]) continue;
-      const Vec<T, NP> a = load_vec<T, NP>(src + lo[i]), b = load_vec<T, NP>(src + hi[i]);
 #pragma unroll
       for (int e = 0; e < NP; ++e) {
-        x[i][e] = to_f32(a.v[e]);
-        x[i][NP + e] = to_f32(b.v[e]);
+        x[i][e] = to_f32(na[i].v[e]);
+        x[i][NP + e] = to_f32(nb[i].v[e]);
       }
 #pragma unroll
       for (int e = 0; e < 2 * NP; ++e) sum = fmaf(x[i][e], x[i][e], sum);
     }
-    if (h < Hq + Hkv) {
+    h += groups;
+    while (h >= n) h -= n, ++u;
+    if (u < nt) load();
+    if (at < 0) continue;
+    if (hh < Hq + Hkv) {
       for (int off = lph >> 1; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
       const float r = 1.f / sqrtf(fmaf(sum, inv_d, nm.eps));
-      const bool is_q = h < Hq;
+      const bool is_q = hh < Hq;
 #pragma unroll
-      for (int i = 0; i < kNormItems; ++i) {
+      for (int i = 0; i < kItems; ++i) {
         if (!live[i]) continue;
         const int p0 = (lane + i * lph) * NP;
 #pragma unroll
@@ -365,7 +394,7 @@ __global__ __launch_bounds__(kRopeThreads) void norm_rope_append_kernel(
         if (p0 >= half) continue;
 #pragma unroll
         for (int e = 0; e < NP; ++e) {
-          const float2 cs = sm_cs[u][p0 + e];
+          const float2 cs = sm_cs[was][p0 + e];
           const int re = halves ? e : 2 * e, im = halves ? NP + e : 2 * e + 1;
           const float a = x[i][re], b = x[i][im];
           x[i][re] = as_f32_value(fmaf(a, cs.x, -(b * cs.y)));
@@ -374,7 +403,7 @@ __global__ __launch_bounds__(kRopeThreads) void norm_rope_append_kernel(
       }
     }
 #pragma unroll
-    for (int i = 0; i < kNormItems; ++i) {
+    for (int i = 0; i < kItems; ++i) {
       if (!live[i]) continue;
       float ya[NP], yb[NP];
 #pragma unroll
@@ -382,12 +411,12 @@ __global__ __launch_bounds__(kRopeThreads) void norm_rope_append_kernel(
         ya[e] = as_f32_value(x[i][e]);
         yb[e] = as_f32_value(x[i][NP + e]);
       }
-      if (h < Hq) {
-        T* dst = q_out + tok * in.o_token + h * in.o_head;
+      if (hh < Hq) {
+        T* dst = q_out + tok * in.o_token + hh * in.o_head;
         store_vec<T, NP>(dst + lo[i], ya);
         store_vec<T, NP>(dst + hi[i], yb);
       } else {
-        TK* dst = (h < Hq + Hkv ? kp + (int64_t)(h - Hq) * P * D : vp + (int64_t)(h - Hq - Hkv) * P * D) + at;
+        TK* dst = (hh < Hq + Hkv ? kp + (int64_t)(hh - Hq) * P * D : vp + (int64_t)(hh - Hq - Hkv) * P * D) + at;
         store_vec<TK, NP>(dst + lo[i], ya);
         store_vec<TK, NP>(dst + hi[i], yb);
       }

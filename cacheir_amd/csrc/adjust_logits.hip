@@ -16,11 +16,14 @@ namespace {
 // One workgroup takes kChunk tokens of the vocabulary for some of a sequence's rows.  Counts
 // of a whole vocabulary do not fit LDS, so each chunk's workgroup reads the sequence's history
 // by itself (from L2: 64 KB for 8000 tokens) and counts what falls into its chunk, once for all
-// of its rows; the drafted tokens on a row's path are added before the row and taken off after
-// it.  A word per token: how often it was said, its place in the bias list, and whether it was
-// given in the prompt.  Bound by the read and write of the logits.
+// of its rows; between two rows the drafted tokens on the one's path and not on the other's are
+// added or taken off.  A word per token: how often it was said, its place in the bias list, and
+// whether it was given in the prompt.  Bound by the read and write of the logits: a row's are on
+// their way while the one before is worked on, the first row's while the history is counted.
+// 485 rows of 152064 in fp16 (295 MB, histories of up to 4000): 73 us, a copy of them takes 57; with 512 threads 77.  Chunks
+// of 4096 or 16384 tokens, which read the history twice or half as often: 90 and 85.
 constexpr int kChunk = 8192;
-constexpr int kThreads = 512;
+constexpr int kThreads = 1024;
 constexpr int kCountBits = 20;                        // history and drafts hold fewer than 2^20 tokens
 constexpr uint32_t kCount = (1u << kCountBits) - 1;
 constexpr int kMaxBias = (1 << (31 - kCountBits)) - 1;  // 11 bits: index + 1
@@ -41,10 +44,27 @@ struct Args {
   int rows, vocab, history_width, bias_width, words, allowed_words, in_place;
 };
 
-template <typename T, int VE>
+template <typename T>
+__device__ __forceinline__ uint32_t raw_of(T x) {
+  if constexpr (sizeof(T) == 2) return __builtin_bit_cast(uint16_t, x);
+  else return __builtin_bit_cast(uint32_t, x);
+}
+template <typename T>
+__device__ __forceinline__ T elem_of(uint32_t raw) {
+  if constexpr (sizeof(T) == 2) return __builtin_bit_cast(T, (uint16_t)raw);
+  else return __builtin_bit_cast(T, raw);
+}
+
+template <typename T>
 __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const T* in, T* out, Args A) {
-  typedef T vt __attribute__((ext_vector_type(VE)));
-  __shared__ uint32_t sm_tab[kChunk];
+  constexpr int VE = 16 / sizeof(T), J = kChunk / (kThreads * VE);  // tokens of a vector, vectors of a thread
+  constexpr uint32_t kAll = (1u << VE) - 1;
+  // (rows of any stride and address: the hardware takes vectors at any element)
+  typedef T mt __attribute__((ext_vector_type(VE), aligned(sizeof(T))));
+  typedef uint32_t vt __attribute__((ext_vector_type(4)));
+  constexpr int kBits = 8 * sizeof(T), kPer = 32 / kBits;  // of an element; elements of a word
+  constexpr uint32_t kElem = kPer == 1 ? ~0u : (1u << kBits % 32) - 1;
+  __shared__ uint32_t sm_tab[kChunk], sm_drafted[kChunk / 32];
   const int t = threadIdx.x, b = blockIdx.y;
   const int v0 = blockIdx.x * kChunk, nv = min(kChunk, A.vocab - v0);
   // The sequence's rows, and this workgroup's share of them.
@@ -58,9 +78,50 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const T* in, T*
   if (i0 >= i1) return;  // uniform
   const int drafts = A.drafts ? min(n, 64 * A.words) : 0;
 
-  for (int i = t; i < kChunk; i += kThreads) sm_tab[i] = 0;
-  __syncthreads();
+  // Tokens of vector k that the mask of the sequence's row i allows (none behind the vocabulary).
+  const auto allowed = [&](int i, uint32_t (&ok)[J]) __attribute__((always_inline)) {
+    const uint8_t* bits = reinterpret_cast<const uint8_t*>(A.allowed + (int64_t)(first + i) * A.allowed_words) + v0 / 8;
+#pragma unroll
+    for (int k = 0; k < J; ++k) {
+      const int j = (t + k * kThreads) * VE;
+      ok[k] = j >= nv || i >= i1 ? 0 : A.allowed ? bits[j >> 3] >> (j & 7) & kAll : kAll;
+    }
+  };
+  const auto load = [&](int i, int k) __attribute__((always_inline)) {
+    const T* src = in + (first + i) * A.ld_in + v0 + (t + k * kThreads) * VE;
+    const int rest = nv - (t + k * kThreads) * VE;
+    if (rest >= VE) return __builtin_bit_cast(vt, *reinterpret_cast<const mt*>(src));
+    vt x = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < VE; ++e)
+      if (e < rest) x[e / kPer] |= raw_of(src[e]) << e % kPer * kBits;
+    return x;
+  };
+  // The draft token of this thread: its place in the chunk.
+  int place = -1;
   const auto in_chunk = [&](int64_t id) { return (uint64_t)(id - v0) < (uint64_t)nv; };
+  const auto on_path = [&](int i) __attribute__((always_inline)) {
+    return place >= 0 && i < i1 && (A.masks[(int64_t)(first + i) * A.words + (t >> 6)] >> (t & 63) & 1);
+  };
+  vt x[J], xn[J];
+  uint32_t ok[J], okn[J];
+  allowed(i0, ok);
+  allowed(i0 + 1, okn);
+  if (!A.in_place) {  // (in place most vectors need no load: below)
+#pragma unroll
+    for (int k = 0; k < J; ++k)
+      if (ok[k]) x[k] = load(i0, k);
+  }
+  if (t < drafts) {
+    const int64_t id = A.drafts[first + t];
+    if (in_chunk(id)) place = (int)(id - v0);
+  }
+  bool on = on_path(i0), was = false;
+
+  for (int i = t; i < kChunk / 4; i += kThreads) *reinterpret_cast<uint4*>(sm_tab + 4 * i) = make_uint4(0, 0, 0, 0);
+  for (int i = t; i < kChunk / 32; i += kThreads) sm_drafted[i] = 0;
+  const bool tree = __syncthreads_or(place >= 0);  // some token of the sequence's tree lies in the chunk
+  if (place >= 0) atomicOr(&sm_drafted[place >> 5], 1u << (place & 31));
   if (A.bias_ids) {  // (of equal ids the last one counts)
     for (int k = t; k < A.bias_width; k += kThreads) {
       const int64_t id = A.bias_ids[(int64_t)b * A.bias_width + k];
@@ -69,16 +130,43 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const T* in, T*
     __syncthreads();
   }
   if (A.history) {
+    constexpr int U = 4;  // pairs on their way
+    typedef int64_t i64x2 __attribute__((ext_vector_type(2), aligned(8)));
     const int len = min(max(A.history_lens[b], 0), A.history_width);
     const int prompt = A.prompt_lens ? A.prompt_lens[b] : 0;
     const int64_t* h = A.history + (int64_t)b * A.history_width;
-    for (int k = t; k < len; k += kThreads) {
-      const int64_t id = h[k];
-      if (in_chunk(id)) {
-        if (k < prompt) atomicOr(&sm_tab[id - v0], kGiven);
-        else atomicAdd(&sm_tab[id - v0], 1u);
+    const auto count = [&](int64_t id, int k) __attribute__((always_inline)) {
+      if (!in_chunk(id)) return;
+      if (k < prompt) atomicOr(&sm_tab[id - v0], kGiven);
+      else atomicAdd(&sm_tab[id - v0], 1u);
+    };
+    for (int k0 = 0; k0 < len; k0 += 2 * U * kThreads) {
+      i64x2 id[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + 2 * (t + u * kThreads);
+        id[u] = i64x2{-1, -1};
+        if (k + 1 < len) id[u] = *reinterpret_cast<const i64x2*>(h + k);
+        else if (k < len) id[u].x = h[k];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + 2 * (t + u * kThreads);
+        count(id[u].x, k);
+        count(id[u].y, k + 1);
       }
     }
+  }
+  __syncthreads();
+  // Tokens of the thread's vectors that some row adjusts.  They are few, so a lane works on its own one after another: the
+  // same for every element, needed or not, took as long as the memory (85 us instead of 77).
+  uint32_t touched[J];
+#pragma unroll
+  for (int k = 0; k < J; ++k) {
+    const int j = (t + k * kThreads) * VE;
+    touched[k] = sm_drafted[j >> 5] >> (j & 31) & kAll;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) touched[k] |= sm_tab[j + e] ? 1u << e : 0;
   }
   const float rep = A.rep ? A.rep[b] : 1.f, pres = A.pres ? A.pres[b] : 0.f, freq = A.freq ? A.freq[b] : 0.f;
   const auto adjust = [&](float x, uint32_t w) __attribute__((always_inline)) {
@@ -89,40 +177,60 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const T* in, T*
     return x;
   };
   for (int i = i0; i < i1; ++i) {
-    const int row = first + i;
-    // Whether token t of the row's tree is on its path, and falls into the chunk.
-    int64_t said = -1;
-    if (t < drafts && (A.masks[(int64_t)row * A.words + (t >> 6)] >> (t & 63) & 1)) {
-      const int64_t id = A.drafts[first + t];
-      if (in_chunk(id)) said = id - v0;
+    if (tree) __syncthreads();  // uniform: the row before is done
+    if (on != was) atomicAdd(&sm_tab[place], on ? 1u : ~0u);
+    was = on;
+    on = on_path(i + 1);
+    if (!A.in_place) {
+#pragma unroll
+      for (int k = 0; k < J; ++k)
+        if (okn[k]) xn[k] = load(i + 1, k);
     }
-    __syncthreads();  // (the history is counted, the row before is done)
-    if (said >= 0) atomicAdd(&sm_tab[said], 1u);
-    __syncthreads();
-    const T* src = in + row * A.ld_in + v0;
-    T* dst = out + row * A.ld_out + v0;
-    const int32_t* bits = A.allowed ? A.allowed + (int64_t)row * A.allowed_words + v0 / 32 : nullptr;
-    for (int j = t * VE; j < nv; j += kThreads * VE) {  // (nv is a multiple of VE)
-      constexpr uint32_t kAll = (1u << VE) - 1;
-      const uint32_t ok = bits ? ((uint32_t)bits[j >> 5] >> (j & 31)) & kAll : kAll;
-      uint32_t w[VE], any = 0;
+    uint32_t oka[J];
+    allowed(i + 2, oka);
+    if (tree) __syncthreads();  // uniform
+    T* dst = out + (first + i) * A.ld_out + v0;
 #pragma unroll
-      for (int e = 0; e < VE; ++e) any |= w[e] = sm_tab[j + e];
-      if (A.in_place && ok == kAll && !any) continue;
-      vt x = {};
-      if (ok) x = *reinterpret_cast<const vt*>(src + j);
-      if (any | (ok ^ kAll)) {
-#pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          const float y = adjust(to_f32<T>(x[e]), w[e]);
-          x[e] = ok >> e & 1 ? w[e] ? from_f32<T>(y) : x[e] : from_f32<T>(-INFINITY);
-        }
+    for (int k = 0; k < J; ++k) {
+      const int j = (t + k * kThreads) * VE;
+      if (j >= nv) break;
+      uint32_t left = touched[k] & ok[k];
+      if (A.in_place) {
+        if (ok[k] == kAll && !left) continue;
+        if (ok[k]) x[k] = load(i, k);
       }
-      *reinterpret_cast<vt*>(dst + j) = x;
+      while (left) {
+        const int e = __builtin_ctz(left);
+        left &= left - 1;
+        const uint32_t w = sm_tab[j + e];
+        const int d = e / kPer, shift = e % kPer * kBits;
+        const uint32_t word = d == 0 ? x[k][0] : d == 1 ? x[k][1] : d == 2 ? x[k][2] : x[k][3];
+        const T old = elem_of<T>(word >> shift);
+        const uint32_t y = raw_of(w ? from_f32<T>(adjust(to_f32<T>(old), w)) : old) << shift;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[k][i] = d == i ? (x[k][i] & ~(kElem << shift)) | y : x[k][i];
+      }
+      const uint32_t lowest = raw_of(from_f32<T>(-INFINITY));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t off = 0;  // the elements that the mask takes out
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) off |= ok[k] >> (i * kPer + e) & 1 ? 0 : kElem << e * kBits;
+        x[k][i] = (x[k][i] & ~off) | ((kPer == 1 ? lowest : lowest * 0x10001u) & off);
+      }
+      if (nv - j >= VE) {
+        *reinterpret_cast<mt*>(dst + j) = __builtin_bit_cast(mt, x[k]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+          if (e < nv - j) dst[j + e] = elem_of<T>(x[k][e / kPer] >> e % kPer * kBits);
+      }
     }
-    if (i + 1 < i1) {
-      __syncthreads();
-      if (said >= 0) atomicSub(&sm_tab[said], 1u);
+#pragma unroll
+    for (int k = 0; k < J; ++k) {
+      x[k] = xn[k];
+      ok[k] = okn[k];
+      okn[k] = oka[k];
     }
   }
 }
@@ -160,20 +268,16 @@ extern "C" int cir_adjust_logits(const void* logits, int64_t ld_in, void* out, i
   const uintptr_t z_bytes = ((uintptr_t)(rows - 1) * ld_out + vocab) * size;
   CIR_CHECK_ARG(a == z ? (rows == 1 || ld_in == ld_out) : a < z ? z - a >= a_bytes : a - z >= z_bytes,
                 "adjust_logits: out overlaps the logits");
-  const Args A{offsets, history_width ? history : nullptr, history_lens, prompt_lens, drafts, masks, repetition, presence, frequency,
-               bias_width ? bias_ids : nullptr, bias, allowed, ld_in, ld_out, rows, vocab, history_width, bias_width,
-               words, (vocab + 31) / 32, a == z};
   const int chunks = (vocab + kChunk - 1) / kChunk;
-  // Rows of a sequence are shared out until some 2048 workgroups fill the GPU.
+  // Rows of a sequence are shared out until some 2048 workgroups fill the GPU, four times over (1024: 87 us instead of 76,
+  // 4096: 80, each workgroup counts the history again).
   const int mean = (rows + batch - 1) / batch;
   const int shares = max(1, min(min(mean, 64), (int)(2048 / ((long)chunks * batch))));
-  const int ve = 16 / size;
-  const bool wide = (a | z) % 16 == 0 && ld_in % ve == 0 && ld_out % ve == 0 && vocab % ve == 0;
+  const Args A{offsets, history_width ? history : nullptr, history_lens, prompt_lens, drafts, masks, repetition, presence,
+               frequency, bias_width ? bias_ids : nullptr, bias, allowed, ld_in, ld_out, rows, vocab, history_width, bias_width,
+               words, (vocab + 31) / 32, a == z};
   const dim3 grid(chunks, batch, shares);
-  const auto go = [&]<typename T, int VE>() {
-    adjust_logits_kernel<T, VE><<<grid, kThreads, 0, as_stream(stream)>>>((const T*)logits, (T*)out, A);
-  };
-  if (dt == CIR_F16) wide ? go.template operator()<f16, 8>() : go.template operator()<f16, 1>();
-  else wide ? go.template operator()<float, 4>() : go.template operator()<float, 1>();
+  if (dt == CIR_F16) adjust_logits_kernel<<<grid, kThreads, 0, as_stream(stream)>>>((const f16*)logits, (f16*)out, A);
+  else adjust_logits_kernel<<<grid, kThreads, 0, as_stream(stream)>>>((const float*)logits, (float*)out, A);
   return launch_status();
 }

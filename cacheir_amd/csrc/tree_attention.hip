@@ -65,8 +65,9 @@ __device__ __forceinline__ bool sees(const Args& A, const Row& r, int j) {
 
 // -------------------------------------------------------------- any sizes -----
 // fp32 arithmetic for any head_dim up to 256, type and page size.  A workgroup takes up to kVec query vectors of one row
-// and KV head (a tile) over a stretch of the row's tokens, 64 at a time: K and V through LDS as fp32, a wavefront's
-// lanes are tokens for the scores and dims for the sum over V, each wavefront with its own four vectors.
+// and KV head (a tile) over a stretch of the row's tokens, 64 at a time: K and V through LDS as fp32 (the next 64 on their
+// way in registers), a wavefront's lanes are tokens for the scores and dims for the sum over V, each wavefront with its own
+// four vectors.
 constexpr int kGenThreads = 256;
 constexpr int kGenWaves = kGenThreads / 64;
 constexpr int kPerWave = 4;
@@ -80,10 +81,14 @@ template <typename T, int DM>  // DM: head_dim at most
 __global__ __launch_bounds__(kGenThreads) void tree_generic(const T* __restrict__ q, const T* __restrict__ kp,
                                                             const T* __restrict__ vp, T* __restrict__ out, Args A) {
   constexpr int ldk = DM + 4;
+  constexpr int VE = 16 / sizeof(T), kRowThreads = DM / VE;   // 16-byte vectors (at any address): of a row, a thread each
+  constexpr int kStep = kGenThreads / kRowThreads, PS = kTok / kStep;  // rows at a time
+  typedef T mt __attribute__((ext_vector_type(VE), aligned(sizeof(T))));
+  typedef T vt __attribute__((ext_vector_type(VE)));
   __shared__ __align__(16) float sm_q[kVec * DM], sm_k[kTok * ldk], sm_v[kTok * DM];
   __shared__ int sm_sum[kGenWaves], sm_find[2];
-  const int D = A.D, Dp = (D + 3) / 4 * 4;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int D = A.D;
+  const int t = threadIdx.x, lane = t & 63, wave = uni(t >> 6);
   const int G = A.Hq / A.Hkv, h = blockIdx.y;
 
   // The row and tile of this workgroup: tiles are numbered row after row.
@@ -125,12 +130,41 @@ __global__ __launch_bounds__(kGenThreads) void tree_generic(const T* __restrict_
   const int stretch = ((r.limit + A.splits - 1) / A.splits + kTok - 1) / kTok * kTok;
   const int k0 = min((int64_t)r.limit, (int64_t)blockIdx.z * stretch), k1 = min(r.limit, k0 + stretch);
 
-  for (int i = t; i < kVec * Dp; i += kGenThreads) {
-    const int v = i / Dp, d = i - v * Dp, vv = v0 + v;
-    float x = 0.f;
-    if (v < nv && d < D)
-      x = to_f32(q[((size_t)(r.first + vv / G) * A.Hq + (size_t)h * G + vv % G) * D + d]) * A.scale_log2;
-    sm_q[i] = x;
+  const int t_row = t / kRowThreads, d0 = t % kRowThreads * VE;
+  const auto part_of = [&](const T* row) __attribute__((always_inline)) {  // dims d0 .. of a row, zeros past the last
+    if (d0 + VE <= D) return static_cast<vt>(*reinterpret_cast<const mt*>(row + d0));
+    vt x = {};
+#pragma unroll
+    for (int e = 0; e < VE; ++e)
+      if (d0 + e < D) x[e] = row[d0 + e];
+    return x;
+  };
+  const auto put = [&](float* to, vt x, float by) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < VE; e += 4)
+      *reinterpret_cast<f32x4*>(to + d0 + e) =
+          f32x4{to_f32(x[e]) * by, to_f32(x[e + 1]) * by, to_f32(x[e + 2]) * by, to_f32(x[e + 3]) * by};
+  };
+  vt nk[PS], nv_[PS];  // the next tokens' K and V
+  const auto load = [&](int k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PS; ++i) {
+      const int pos = k + t_row + i * kStep;
+      nk[i] = nv_[i] = vt{};
+      if (pos >= k1) continue;
+      const int page = pos / A.P;
+      const size_t at = (((size_t)A.table[(size_t)b * A.max_pages + page] * A.Hkv + h) * A.P + (pos - page * A.P)) * D;
+      nk[i] = part_of(kp + at);
+      nv_[i] = part_of(vp + at);
+    }
+  };
+  if (k0 < k1) load(k0);  // uniform
+#pragma unroll
+  for (int i = 0; i < (kVec + kStep - 1) / kStep; ++i) {
+    const int v = t_row + i * kStep, vv = v0 + v;
+    if (v < kVec)
+      put(sm_q + v * DM, v < nv ? part_of(q + ((size_t)(r.first + vv / G) * A.Hq + (size_t)h * G + vv % G) * D) : vt{},
+          A.scale_log2);
   }
   float m[kPerWave], l[kPerWave], acc[kPerWave][DM / 64];
   int row[kPerWave];
@@ -145,27 +179,21 @@ __global__ __launch_bounds__(kGenThreads) void tree_generic(const T* __restrict_
   for (int k = k0; k < k1; k += kTok) {  // uniform
     const int nt = min(kTok, k1 - k);
     __syncthreads();
-    for (int i = t; i < kTok * Dp; i += kGenThreads) {
-      const int tok = i / Dp, d = i - tok * Dp;
-      float x = 0.f, y = 0.f;
-      if (tok < nt && d < D) {
-        const int pos = k + tok, page = pos / A.P;
-        const size_t at = (((size_t)A.table[(size_t)b * A.max_pages + page] * A.Hkv + h) * A.P + (pos - page * A.P)) * D + d;
-        x = to_f32(kp[at]);
-        y = to_f32(vp[at]);
-      }
-      sm_k[tok * ldk + d] = x;
-      sm_v[tok * Dp + d] = y;
+#pragma unroll
+    for (int i = 0; i < PS; ++i) {
+      put(sm_k + (t_row + i * kStep) * ldk, nk[i], 1.f);
+      put(sm_v + (t_row + i * kStep) * DM, nv_[i], 1.f);
     }
     __syncthreads();
+    if (k + kTok < k1) load(k + kTok);  // uniform
     float s[kPerWave];
 #pragma unroll
     for (int i = 0; i < kPerWave; ++i) s[i] = 0.f;
-    for (int d = 0; d < Dp; d += 4) {
+    for (int d = 0; d < D; d += 4) {
       const f32x4 x = *reinterpret_cast<const f32x4*>(sm_k + lane * ldk + d);
 #pragma unroll
       for (int i = 0; i < kPerWave; ++i) {
-        const f32x4 y = *reinterpret_cast<const f32x4*>(sm_q + (wave * kPerWave + i) * Dp + d);
+        const f32x4 y = *reinterpret_cast<const f32x4*>(sm_q + (wave * kPerWave + i) * DM + d);
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[i] = fmaf(x[e], y[e], s[i]);
       }
@@ -187,20 +215,26 @@ __global__ __launch_bounds__(kGenThreads) void tree_generic(const T* __restrict_
 #pragma unroll
       for (int c = 0; c < DM / 64; ++c) acc[i][c] *= alpha;
     }
-    for (int tok = 0; tok < nt; ++tok) {
-      float p[kPerWave];
-#pragma unroll
-      for (int i = 0; i < kPerWave; ++i) p[i] = __shfl(s[i], tok, 64);
-#pragma unroll
-      for (int c = 0; c < DM / 64; ++c) {
-        const int d = lane + 64 * c;
-        if (64 * c >= D) break;  // uniform
-        const float y = d < D ? sm_v[tok * Dp + d] : 0.f;
+    const auto sums = [&]<bool DRAFTED>() __attribute__((always_inline)) {
+#pragma unroll 8
+      for (int tok = 0; tok < (nt + 7) / 8 * 8; ++tok) {  // (tokens from nt on: zeros)
+        float p[kPerWave];
 #pragma unroll
         for (int i = 0; i < kPerWave; ++i)
-          if (!drafted || (seen[i] >> tok & 1)) acc[i][c] = fmaf(p[i], y, acc[i][c]);  // (what is not seen may be NaN)
+          p[i] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s[i]), tok));
+#pragma unroll
+        for (int c = 0; c < DM / 64; ++c) {  // (dims from D on are zero or not written, and go nowhere)
+          const float y = sm_v[tok * DM + lane + 64 * c];
+#pragma unroll
+          for (int i = 0; i < kPerWave; ++i) {
+            const float z = fmaf(p[i], y, acc[i][c]);
+            acc[i][c] = !DRAFTED || (seen[i] >> tok & 1) ? z : acc[i][c];  // (what is not seen may be NaN)
+          }
+        }
       }
-    }
+    };
+    if (drafted) sums.template operator()<true>();
+    else sums.template operator()<false>();
   }
 #pragma unroll
   for (int i = 0; i < kPerWave; ++i) {

@@ -64,15 +64,17 @@ __device__ __forceinline__ bool sees(const Args& A, const Row& r, int j) {
 }
 
 // -------------------------------------------------------------- any sizes -----
-// fp32 arithmetic for any head_dim up to 256, type and page size.  A workgroup takes up to kVec query vectors of one row
-// and KV head (a tile) over a stretch of the row's tokens, 64 at a time: K and V through LDS as fp32 (the next 64 on their
-// way in registers), a wavefront's lanes are tokens for the scores and dims for the sum over V, each wavefront with its own
-// four vectors.
+// Any head_dim up to 256, type and page size, in fp32.  A workgroup takes up to 16 query vectors of one row and KV head (a
+// tile) over a stretch of the row's tokens; its wavefronts take turns at blocks of 16 tokens, each with a softmax of its
+// own, and are joined through LDS at the end.  MFMA 16x16x4 in fp32, S^T = K Q^T and O^T = V^T P^T, from registers alone:
+// the order of the summed dims and tokens is free, so lane l takes dims 16 c + 4 (l / 16) .. of K and Q by one load, its
+// scores are those of tokens 4 (l / 16) .. of vector l % 16, which is how the second product wants the weights, and its
+// rows of V^T are dims 64 g + 4 (l % 16) .., again one load.  K of the next block and V of this one are on their way
+// during the products.
 constexpr int kGenThreads = 256;
 constexpr int kGenWaves = kGenThreads / 64;
-constexpr int kPerWave = 4;
-constexpr int kVec = kGenWaves * kPerWave;
-constexpr int kTok = 64;
+constexpr int kVec = 16;
+constexpr int kTok = 16;
 constexpr int kMaxD = 256;
 
 __device__ __forceinline__ int tiles_of(const Args& A, int n) { return (n * (A.Hq / A.Hkv) + kVec - 1) / kVec; }
@@ -80,17 +82,15 @@ __device__ __forceinline__ int tiles_of(const Args& A, int n) { return (n * (A.H
 template <typename T, int DM>  // DM: head_dim at most
 __global__ __launch_bounds__(kGenThreads) void tree_generic(const T* __restrict__ q, const T* __restrict__ kp,
                                                             const T* __restrict__ vp, T* __restrict__ out, Args A) {
-  constexpr int ldk = DM + 4;
-  constexpr int VE = 16 / sizeof(T), kRowThreads = DM / VE;   // 16-byte vectors (at any address): of a row, a thread each
-  constexpr int kStep = kGenThreads / kRowThreads, PS = kTok / kStep;  // rows at a time
-  typedef T mt __attribute__((ext_vector_type(VE), aligned(sizeof(T))));
-  typedef T vt __attribute__((ext_vector_type(VE)));
-  __shared__ __align__(16) float sm_q[kVec * DM], sm_k[kTok * ldk], sm_v[kTok * DM];
+  constexpr int C = DM / 16, NGr = DM / 64;
+  typedef T mt __attribute__((ext_vector_type(4), aligned(sizeof(T))));  // (at any address)
+  typedef T vt __attribute__((ext_vector_type(4)));
+  __shared__ __align__(16) float sm_o[kGenWaves][kVec][DM + 4];
+  __shared__ float sm_ml[kGenWaves][2][kVec];
   __shared__ int sm_sum[kGenWaves], sm_find[2];
   const int D = A.D;
-  const int t = threadIdx.x, lane = t & 63, wave = uni(t >> 6);
+  const int t = threadIdx.x, lane = t & 63, wave = uni(t >> 6), col = lane & 15, quarter = lane >> 4;
   const int G = A.Hq / A.Hkv, h = blockIdx.y;
-
   // The row and tile of this workgroup: tiles are numbered row after row.
   if (t == 0) sm_find[0] = -1;
   int before = 0;
@@ -127,133 +127,182 @@ __global__ __launch_bounds__(kGenThreads) void tree_generic(const T* __restrict_
   const Row r = row_of(A, b);
   const int v0 = uni(sm_find[1]) * kVec, nv = min(kVec, r.n * G - v0);
   // This workgroup's stretch of the row's tokens.
-  const int stretch = ((r.limit + A.splits - 1) / A.splits + kTok - 1) / kTok * kTok;
+  constexpr int kTurn = kTok * kGenWaves;
+  const int stretch = ((r.limit + A.splits - 1) / A.splits + kTurn - 1) / kTurn * kTurn;
   const int k0 = min((int64_t)r.limit, (int64_t)blockIdx.z * stretch), k1 = min(r.limit, k0 + stretch);
 
-  const int t_row = t / kRowThreads, d0 = t % kRowThreads * VE;
-  const auto part_of = [&](const T* row) __attribute__((always_inline)) {  // dims d0 .. of a row, zeros past the last
-    if (d0 + VE <= D) return static_cast<vt>(*reinterpret_cast<const mt*>(row + d0));
+  const auto part_of = [&](const T* row, int d) __attribute__((always_inline)) {  // dims d .. d + 3 of a row, zeros past the last
+    if (d + 4 <= D) return static_cast<vt>(*reinterpret_cast<const mt*>(row + d));
     vt x = {};
 #pragma unroll
-    for (int e = 0; e < VE; ++e)
-      if (d0 + e < D) x[e] = row[d0 + e];
+    for (int e = 0; e < 3; ++e)
+      if (d + e < D) x[e] = row[d + e];
     return x;
   };
-  const auto put = [&](float* to, vt x, float by) __attribute__((always_inline)) {
-#pragma unroll
-    for (int e = 0; e < VE; e += 4)
-      *reinterpret_cast<f32x4*>(to + d0 + e) =
-          f32x4{to_f32(x[e]) * by, to_f32(x[e + 1]) * by, to_f32(x[e + 2]) * by, to_f32(x[e + 3]) * by};
+  const auto f32_of = [](vt x) { return f32x4{to_f32(x[0]), to_f32(x[1]), to_f32(x[2]), to_f32(x[3])}; };
+  // Token k + l % 16 of block k: its page, and the place of its row in the pools (-1: none).
+  const auto page_of = [&](int64_t k) { return k + col < k1 ? A.table[(size_t)b * A.max_pages + (int)(k + col) / A.P] : -1; };
+  const auto row_at = [&](int64_t k, int page) {
+    return k + col < k1 ? (((int64_t)page * A.Hkv + h) * A.P + (int)(k + col) % A.P) * D : (int64_t)-1;
   };
-  vt nk[PS], nv_[PS];  // the next tokens' K and V
-  const auto load = [&](int k) __attribute__((always_inline)) {
+  vt nk[C];
+  const auto load_k = [&](int64_t at) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < PS; ++i) {
-      const int pos = k + t_row + i * kStep;
-      nk[i] = nv_[i] = vt{};
-      if (pos >= k1) continue;
-      const int page = pos / A.P;
-      const size_t at = (((size_t)A.table[(size_t)b * A.max_pages + page] * A.Hkv + h) * A.P + (pos - page * A.P)) * D;
-      nk[i] = part_of(kp + at);
-      nv_[i] = part_of(vp + at);
+    for (int c = 0; c < C; ++c) {
+      nk[c] = vt{};
+      if (16 * c < D && at >= 0) nk[c] = part_of(kp + at, 16 * c + 4 * quarter);
     }
   };
-  if (k0 < k1) load(k0);  // uniform
+  int64_t k = (int64_t)k0 + kTok * wave;
+  int64_t at = row_at(k, page_of(k));
+  load_k(at);
+  const int live = min(v0 + col, r.n * G - 1), j = r.first + live / G;  // (vectors past the last: the last one again)
+  f32x4 qf[C];
 #pragma unroll
-  for (int i = 0; i < (kVec + kStep - 1) / kStep; ++i) {
-    const int v = t_row + i * kStep, vv = v0 + v;
-    if (v < kVec)
-      put(sm_q + v * DM, v < nv ? part_of(q + ((size_t)(r.first + vv / G) * A.Hq + (size_t)h * G + vv % G) * D) : vt{},
-          A.scale_log2);
+  for (int c = 0; c < C; ++c) {
+    qf[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (16 * c >= D) continue;  // uniform
+    const T* row = q + ((size_t)j * A.Hq + (size_t)h * G + live % G) * D;
+    qf[c] = f32_of(part_of(row, 16 * c + 4 * quarter)) * A.scale_log2;
   }
-  float m[kPerWave], l[kPerWave], acc[kPerWave][DM / 64];
-  int row[kPerWave];
+  float m = -INFINITY, l = 0.f;
+  f32x4 acc[NGr][4];  // [64 dims][dim % 4]: dims 64 g + 16 (l / 16) + 4 i + dim % 4
 #pragma unroll
-  for (int i = 0; i < kPerWave; ++i) {
-    m[i] = -INFINITY;
-    l[i] = 0.f;
-    row[i] = r.first + min(v0 + wave * kPerWave + i, r.n * G - 1) / G;
+  for (int g = 0; g < NGr; ++g)
 #pragma unroll
-    for (int c = 0; c < DM / 64; ++c) acc[i][c] = 0.f;
-  }
-  for (int k = k0; k < k1; k += kTok) {  // uniform
-    const int nt = min(kTok, k1 - k);
-    __syncthreads();
+    for (int e = 0; e < 4; ++e) acc[g][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (; k < k1; k += kTurn) {  // uniform in a wavefront
+    const int page = page_of(k + kTurn);
+    vt nv_[4][NGr];
+    int64_t rows[4];
 #pragma unroll
-    for (int i = 0; i < PS; ++i) {
-      put(sm_k + (t_row + i * kStep) * ldk, nk[i], 1.f);
-      put(sm_v + (t_row + i * kStep) * DM, nv_[i], 1.f);
-    }
-    __syncthreads();
-    if (k + kTok < k1) load(k + kTok);  // uniform
-    float s[kPerWave];
+    for (int i = 0; i < 4; ++i) {  // token 4 (l / 16) + i
+      rows[i] = __shfl(at, 4 * quarter + i, 64);
 #pragma unroll
-    for (int i = 0; i < kPerWave; ++i) s[i] = 0.f;
-    for (int d = 0; d < D; d += 4) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(sm_k + lane * ldk + d);
-#pragma unroll
-      for (int i = 0; i < kPerWave; ++i) {
-        const f32x4 y = *reinterpret_cast<const f32x4*>(sm_q + (wave * kPerWave + i) * DM + d);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[i] = fmaf(x[e], y[e], s[i]);
+      for (int g = 0; g < NGr; ++g) {
+        nv_[i][g] = vt{};
+        if (64 * g < D && rows[i] >= 0) nv_[i][g] = part_of(vp + rows[i], 64 * g + 4 * col);
       }
     }
-    const bool drafted = k + nt > r.context;  // uniform: some tokens that not every vector sees
-    uint64_t seen[kPerWave];
+    f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int i = 0; i < kPerWave; ++i) {
-      seen[i] = nt < 64 ? (1ull << nt) - 1 : ~0ull;
-      if (drafted)
-        seen[i] &= seen_from(A, row[i], k, r.context, r.n) | (uint64_t)seen_from(A, row[i], k + 32, r.context, r.n) << 32;
-      const bool mine = seen[i] >> lane & 1;
-      const float x = mine ? s[i] : -INFINITY;
-      const float mn = fmaxf(m[i], wave_max(x)), ms = mn == -INFINITY ? 0.f : mn;
-      const float alpha = __builtin_amdgcn_exp2f(m[i] - ms);
-      s[i] = mine ? __builtin_amdgcn_exp2f(s[i] - ms) : 0.f;
-      l[i] = fmaf(l[i], alpha, wave_sum(s[i]));
-      m[i] = mn;
+    for (int c = 0; c < C; ++c) {
+      if (16 * c >= D) continue;  // uniform
+      const f32x4 x = f32_of(nk[c]);
 #pragma unroll
-      for (int c = 0; c < DM / 64; ++c) acc[i][c] *= alpha;
+      for (int e = 0; e < 4; ++e) s[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], qf[c][e], s[e & 1], 0, 0, 0);
     }
-    const auto sums = [&]<bool DRAFTED>() __attribute__((always_inline)) {
-#pragma unroll 8
-      for (int tok = 0; tok < (nt + 7) / 8 * 8; ++tok) {  // (tokens from nt on: zeros)
-        float p[kPerWave];
+    const int64_t here = at;
+    at = row_at(k + kTurn, page);
+    load_k(at);
+    const int nt = (int)min((int64_t)kTok, k1 - k);
+    const bool drafted = k + nt > r.context;  // uniform: some tokens that not every vector sees
+    uint32_t seen = (1u << nt) - 1;
+    if (drafted) seen &= seen_from(A, j, (int)k, r.context, r.n);
+    float p[4], mx = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kPerWave; ++i)
-          p[i] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s[i]), tok));
+    for (int i = 0; i < 4; ++i) {
+      p[i] = seen >> (4 * quarter + i) & 1 ? as_f32_value(s[0][i] + s[1][i]) : -INFINITY;
+      mx = fmaxf(mx, p[i]);
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - ms);
+    l *= alpha;
+    m = mn;
 #pragma unroll
-        for (int c = 0; c < DM / 64; ++c) {  // (dims from D on are zero or not written, and go nowhere)
-          const float y = sm_v[tok * DM + lane + 64 * c];
+    for (int i = 0; i < 4; ++i) {
+      p[i] = __builtin_amdgcn_exp2f(p[i] - ms);
+      l += p[i];
+    }
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {  // uniform
 #pragma unroll
-          for (int i = 0; i < kPerWave; ++i) {
-            const float z = fmaf(p[i], y, acc[i][c]);
-            acc[i][c] = !DRAFTED || (seen[i] >> tok & 1) ? z : acc[i][c];  // (what is not seen may be NaN)
+      for (int g = 0; g < NGr; ++g)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[g][e] *= alpha;
+    }
+    bool dirty = false;
+#pragma unroll
+    for (int g = 0; g < NGr; ++g) {
+      if (64 * g >= D) continue;  // uniform
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f32x4 x = f32_of(nv_[i][g]);
+        if (drafted) {  // uniform: what is no finite number must not meet the zero weights of what is not seen
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool bad = !(fabsf(x[e]) < INFINITY);
+            dirty |= bad;
+            x[e] = bad ? 0.f : x[e];
           }
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[g][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], p[i], acc[g][e], 0, 0, 0);
       }
-    };
-    if (drafted) sums.template operator()<true>();
-    else sums.template operator()<false>();
+    }
+    if (__builtin_amdgcn_ballot_w64(dirty) != 0) {  // uniform: and is added to the sums of the vectors that see its token
+#pragma unroll 1
+      for (int tok = 0; tok < nt; ++tok) {
+        const T* row = vp + __shfl(here, tok, 64);
+#pragma unroll
+        for (int g = 0; g < NGr; ++g)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int d = 64 * g + 16 * quarter + 4 * i + e;
+              const float x = d < D ? to_f32(row[d]) : 0.f;
+              if ((seen >> tok & 1) && !(fabsf(x) < INFINITY)) acc[g][e][i] += x;
+            }
+      }
+    }
   }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
 #pragma unroll
-  for (int i = 0; i < kPerWave; ++i) {
-    const int v = wave * kPerWave + i;
-    if (v >= nv) continue;
-    const int j = r.first + (v0 + v) / G, head = h * G + (v0 + v) % G;
-    const size_t id = (size_t)j * A.Hq + head;
-    const size_t at = id * A.splits + blockIdx.z;
-    const float inv = A.splits > 1 ? 1.f : l[i] != 0.f ? 1.f / l[i] : sees(A, r, j) ? NAN : 0.f;
+  for (int g = 0; g < NGr; ++g)
 #pragma unroll
-    for (int c = 0; c < DM / 64; ++c) {
-      if (lane + 64 * c >= D) continue;
-      if (A.splits > 1) A.part_o[at * D + lane + 64 * c] = acc[i][c];
-      else out[id * D + lane + 64 * c] = from_f32<T>(as_f32_value(l[i] != 0.f ? acc[i][c] * inv : inv));
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<f32x4*>(&sm_o[wave][col][64 * g + 16 * quarter + 4 * i]) =
+          f32x4{acc[g][0][i], acc[g][1][i], acc[g][2][i], acc[g][3][i]};
+  if (quarter == 0) {
+    sm_ml[wave][0][col] = m;
+    sm_ml[wave][1][col] = l;
+  }
+  __syncthreads();
+  // 16 threads per vector from here on.
+  const int v = t >> 4, part = t & 15;
+  if (v >= nv) return;
+  float M = -INFINITY, f[kGenWaves], den = 0.f;
+#pragma unroll
+  for (int w = 0; w < kGenWaves; ++w) M = fmaxf(M, sm_ml[w][0][v]);
+#pragma unroll
+  for (int w = 0; w < kGenWaves; ++w) {
+    f[w] = __builtin_amdgcn_exp2f(sm_ml[w][0][v] - (M == -INFINITY ? 0.f : M));
+    den = fmaf(sm_ml[w][1][v], f[w], den);
+  }
+  const int token = r.first + (v0 + v) / G;
+  const size_t id = (size_t)token * A.Hq + h * G + (v0 + v) % G;
+  const size_t place = id * A.splits + blockIdx.z;
+  const float inv = den != 0.f ? 1.f / den : 0.f, none = den != 0.f || !sees(A, r, token) ? 0.f : NAN;
+#pragma unroll
+  for (int g = 0; g < NGr; ++g) {
+    const int d = 64 * g + 4 * part;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kGenWaves; ++w)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(sm_o[w][v][d + e], f[w], o[e]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (d + e >= D) continue;
+      if (A.splits > 1) A.part_o[place * D + d + e] = o[e];
+      else out[id * D + d + e] = from_f32<T>(as_f32_value(den != 0.f ? o[e] * inv : none));
     }
-    if (A.splits > 1 && lane == 0) {
-      A.part_ml[2 * at] = m[i];
-      A.part_ml[2 * at + 1] = l[i];
-    }
+  }
+  if (A.splits > 1 && part == 0) {
+    A.part_ml[2 * place] = M;
+    A.part_ml[2 * place + 1] = den;
   }
 }
 
@@ -1073,8 +1122,9 @@ Layout layout(int tokens, int batch, int Hq, int Hkv) {
 bool fast_sizes(int tokens, int batch, int Hq, int Hkv, int head_dim, int P, int max_pages, int kv_dtype) {
   const long blocks = (long)max_pages * P / kBlock + 1 + kItemCost;
   const long tiles = (long)tokens * (Hq / Hkv) / kTileVec + batch;
-  return kv_dtype == CIR_F16 && head_dim == D && P % 16 == 0 && Hq / Hkv <= kMaxGroup && (long)max_pages * P / 16 * (P / 16) < (1L << 32) &&
-         batch <= kMaxRows && blocks * tiles < (1L << 31) - kWorkgroups;
+  return kv_dtype == CIR_F16 && head_dim == D && P % 16 == 0 && Hq / Hkv <= kMaxGroup && batch <= kMaxRows &&
+         (long)max_pages * P / 16 * (P / 16) < (1L << 32) && (long)max_pages * P < (1L << 31) - 4096 &&
+         blocks * tiles < (1L << 31) - kWorkgroups;
 }
 
 }  // namespace

@@ -432,8 +432,7 @@ struct Piece {
 struct Smem {
   float ml[kWaves][2][2 * kGroup];
   uint32_t mask[kTileVec][2 * kMaxDrafts / 64 + 1];
-  int place[kMaxRows + 1], len[kMaxRows], first[kMaxRows];
-  int16_t n[kMaxRows];
+  int4 row[kMaxRows + 1];  // first token, their number, length, place on the axis
   int scan[kWaves], find;
 };
 
@@ -486,7 +485,9 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
   constexpr int PW = 2 / CW;          // blocks of a stage that a wavefront takes
   static_assert(CW == 1 || CW == 2, "");
   const Args& A = F.a;
-  const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));  // (else what all variants form from it is formed, and kept, before the first piece: 500 lines)
+  const int wave = uni(t >> 6), lane = t & 63;
   const int l32 = lane & 31, h = lane >> 5;
   const int col = wave % VW, par = wave / VW;
   const float sc = fabsf(A.scale_log2);
@@ -527,7 +528,7 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
   fetch(0);
   issue(0);
 
-  // Q^T as the B operand: lane l32's vector of each group, dims 16 s + 8 h + e (zero past the last vector); a negative
+  // Q^T as the B operand: lane l32's vector of each group, dims 16 s + 8 h + e; a negative
   // scale goes into its sign, so that the maximum can be taken before scaling.
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   const uint32_t flip = A.scale_log2 < 0.f ? 0x80008000u : 0u;
@@ -535,27 +536,28 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
     const int v = (col * NG + g) * kGroup + l32;
-    const bool live = v < p.nv;
-    const int vv = p.v0 + (live ? v : 0), tok = token_of(F, G, vv);
+    const int vv = p.v0 + min(v, p.nv - 1), tok = token_of(F, G, vv);  // (vectors past the last: the last one again)
     const f16* row = p.q + ((size_t)(p.r.first + tok) * A.Hq + (size_t)p.h * G + (vv - tok * G)) * D + 8 * h;
 #pragma unroll
+    for (int s = 0; s < 8; ++s) qb[g][s] = *reinterpret_cast<const f16x8*>(row + 16 * s);
+  }
+#pragma unroll
+  for (int g = 0; g < NG; ++g)
+#pragma unroll
     for (int s = 0; s < 8; ++s) {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(row + 16 * s) ^ flip;
-      qb[g][s] = live ? __builtin_bit_cast(f16x8, x) : f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      qb[g][s] = __builtin_bit_cast(f16x8, __builtin_bit_cast(u32x4, qb[g][s]) ^ flip);
       // (Here, before the next stages are on their way: its wait would be for them too.  In accumulator registers, which an
       // MFMA reads as well as the others.)
       asm volatile("" : "+a"(qb[g][s]));
     }
-  }
   // The masks of the tile's vectors, where a block of the piece holds drafted tokens.
   const int drafts = min(p.r.n, p.r.limit - p.r.context);  // of the row, as far as the table holds them
   if (p.blk1 * kBlock > p.r.context) {                     // uniform
-    const int v = threadIdx.x;
     static_assert(kTileVec <= kThreads, "");
-    if (v < p.nv) {
-      const int j = p.r.first + token_of(F, G, p.v0 + v);
+    if (t < p.nv) {
+      const int j = p.r.first + token_of(F, G, p.v0 + t);
 #pragma unroll 1
-      for (int w = 0; w < 2 * A.words; ++w) sm.mask[v][w] = mask_word(A, j, w, drafts);
+      for (int w = 0; w < 2 * A.words; ++w) sm.mask[t][w] = mask_word(A, j, w, drafts);
     }
   }
 
@@ -583,7 +585,7 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
   // Tokens of a block that the lane's vector of group g sees; score r is that of token bit_of(r).
   const auto seen_of = [&](int g, int blk) __attribute__((always_inline)) {
     const int k = blk * kBlock - p.r.context, rest = limit - blk * kBlock;  // drafted token of the block's first
-    const uint32_t* m = sm.mask[(col * NG + g) * kGroup + l32];
+    const uint32_t* m = sm.mask[min((col * NG + g) * kGroup + l32, p.nv - 1)];
     const int w = k >> 5, s = k & 31;
     const uint32_t lo = k < 0 ? 0xffffffffu : w < 2 * A.words ? m[w] : 0;
     const uint32_t hi = w + 1 >= 0 && w + 1 < 2 * A.words ? m[w + 1] : 0;
@@ -854,70 +856,58 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
     }
   }
 
-  // Wavefronts that took turns at the blocks are joined through LDS: the second leaves its (m, l, O) there, the first adds
-  // its own and writes.  16-byte chunk c of vector v in slot c ^ (v % 32) of its 512 bytes.
+  // The wavefronts' (m, l, O) go to LDS, 16-byte chunk c of vector v in slot c ^ (v % 32) of its 512 bytes; all threads join
+  // those of wavefronts that took turns at the blocks, and write rows.
+  static_assert(kWaves * 2 * kGroup * D * sizeof(float) <= 4 * kStage, "");
+  dma_wait_barrier();  // (every wavefront is done with its blocks, and no DMA is on its way into them)
 #pragma unroll
-  for (int g = 0; g < NG; ++g) a[g].l += __shfl_xor(a[g].l, 32, 64);
-  float part[NG][2];  // the factors of the two parts' O, and (m, l) of both
+  for (int g = 0; g < NG; ++g) {
+    uint8_t* to = ring + (wave * NG + g) * kGroup * 512 + l32 * 512;
 #pragma unroll
-  for (int g = 0; g < NG; ++g) part[g][0] = 1.f, part[g][1] = 0.f;
-  if constexpr (CW == 2) {
-    dma_wait_barrier();  // (every wavefront is done with its blocks, and no DMA is on its way into them)
-    if (par == 1) {
+    for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        uint8_t* to = ring + col * kStage + (g * kGroup + l32) * 512;
-#pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<f32x4*>(to + 16 * ((8 * dt + 2 * j + h) ^ l32)) =
-                f32x4{a[g].acc[dt][4 * j], a[g].acc[dt][4 * j + 1], a[g].acc[dt][4 * j + 2], a[g].acc[dt][4 * j + 3]};
-        if (h == 0) {
-          sm.ml[wave][0][g * kGroup + l32] = a[g].m;
-          sm.ml[wave][1][g * kGroup + l32] = a[g].l;
-        }
-      }
-    }
-    __syncthreads();
-    if (par == 0) {
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const float m1 = sm.ml[wave + VW][0][g * kGroup + l32], l1 = sm.ml[wave + VW][1][g * kGroup + l32];
-        const float M = fmaxf(a[g].m, m1), ms = M == -INFINITY ? 0.f : M;
-        part[g][0] = __builtin_amdgcn_exp2f(a[g].m - ms);
-        part[g][1] = __builtin_amdgcn_exp2f(m1 - ms);
-        a[g].l = fmaf(l1, part[g][1], a[g].l * part[g][0]);
-        a[g].m = M;
-      }
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<f32x4*>(to + 16 * ((8 * dt + 2 * j + h) ^ l32)) =
+            f32x4{a[g].acc[dt][4 * j], a[g].acc[dt][4 * j + 1], a[g].acc[dt][4 * j + 2], a[g].acc[dt][4 * j + 3]};
+    a[g].l += __shfl_xor(a[g].l, 32, 64);
+    if (h == 0) {
+      sm.ml[wave][0][g * kGroup + l32] = a[g].m;
+      sm.ml[wave][1][g * kGroup + l32] = a[g].l;
     }
   }
-  if (CW == 1 || par == 0) {
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const int v = (col * NG + g) * kGroup + l32;
-      if (v >= p.nv) continue;
-      const size_t at = (p.at + v) * A.Hkv + p.h;
-      const uint8_t* other = ring + col * kStage + (g * kGroup + l32) * 512;
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          f32x4 o = {a[g].acc[dt][4 * j], a[g].acc[dt][4 * j + 1], a[g].acc[dt][4 * j + 2], a[g].acc[dt][4 * j + 3]};
-          if constexpr (CW == 2) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(other + 16 * ((8 * dt + 2 * j + h) ^ l32));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], part[g][1], o[e] * part[g][0]);
-          }
-          *reinterpret_cast<f32x4*>(F.o + at * D + 32 * dt + 8 * j + 4 * h) = o;
-        }
-      if (h == 0) {
-        F.ml[2 * at] = a[g].m;
-        F.ml[2 * at + 1] = a[g].l;
-      }
+  __syncthreads();
+  if (t < p.nv) {  // (max, sum) of vector t, and the factors of its parts' O
+    constexpr int V = NG * kGroup;  // vectors of a wavefront
+    float* m0 = &sm.ml[t / V][0][t % V];
+    const size_t at = (p.at + t) * A.Hkv + p.h;
+    float m = m0[0], l = m0[2 * kGroup];
+    if constexpr (CW == 2) {
+      float* m1 = &sm.ml[t / V + VW][0][t % V];
+      const float M = fmaxf(m, m1[0]), ms = M == -INFINITY ? 0.f : M;
+      const float f0 = __builtin_amdgcn_exp2f(m - ms), f1 = __builtin_amdgcn_exp2f(m1[0] - ms);
+      l = fmaf(m1[2 * kGroup], f1, l * f0);
+      m = M;
+      m0[0] = f0;
+      m1[0] = f1;
     }
+    F.ml[2 * at] = m;
+    F.ml[2 * at + 1] = l;
   }
-  dma_wait_barrier();  // the next piece writes the same LDS
+  if constexpr (CW == 2) __syncthreads();
+#pragma unroll 4
+  for (int id = t; id < p.nv * (D / 4); id += kThreads) {
+    const int v = id / (D / 4), c = id % (D / 4), slot = v * 512 + 16 * (c ^ (v & 31));
+    f32x4 o = *reinterpret_cast<const f32x4*>(ring + slot);
+    if constexpr (CW == 2) {
+      constexpr int V = NG * kGroup;
+      const float f0 = sm.ml[v / V][0][v % V], f1 = sm.ml[v / V + VW][0][v % V];
+      const f32x4 x = *reinterpret_cast<const f32x4*>(ring + VW * V * 512 + slot);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f1, o[e] * f0);
+    }
+    *reinterpret_cast<f32x4*>(F.o + ((p.at + v) * A.Hkv + p.h) * D + 4 * c) = o;
+  }
+  __syncthreads();  // the next piece writes the same LDS
 }
 
 __global__ __launch_bounds__(kThreads, 1) void tree_f16_d128(const f16* __restrict__ q, const f16* __restrict__ kp,
@@ -934,13 +924,12 @@ __global__ __launch_bounds__(kThreads, 1) void tree_f16_d128(const f16* __restri
   for (int b0 = 0; b0 < B; b0 += kThreads) {  // uniform
     const int b = b0 + t;
     int cost = 0;
+    int4 row = make_int4(0, 0, 0, 0);
     if (b < B) {
       const Row r = row_of(A, b);
       const int blocks = (r.limit + kBlock - 1) / kBlock, tiles = (r.n * G + kTileVec - 1) / kTileVec;
       cost = blocks > 0 ? tiles * (blocks + kItemCost) : 0;
-      sm.first[b] = r.first;
-      sm.n[b] = (int16_t)r.n;
-      sm.len[b] = A.lens[b];
+      row = make_int4(r.first, r.n, max(0, A.lens[b]), 0);
     }
     int upto = cost;
 #pragma unroll
@@ -956,54 +945,50 @@ __global__ __launch_bounds__(kThreads, 1) void tree_f16_d128(const f16* __restri
       upto += i < wave ? sm.scan[i] : 0;
       total += sm.scan[i];
     }
-    if (b < B) sm.place[b] = all + upto - cost;
+    row.w = all + upto - cost;
+    if (b < B) sm.row[b] = row;
     all += total;
     __syncthreads();
   }
-  if (t == 0) sm.place[B] = all;
+  if (t == 0) sm.row[B].w = all;
   const int teams = gridDim.x / Hkv;
   const int stretch = max((all + teams - 1) / teams, kMinStretch);
   const int lo = w * stretch, hi = min(all, lo + stretch);
   __syncthreads();
-  const auto row_at = [&](int b) __attribute__((always_inline)) {
-    Row r;
-    r.first = uni(sm.first[b]);
-    r.n = uni(sm.n[b]);
-    const int len = uni(sm.len[b]);
-    r.context = max(0, len - r.n);
-    r.limit = max(0, min(len, A.max_pages * A.P));
-    return r;
-  };
-
   // What the join needs, shared out over the workgroups from the last one on (the ones without work of their own).
   const int id = (int)(gridDim.x - 1 - blockIdx.x) + t * (int)gridDim.x, step = kThreads * (int)gridDim.x;
   if (id == 0) F.stretch[0] = stretch;
-  for (int b = id; b < B; b += step)
-    F.rows[b] = RowRec{sm.first[b], sm.n[b], sm.place[b] + kItemCost,
-                       (max(0, min(sm.len[b], A.max_pages * A.P)) + kBlock - 1) / kBlock};
+  for (int b = id; b < B; b += step) {
+    const int4 r = sm.row[b];
+    F.rows[b] = RowRec{r.x, r.y, r.w + kItemCost, (max(0, min(r.z, A.max_pages * A.P)) + kBlock - 1) / kBlock};
+  }
   for (int j = id; j < A.tokens; j += step) {
     int a = 0, z = B - 1;  // the last row that begins at or before j (rows without tokens begin where the next does)
     while (a < z) {
       const int m = (a + z + 1) >> 1;
-      if (sm.first[m] <= j) a = m;
+      if (sm.row[m].x <= j) a = m;
       else z = m - 1;
     }
-    F.row_of[j] = j >= sm.first[a] && j < sm.first[a] + sm.n[a] ? a : -1;
+    F.row_of[j] = j >= sm.row[a].x && j < sm.row[a].x + sm.row[a].y ? a : -1;
   }
   if (lo >= hi) return;  // uniform
   for (int b = t; b < B; b += kThreads)
-    if (sm.place[b] <= lo && lo < sm.place[b + 1]) sm.find = b;
+    if (sm.row[b].w <= lo && lo < sm.row[b + 1].w) sm.find = b;
   __syncthreads();
 
   for (int b = uni(sm.find); b < B; ++b) {  // uniform
-    const int start = uni(sm.place[b]);
+    const int4 row = sm.row[b];
+    const int start = uni(row.w);
     if (start >= hi) break;
-    if (uni(sm.place[b + 1]) == start) continue;
+    if (uni(sm.row[b + 1].w) == start) continue;
     Piece p;
-    p.r = row_at(b);
+    p.r.first = uni(row.x);
+    p.r.n = uni(row.y);
+    p.r.context = max(0, uni(row.z) - p.r.n);
+    p.r.limit = min(uni(row.z), A.max_pages * A.P);
     const int blocks = (p.r.limit + kBlock - 1) / kBlock, cost = blocks + kItemCost;
     const int tiles = (p.r.n * G + kTileVec - 1) / kTileVec;
-    for (int i = max(0, (lo - start) / cost); i < tiles && start + i * cost < hi; ++i) {
+    for (int i = start >= lo || tiles == 1 ? 0 : (lo - start) / cost; i < tiles && start + i * cost < hi; ++i) {
       const int at = start + i * cost + kItemCost;
       const int k0 = max(0, min(lo - at, blocks)), k1 = max(0, min(hi - at, blocks));
       if (k0 >= k1) continue;

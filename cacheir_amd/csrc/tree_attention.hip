@@ -388,7 +388,7 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kTileVec = 256;    // query vectors of a tile
 constexpr int kWorkgroups = 256;
-constexpr int kItemCost = 6;     // a piece's start and join, in blocks
+constexpr int kItemCost = 10;    // a piece's start and join, in blocks
 constexpr int kMinStretch = 4;
 constexpr int kMaxRows = 1024;
 constexpr int kMaxGroup = 2048;   // query heads per KV head (256 G G < 2^32: token_of is exact)
@@ -526,7 +526,6 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
     for_each4([&]<int U>() __attribute__((always_inline)) { dma16<U>(r.v, r.to + kStage / 2, at_v ^ (16 * U)); });
   };
   fetch(0);
-  issue(0);
 
   // Q^T as the B operand: lane l32's vector of each group, dims 16 s + 8 h + e; a negative
   // scale goes into its sign, so that the maximum can be taken before scaling.
@@ -541,15 +540,7 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
 #pragma unroll
     for (int s = 0; s < 8; ++s) qb[g][s] = *reinterpret_cast<const f16x8*>(row + 16 * s);
   }
-#pragma unroll
-  for (int g = 0; g < NG; ++g)
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      qb[g][s] = __builtin_bit_cast(f16x8, __builtin_bit_cast(u32x4, qb[g][s]) ^ flip);
-      // (Here, before the next stages are on their way: its wait would be for them too.  In accumulator registers, which an
-      // MFMA reads as well as the others.)
-      asm volatile("" : "+a"(qb[g][s]));
-    }
+  issue(0);
   // The masks of the tile's vectors, where a block of the piece holds drafted tokens.
   const int drafts = min(p.r.n, p.r.limit - p.r.context);  // of the row, as far as the table holds them
   if (p.blk1 * kBlock > p.r.context) {                     // uniform
@@ -765,6 +756,15 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
     dma16<0>(rows.v, rows.to + kStage / 2, at_v);
     dma16<1>(rows.v, rows.to + kStage / 2, at_v ^ 16);
   }
+#pragma unroll
+  for (int g = 0; g < NG; ++g)
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      qb[g][s] = __builtin_bit_cast(f16x8, __builtin_bit_cast(u32x4, qb[g][s]) ^ flip);
+      // (Here, before the next stages are on their way: its wait would be for them too.  In accumulator registers, which an
+      // MFMA reads as well as the others.)
+      asm volatile("" : "+a"(qb[g][s]));
+    }
   asm volatile("" ::: "memory");
   // Block 0 and K of block 1 have landed, the masks are written: lgkmcnt(0), vmcnt(12) (a stage and K of one) or 14.
   __builtin_amdgcn_s_waitcnt(PW == 1 ? 0x007C : 0x007E);
@@ -932,12 +932,11 @@ __global__ __launch_bounds__(kThreads, 1) void tree_f16_d128(const f16* __restri
       row = make_int4(r.first, r.n, max(0, A.lens[b]), 0);
     }
     int upto = cost;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
+    for (int off = 1; off < min(B, 64); off <<= 1) {  // uniform
       const int o = __shfl_up(upto, off, 64);
       upto += lane >= off ? o : 0;
     }
-    if (lane == 63) sm.scan[wave] = upto;
+    if (lane == min(B, 64) - 1) sm.scan[wave] = upto;
     __syncthreads();
     int total = 0;
 #pragma unroll

@@ -396,14 +396,14 @@ constexpr int kRowB = 2 * D;     // bytes of a K or V row
 constexpr int kStageTok = 64;    // tokens of a stage
 constexpr int kStage = 2 * kStageTok * kRowB;  // bytes: K, then V
 
-struct RowRec {
-  int first, n, start, blocks;  // first token, their number, place of the first tile's blocks, blocks
+// What the join wants to know of a token's row: place of the first tile's blocks on the axis, their number (-1: no row counts
+// the token), the stretch, and 256 row + the token's number in it.
+struct TokRec {
+  int start, blocks, stretch, row;
 };
 struct Fast {
   Args a;
-  RowRec* rows;
-  int* row_of;      // [tokens]: the row that counts a token, or -1
-  int* stretch;
+  TokRec* rec;      // [tokens]
   float *o, *ml;    // [vector of the workspace][KV head][D] and [2]
   int P16;          // page size / 16
   uint32_t page_magic;  // ceil(2^32 / P16): n / P16 = n * page_magic >> 32 (P16 > 1)
@@ -956,11 +956,6 @@ __global__ __launch_bounds__(kThreads, 1) void tree_f16_d128(const f16* __restri
   __syncthreads();
   // What the join needs, shared out over the workgroups from the last one on (the ones without work of their own).
   const int id = (int)(gridDim.x - 1 - blockIdx.x) + t * (int)gridDim.x, step = kThreads * (int)gridDim.x;
-  if (id == 0) F.stretch[0] = stretch;
-  for (int b = id; b < B; b += step) {
-    const int4 r = sm.row[b];
-    F.rows[b] = RowRec{r.x, r.y, r.w + kItemCost, (max(0, min(r.z, A.max_pages * A.P)) + kBlock - 1) / kBlock};
-  }
   for (int j = id; j < A.tokens; j += step) {
     int a = 0, z = B - 1;  // the last row that begins at or before j (rows without tokens begin where the next does)
     while (a < z) {
@@ -968,7 +963,10 @@ __global__ __launch_bounds__(kThreads, 1) void tree_f16_d128(const f16* __restri
       if (sm.row[m].x <= j) a = m;
       else z = m - 1;
     }
-    F.row_of[j] = j >= sm.row[a].x && j < sm.row[a].x + sm.row[a].y ? a : -1;
+    const int4 r = sm.row[a];
+    const bool counted = j >= r.x && j < r.x + r.y;
+    F.rec[j] = TokRec{r.w + kItemCost, counted ? (min(r.z, A.max_pages * A.P) + kBlock - 1) / kBlock : -1, stretch,
+                      kMaxDrafts * a + (j - r.x)};
   }
   if (lo >= hi) return;  // uniform
   for (int b = t; b < B; b += kThreads)
@@ -1018,15 +1016,14 @@ __global__ __launch_bounds__(256) void tree_join(Fast F, f16* __restrict__ out) 
   const int part = threadIdx.x >> 5, lane = threadIdx.x & 31, s = part % W, vec = part / W;
   const int id = blockIdx.x * kVecs + vec, G = A.Hq / A.Hkv;
   const int j = id / A.Hq, head = id - j * A.Hq, h = head / G;
-  const int b = id < A.tokens * A.Hq ? F.row_of[j] : -1;
-  const bool live = b >= 0;
-  const RowRec rec = F.rows[live ? b : 0];
-  const int stretch = F.stretch[0];
-  const int v = (j - rec.first) * G + (head - h * G), tile = v / kTileVec;
-  const int start = rec.start + tile * (rec.blocks + kItemCost), w0 = start / stretch;
-  const int n = live && rec.blocks > 0 ? (start + rec.blocks - 1) / stretch - w0 + 1 : 0;
+  TokRec rec = F.rec[min(j, A.tokens - 1)];
+  if (j >= A.tokens) rec.blocks = -1;
+  const bool live = rec.blocks >= 0;
+  const int v = rec.row % kMaxDrafts * G + (head - h * G), tile = v / kTileVec;
+  const int start = rec.start + tile * (rec.blocks + kItemCost), w0 = start / rec.stretch;
+  const int n = live && rec.blocks > 0 ? (start + rec.blocks - 1) / rec.stretch - w0 + 1 : 0;
   const auto at = [&](int k) {
-    return ((size_t)(w0 + k) * kTileVec + (size_t)rec.first * G + v) * A.Hkv + h;
+    return ((size_t)(w0 + k) * kTileVec + (size_t)j * G + (head - h * G)) * A.Hkv + h;
   };
   const auto ml_of = [&](int k) { return *reinterpret_cast<const float2*>(F.ml + 2 * at(k)); };
   const auto o_of = [&](int k) { return *reinterpret_cast<const f32x4*>(F.o + D * at(k) + 4 * lane); };
@@ -1070,7 +1067,7 @@ __global__ __launch_bounds__(256) void tree_join(Fast F, f16* __restrict__ out) 
   if (s > 0 || !live) return;
   o += sm_o[vec][lane];
   float inv = 1.f / den;
-  if (den == 0.f) inv = n > 0 && sees(A, row_of(A, b), j) ? NAN : 0.f;
+  if (den == 0.f) inv = n > 0 && sees(A, row_of(A, rec.row / kMaxDrafts), j) ? NAN : 0.f;
   f16x4 y;
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] = static_cast<f16>(as_f32_value(o[e] * inv));
@@ -1082,9 +1079,9 @@ int teams_of(int Hkv) { return max(1, kWorkgroups / Hkv); }
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
 struct Layout {
-  size_t rows, row_of, stretch, o, ml, total;  // bytes
+  size_t rec, o, ml, total;  // bytes
 };
-Layout layout(int tokens, int batch, int Hq, int Hkv) {
+Layout layout(int tokens, int Hq, int Hkv) {
   Layout l{};
   size_t at = 0;
   const auto take = [&](size_t bytes) {
@@ -1093,9 +1090,7 @@ Layout layout(int tokens, int batch, int Hq, int Hkv) {
     return p;
   };
   const size_t vectors = ((size_t)teams_of(Hkv) * kTileVec + (size_t)tokens * (Hq / Hkv)) * Hkv;
-  l.rows = take(sizeof(RowRec) * batch);
-  l.row_of = take(sizeof(int) * tokens);
-  l.stretch = take(sizeof(int));
+  l.rec = take(sizeof(TokRec) * tokens);
   l.o = take(vectors * D * sizeof(float));
   l.ml = take(vectors * 2 * sizeof(float));
   l.total = at;
@@ -1126,7 +1121,7 @@ extern "C" size_t cir_tree_attention_workspace_bytes(int tokens, int batch, int 
   const GenericPlan g = generic_plan(tokens, batch, num_heads, num_kv_heads, page_size, max_pages);
   const size_t plain = generic_floats(g, tokens, num_heads, head_dim) * sizeof(float);
   if (!fast_sizes(tokens, batch, num_heads, num_kv_heads, head_dim, page_size, max_pages, kv_dtype)) return plain;
-  return std::max(plain, layout(tokens, batch, num_heads, num_kv_heads).total);
+  return std::max(plain, layout(tokens, num_heads, num_kv_heads).total);
 }
 
 extern "C" int cir_paged_tree_attention(const void* q, const void* k_pool, const void* v_pool,
@@ -1157,13 +1152,12 @@ extern "C" int cir_paged_tree_attention(const void* q, const void* k_pool, const
   // DMA takes 16-byte groups of the pools; q is read by 16 bytes, out written by 8.
   if (fast_sizes(tokens, batch, num_heads, num_kv_heads, head_dim, page_size, max_pages, kv_dtype) &&
       ((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool) % 16 == 0 && (uintptr_t)out % 8 == 0) {
-    const Layout l = layout(tokens, batch, num_heads, num_kv_heads);
+    const Layout l = layout(tokens, num_heads, num_kv_heads);
     CIR_CHECK_ARG(workspace && workspace_bytes >= l.total && (uintptr_t)workspace % 16 == 0,
                   "tree_attention: workspace too small or not on 16 bytes (%zu < %zu)", workspace_bytes, l.total);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     const uint32_t P16 = page_size / 16, G = num_heads / num_kv_heads;
-    const Fast F{A, reinterpret_cast<RowRec*>(ws + l.rows), reinterpret_cast<int*>(ws + l.row_of),
-                 reinterpret_cast<int*>(ws + l.stretch), reinterpret_cast<float*>(ws + l.o),
+    const Fast F{A, reinterpret_cast<TokRec*>(ws + l.rec), reinterpret_cast<float*>(ws + l.o),
                  reinterpret_cast<float*>(ws + l.ml), (int)P16, (uint32_t)(((1ull << 32) + P16 - 1) / P16),
                  (uint32_t)(((1ull << 32) + G - 1) / G)};
     tree_f16_d128<<<teams_of(num_kv_heads) * num_kv_heads, kThreads, 0, s>>>(

@@ -351,6 +351,86 @@ def test_tree_attention_many_rows(device, rows, nodes, hq, hkv):
         check_tree(one, got[lo:hi])
 
 
+def tree_heads64(c, scale):
+    """attention64 for as many query as KV heads and one row, head by head in float64 on the tensors' device: (out,
+    tolerance)."""
+    q, length, n = c["q"].double(), int(c["seq_lens"][0]), c["q"].shape[0]
+    t = torch.arange(length, device=q.device)
+    pages, psize = c["page_table"][0].long()[t // c["k_pool"].shape[2]], c["k_pool"].shape[2]
+    seen = torch.ones((n, length), dtype=torch.bool)
+    seen[:, length - n:] = bits_of(c["masks"].cpu(), n)
+    seen = seen.to(q.device)
+    out, tol = torch.empty_like(q), torch.empty_like(q)
+    for h in range(q.shape[1]):
+        k, v = c["k_pool"][pages, h, t % psize].double(), c["v_pool"][pages, h, t % psize].double()
+        s = (q[:, h] @ k.T * scale).masked_fill(~seen, -math.inf)
+        e = torch.exp(s - s.max(dim=1, keepdim=True).values)
+        l = e.sum(dim=1, keepdim=True)
+        out[:, h] = e @ v / l
+        off = 260 * U32 * abs(scale) * (q[:, h].abs() @ k.abs().T).max(dim=1, keepdim=True).values
+        tol[:, h] = (e @ v.abs() / l) * (2 * U16 + 2 * off) + v.abs().sum(dim=0) * 2.0 ** -25 / l + U16 * out[:, h].abs()
+    return out, tol
+
+
+@pytest.mark.parametrize("heads,n,context", [
+    (256, 2, 4500), (256, 100, 4600), (256, 200, 4433),  # one workgroup a head: 70 stages, pages of 64 of them at a time
+    (1, 3, 9000), (1, 150, 17000),                       # 256 workgroups: a tile's pieces are more than 32
+])
+def test_tree_attention_long(device, heads, n, context):
+    g = torch.Generator(device).manual_seed(n)
+    pages = -(-(context + n) // 16)
+    pool = lambda: torch.randn((pages + 3, heads, 16, 128), generator=g, dtype=torch.float16, device=device)
+    c = dict(q=torch.randn((n, heads, 128), generator=g, dtype=torch.float16, device=device), k_pool=pool(), v_pool=pool(),
+             page_table=torch.randperm(pages + 3, generator=g, device=device)[None, :pages].int(),
+             seq_lens=i32([context + n]).to(device), offsets=i32([0, n]).to(device), counts=i32([n]).to(device),
+             masks=mask_words(seen_sets(tree(n, 5, "any")), 4).to(device))
+    ref, tol = tree_heads64(c, 128 ** -0.5)
+    got = run_tree(c, device)
+    assert bool(((got.double() - ref).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype", KINDS)
+@pytest.mark.parametrize("nodes", [[3], [40], [64, 7]])
+def test_tree_attention_of_huge_scores(device, hq, hkv, d, dtype, nodes):
+    """Scores of up to 10^8 that are exact, 2^20 apart or equal: a token's answer is the mean of V over those of the greatest,
+    off by the rounding of the weights (equal: they are 1, or 2^x with one x for all), of the sums and of the answer."""
+    c = tree_case(21, nodes, [70] * len(nodes), hq, hkv, d=d, dtype=dtype)
+    g = torch.Generator().manual_seed(2)
+    steps = torch.randint(-90, 91, c["k_pool"].shape[:3], generator=g)
+    c["k_pool"].zero_()
+    c["k_pool"][..., 0] = steps.to(dtype)
+    c["q"].zero_()
+    c["q"][..., 0] = torch.tensor([1.0, -1.0])[torch.randint(0, 2, c["q"].shape[:2], generator=g)].to(dtype)
+    got = run_tree(c, device, scale=2.0 ** 20).cpu().double()
+    for b, n in enumerate(nodes):
+        first, t = int(c["offsets"][b]), torch.arange(70 + n)
+        pages = c["page_table"][b].long()[t // 16]
+        for i in range(n):
+            seen = torch.cat([torch.ones(70, dtype=torch.bool), bits_of(c["masks"][first + i: first + i + 1], n)[0]])
+            for h in range(hq):
+                s = steps[pages, h // (hq // hkv), t % 16] * float(c["q"][first + i, h, 0])
+                best = (s == s[seen].max()) & seen
+                v = c["v_pool"][pages[best], h // (hq // hkv), t[best] % 16].double()
+                tol = (2 * U16 if dtype == torch.float16 else 100 * U32) * v.abs().mean(dim=0) + 2.0 ** -25
+                assert bool(((got[first + i, h] - v.mean(dim=0)).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("d,dtype", [(128, torch.float16), (64, torch.float32)])
+def test_tree_attention_far_in_the_pools(device, d, dtype):
+    """Pages whose elements have numbers past 2^31: the same bits as from the start of small pools."""
+    c = tree_case(13, [20, 3], [100, 40], 8, 2, d=d, dtype=dtype)
+    want = run_tree(c, device)
+    small = c["k_pool"].shape[0]
+    slots = 2 ** 31 // (2 * 16 * d) + small
+    pools = {}
+    for name in ("k_pool", "v_pool"):
+        pools[name] = torch.empty((slots, 2, 16, d), dtype=dtype, device=device)
+        pools[name][-small:] = c[name].to(device)
+    far = {**{k: v.to(device) for k, v in c.items()}, **pools}
+    far["page_table"] = far["page_table"] + (slots - small)
+    assert torch.equal(run_tree(far, device), want)
+
+
 def test_tree_attention_chain_is_causal_prefill(device):
     from cacheir_amd import kernels
 
@@ -519,6 +599,23 @@ def test_norm_rope_append(device, tokens, hq, hkv, d, rot, layout, dt, kvdt, wdt
         kernels.norm_rope_append(gq, gk, gv, on(qw), on(kw), eps, on(pos), on(slots), on(freq), kp, vp, layout=layout,
                                  factor=factor, out=gq)
         assert torch.equal(gq.cpu()[~dead], got.cpu()[~dead]) and torch.equal(gq.cpu()[dead], q[dead])
+
+
+def test_norm_rope_append_far_in_the_pools(device):
+    """Slots whose elements have numbers past 2^31: the bits of a small pool."""
+    from cacheir_amd import kernels
+
+    g = torch.Generator(device).manual_seed(6)
+    q, k, v = (torch.randn((9, h, 128), generator=g, dtype=torch.float16, device=device) for h in (4, 2, 2))
+    w = torch.ones(128, device=device)
+    pos, freq = torch.arange(9, device=device, dtype=torch.int32), kernels.rope_frequencies(128, 10000.0, device=device)
+    slots = torch.arange(9, device=device) * 5
+    pages = 2 ** 31 // (2 * 16 * 128)
+    small, far = ([torch.zeros((n, 2, 16, 128), dtype=torch.float16, device=device) for _ in range(2)] for n in (3, pages + 3))
+    go = lambda pools, at: kernels.norm_rope_append(q, k, v, w, w, 1e-6, pos, at, freq, *pools)
+    assert torch.equal(go(small, slots), go(far, slots + 16 * pages))
+    for a, b in zip(small, far):
+        assert torch.equal(a, b[pages:]) and not b[:pages].any()
 
 
 def test_norm_rope_append_of_extreme_heads(device):
@@ -752,6 +849,41 @@ def test_adjust_logits_in_graphs(device):
         assert torch.equal(go(), replayed)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_adjust_logits_at_any_address(device, dtype):
+    """Rows that begin one element behind a 16-byte boundary, of odd strides, and their out alike."""
+    from cacheir_amd import kernels
+
+    c = logits_case(41, [9, 2], 8201, 300, dtype, pad=4)
+    ref, tol = reference_logits(c)
+    wide = torch.full((11, 8201 + 4), 3.5, dtype=dtype, device=device)
+    wide[:, 1: 8202] = c["logits"].to(device)
+    d = {**{k: v.to(device) for k, v in c.items()}, "logits": wide[:, 1: 8202]}
+    into = torch.full((11, 8201 + 6), 3.5, dtype=dtype, device=device)
+    near_logits(kernels.adjust_logits(**d, out=into[:, 3: 8204]), ref, tol)
+    assert (into[:, :3] == 3.5).all() and (into[:, 8204:] == 3.5).all()
+    near_logits(kernels.adjust_logits(**d, out=d["logits"]), ref, tol)
+    assert (wide[:, :1] == 3.5).all() and (wide[:, 8202:] == 3.5).all()
+
+
+def test_adjust_logits_of_many_rows(device):
+    """Logits of more than 2^31 elements, in place: the last rows as in a small call."""
+    from cacheir_amd import kernels
+
+    vocab, rows = 152064, 2 ** 31 // 152064 + 5
+    x = torch.zeros((rows, vocab), dtype=torch.float16, device=device)
+    g = torch.Generator(device).manual_seed(4)
+    x[-4:] = torch.randn((4, vocab), generator=g, dtype=torch.float16, device=device)
+    hist = torch.randint(0, vocab, (4, 50), generator=g, device=device)
+    kw = dict(repetition=torch.full((4,), 1.5, device=device), frequency=torch.full((4,), 0.25, device=device))
+    want = kernels.adjust_logits(x[-4:], history=hist, history_lens=i32([50] * 4).to(device), **kw)
+    offsets = torch.tensor([0] + [rows - 4 + i for i in range(5)], device=device, dtype=torch.int32)  # (rows 0 .. : row 0's)
+    full = lambda t: torch.cat([torch.ones((1, *t.shape[1:]), dtype=t.dtype, device=device), t])
+    kernels.adjust_logits(x, offsets, history=full(hist), history_lens=i32([0] + [50] * 4).to(device),
+                          **{k: full(v) for k, v in kw.items()}, out=x)
+    assert torch.equal(x[-4:], want) and not x[:-4].any()
+
+
 def test_adjust_logits_refusals(device):
     from cacheir_amd import kernels
 
@@ -839,6 +971,24 @@ def test_accept_drafts(device, nodes, contexts, layers, hkv, d, psize, dtype, mo
     assert got.tokens.tolist() == tokens and got.seq_lens.tolist() == ends
     assert torch.equal(s["k_pools"].cpu(), kp) and torch.equal(s["v_pools"].cpu(), vp)
     assert torch.equal(s["seq_lens"].cpu(), c["seq_lens"])
+
+
+def test_accept_drafts_far_in_the_pools(device):
+    """Layers of more than 2^32 bytes: what moves is where it belongs, and nothing else is written."""
+    from cacheir_amd import kernels
+
+    c = accept_case(51, [40, 9], [30, 3], 2, 2, 64, 16, torch.float32, ids=2, shape="chain")
+    _, _, _, _, kp, vp = accept_ref(c, 256)
+    small = c["k_pools"].shape[1]
+    slots = 2 ** 30 // (2 * 16 * 64) + small
+    s = {k: v.to(device) for k, v in c.items()}
+    s["page_table"] = s["page_table"] + (slots - small)
+    for name in ("k_pools", "v_pools"):
+        s[name] = torch.zeros((2, slots, 2, 16, 64), device=device)
+        s[name][:, -small:] = c[name].to(device)
+    kernels.accept_drafts(**s, most=256)
+    for name, want in (("k_pools", kp), ("v_pools", vp)):
+        assert torch.equal(s[name][:, -small:].cpu(), want) and not s[name][:, :-small].any()
 
 
 def test_accept_drafts_gives_pages_back(device):

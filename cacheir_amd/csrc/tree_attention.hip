@@ -79,7 +79,7 @@ constexpr int kMaxD = 256;
 
 __device__ __forceinline__ int tiles_of(const Args& A, int n) { return (n * (A.Hq / A.Hkv) + kVec - 1) / kVec; }
 
-template <typename T, int DM>  // DM: head_dim at most
+template <typename T, int DM, bool QUADS>  // DM: head_dim at most; QUADS: it is a multiple of 4
 __global__ __launch_bounds__(kGenThreads) void tree_generic(const T* __restrict__ q, const T* __restrict__ kp,
                                                             const T* __restrict__ vp, T* __restrict__ out, Args A) {
   constexpr int C = DM / 16, NGr = DM / 64;
@@ -131,31 +131,37 @@ __global__ __launch_bounds__(kGenThreads) void tree_generic(const T* __restrict_
   const int stretch = ((r.limit + A.splits - 1) / A.splits + kTurn - 1) / kTurn * kTurn;
   const int k0 = min((int64_t)r.limit, (int64_t)blockIdx.z * stretch), k1 = min(r.limit, k0 + stretch);
 
-  const auto part_of = [&](const T* row, int d) __attribute__((always_inline)) {  // dims d .. d + 3 of a row, zeros past the last
-    if (d + 4 <= D) return static_cast<vt>(*reinterpret_cast<const mt*>(row + d));
-    vt x = {};
+  // Dims d .. d + 3 of a row; what stands for those past the last is some other dim's.  Without a branch, and so is what
+  // follows: where lanes take different paths to a register, the compiler waits for the load there.
+  const auto part_of = [&](const T* row, int d) __attribute__((always_inline)) {
+    if constexpr (QUADS) return static_cast<vt>(*reinterpret_cast<const mt*>(row + min(d, D - 4)));
+    vt x;
 #pragma unroll
-    for (int e = 0; e < 3; ++e)
-      if (d + e < D) x[e] = row[d + e];
+    for (int e = 0; e < 4; ++e) x[e] = row[min(d + e, D - 1)];
     return x;
   };
   const auto f32_of = [](vt x) { return f32x4{to_f32(x[0]), to_f32(x[1]), to_f32(x[2]), to_f32(x[3])}; };
-  // Token k + l % 16 of block k: its page, and the place of its row in the pools (-1: none).
-  const auto page_of = [&](int64_t k) { return k + col < k1 ? A.table[(size_t)b * A.max_pages + (int)(k + col) / A.P] : -1; };
-  const auto row_at = [&](int64_t k, int page) {
-    return k + col < k1 ? (((int64_t)page * A.Hkv + h) * A.P + (int)(k + col) % A.P) * D : (int64_t)-1;
+  const auto dims_of = [&](f32x4 x, int d) __attribute__((always_inline)) {  // zeros past the last dim
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = d + e < D ? x[e] : 0.f;
+    return x;
   };
+  // Token k + l % 16 of block k, or the stretch's last: its page, and the place of its row in the pools.
+  const auto token_at = [&](int64_t k) { return (int)min(k + col, (int64_t)k1 - 1); };
+  const auto page_of = [&](int64_t k) { return A.table[(size_t)b * A.max_pages + token_at(k) / A.P]; };
+  const auto row_at = [&](int64_t k, int page) { return (((int64_t)page * A.Hkv + h) * A.P + token_at(k) % A.P) * D; };
   vt nk[C];
   const auto load_k = [&](int64_t at) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      nk[c] = vt{};
-      if (16 * c < D && at >= 0) nk[c] = part_of(kp + at, 16 * c + 4 * quarter);
-    }
+    for (int c = 0; c < C; ++c)
+      if (16 * c < D) nk[c] = part_of(kp + at, 16 * c + 4 * quarter);  // uniform
   };
   int64_t k = (int64_t)k0 + kTok * wave;
-  int64_t at = row_at(k, page_of(k));
-  load_k(at);
+  int64_t at = 0;
+  if (k < k1) {  // uniform in a wavefront
+    at = row_at(k, page_of(k));
+    load_k(at);
+  }
   const int live = min(v0 + col, r.n * G - 1), j = r.first + live / G;  // (vectors past the last: the last one again)
   f32x4 qf[C];
 #pragma unroll
@@ -163,7 +169,7 @@ __global__ __launch_bounds__(kGenThreads) void tree_generic(const T* __restrict_
     qf[c] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (16 * c >= D) continue;  // uniform
     const T* row = q + ((size_t)j * A.Hq + (size_t)h * G + live % G) * D;
-    qf[c] = f32_of(part_of(row, 16 * c + 4 * quarter)) * A.scale_log2;
+    qf[c] = dims_of(f32_of(part_of(row, 16 * c + 4 * quarter)) * A.scale_log2, 16 * c + 4 * quarter);
   }
   float m = -INFINITY, l = 0.f;
   f32x4 acc[NGr][4];  // [64 dims][dim % 4]: dims 64 g + 16 (l / 16) + 4 i + dim % 4
@@ -174,21 +180,19 @@ __global__ __launch_bounds__(kGenThreads) void tree_generic(const T* __restrict_
   for (; k < k1; k += kTurn) {  // uniform in a wavefront
     const int page = page_of(k + kTurn);
     vt nv_[4][NGr];
-    int64_t rows[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // token 4 (l / 16) + i
-      rows[i] = __shfl(at, 4 * quarter + i, 64);
+      const T* row = vp + __shfl(at, 4 * quarter + i, 64);
 #pragma unroll
-      for (int g = 0; g < NGr; ++g) {
-        nv_[i][g] = vt{};
-        if (64 * g < D && rows[i] >= 0) nv_[i][g] = part_of(vp + rows[i], 64 * g + 4 * col);
-      }
+      for (int g = 0; g < NGr; ++g)
+        if (64 * g < D) nv_[i][g] = part_of(row, 64 * g + 4 * col);  // uniform
     }
     f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       if (16 * c >= D) continue;  // uniform
-      const f32x4 x = f32_of(nk[c]);
+      f32x4 x = f32_of(nk[c]);
+      if (16 * c + 16 > D) x = dims_of(x, 16 * c + 4 * quarter);  // uniform
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], qf[c][e], s[e & 1], 0, 0, 0);
     }
@@ -228,6 +232,10 @@ __global__ __launch_bounds__(kGenThreads) void tree_generic(const T* __restrict_
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         f32x4 x = f32_of(nv_[i][g]);
+        if (nt < kTok) {  // uniform: the last token again
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = 4 * quarter + i < nt ? x[e] : 0.f;
+        }
         if (drafted) {  // uniform: what is no finite number must not meet the zero weights of what is not seen
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -306,41 +314,45 @@ __global__ __launch_bounds__(kGenThreads) void tree_generic(const T* __restrict_
   }
 }
 
-// out = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s over the stretches.  One workgroup per token.
+// out = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s over the stretches.  A wavefront per token and head: lanes are stretches
+// for the statistics, dims for the sums, 16 O on their way.
+constexpr int kMaxSplits = 64;
 template <typename T>
 __global__ __launch_bounds__(kGenThreads) void tree_generic_join(T* __restrict__ out, Args A) {
-  const int j = blockIdx.x, t = threadIdx.x;
+  const int lane = threadIdx.x & 63;
+  const int64_t id = (int64_t)blockIdx.x * kGenWaves + uni(threadIdx.x >> 6);
+  const int j = (int)(id / A.Hq);
+  if (j >= A.tokens) return;  // uniform in a wavefront
+  const float2 ml = lane < A.splits ? *reinterpret_cast<const float2*>(A.part_ml + 2 * (id * A.splits + lane))
+                                    : make_float2(-INFINITY, 0.f);
   int b = -1;  // the row whose tokens hold j
-  for (int b0 = 0; b0 < A.batch; b0 += kGenThreads) {  // uniform
-    const int mine = b0 + t < A.batch ? b0 + t : -1;
+  for (int b0 = 0; b0 < A.batch && b < 0; b0 += 64) {  // uniform
     bool has = false;
-    if (mine >= 0) {
-      const Row r = row_of(A, mine);
+    if (b0 + lane < A.batch) {
+      const Row r = row_of(A, b0 + lane);
       has = j >= r.first && j < r.first + r.n;
     }
-    __shared__ int sm_row;
-    if (t == 0) sm_row = -1;
-    __syncthreads();
-    if (has) sm_row = mine;
-    __syncthreads();
-    b = uni(sm_row);
-    if (b >= 0) break;  // uniform
-    __syncthreads();
+    const uint64_t rows = __builtin_amdgcn_ballot_w64(has);
+    if (rows) b = b0 + __builtin_ctzll(rows);
   }
   if (b < 0) return;  // uniform: a token of no row is left as it was
-  const bool any = sees(A, row_of(A, b), j);
-  for (int i = t; i < A.Hq * A.D; i += kGenThreads) {
-    const int head = i / A.D, d = i - head * A.D;
-    const size_t at = ((size_t)j * A.Hq + head) * A.splits;
-    float M = -INFINITY, den = 0.f, o = 0.f;
-    for (int s = 0; s < A.splits; ++s) M = fmaxf(M, A.part_ml[2 * (at + s)]);
-    const float ms = M == -INFINITY ? 0.f : M;
-    for (int s = 0; s < A.splits; ++s) {
-      const float f = __builtin_amdgcn_exp2f(A.part_ml[2 * (at + s)] - ms);
-      den = fmaf(A.part_ml[2 * (at + s) + 1], f, den);
-      o = fmaf(A.part_o[(at + s) * A.D + d], f, o);
+  const float M = wave_max(ml.x), f = __builtin_amdgcn_exp2f(ml.x - (M == -INFINITY ? 0.f : M)), den = wave_sum(ml.y * f);
+  const float none = den != 0.f || !sees(A, row_of(A, b), j) ? 0.f : NAN;
+  for (int d0 = 0; d0 < A.D; d0 += 64) {  // uniform
+    const int d = min(d0 + lane, A.D - 1);
+    float o = 0.f;
+    constexpr int U = 16;
+    for (int s0 = 0; s0 < A.splits; s0 += U) {  // uniform
+      float x[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) x[i] = A.part_o[(id * A.splits + min(s0 + i, A.splits - 1)) * A.D + d];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const float fi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(s0 + i, 63)));
+        if (s0 + i < A.splits) o = fmaf(x[i], fi, o);
+      }
     }
-    out[((size_t)j * A.Hq + head) * A.D + d] = from_f32<T>(as_f32_value(den != 0.f ? o / den : any ? NAN : 0.f));
+    if (d0 + lane < A.D) out[id * A.D + d] = from_f32<T>(as_f32_value(den != 0.f ? o / den : none));
   }
 }
 
@@ -348,13 +360,13 @@ struct GenericPlan {
   unsigned tiles;
   int splits;
 };
-// Splits that give some 1024 workgroups, of 256 tokens at least (were every row as long as the table).
+// Splits that give some 1024 workgroups, of 128 tokens at least (were every row as long as the table).
 GenericPlan generic_plan(int tokens, int batch, int Hq, int Hkv, int P, int max_pages) {
   const long vectors = (long)tokens * (Hq / Hkv);
   GenericPlan p;
   p.tiles = (unsigned)((vectors + kVec - 1) / kVec + min(batch, tokens));  // (a part of a tile a row besides)
-  const long wgs = (long)p.tiles * Hkv, most = ((long)max_pages * P + 255) / 256;
-  p.splits = (int)max(1L, min(min(32L, most), 1024 / wgs));
+  const long wgs = (long)p.tiles * Hkv, most = ((long)max_pages * P + 127) / 128;
+  p.splits = (int)max(1L, min(min((long)kMaxSplits, most), 1024 / wgs));
   return p;
 }
 size_t generic_floats(const GenericPlan& p, int tokens, int Hq, int D) {
@@ -1171,19 +1183,24 @@ extern "C" int cir_paged_tree_attention(const void* q, const void* k_pool, const
   const size_t floats = generic_floats(g, tokens, num_heads, head_dim), need = floats * sizeof(float);
   CIR_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0),
                 "tree_attention: workspace too small or not on 16 bytes (%zu < %zu)", workspace_bytes, need);
-  A.part_o = static_cast<float*>(workspace);
-  A.part_ml = A.part_o + (size_t)tokens * num_heads * g.splits * head_dim;
+  A.part_ml = static_cast<float*>(workspace);
+  A.part_o = A.part_ml + 2 * (size_t)tokens * num_heads * g.splits;
   A.splits = g.splits;
   A.scale_log2 = scale_log2;
   const auto go = [&]<typename T>() {
     const dim3 grid(g.tiles, num_kv_heads, g.splits);
     const T *qt = static_cast<const T*>(q), *kt = static_cast<const T*>(k_pool), *vt = static_cast<const T*>(v_pool);
-    if (head_dim <= 64) tree_generic<T, 64><<<grid, kGenThreads, 0, s>>>(qt, kt, vt, static_cast<T*>(out), A);
-    else if (head_dim <= 128) tree_generic<T, 128><<<grid, kGenThreads, 0, s>>>(qt, kt, vt, static_cast<T*>(out), A);
-    else tree_generic<T, 256><<<grid, kGenThreads, 0, s>>>(qt, kt, vt, static_cast<T*>(out), A);
+    const auto sized = [&]<int DM>() {
+      if (head_dim % 4 == 0) tree_generic<T, DM, true><<<grid, kGenThreads, 0, s>>>(qt, kt, vt, static_cast<T*>(out), A);
+      else tree_generic<T, DM, false><<<grid, kGenThreads, 0, s>>>(qt, kt, vt, static_cast<T*>(out), A);
+    };
+    if (head_dim <= 64) sized.template operator()<64>();
+    else if (head_dim <= 128) sized.template operator()<128>();
+    else sized.template operator()<256>();
     const int st = launch_status();
     if (st || g.splits == 1) return st;
-    tree_generic_join<T><<<tokens, kGenThreads, 0, s>>>(static_cast<T*>(out), A);
+    const unsigned wgs = (unsigned)(((long)tokens * num_heads + kGenWaves - 1) / kGenWaves);
+    tree_generic_join<T><<<wgs, kGenThreads, 0, s>>>(static_cast<T*>(out), A);
     return launch_status();
   };
   return kv_dtype == CIR_F16 ? go.template operator()<f16>() : go.template operator()<float>();

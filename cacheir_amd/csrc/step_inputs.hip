@@ -275,7 +275,8 @@ __global__ __launch_bounds__(kRopeThreads) void rope_append_kernel(
 // y = factor * R(pos * f_i) (x / sqrt(mean x^2 + eps) * w), heads of q and k; v is copied: the rotary append with the
 // norm of each head before the turn, x read once and y rounded once.  A head is taken by LPH lanes (a power of two, items
 // of NP pairs as above, at most two a lane), which join their sums of squares by shuffles, so nothing passes through LDS
-// but the sines.  A lane keeps its own part of both weights.
+// but the sines.  A lane keeps its own part of both weights.  Bound by the copy: 100.6 MB of 4093 tokens of 48 heads in 20.7
+// us (4.9 TB/s; without the next head's values on their way and with weights one by one 31.6), of one token by latency (3.4).
 struct NormIn {
   const void *qw, *kw;
   int wf32;  // weights in fp32 (else fp16)

@@ -70,7 +70,8 @@ __device__ __forceinline__ bool sees(const Args& A, const Row& r, int j) {
 // the order of the summed dims and tokens is free, so lane l takes dims 16 c + 4 (l / 16) .. of K and Q by one load, its
 // scores are those of tokens 4 (l / 16) .. of vector l % 16, which is how the second product wants the weights, and its
 // rows of V^T are dims 64 g + 4 (l % 16) .., again one load.  K of the next block and V of this one are on their way
-// during the products.
+// during the products.  16 rows of 1 or 2 tokens over 7800, 16 heads on 8 of 96 dims in fp32 (767 MB): 128 us, 6.0 TB/s;
+// 7 tokens over 97, 4 heads on 2 of 64 dims: 8.4, latency (plan, table, K, two blocks, the join through LDS).
 constexpr int kGenThreads = 256;
 constexpr int kGenWaves = kGenThreads / 64;
 constexpr int kVec = 16;
@@ -389,10 +390,18 @@ __device__ __forceinline__ uint32_t not_finite(f16 x) {
 // vectors, so pieces do not overlap, and the join finds a tile's pieces from its start and the stretch alone.
 //
 // Body (4 wavefronts, one workgroup per CU, up to 512 registers a lane).  Each wavefront takes NG groups of 32 query
-// vectors (Q in registers) and, of VW = 4 / CW wavefronts side by side, every CW-th block.  Stages of 64 tokens of K and V
-// come by DMA into a ring of four in LDS: two are on their way while one is worked on.  S^T = K Q^T and O^T = V^T P^T on
-// MFMA 32x32x16: a lane holds one vector's scores and sums, 64 vectors a wavefront halve the LDS reads of 32.  The scores
-// of the next block run on the matrix cores while the VALU takes this block's exponentials.
+// vectors (Q in accumulator registers) and, of VW = 4 / CW wavefronts side by side, every CW-th block.  Stages of 64 tokens
+// of K and V come by DMA into a ring of four in LDS: two are on their way while one is worked on.  S^T = K Q^T and
+// O^T = V^T P^T on MFMA 32x32x16: a lane holds one vector's scores and sums, 64 vectors a wavefront halve the LDS reads of
+// 32.  The scores of the next block run on the matrix cores while the VALU takes this block's exponentials.
+//
+// Bound, and measured (kernel, then join): 8 trees of 57 to 64 tokens over 11000 to 16000, 32 query heads on 8 (107 GFLOP):
+// 168 + 10 us, 640 TFLOP/s, the matrix cores busy 40% of the cycles: a block of 32 tokens and 64 vectors a wavefront takes
+// 2500 cycles for 1024 of products, since one wavefront per SIMD issues an instruction in 4 to 5 cycles and products hide only
+// what stands between them.  32 trees of 5 to 16 tokens, 28 heads on 4 (238 MB of K and V): 63 + 6 us, 3.8 TB/s; 26 us of it
+// are what comes before and behind the blocks of a workgroup's one or two pieces (plan 3.3 us, a piece's first loads 4, its
+// sums 3).  4 trees of 26 tokens over 300 to 3000: 22 + 5, all of it such.  K and V straight into registers, without a ring,
+// took 32 and 100 us where this took 31 and 75.
 constexpr int D = 128;
 constexpr int kBlock = 32;       // tokens of an MFMA tile
 constexpr int kGroup = 32;       // query vectors of an MFMA tile
@@ -400,7 +409,8 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kTileVec = 256;    // query vectors of a tile
 constexpr int kWorkgroups = 256;
-constexpr int kItemCost = 10;    // a piece's start and join, in blocks
+constexpr int kItemCost = 10;    // a piece's start and join, in blocks (32 and 8 trees above: 63 and 168 us, with 6 70 and 176,
+                                 // with 16 63 and 174)
 constexpr int kMinStretch = 4;
 constexpr int kMaxRows = 1024;
 constexpr int kMaxGroup = 2048;   // query heads per KV head (256 G G < 2^32: token_of is exact)
@@ -819,9 +829,7 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
       block.template operator()<SPECIAL>(i, blk, blk + CW, place(i + 2), place(i));
     }
   };
-  // (A block scores the next one too.  Short pieces stay with the code of the special blocks, which they need besides: each
-  // line of code is loaded once a launch, and a piece of 8 blocks waits for that most of its time.)
-  const int plain = nst <= 6 ? 0 : max(0, min(nst * PW, (special - p.blk0) / CW - 1));
+  const int plain = max(0, min(nst * PW, (special - p.blk0) / CW - 1));  // (a block scores the next one too)
   turns.template operator()<false>(0, plain);
   turns.template operator()<true>(plain, nst * PW);
   // Infinities and NaN of V among the drafted tokens: each is added to the sums of the vectors that see its token.
@@ -1011,6 +1019,8 @@ __global__ __launch_bounds__(kThreads, 1) void tree_f16_d128(const f16* __restri
       p.blk0 = k0;
       p.blk1 = k1;
       p.at = (size_t)w * kTileVec + (size_t)p.r.first * G + p.v0;
+      // The fewest vectors a wavefront that hold the tile; 112 vectors of 32 trees: 63 us, as <4, 2> 92; up to 48 of 32 trees
+      // over up to 4000 tokens: 62, as <2, 2> 71, as <4, 2> 101.
       if (p.nv <= 2 * kGroup) tree_piece<2, 1>(F, p, sm, ring);
       else if (p.nv <= 4 * kGroup) tree_piece<2, 2>(F, p, sm, ring);
       else tree_piece<4, 2>(F, p, sm, ring);
@@ -1018,15 +1028,16 @@ __global__ __launch_bounds__(kThreads, 1) void tree_f16_d128(const f16* __restri
   }
 }
 
-// out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i over the pieces of a vector's tile.  Two half-wavefronts per vector, each
-// with every second piece, four dims a lane; lane k takes (m, l) of every 32nd piece.  Bound by latency (row, record, then
-// pieces), so a half-wavefront has four O on their way, the first ones along with the (m, l).
-__global__ __launch_bounds__(256) void tree_join(Fast F, f16* __restrict__ out) {
-  constexpr int W = 2, U = 4, kVecs = 8 / W;
-  __shared__ f32x4 sm_o[kVecs][32];
+// out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i over the pieces of a vector's tile.  Half a wavefront per vector, four dims
+// a lane; lane k takes (m, l) of every 32nd piece.  Bound by latency (record, then pieces): four O are on their way, the first
+// ones along with the (m, l).  15.5k vectors of 4 to 5 pieces: 10.1 us, of 41k vectors with one or two 12.3; two halves per
+// vector, with every second piece each: 12.8 and 22.5, eight O on their way 10.5 and 14.4.
+constexpr int kJoinVec = 8;  // of a workgroup
+__global__ __launch_bounds__(32 * kJoinVec) void tree_join(Fast F, f16* __restrict__ out) {
+  constexpr int U = 4;
   const Args& A = F.a;
-  const int part = threadIdx.x >> 5, lane = threadIdx.x & 31, s = part % W, vec = part / W;
-  const int id = blockIdx.x * kVecs + vec, G = A.Hq / A.Hkv;
+  const int lane = threadIdx.x & 31;
+  const int id = blockIdx.x * kJoinVec + (threadIdx.x >> 5), G = A.Hq / A.Hkv;
   const int j = id / A.Hq, head = id - j * A.Hq, h = head / G;
   TokRec rec = F.rec[min(j, A.tokens - 1)];
   if (j >= A.tokens) rec.blocks = -1;
@@ -1046,7 +1057,7 @@ __global__ __launch_bounds__(256) void tree_join(Fast F, f16* __restrict__ out) 
     f32x4 x[U];
     const auto load = [&](int k0) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < U; ++i) x[i] = o_of(min(k0 + s + W * i, n - 1));
+      for (int i = 0; i < U; ++i) x[i] = o_of(min(k0 + i, n - 1));
     };
     load(0);
     float M = ml.x;
@@ -1058,26 +1069,23 @@ __global__ __launch_bounds__(256) void tree_join(Fast F, f16* __restrict__ out) 
       if (k0) ml = k0 + lane < n ? ml_of(k0 + lane) : make_float2(-INFINITY, 0.f);
       const float f = __builtin_amdgcn_exp2f(ml.x - ms);
       den = fmaf(ml.y, f, den);
-      for (int j0 = k0; j0 < min(n, k0 + 32); j0 += W * U) {
+      for (int j0 = k0; j0 < min(n, k0 + 32); j0 += U) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-          const int k = j0 + s + W * i;
+          const int k = j0 + i;
           const float fk = __shfl(f, k - k0, 32);
           if (k < n) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] = fmaf(x[i][e], fk, o[e]);
           }
         }
-        if (j0 + W * U < n) load(j0 + W * U);
+        if (j0 + U < n) load(j0 + U);
       }
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) den += __shfl_xor(den, d, 32);
   }
-  if (s > 0) sm_o[vec][lane] = o;
-  __syncthreads();
-  if (s > 0 || !live) return;
-  o += sm_o[vec][lane];
+  if (!live) return;
   float inv = 1.f / den;
   if (den == 0.f) inv = n > 0 && sees(A, row_of(A, rec.row / kMaxDrafts), j) ? NAN : 0.f;
   f16x4 y;
@@ -1109,7 +1117,8 @@ Layout layout(int tokens, int Hq, int Hkv) {
   return l;
 }
 
-// Sizes that the MFMA kernel takes; others run the generic one.
+// Sizes that the MFMA kernel takes; others run the generic one (which takes 107, 544 and 2104 us for the three above, and 13
+// where this takes 9: 7 tokens over 97).
 bool fast_sizes(int tokens, int batch, int Hq, int Hkv, int head_dim, int P, int max_pages, int kv_dtype) {
   const long blocks = (long)max_pages * P / kBlock + 1 + kItemCost;
   const long tiles = (long)tokens * (Hq / Hkv) / kTileVec + batch;
@@ -1176,7 +1185,7 @@ extern "C" int cir_paged_tree_attention(const void* q, const void* k_pool, const
         static_cast<const f16*>(q), static_cast<const f16*>(k_pool), static_cast<const f16*>(v_pool), page_table, F);
     const int st = launch_status();
     if (st) return st;
-    tree_join<<<((unsigned)tokens * num_heads + 3) / 4, 256, 0, s>>>(F, static_cast<f16*>(out));
+    tree_join<<<((unsigned)tokens * num_heads + kJoinVec - 1) / kJoinVec, 32 * kJoinVec, 0, s>>>(F, static_cast<f16*>(out));
     return launch_status();
   }
   const GenericPlan g = generic_plan(tokens, batch, num_heads, num_kv_heads, page_size, max_pages);

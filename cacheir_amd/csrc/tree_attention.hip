@@ -136,6 +136,7 @@ __global__ __launch_bounds__(kGenThreads) void tree_generic(const T* __restrict_
   // follows: where lanes take different paths to a register, the compiler waits for the load there.
   const auto part_of = [&](const T* row, int d) __attribute__((always_inline)) {
     if constexpr (QUADS) return static_cast<vt>(*reinterpret_cast<const mt*>(row + min(d, D - 4)));
+    asm volatile("" : "+v"(d));  // (else the places of all elements are kept through the loop: 20 registers too many at 256)
     vt x;
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = row[min(d + e, D - 1)];

@@ -103,6 +103,22 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const T* in, T*
   const auto on_path = [&](int i) __attribute__((always_inline)) {
     return place >= 0 && i < i1 && (A.masks[(int64_t)(first + i) * A.words + (t >> 6)] >> (t & 63) & 1);
   };
+  // The first tokens of the history, before the logits: loads come back in order.
+  constexpr int U = 4;  // pairs on their way
+  typedef int64_t i64x2 __attribute__((ext_vector_type(2), aligned(8)));
+  const int len = A.history ? min(max(A.history_lens[b], 0), A.history_width) : 0;
+  const int64_t* hist = A.history + (int64_t)b * A.history_width;
+  i64x2 said[U];
+  const auto said_from = [&](int k0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + 2 * (t + u * kThreads);
+      said[u] = i64x2{-1, -1};
+      if (k + 1 < len) said[u] = *reinterpret_cast<const i64x2*>(hist + k);
+      else if (k < len) said[u].x = hist[k];
+    }
+  };
+  said_from(0);
   vt x[J], xn[J];
   uint32_t ok[J], okn[J];
   allowed(i0, ok);
@@ -129,32 +145,19 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const T* in, T*
     }
     __syncthreads();
   }
-  if (A.history) {
-    constexpr int U = 4;  // pairs on their way
-    typedef int64_t i64x2 __attribute__((ext_vector_type(2), aligned(8)));
-    const int len = min(max(A.history_lens[b], 0), A.history_width);
-    const int prompt = A.prompt_lens ? A.prompt_lens[b] : 0;
-    const int64_t* h = A.history + (int64_t)b * A.history_width;
-    const auto count = [&](int64_t id, int k) __attribute__((always_inline)) {
-      if (!in_chunk(id)) return;
-      if (k < prompt) atomicOr(&sm_tab[id - v0], kGiven);
-      else atomicAdd(&sm_tab[id - v0], 1u);
-    };
-    for (int k0 = 0; k0 < len; k0 += 2 * U * kThreads) {
-      i64x2 id[U];
+  const int prompt = A.prompt_lens ? A.prompt_lens[b] : 0;
+  const auto count = [&](int64_t id, int k) __attribute__((always_inline)) {
+    if (!in_chunk(id)) return;
+    if (k < prompt) atomicOr(&sm_tab[id - v0], kGiven);
+    else atomicAdd(&sm_tab[id - v0], 1u);
+  };
+  for (int k0 = 0; k0 < len; k0 += 2 * U * kThreads) {
+    if (k0) said_from(k0);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int k = k0 + 2 * (t + u * kThreads);
-        id[u] = i64x2{-1, -1};
-        if (k + 1 < len) id[u] = *reinterpret_cast<const i64x2*>(h + k);
-        else if (k < len) id[u].x = h[k];
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int k = k0 + 2 * (t + u * kThreads);
-        count(id[u].x, k);
-        count(id[u].y, k + 1);
-      }
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + 2 * (t + u * kThreads);
+      count(said[u].x, k);
+      count(said[u].y, k + 1);
     }
   }
   __syncthreads();

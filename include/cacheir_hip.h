@@ -203,9 +203,10 @@ int cir_paged_decode_attention_shared(const void* q, const void* k_pool, const v
  * counts are not read and their out is left as it was.  A token that sees nothing yields
  * zeros, one whose scores are all -inf NaN; K and V that a token does not see do not enter
  * its result, NaN and infinities among them.  Tokens past the table (max_pages * page_size)
- * are not seen.  fp16 with head_dim 128 runs on MFMA, other sizes (head_dim <= 256) in fp32
- * arithmetic.  A row's last bits depend on the batch it is in.  tokens * num_heads < 2^26,
- * num_kv_heads < 2^16, batch < 2^20.
+ * are not seen.  fp16 with head_dim 128 and pages of a multiple of 16 tokens holds the weights
+ * in fp16 (statistics and sums in fp32), other sizes (head_dim <= 256) run in fp32 arithmetic.
+ * A row's last bits depend on the batch it is in.  out overlaps no input.  tokens * num_heads
+ * < 2^26, num_kv_heads < 2^16, batch < 2^20.
  * workspace: cir_tree_attention_workspace_bytes bytes on a 16-byte address (0: NULL will do),
  * written by the call (calls that overlap need one each); nothing in it needs clearing.
  * The reference attends one new token a row (cacheir/backends/triton_kernels.py:174-217). */

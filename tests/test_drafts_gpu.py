@@ -743,6 +743,7 @@ def near_logits(got, ref, tol):
     ([5, 1, 12], 8192, 300, torch.float32, 1, 0), ([70, 3], 8193, 50, torch.float16, 2, 0),
     ([64, 0, 33, 1], 16384, 1000, torch.float16, 1, 0), ([2, 9], 20001, 5000, torch.float32, 1, 3),
     ([3, 200], 1000, 64, torch.float32, 4, 0), ([4, 4], 24576, 10, torch.float16, 1, 8), ([3, 1], 16390, 7, torch.float16, 1, 2),
+    ([64, 6], 152064, 300, torch.float32, 1, 0), ([100, 12], 152063, 3000, torch.float16, 2, 1),  # more than 32 MB
 ])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_adjust_logits(device, nodes, vocab, width, dtype, words, pad, in_place):

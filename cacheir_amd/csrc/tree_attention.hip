@@ -129,8 +129,8 @@ __global__ __launch_bounds__(kGenThreads) void tree_generic(const T* __restrict_
   const int v0 = uni(sm_find[1]) * kVec, nv = min(kVec, r.n * G - v0);
   // This workgroup's stretch of the row's tokens.
   constexpr int kTurn = kTok * kGenWaves;
-  const int stretch = ((r.limit + A.splits - 1) / A.splits + kTurn - 1) / kTurn * kTurn;
-  const int k0 = min((int64_t)r.limit, (int64_t)blockIdx.z * stretch), k1 = min(r.limit, k0 + stretch);
+  const int64_t stretch = (((int64_t)r.limit + A.splits - 1) / A.splits + kTurn - 1) / kTurn * kTurn;
+  const int k0 = (int)min((int64_t)r.limit, blockIdx.z * stretch), k1 = (int)min((int64_t)r.limit, k0 + stretch);
 
   // Dims d .. d + 3 of a row; what stands for those past the last is some other dim's.  Without a branch, and so is what
   // follows: where lanes take different paths to a register, the compiler waits for the load there.

@@ -412,7 +412,7 @@ constexpr int kTileVec = 256;    // query vectors of a tile
 constexpr int kWorkgroups = 256;
 constexpr int kItemCost = 10;    // a piece's start and join, in blocks (32 and 8 trees above: 63 and 168 us, with 6 70 and 176,
                                  // with 16 63 and 174)
-constexpr int kMinStretch = 4;
+constexpr int kMinStretch = 4;   // (2 trees of 5 and 26 tokens over 300: 15 us, with 8 17, with 16 23)
 constexpr int kMaxRows = 1024;
 constexpr int kMaxGroup = 2048;   // query heads per KV head (256 G G < 2^32: token_of is exact)
 constexpr int kRowB = 2 * D;     // bytes of a K or V row

@@ -13,16 +13,18 @@ namespace {
 constexpr int kMaxDrafts = 256;  // of a row: one per thread
 constexpr int kThreads = 256;
 
-// A row's first token and their number, inside the step's tokens whatever the device's numbers are.
+// A row's first token and their number, inside the step's tokens whatever the device's numbers are.  The cache holds all of
+// them behind the context, however many a kernel takes.
 struct Drafts {
-  int first, n, end;  // end: where the next row's begin
+  int first, all, n, end;  // n: of all, those that the kernel takes (`most` at most); end: where the next row's begin
 };
 __device__ __forceinline__ Drafts drafts_of(const int32_t* offsets, const int32_t* counts, int b, int tokens, int most) {
   const int o = offsets[b], e = offsets[b + 1], c = counts[b];
   Drafts d;
   d.first = min(max(o, 0), tokens);
   d.end = min(max(e, d.first), tokens);
-  d.n = max(0, min(min(c, most), d.end - d.first));
+  d.all = max(0, min(c, d.end - d.first));
+  d.n = min(d.all, most);
   return d;
 }
 
@@ -116,7 +118,7 @@ __global__ __launch_bounds__(kThreads) void accept_kernel(AcceptArgs A) {
   __shared__ int64_t sm_of[kMaxDrafts], sm_to[kMaxDrafts];  // byte of the token's row in head 0 of a layer's pool
   const int b = blockIdx.x, t = threadIdx.x;
   const Drafts d = drafts_of(A.offsets, A.counts, b, A.tokens, kMaxDrafts);
-  const int len = A.lens[b], ctx = max(0, len - d.n);
+  const int len = A.lens[b], ctx = max(0, len - d.all);
   const bool in = t < d.n;
   const int p = in ? A.parents[d.first + t] : -1;
   const int64_t draft = in ? A.drafts[d.first + t] : 0;
@@ -195,7 +197,7 @@ __global__ __launch_bounds__(kThreads) void settle_kernel(const int32_t* lens, c
   const auto row = [&](int b, int& keep, int& now, int& had) __attribute__((always_inline)) {
     const Drafts d = drafts_of(offsets, counts, b, tokens, kMaxDrafts);
     const int len = max(0, lens[b]);
-    keep = max(0, len - d.n) + accepted[b];
+    keep = max(0, len - d.all) + accepted[b];
     now = pages(keep);
     had = pages(len);
   };

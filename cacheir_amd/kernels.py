@@ -546,8 +546,8 @@ def accept_drafts(parents: torch.Tensor, drafts: torch.Tensor, targets: torch.Te
                   v_pools: torch.Tensor, *, most: int, free_slots: torch.Tensor | None = None,
                   free_head: torch.Tensor | None = None, out: AcceptedDrafts | None = None) -> AcceptedDrafts:
     """The drafted tokens that the model's choices confirm: from the row's token 0 on, the child whose ``drafts`` (int64
-    ``[T]``) equals ``targets`` (int64 ``[T]``, chosen after each token), ``most`` tokens at most.  K and V of the path
-    move behind the context in the pools of all layers (``[layers, slots, kv_heads, page_size, head_dim]``).  With
+    ``[T]``) equals ``targets`` (int64 ``[T]``, chosen after each token), ``most`` tokens at most, none past the row's
+    first 256.  K and V of the path move behind the context in the pools of all layers (``[layers, slots, kv_heads, page_size, head_dim]``).  With
     ``free_slots`` and ``free_head`` (as ``extend_page_tables`` takes them) pages behind the new lengths go back.
     ``out.seq_lens`` may be ``seq_lens``.  See ``cir_accept_drafts``."""
     dev, i32, i64 = parents.get_device(), torch.int32, torch.int64

@@ -494,8 +494,8 @@ int cir_norm_rope_append(const void* q, int64_t q_token_stride, int64_t q_head_s
 int cir_draft_tree(const int32_t* parents, const int32_t* seq_lens, const int32_t* offsets, const int32_t* counts,
                    int64_t* masks, int32_t* positions, int tokens, int batch, int words, void* stream);
 
-/* The drafted tokens that the model confirms.  Rows as in cir_draft_tree (up to 256 tokens
- * each, later ones are never taken); drafts int64 [tokens] are the tokens fed to the model,
+/* The drafted tokens that the model confirms.  Rows as in cir_draft_tree, of any number of
+ * tokens n, of which those from the 256th on are never taken; drafts int64 [tokens] are the tokens fed to the model,
  * targets int64 [tokens] what it chose after each.  The path starts at the row's token 0,
  * which stands, and goes on from token p to its first child whose draft equals targets[p]:
  *   accepted[b]   tokens on the path: at least 1 (0 in a row without tokens), at most `most`

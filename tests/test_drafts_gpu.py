@@ -974,6 +974,34 @@ def test_accept_drafts(device, nodes, contexts, layers, hkv, d, psize, dtype, mo
     assert torch.equal(s["seq_lens"].cpu(), c["seq_lens"])
 
 
+@pytest.mark.parametrize("shape,ids,most", [("any", 2, 256), ("any", 1, 256), ("chain", 1, 256), ("forest", 2, 9)])
+@pytest.mark.parametrize("give_back", [False, True])
+def test_accept_drafts_of_rows_past_256_tokens(device, shape, ids, most, give_back):
+    """The context ends before all of a row's drafted tokens; those from the 256th on are never taken."""
+    from cacheir_amd import kernels
+
+    nodes, contexts, psize = [300, 5, 257, 1000, 256], [37, 9, 0, 130, 16], 16
+    c = accept_case(91, nodes, contexts, 2, 2, 64, psize, torch.float16, ids, gaps=[0, 2, 0, 1, 0], shape=shape)
+    ref = dict(c, parents=c["parents"].clone())
+    for first, n in zip(c["offsets"].tolist(), nodes):
+        ref["parents"][first + 256: first + max(n, 256)] = -1  # (accept_ref takes tokens by their parents)
+    accepted, paths, tokens, ends, kp, vp = accept_ref(ref, most)
+    s = {k: v.to(device) for k, v in c.items()}
+    kw, back = {}, []
+    if give_back:
+        for b, (end, length) in enumerate(zip(ends, c["seq_lens"].tolist())):
+            back += c["page_table"][b, -(-end // psize): -(-length // psize)].tolist()
+        kw = dict(free_slots=torch.zeros(len(back) + 5, dtype=torch.int32, device=device),
+                  free_head=i32([len(back) + 2]).to(device),
+                  out=kernels.AcceptedDrafts.empty(len(nodes), most, device)._replace(seq_lens=s["seq_lens"]))
+    got = kernels.accept_drafts(**s, most=most, **kw)
+    assert got.accepted.tolist() == accepted and got.path.tolist() == paths and got.tokens.tolist() == tokens
+    assert got.seq_lens.tolist() == ends
+    assert torch.equal(s["k_pools"].cpu(), kp) and torch.equal(s["v_pools"].cpu(), vp)
+    if give_back:
+        assert kw["free_head"].item() == 2 and kw["free_slots"].tolist() == [0, 0] + back + [0] * 3
+
+
 def test_accept_drafts_far_in_the_pools(device):
     """Layers of more than 2^32 bytes: what moves is where it belongs, and nothing else is written."""
     from cacheir_amd import kernels

@@ -35,6 +35,8 @@ __device__ __forceinline__ Drafts drafts_of(const int32_t* offsets, const int32_
 // parent to parent is one LDS latency a step: some 8 us for the chain).  One workgroup per
 // row, one token per thread; a token's depth is the number of its ancestors.  Bound by
 // latency: offsets, then parents, then the rounds (26 tokens 2.6 us, 128 rows of up to 200 6.0).
+// A row of more tokens than masks of W words have bits for is refused: all of its masks are
+// empty, and its positions, as if the first 64 W tokens were all it has, mean nothing.
 template <int W>
 __global__ __launch_bounds__(kThreads) void draft_tree_kernel(const int32_t* __restrict__ parents,
                                                               const int32_t* __restrict__ lens,
@@ -74,7 +76,7 @@ __global__ __launch_bounds__(kThreads) void draft_tree_kernel(const int32_t* __r
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       above += __popcll(m[w]);
-      masks[(size_t)(d.first + t) * W + w] = (int64_t)m[w];
+      masks[(size_t)(d.first + t) * W + w] = d.all > 64 * W ? 0 : (int64_t)m[w];
     }
     positions[d.first + t] = max(0, len - d.n) + above;
   }

@@ -26,17 +26,19 @@ struct Args {
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // A row's first token, their number, where they begin in its context, and what is stored of it; inside the step's
-// tokens and the table whatever the device's numbers are.
+// tokens and the table whatever the device's numbers are.  A row of more tokens than the masks have bits for is refused:
+// what its tokens see is not known, so nothing is stored of it and all of them yield NaN.
 struct Row {
   int first, n, context, limit;
 };
+__device__ __forceinline__ bool refused(const Args& A, int n) { return n > 64 * A.words; }
 __device__ __forceinline__ Row row_of(const Args& A, int b) {
   const int o = A.offsets[b], e = A.offsets[b + 1], c = A.counts[b], len = A.lens[b];
   Row r;
   r.first = min(max(o, 0), A.tokens);
-  r.n = max(0, min(min(c, 64 * A.words), min(e, A.tokens) - r.first));
+  r.n = max(0, min(c, min(e, A.tokens) - r.first));
   r.context = max(0, len - r.n);
-  r.limit = max(0, min(len, A.max_pages * A.P));
+  r.limit = refused(A, r.n) ? 0 : max(0, min(len, A.max_pages * A.P));
   return r;
 }
 // Drafted tokens 32 w .. 32 w + 31 that token j sees.
@@ -54,9 +56,9 @@ __device__ __forceinline__ uint32_t seen_from(const Args& A, int j, int token, i
   return s ? (lo >> s) | (hi << (32 - s)) : lo;
 }
 
-// Whether token j sees any token at all.
+// Whether token j sees any token at all (and yields NaN if none of them counts).
 __device__ __forceinline__ bool sees(const Args& A, const Row& r, int j) {
-  if (min(r.context, r.limit) > 0) return true;
+  if (min(r.context, r.limit) > 0 || refused(A, r.n)) return true;
   const int n = min(r.n, r.limit - r.context);
   uint32_t any = 0;
   for (int w = 0; 32 * w < n; ++w) any |= mask_word(A, j, w, n);
@@ -419,8 +421,9 @@ constexpr int kRowB = 2 * D;     // bytes of a K or V row
 constexpr int kStageTok = 64;    // tokens of a stage
 constexpr int kStage = 2 * kStageTok * kRowB;  // bytes: K, then V
 
-// What the join wants to know of a token's row: place of the first tile's blocks on the axis, their number (-1: no row counts
-// the token), the stretch, and 256 row + the token's number in it.
+// What the join wants to know of a token's row: place of the first tile's blocks on the axis, their number (kNoRow: no row
+// counts the token, kRefused: its row is), the stretch, and 256 row + the token's number in it.
+constexpr int kNoRow = -1, kRefused = -2;
 struct TokRec {
   int start, blocks, stretch, row;
 };
@@ -455,7 +458,7 @@ struct Piece {
 struct Smem {
   float ml[kWaves][2][2 * kGroup];
   uint32_t mask[kTileVec][2 * kMaxDrafts / 64 + 1];
-  int4 row[kMaxRows + 1];  // first token, their number, length, place on the axis
+  int4 row[kMaxRows + 1];  // first token, their number, length (kRefused), place on the axis
   int scan[kWaves], find;
 };
 
@@ -950,7 +953,7 @@ __global__ __launch_bounds__(kThreads, 1) void tree_f16_d128(const f16* __restri
       const Row r = row_of(A, b);
       const int blocks = (r.limit + kBlock - 1) / kBlock, tiles = (r.n * G + kTileVec - 1) / kTileVec;
       cost = blocks > 0 ? tiles * (blocks + kItemCost) : 0;
-      row = make_int4(r.first, r.n, max(0, A.lens[b]), 0);
+      row = make_int4(r.first, r.n, refused(A, r.n) ? kRefused : max(0, A.lens[b]), 0);
     }
     int upto = cost;
     for (int off = 1; off < min(B, 64); off <<= 1) {  // uniform
@@ -986,8 +989,8 @@ __global__ __launch_bounds__(kThreads, 1) void tree_f16_d128(const f16* __restri
     }
     const int4 r = sm.row[a];
     const bool counted = j >= r.x && j < r.x + r.y;
-    F.rec[j] = TokRec{r.w + kItemCost, counted ? (min(r.z, A.max_pages * A.P) + kBlock - 1) / kBlock : -1, stretch,
-                      kMaxDrafts * a + (j - r.x)};
+    const int blocks = r.z == kRefused ? kRefused : (min(r.z, A.max_pages * A.P) + kBlock - 1) / kBlock;
+    F.rec[j] = TokRec{r.w + kItemCost, counted ? blocks : kNoRow, stretch, kMaxDrafts * a + (j - r.x)};
   }
   if (lo >= hi) return;  // uniform
   for (int b = t; b < B; b += kThreads)
@@ -1041,8 +1044,8 @@ __global__ __launch_bounds__(32 * kJoinVec) void tree_join(Fast F, f16* __restri
   const int id = blockIdx.x * kJoinVec + (threadIdx.x >> 5), G = A.Hq / A.Hkv;
   const int j = id / A.Hq, head = id - j * A.Hq, h = head / G;
   TokRec rec = F.rec[min(j, A.tokens - 1)];
-  if (j >= A.tokens) rec.blocks = -1;
-  const bool live = rec.blocks >= 0;
+  if (j >= A.tokens) rec.blocks = kNoRow;
+  const bool live = rec.blocks != kNoRow;
   const int v = rec.row % kMaxDrafts * G + (head - h * G), tile = v / kTileVec;
   const int start = rec.start + tile * (rec.blocks + kItemCost), w0 = start / rec.stretch;
   const int n = live && rec.blocks > 0 ? (start + rec.blocks - 1) / rec.stretch - w0 + 1 : 0;
@@ -1088,7 +1091,8 @@ __global__ __launch_bounds__(32 * kJoinVec) void tree_join(Fast F, f16* __restri
   }
   if (!live) return;
   float inv = 1.f / den;
-  if (den == 0.f) inv = n > 0 && sees(A, row_of(A, rec.row / kMaxDrafts), j) ? NAN : 0.f;
+  if (den == 0.f)
+    inv = rec.blocks == kRefused || (n > 0 && sees(A, row_of(A, rec.row / kMaxDrafts), j)) ? NAN : 0.f;
   f16x4 y;
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] = static_cast<f16>(as_f32_value(o[e] * inv));

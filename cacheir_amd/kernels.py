@@ -308,7 +308,8 @@ def paged_tree_attention(q, k_pool, v_pool, page_table, seq_lens, offsets, count
     """Attention of drafted tokens q ``[T, Hq, D]``: row b's are ``q[offsets[b] : offsets[b] + counts[b]]`` (int32
     ``[B + 1]``, ``[B]``; ``StepTables.offsets`` and ``.granted``), the last of its ``seq_lens[b]`` tokens in the pages.
     Each sees the tokens before the drafted ones, and drafted token k of its row where bit k % 64 of its
-    ``masks[:, k // 64]`` (int64 ``[T, words]``, ``draft_tree``) is set.  Rows of q that no row counts keep their ``out``.
+    ``masks[:, k // 64]`` (int64 ``[T, words]``, ``draft_tree``) is set.  Rows of q that no row counts keep their ``out``;
+    all of a row of more tokens than its masks have bits for become NaN.
     ``check_tables`` checks lengths, offsets and pages on the host (a device sync)."""
     dev, dt, i32 = q.get_device(), q.dtype, torch.int32
     qs, ps, ts, ms = q.shape, k_pool.shape, page_table.shape, masks.shape
@@ -505,8 +506,8 @@ def draft_tree(parents: torch.Tensor, seq_lens: torch.Tensor, offsets: torch.Ten
                out: DraftTree | None = None) -> DraftTree:
     """What each drafted token sees of its row's tree (itself and its ancestors) and its rotary position, from
     ``parents`` (int32 ``[T]``, places in the row's tree, negative: it follows the context).  Row b's tokens are
-    ``offsets[b] .. offsets[b] + counts[b] - 1``, up to ``64 * words`` (words 1..4), and the last of its ``seq_lens[b]``;
-    see ``cir_draft_tree``."""
+    ``offsets[b] .. offsets[b] + counts[b] - 1``, up to ``64 * words`` (words 1..4; a row of more gets empty masks), and the
+    last of its ``seq_lens[b]``; see ``cir_draft_tree``."""
     dev, i32 = parents.get_device(), torch.int32
     tokens, batch = parents.numel(), counts.numel()
     if not (dev >= 0 and _fits(parents, dev, i32, (tokens,)) and _fits(counts, dev, i32, (batch,))

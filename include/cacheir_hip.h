@@ -199,8 +199,9 @@ int cir_paged_decode_attention_shared(const void* q, const void* k_pool, const v
  * cir_draft_tree writes them, or any others).  Head h reads KV head h / (num_heads /
  * num_kv_heads).  offsets int32 [batch + 1] and counts int32 [batch] are as
  * cir_extend_page_tables writes them (offsets, granted); a row has at most
- * offsets[b + 1] - offsets[b] and 64 * words tokens, words 1..4.  Rows of q that no row
- * counts are not read and their out is left as it was.  A token that sees nothing yields
+ * offsets[b + 1] - offsets[b] and 64 * words tokens, words 1..4; all tokens of a row of more
+ * than 64 * words yield NaN.  Rows of q that no row counts are not read and their out is left
+ * as it was.  A token that sees nothing yields
  * zeros, one whose scores are all -inf NaN; K and V that a token does not see do not enter
  * its result, NaN and infinities among them.  Tokens past the table (max_pages * page_size)
  * are not seen.  fp16 with head_dim 128 and pages of a multiple of 16 tokens holds the weights
@@ -489,8 +490,9 @@ int cir_norm_rope_append(const void* q, int64_t q_token_stride, int64_t q_head_s
  *   masks[j][w] (int64 [tokens, words]): bit k of word w set where token 64 w + k of the row is
  *     j or one of its ancestors
  *   positions[j] = seq_lens[b] - n + the number of j's ancestors
- * Tokens that no row counts get empty masks and position 0.  batch < 2^24.  No counterpart in
- * the reference, which decodes one token at a time. */
+ * Tokens that no row counts get empty masks and position 0; a row of more than 64 * words
+ * tokens gets empty masks, and its positions mean nothing (cir_paged_tree_attention gives NaN
+ * for it).  batch < 2^24.  No counterpart in the reference, which decodes one token at a time. */
 int cir_draft_tree(const int32_t* parents, const int32_t* seq_lens, const int32_t* offsets, const int32_t* counts,
                    int64_t* masks, int32_t* positions, int tokens, int batch, int words, void* stream);
 

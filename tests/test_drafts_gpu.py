@@ -98,6 +98,25 @@ def test_draft_tree_of_odd_numbers(device):
     assert t.masks.shape == (0, 1)
 
 
+@pytest.mark.parametrize("words", [1, 2, 4])
+def test_draft_tree_rows_past_their_masks(device, words):
+    """A row of more tokens than its masks have bits for is refused: all of its masks are empty; other rows are as ever."""
+    from cacheir_amd import kernels
+
+    top = 64 * words
+    nodes, parents, masks, offsets = [3, top + 1, top, 2 * top + 9, 5], [], [], [0]
+    for b, n in enumerate(nodes):
+        p = tree(n, b)
+        parents += p
+        masks += seen_sets(p) if n <= top else [0] * n
+        offsets.append(len(parents))
+    lens = [n + 40 for n in nodes]
+    got = kernels.draft_tree(*(i32(x).to(device) for x in (parents, lens, offsets, nodes)), words=words)
+    assert torch.equal(got.masks.cpu(), mask_words(masks, words))
+    live = [j for b, n in enumerate(nodes) if n <= top for j in range(offsets[b], offsets[b + 1])]
+    assert [got.positions.tolist()[j] for j in live] == [39 + bin(masks[j]).count("1") for j in live]
+
+
 # --------------------------------------------------------------- attention -----
 def tree_case(seed, nodes, contexts, hq, hkv, d=128, psize=16, words=1, dtype=torch.float16, shape="any", gaps=None,
               extra=2):
@@ -336,6 +355,31 @@ def test_tree_attention_leaves_other_rows(device, hq, hkv, d, dtype):
     assert got is out
     check_tree(c, got)
     assert (got.cpu()[dead] == 7.0).all()
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype", KINDS)
+@pytest.mark.parametrize("nodes,words,context", [([5, 65, 64, 0, 9], 1, 0), ([300, 3], 2, 70), ([2, 257, 200, 600], 4, 3000)])
+def test_tree_attention_rows_past_their_masks(device, hq, hkv, d, dtype, nodes, words, context):
+    """A row of more tokens than its masks have bits for is refused: its tokens yield NaN (nothing says which drafted tokens
+    they see, and the first ones are no context); other rows are as ever, and check_tables raises."""
+    c = tree_case(len(nodes), nodes, [context + 3 * b for b in range(len(nodes))], hq, hkv, d=d, words=words, dtype=dtype,
+                  gaps=[b % 2 for b in range(len(nodes))])
+    over = [b for b, n in enumerate(nodes) if n > 64 * words]
+    out = torch.full_like(c["q"], 7.0).to(device)
+    got = run_tree(c, device, out=out).cpu()
+    refused = torch.zeros(got.shape[0], dtype=torch.bool)
+    for b in over:
+        first = int(c["offsets"][b])
+        refused[first: first + nodes[b]] = True
+    assert got[refused].isnan().all()
+    with pytest.raises(ValueError, match=f"row {over[0]}: counts exceed"):
+        run_tree(c, device, check_tables=True)
+    c["counts"][over] = 0
+    ref, tol = attention64(c, d ** -0.5)
+    idle = ref.isnan() & ~refused[:, None, None]
+    assert (got[idle] == 7.0).all()
+    live = ~ref.isnan()
+    assert bool(((got.double() - ref).abs()[live] <= tol[live]).all())
 
 
 @pytest.mark.parametrize("rows,nodes,hq,hkv", [(300, 3, 8, 2), (700, 1, 4, 4), (2300, 2, 4, 4), (40, 200, 8, 2)])

@@ -845,6 +845,40 @@ def test_adjust_logits_a_row_each(device):
     assert (got[2] == -math.inf).all()  # a mask without a bit
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("drafts", [False, True])
+def test_adjust_logits_values_and_bits(device, dtype, in_place, drafts):
+    """Every value that some rule names, in rows of their own and in rows of trees, and the bits of those that none names:
+    NaN of any payload, infinities, negative zeros and numbers below the normal range among them."""
+    from cacheir_amd import kernels
+
+    c = logits_case(13, [7, 1, 30] if drafts else [1] * 9, 9001, 200, dtype, drafts=drafts)
+    if not drafts:
+        for name in ("offsets", "drafts", "masks"):
+            del c[name]
+    kind, odd = ((torch.int32, [0x7fc01234, 0x7f800001, -0x3fffff, 0x7f800000, -0x800000, -2 ** 31, 1, -2 ** 31 + 77])
+                 if dtype == torch.float32 else
+                 (torch.int16, [0x7e21, 0x7c01, -0x1ff, 0x7c00, -0x400, -2 ** 15, 1, -2 ** 15 + 77]))
+    bits = c["logits"].contiguous().view(kind).clone()
+    for i, x in enumerate(odd):
+        bits[:, 11 + i:: 50] = x
+    c["logits"] = bits.view(dtype)
+    ref, tol = reference_logits(c)
+    d = {k: v.to(device) for k, v in c.items()}
+    got = kernels.adjust_logits(**d, out=d["logits"] if in_place else None).cpu()
+    kept = (tol == 0) & (ref != -math.inf) | (bits == odd[4]) & (ref == -math.inf)  # (-inf stays so under every rule)
+    kept |= ref.isnan() & ~tol.isnan()
+    assert torch.equal(got.view(kind)[kept], bits[kept]) and int(kept.sum()) > got.numel() // 3
+    finite = ref.isfinite()
+    # Below 2^-126 fp32 numbers lie 2^-149 apart, so each of the four roundings that logits64 counts in relative terms (a
+    # quotient or product, an FMA, two sums) may be off by half of that, 2^-150, instead.
+    tol = tol + (4 * 2.0 ** -150 if dtype == torch.float32 else 0.0)
+    assert bool(((got.double() - ref).abs()[finite] <= tol[finite]).all()) and int((finite & ~kept).sum()) > 100
+    assert torch.equal(got == -math.inf, ref == -math.inf) and torch.equal(got.isnan(), ref.isnan())
+    assert torch.equal(got == math.inf, ref == math.inf)
+
+
 def test_adjust_logits_the_same_token_many_times(device):
     from cacheir_amd import kernels
 

@@ -917,7 +917,8 @@ def adjust_logits(logits: torch.Tensor, offsets: torch.Tensor | None = None, *, 
     row stride).  Sequence b has the rows ``offsets[b] .. offsets[b + 1] - 1`` (int32 ``[B + 1]``; None: a row each),
     tokens ``history[b, : history_lens[b]]`` (int64 ``[B, L]``, int32 ``[B]``; the first ``prompt_lens[b]`` count for
     ``repetition`` only), and, where ``drafts`` (int64 ``[rows]``) and ``masks`` (``draft_tree``) are given, the drafted
-    tokens on the row's path.  ``repetition``, ``presence``, ``frequency``: float32 ``[B]``; ``bias_ids`` (int64, -1:
+    tokens on the row's path (the history ends before them, and before the token that opens the tree, which is one of
+    them: what stands in both counts twice).  ``repetition``, ``presence``, ``frequency``: float32 ``[B]``; ``bias_ids`` (int64, -1:
     unused) and ``bias`` (float32) ``[B, K]``; ``allowed``: int32 ``[rows, ceil(vocab / 32)]``, a bit per token.  ``out``
     may be ``logits``.  See ``cir_adjust_logits``."""
     _req(isinstance(logits, torch.Tensor), "logits must be a torch.Tensor", TypeError)

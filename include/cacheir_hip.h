@@ -204,8 +204,11 @@ int cir_paged_decode_attention_shared(const void* q, const void* k_pool, const v
  * as it was.  A token that sees nothing yields
  * zeros, one whose scores are all -inf NaN; K and V that a token does not see do not enter
  * its result, NaN and infinities among them.  Tokens past the table (max_pages * page_size)
- * are not seen.  fp16 with head_dim 128 and pages of a multiple of 16 tokens holds the weights
- * in fp16 (statistics and sums in fp32), other sizes (head_dim <= 256) run in fp32 arithmetic.
+ * are not seen.  fp16 with head_dim 128, pages of a multiple of 16 tokens, up to 1024 rows
+ * and 2048 query heads a KV head holds the weights in fp16 (statistics and sums in fp32); other
+ * sizes (head_dim <= 256) run in fp32 arithmetic, slower, and so do tables of W = max_pages *
+ * page_size tokens with W * (batch + tokens * heads per KV head / 256) near 2^36 or W *
+ * page_size past 2^40.
  * A row's last bits depend on the batch it is in.  out overlaps no input.  tokens * num_heads
  * < 2^26, num_kv_heads < 2^16, batch < 2^20.
  * workspace: cir_tree_attention_workspace_bytes bytes on a 16-byte address (0: NULL will do),
@@ -407,7 +410,8 @@ int cir_token_logprobs(const void* logits, int dt, int64_t ld, const int64_t* id
  * history int64 [batch, history_width] (entries from history_lens[b] on are not read, and
  * ids outside 0 .. vocab - 1 name no token), prompt_lens NULL: no prompt; drafts int64 and
  * masks int64 [rows, words] as cir_draft_tree writes them: the row's path are the tokens
- * drafts[offsets[b] + k] of the bits k of masks[row], its own among them; repetition (> 0),
+ * drafts[offsets[b] + k] of the bits k of masks[row], its own among them (the history ends
+ * before them: a token that is said once and stands in both counts twice); repetition (> 0),
  * presence and frequency float [batch] (NULL: 1, 0, 0); bias_ids int64 and bias float
  * [batch, bias_width] (ids outside the vocabulary: unused); allowed int32 [rows,
  * ceil(vocab / 32)].  What is NULL is left out.  out may be logits (at the same stride, then

@@ -399,9 +399,10 @@ __device__ __forceinline__ uint32_t not_finite(f16 x) {
 // 32.  The scores of the next block run on the matrix cores while the VALU takes this block's exponentials.
 //
 // Bound, and measured (kernel, then join): 8 trees of 57 to 64 tokens over 11000 to 16000, 32 query heads on 8 (107 GFLOP):
-// 168 + 10 us, 640 TFLOP/s, the matrix cores busy 40% of the cycles: a block of 32 tokens and 64 vectors a wavefront takes
-// 2500 cycles for 1024 of products, since one wavefront per SIMD issues an instruction in 4 to 5 cycles and products hide only
-// what stands between them.  32 trees of 5 to 16 tokens, 28 heads on 4 (238 MB of K and V): 63 + 6 us, 3.8 TB/s; 26 us of it
+// 155 + 10 us in a long run of calls, 690 TFLOP/s (up to 181 where the card's clocks fall), the matrix cores busy 40% of the
+// cycles: a block of 32 tokens and 64 vectors a wavefront takes 2500 cycles for 1024 of products.  Its 330 instructions, one
+// in 4 to 5 cycles from one wavefront per SIMD and 32 exponentials at a quarter of that rate, make some 2000 of them; what
+// the rest waits for is not known.  32 trees of 5 to 16 tokens, 28 heads on 4 (238 MB of K and V): 63 + 6 us, 3.8 TB/s; 26 us of it
 // are what comes before and behind the blocks of a workgroup's one or two pieces (plan 3.3 us, a piece's first loads 4, its
 // sums 3).  4 trees of 26 tokens over 300 to 3000: 22 + 5, all of it such.  K and V straight into registers, without a ring,
 // took 32 and 100 us where this took 31 and 75.

@@ -636,7 +636,9 @@ __device__ __forceinline__ void tree_piece(const Fast& F, const Piece& p, Smem& 
   // One block, `blk` (its V at byte `vcur` of the ring), and the scores of the next one, `bnext`; K of the one after that
   // (at `kafter`) is read beside the second products.
   //
-  // p = 2^(c sc - m) by one FMA, in fp16: the B operand of the second product.  The first block's scores set m, which
+  // p = 2^(c sc - m) by one FMA, in fp16: the B operand of the second product, since fp32 products are an eighth as fast.
+  // Each weight is rounded once (2^-11 of it, or 2^-25 below fp16's normal range) and the sum takes the rounded ones; the
+  // results' error against 64 bits is 2.8e-4 where fp32 weights, and the same fp16 output, leave 2.1e-4.  The first block's scores set m, which
   // follows the maximum only once a lane's 16 weights of a block sum to more than 2^8: then no p is larger, and fp16 holds it
   // as exactly as p <= 1; after a piece's first blocks the accumulators are hardly ever scaled, and no maximum is taken.
   // m is a rounded product, off by up to half an ulp: a factor that all p of the vector share.  From |m| = 2^24 on (where it

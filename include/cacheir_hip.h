@@ -200,17 +200,17 @@ int cir_paged_decode_attention_shared(const void* q, const void* k_pool, const v
  * num_kv_heads).  offsets int32 [batch + 1] and counts int32 [batch] are as
  * cir_extend_page_tables writes them (offsets, granted); a row has at most
  * offsets[b + 1] - offsets[b] and 64 * words tokens, words 1..4; all tokens of a row of more
- * than 64 * words yield NaN.  Rows of q that no row counts are not read and their out is left
- * as it was.  A token that sees nothing yields
- * zeros, one whose scores are all -inf NaN; K and V that a token does not see do not enter
- * its result, NaN and infinities among them.  Tokens past the table (max_pages * page_size)
- * are not seen.  fp16 with head_dim 128, pages of a multiple of 16 tokens, up to 1024 rows
- * and 2048 query heads a KV head holds the weights in fp16 (statistics and sums in fp32); other
- * sizes (head_dim <= 256) run in fp32 arithmetic, slower, and so do tables of W = max_pages *
- * page_size tokens with W * (batch + tokens * heads per KV head / 256) near 2^36 or W *
- * page_size past 2^40.
- * A row's last bits depend on the batch it is in.  out overlaps no input.  tokens * num_heads
- * < 2^26, num_kv_heads < 2^16, batch < 2^20.
+ * than 64 * words yield NaN.  Rows of q that no row counts are not read and their out is
+ * left as it was.  A token that sees nothing yields zeros, one whose scores are all -inf
+ * NaN; K and V that a token does not see do not enter its result, NaN and infinities among
+ * them.  Tokens past the table (max_pages * page_size) are not seen.  fp16 with head_dim
+ * 128, pages of a multiple of 16 tokens, up to 1024 rows and 2048 query heads a KV head
+ * holds the weights in fp16 (statistics and sums in fp32; weights below 2^-25 of a token's
+ * largest may count as zero); other sizes (head_dim <= 256) run in fp32 arithmetic, slower,
+ * and so do tables of W = max_pages * page_size tokens with W * (batch + tokens * heads per
+ * KV head / 256) near 2^36 or W * page_size past 2^40. A row's last bits depend on the
+ * batch it is in.  out overlaps no input.  tokens * num_heads < 2^26, num_kv_heads < 2^16,
+ * batch < 2^20.
  * workspace: cir_tree_attention_workspace_bytes bytes on a 16-byte address (0: NULL will do),
  * written by the call (calls that overlap need one each); nothing in it needs clearing.
  * The reference attends one new token a row (cacheir/backends/triton_kernels.py:174-217). */
@@ -411,14 +411,14 @@ int cir_token_logprobs(const void* logits, int dt, int64_t ld, const int64_t* id
  * ids outside 0 .. vocab - 1 name no token), prompt_lens NULL: no prompt; drafts int64 and
  * masks int64 [rows, words] as cir_draft_tree writes them: the row's path are the tokens
  * drafts[offsets[b] + k] of the bits k of masks[row], its own among them (the history ends
- * before them: a token that is said once and stands in both counts twice); repetition (> 0),
- * presence and frequency float [batch] (NULL: 1, 0, 0); bias_ids int64 and bias float
- * [batch, bias_width] (ids outside the vocabulary: unused); allowed int32 [rows,
- * ceil(vocab / 32)].  What is NULL is left out.  out may be logits (at the same stride, then
- * only what changes is written) and otherwise overlaps no input.  Rows that offsets do not
- * name are left as they were.  rows < 2^24, batch < 2^16, vocab <= 2^30, history_width <=
- * 2^20 - 257, bias_width <= 2047, words 1..4.  No counterpart in the reference, whose
- * sampling is greedy over all tokens (scheduler.py:535-543). */
+ * before them: a token that is said once and stands in both counts twice); repetition (>
+ * 0), presence and frequency float [batch] (NULL: 1, 0, 0); bias_ids int64 and bias float
+ * [batch, bias_width] (ids outside the vocabulary: unused); allowed int32 [rows, ceil(vocab
+ * / 32)].  What is NULL is left out.  out may be logits (at the same stride, then only what
+ * changes is written) and otherwise overlaps no input.  Rows that offsets do not name are
+ * left as they were.  rows < 2^24, batch < 2^16, vocab <= 2^30, history_width <= 2^20 -
+ * 257, bias_width <= 2047, words 1..4.  No counterpart in the reference, whose sampling is
+ * greedy over all tokens (scheduler.py:535-543). */
 int cir_adjust_logits(const void* logits, int64_t ld_in, void* out, int64_t ld_out, int dt, const int32_t* offsets,
                       const int64_t* history, const int32_t* history_lens, const int32_t* prompt_lens,
                       int history_width, const int64_t* drafts, const int64_t* masks, int words,
@@ -501,9 +501,9 @@ int cir_draft_tree(const int32_t* parents, const int32_t* seq_lens, const int32_
                    int64_t* masks, int32_t* positions, int tokens, int batch, int words, void* stream);
 
 /* The drafted tokens that the model confirms.  Rows as in cir_draft_tree, of any number of
- * tokens n, of which those from the 256th on are never taken; drafts int64 [tokens] are the tokens fed to the model,
- * targets int64 [tokens] what it chose after each.  The path starts at the row's token 0,
- * which stands, and goes on from token p to its first child whose draft equals targets[p]:
+ * tokens n, of which token 256 and later ones are never taken; drafts int64 [tokens] are the
+ * tokens fed to the model, targets int64 [tokens] what it chose after each.  The path starts
+ * at the row's token 0, which stands, and goes on from token p to its first child whose draft equals targets[p]:
  *   accepted[b]   tokens on the path: at least 1 (0 in a row without tokens), at most `most`
  *   path[b][i]    their places in the row's tree, then -1         int32 [batch, most]
  *   tokens_out[b][i]  targets[path[i]], what the row says, then -1  int64 [batch, most]

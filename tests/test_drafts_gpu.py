@@ -1055,7 +1055,7 @@ def test_accept_drafts(device, nodes, contexts, layers, hkv, d, psize, dtype, mo
 @pytest.mark.parametrize("shape,ids,most", [("any", 2, 256), ("any", 1, 256), ("chain", 1, 256), ("forest", 2, 9)])
 @pytest.mark.parametrize("give_back", [False, True])
 def test_accept_drafts_of_rows_past_256_tokens(device, shape, ids, most, give_back):
-    """The context ends before all of a row's drafted tokens; those from the 256th on are never taken."""
+    """The context ends before all of a row's drafted tokens; those past the first 256 are never taken."""
     from cacheir_amd import kernels
 
     nodes, contexts, psize = [300, 5, 257, 1000, 256], [37, 9, 0, 130, 16], 16
